@@ -27,8 +27,12 @@ TEXTGEN = os.path.join(HERE, "libgtk_textgen.so")
 PYMOD = os.path.join(HERE, "gputok_gpu" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 CLI = os.path.join(HERE, "gpu_tokenizer_blockbpe")
 
+CUDA_SOURCES = [os.path.join(CSRC, f) for f in ("gtk_kernels.cu", "gtk_api.cu", "gtk_embed.cu", "gtk_logprobs.cu", "gtk_table.cpp")]
+CUDA_DEPENDENCIES = CUDA_SOURCES + [os.path.join(CSRC, f) for f in (
+    "gtk_device.cuh", "gtk_tile.cuh", "gtk_rows.cuh", "gtk_table.hpp", "gtk_crew.hpp")] + [os.path.join(INCLUDE, "gputok_b200.h")]
+
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
-              "-Xcompiler", "-fPIC,-fvisibility=hidden", "-shared"]
+              "-Xcompiler", "-fPIC,-fvisibility=hidden", "-shared", "-t", "0"]
 
 
 def _stale(target: str, sources: list[str]) -> bool:
@@ -44,9 +48,7 @@ def _run(cmd: list[str]) -> None:
 
 
 def build_cuda(force: bool = False, ptxas_verbose: bool = False) -> str:
-    srcs = [os.path.join(CSRC, f) for f in ("gtk_kernels.cu", "gtk_api.cu", "gtk_table.cpp")]
-    deps = srcs + [os.path.join(CSRC, f) for f in ("gtk_device.cuh", "gtk_tile.cuh", "gtk_table.hpp", "gtk_crew.hpp")] + \
-        [os.path.join(INCLUDE, "gputok_b200.h")]
+    srcs, deps = CUDA_SOURCES, CUDA_DEPENDENCIES
     if force or _stale(LIB, deps):
         nvcc = os.environ.get("NVCC", "nvcc")
         extra = ["-Xptxas", "-v"] if ptxas_verbose else []
@@ -56,9 +58,7 @@ def build_cuda(force: bool = False, ptxas_verbose: bool = False) -> str:
 
 def build_cuda_checked(force: bool = False) -> str:
     """The bounds-checked build (stands in for a memory sanitizer, which this pool does not offer)."""
-    srcs = [os.path.join(CSRC, f) for f in ("gtk_kernels.cu", "gtk_api.cu", "gtk_table.cpp")]
-    deps = srcs + [os.path.join(CSRC, f) for f in ("gtk_device.cuh", "gtk_tile.cuh", "gtk_table.hpp", "gtk_crew.hpp")] + \
-        [os.path.join(INCLUDE, "gputok_b200.h")]
+    srcs, deps = CUDA_SOURCES, CUDA_DEPENDENCIES
     if force or _stale(LIB_CHECKED, deps):
         nvcc = os.environ.get("NVCC", "nvcc")
         _run([nvcc] + NVCC_FLAGS + ["-DGTK_CHECKED"] + srcs + ["-o", LIB_CHECKED])

@@ -1,0 +1,110 @@
+// gtk_rows.cuh -- what the operators on rows of numbers share (gtk_embed.cu, gtk_logprobs.cu): element types,
+// vector loads and stores, and the frame of their entry points.
+#pragma once
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+#include <mutex>
+#include <new>
+#include <string>
+
+#include "../../include/gputok_b200.h"
+#include "gtk_device.cuh"
+
+namespace gtk {
+
+// ------------------------------------------------------------------------------------------------ device side
+__device__ __forceinline__ float to_float(float x) { return x; }
+__device__ __forceinline__ float to_float(__nv_bfloat16 x) { return __bfloat162float(x); }
+__device__ __forceinline__ float to_float(__half x) { return __half2float(x); }
+
+template <class T>
+__device__ __forceinline__ T from_float(float x);
+template <>
+__device__ __forceinline__ float from_float<float>(float x) { return x; }
+template <>
+__device__ __forceinline__ __nv_bfloat16 from_float<__nv_bfloat16>(float x) { return __float2bfloat16_rn(x); }
+template <>
+__device__ __forceinline__ __half from_float<__half>(float x) { return __float2half_rn(x); }
+
+// V neighbouring elements as they lie in memory, moved in accesses of up to 16 bytes
+template <class T, int V>
+struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Pack {
+  T e[V];
+};
+
+template <class T, int V>
+__device__ __forceinline__ Pack<T, V> load_pack(const T* p) { return *reinterpret_cast<const Pack<T, V>*>(p); }
+template <class T, int V>
+__device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& v) { *reinterpret_cast<Pack<T, V>*>(p) = v; }
+
+// ------------------------------------------------------------------------------------------------ host side
+inline int element_size(int type) { return type == GTK_F32 ? 4 : 2; }
+inline bool known_type(int type) { return type == GTK_F32 || type == GTK_BF16 || type == GTK_F16; }
+inline bool aligned_to(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+// whether all rows of an array start on a multiple of what `pack` elements take, 16 bytes at most
+inline bool rows_aligned(const void* p, int64_t stride, int type, int pack)
+{
+  const int64_t bytes = std::min<int64_t>(16, int64_t(pack) * element_size(type));
+  return aligned_to(p, size_t(bytes)) && stride * element_size(type) % bytes == 0;
+}
+
+// f(T{}) for the C++ type of an element type that known_type() has accepted
+template <class F>
+cudaError_t with_type(int type, F&& f)
+{
+  switch (type) {
+    case GTK_F32: return f(float{});
+    case GTK_BF16: return f(__nv_bfloat16{});
+    default: return f(__half{});
+  }
+}
+
+template <class... Formal, class... Args>
+cudaError_t launch(void (*kernel)(Formal...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args&&... args)
+{
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid, cfg.blockDim = block, cfg.dynamicSmemBytes = smem, cfg.stream = stream;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Formal>(args)...);
+}
+
+// What a refused argument is reported with: a message, or nullptr when there is nothing to refuse.
+using Refusal = const char*;
+
+// An operator's call: check() is asked first, on host-only handles too; then launches(view) runs with the handle's
+// device current and the caller's put back afterwards.  Nothing is thrown past it.
+template <class Check, class Launches>
+int run_operator(gtk_tokenizer* h, Check&& check, Launches&& launches) noexcept
+{
+  HandleView v;
+  if (!handle_view(h, &v)) return GTK_ERR_INVALID_ARG;
+  try {
+    std::lock_guard<std::mutex> lock(*v.mu);
+    handle_view(h, &v);  // the stream as it is under the lock
+    if (const Refusal why = check()) {
+      *v.last_error = why;
+      return GTK_ERR_INVALID_ARG;
+    }
+    if (v.device < 0) {
+      *v.last_error = "host-only handle: no GPU entry points";
+      return GTK_ERR_NO_DEVICE;
+    }
+    int before    = -1;
+    cudaError_t e = cudaGetDevice(&before);
+    if (e == cudaSuccess && before != v.device) e = cudaSetDevice(v.device);
+    if (e == cudaSuccess) e = launches(v);
+    if (before >= 0 && before != v.device) cudaSetDevice(before);
+    if (e != cudaSuccess) {
+      *v.last_error = std::string("launch: ") + cudaGetErrorString(e);
+      return GTK_ERR_CUDA;
+    }
+    return GTK_OK;
+  } catch (...) {  // std::bad_alloc of a message, std::system_error of the lock
+    return GTK_ERR_MEMORY;
+  }
+}
+
+}  // namespace gtk

@@ -12,6 +12,8 @@ GTK_MODE_LOCALMIN = 2  # the reference's other rule (local minimum, max_iters pa
 GTK_RULE_GREEDY = 0
 GTK_RULE_LOCALMIN = 1
 NOALLOC_MAX_CHUNK_BYTES = 16384
+MAX_TOP = 32  # alternatives per row that token_logprobs gives at most
+ELEMENT_TYPES = {"f32": 0, "bf16": 1, "f16": 2}
 
 _PKG_ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 _LIB = None
@@ -82,6 +84,12 @@ def load_library() -> C.CDLL:
     lib.gtk_set_stage_timing.argtypes = [vp, C.c_int]
     lib.gtk_write_token_strings.argtypes = [vp, C.c_char_p, vp, vp, i64]
     lib.gtk_encode_chunks_noalloc.argtypes = [vp, vp, i64, vp, i64, i32, vp, vp]
+    f32 = C.c_float
+    lib.gtk_embed.argtypes = [vp, vp, i64, vp, C.c_int, i64, i64, i64, f32, vp, C.c_int, i64]
+    lib.gtk_embed_grad_workspace.argtypes = [vp, i64, i64, i64, C.POINTER(C.c_size_t)]
+    lib.gtk_embed_grad.argtypes = [vp, vp, i64, vp, C.c_int, i64, f32, i64, i64, vp, C.c_int, i64, C.c_int, vp, C.c_size_t]
+    lib.gtk_token_logprobs.argtypes = [vp, vp, C.c_int, i64, i64, i64, f32, vp, C.c_int, vp, vp, vp, vp, vp]
+    lib.gtk_token_logprobs_grad.argtypes = [vp, vp, C.c_int, i64, i64, i64, f32, vp, vp, vp, vp, vp, vp, i64]
     lib.gtk_pinned_alloc.argtypes = [C.c_size_t]
     lib.gtk_pinned_alloc.restype = vp
     lib.gtk_pinned_free.argtypes = [vp]
@@ -293,6 +301,48 @@ class Tokenizer:
         self._check(self._lib.gtk_encode_chunks_noalloc(self._h, d_bytes, int(n_bytes), d_chunk_offsets,
                                                         int(n_chunks), int(max_chunk_bytes), d_out_ids,
                                                         d_out_counts))
+
+    # ------------------------------------------------------------------ a model's two ends
+    # Raw device pointers (ints), element types by name ("f32", "bf16", "f16"), strides in elements.  Queued on the
+    # handle's stream: the calls return without waiting.
+    def embed(self, d_ids: int, n_ids: int, d_table: int, table_type: str, vocab: int, dim: int, d_out: int, out_type: str,
+              scale: float = 1.0, table_stride: int | None = None, out_stride: int | None = None) -> None:
+        """``out[i] = scale * table[ids[i]]``; a negative id gives zeros, an id >= vocab NaN."""
+        self._check(self._lib.gtk_embed(self._h, d_ids, n_ids, d_table, ELEMENT_TYPES[table_type], vocab, dim,
+                                        dim if table_stride is None else table_stride, scale, d_out, ELEMENT_TYPES[out_type],
+                                        dim if out_stride is None else out_stride))
+
+    def embed_grad_workspace(self, n_ids: int, vocab: int, dim: int) -> int:
+        """Bytes of device memory that ``embed_grad`` needs for a call of this size."""
+        n = C.c_size_t()
+        self._check(self._lib.gtk_embed_grad_workspace(self._h, n_ids, vocab, dim, C.byref(n)))
+        return n.value
+
+    def embed_grad(self, d_ids: int, n_ids: int, d_grad_out: int, out_type: str, vocab: int, dim: int, d_grad_table: int,
+                   table_type: str, d_workspace: int, workspace_bytes: int, scale: float = 1.0, accumulate: bool = False,
+                   out_stride: int | None = None, table_stride: int | None = None) -> None:
+        """Gradient of ``embed`` with respect to the table: all rows, or with ``accumulate`` added to the rows in use."""
+        self._check(self._lib.gtk_embed_grad(self._h, d_ids, n_ids, d_grad_out, ELEMENT_TYPES[out_type],
+                                             dim if out_stride is None else out_stride, scale, vocab, dim, d_grad_table,
+                                             ELEMENT_TYPES[table_type], dim if table_stride is None else table_stride,
+                                             1 if accumulate else 0, d_workspace, workspace_bytes))
+
+    def token_logprobs(self, d_logits: int, type: str, n_rows: int, vocab: int, d_targets: int = 0, d_logprob: int = 0,
+                       d_entropy: int = 0, d_lse: int = 0, top_k: int = 0, d_top_ids: int = 0, d_top_logprobs: int = 0,
+                       scale: float = 1.0, stride: int | None = None) -> None:
+        """Log probabilities of the given ids, entropies, log-sum-exps and the top_k alternatives of every row."""
+        self._check(self._lib.gtk_token_logprobs(self._h, d_logits, ELEMENT_TYPES[type], n_rows, vocab,
+                                                 vocab if stride is None else stride, scale, d_targets, top_k, d_logprob, d_entropy,
+                                                 d_lse, d_top_ids, d_top_logprobs))
+
+    def token_logprobs_grad(self, d_logits: int, type: str, n_rows: int, vocab: int, d_targets: int, d_lse: int,
+                            d_grad_logprob: int, d_grad_logits: int, d_entropy: int = 0, d_grad_entropy: int = 0,
+                            scale: float = 1.0, stride: int | None = None, grad_stride: int | None = None) -> None:
+        """Gradient of log probability and entropy with respect to the logits (in place when the pointers are equal)."""
+        self._check(self._lib.gtk_token_logprobs_grad(self._h, d_logits, ELEMENT_TYPES[type], n_rows, vocab,
+                                                      vocab if stride is None else stride, scale, d_targets, d_lse, d_entropy,
+                                                      d_grad_logprob, d_grad_entropy, d_grad_logits,
+                                                      vocab if grad_stride is None else grad_stride))
 
     # ------------------------------------------------------------------ decode
     def decode(self, ids) -> bytes:

@@ -283,6 +283,81 @@ GTK_API int gtk_encode_chunks_noalloc(gtk_tokenizer* h, const uint8_t* d_bytes, 
                                       const int64_t* d_chunk_offsets, int64_t n_chunks, int32_t max_chunk_bytes,
                                       int32_t* d_out_ids, int32_t* d_out_counts);
 
+/* ---------------------------------------------------------------------------------------------------------------
+ * Where a model takes ids in and gives them out (no counterpart in the reference, which hands its ids to a
+ * framework's model, compare_generation_quality.py:418-459).
+ *
+ * Four operators on device memory, beside gtk_encode_device whose ids they read and gtk_decode which prints the ids
+ * they find.  What they share:
+ *   - ids are int32 and count rows of the table (columns of the logits) as they are: 0 .. vocab-1 in whichever id
+ *     space the model was trained in (see gtk_set_id_space).  A negative id is no token (padding).  An id >= vocab is
+ *     a mistake: it never touches memory and shows as NaN;
+ *   - element types are GTK_F32, GTK_BF16 and GTK_F16; everything is summed in 32-bit floats and rounded once, to
+ *     nearest, where it is stored;
+ *   - strides count elements between the starts of neighbouring rows.  An input's may be anything >= 0 (0: every row is
+ *     the same one), an output's must be >= the row's length; what lies between an output's rows is left alone.
+ *     Pointers must be aligned to their elements, no more; rows that start on multiples of 16 bytes are fastest;
+ *   - they are queued on the handle's stream (gtk_set_stream) and return without waiting, allocate nothing and may be
+ *     captured into a CUDA graph (select the stream before the capture begins).  Only arguments that the host can see
+ *     are reported; they are looked at before anything else, on host-only handles too.  The calling thread's current
+ *     device is left as it was;
+ *   - results do not depend on the run, the stream or what else the GPU does: no sum is formed in the order in which
+ *     atomics arrive.
+ * ------------------------------------------------------------------------------------------------------------- */
+enum { GTK_F32 = 0, GTK_BF16 = 1, GTK_F16 = 2 };
+
+/* out[i][0..dim) = scale * table[ids[i]][0..dim), i < n_ids.  A negative id gives a row of zeros, an id >= vocab a row of
+ * NaN.  d_table is vocab rows of dim elements.  n_ids and vocab < 2^31, dim <= 2^20. */
+GTK_API int gtk_embed(gtk_tokenizer* h, const int32_t* d_ids, int64_t n_ids, const void* d_table, int table_type,
+                      int64_t vocab, int64_t dim, int64_t table_stride, float scale, void* d_out, int out_type,
+                      int64_t out_stride);
+
+/* Device memory that gtk_embed_grad needs for a call of this size (host arithmetic only). */
+GTK_API int gtk_embed_grad_workspace(gtk_tokenizer* h, int64_t n_ids, int64_t vocab, int64_t dim,
+                                     size_t* workspace_bytes);
+
+/* The table's gradient: grad_table[v][0..dim) = (accumulate ? grad_table[v] : 0) + scale * the sum of grad_out[i] over
+ * the i with ids[i] == v, formed in an order that is the same for the same ids.  accumulate == 0 writes every row (zeros
+ * where no id points), accumulate != 0 reads and writes only rows that an id points to: the micro-batches of a step,
+ * or a table whose gradient the model's last layer has written already.  Negative ids and ids >= vocab take no part.
+ * d_workspace: workspace_bytes of device memory, aligned to 16 bytes, at least what gtk_embed_grad_workspace says for
+ * the same sizes; its contents mean nothing before and after.  Calls (and replayed graphs) that may run at the same
+ * time need workspaces of their own.  d_grad_table must not overlap d_grad_out. */
+GTK_API int gtk_embed_grad(gtk_tokenizer* h, const int32_t* d_ids, int64_t n_ids, const void* d_grad_out, int out_type,
+                           int64_t out_stride, float scale, int64_t vocab, int64_t dim, void* d_grad_table,
+                           int table_type, int64_t table_stride, int accumulate, void* d_workspace,
+                           size_t workspace_bytes);
+
+/* Highest number of alternatives per row that gtk_token_logprobs gives. */
+#define GTK_MAX_TOP 32
+
+/* Row r of d_logits (vocab elements) stands for the distribution p_j = exp(scale * x_j - lse), lse = log sum_j
+ * exp(scale * x_j); scale > 0 is the inverse temperature.  Outputs, 32-bit floats, NULL for those that are not wanted
+ * (d_targets may be NULL when d_logprob is):
+ *   d_logprob[r]             log p of d_targets[r]; 0 where that is negative, NaN where it is >= vocab
+ *   d_entropy[r]             -sum_j p_j log p_j
+ *   d_lse[r]                 lse
+ *   d_top_ids[r][0..top_k)   the top_k columns of the highest logits, highest first, of equal ones the lowest column
+ *                            first (int32, rows back to back), and
+ *   d_top_logprobs[r][..]    their log p.  Columns at -inf are no alternatives: places that remain hold -1 and -inf
+ * A row of nothing but -inf (every id masked) has lse -inf, log p -inf, entropy 0 and no alternatives.  A row that holds
+ * a NaN or +inf has NaN everywhere (a negative target's 0 excepted) and no alternatives.  n_rows < 2^31,
+ * vocab <= 2^30, 0 <= top_k <= GTK_MAX_TOP. */
+GTK_API int gtk_token_logprobs(gtk_tokenizer* h, const void* d_logits, int type, int64_t n_rows, int64_t vocab,
+                               int64_t stride, float scale, const int32_t* d_targets, int top_k, float* d_logprob,
+                               float* d_entropy, float* d_lse, int32_t* d_top_ids, float* d_top_logprobs);
+
+/* The gradient of sum_r grad_logprob[r] * logprob[r] + grad_entropy[r] * entropy[r] with respect to the logits:
+ *   grad_logits[r][j] = scale * (g * ([j == t] - p_j) - e * p_j * (log p_j + entropy[r]))
+ * d_lse and d_entropy are what gtk_token_logprobs has given for the same logits and scale.  d_grad_entropy may be NULL
+ * (then d_entropy is not read), and so may d_grad_logprob (then d_targets is not read).  A row whose target is negative
+ * or >= vocab has g = 0; rows that neither part reaches, and rows of nothing but -inf, get zeros whatever they hold.
+ * d_grad_logits has the type of the logits and may be d_logits itself with the same stride; no other overlap. */
+GTK_API int gtk_token_logprobs_grad(gtk_tokenizer* h, const void* d_logits, int type, int64_t n_rows, int64_t vocab,
+                                    int64_t stride, float scale, const int32_t* d_targets, const float* d_lse,
+                                    const float* d_entropy, const float* d_grad_logprob, const float* d_grad_entropy,
+                                    void* d_grad_logits, int64_t grad_stride);
+
 /* Page-locked host memory for inputs (cudaHostAlloc / cudaFreeHost). */
 GTK_API void* gtk_pinned_alloc(size_t bytes);
 GTK_API void  gtk_pinned_free(void* p);

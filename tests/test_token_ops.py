@@ -1,0 +1,744 @@
+"""The operators at a model's two ends (ids to rows of a table, logits to log probabilities, and their gradients)
+against plain implementations in 64 bits, through the C ABI.
+
+Tolerances are bounds, not measurements: u = 2^-24 is half a step of a 32-bit float, a sum of n numbers in any order is
+off by at most (n - 1) u times the sum of their sizes, and storing a value costs half a step of its type.
+"""
+from __future__ import annotations
+
+import math
+
+import numpy as np
+import pytest
+
+from gputok_b200 import GtkError, Tokenizer, load_library
+
+U = 2.0 ** -24
+TYPES = ("f32", "bf16", "f16")
+
+
+# ---------------------------------------------------------------------------------------------------- refusals (CPU)
+@pytest.fixture(scope="module")
+def host(native_built, merges_path):
+    return Tokenizer(merges_path, 2048, 50, device=-1)
+
+
+P = 1 << 20  # an address that no refused call gets to use
+
+EMBED = dict(d_ids=P, n_ids=3, d_table=P, table_type="f32", vocab=10, dim=8, d_out=P, out_type="f32")
+EMBED_GRAD = dict(d_ids=P, n_ids=3, d_grad_out=P, out_type="f32", vocab=10, dim=8, d_grad_table=P, table_type="f32", d_workspace=P,
+                  workspace_bytes=1 << 30)
+SCORE = dict(d_logits=P, type="f32", n_rows=3, vocab=10, d_targets=P, d_logprob=P, d_entropy=P, d_lse=P, top_k=5, d_top_ids=P,
+             d_top_logprobs=P)
+SCORE_GRAD = dict(d_logits=P, type="f32", n_rows=3, vocab=10, d_targets=P, d_lse=P, d_grad_logprob=P, d_grad_logits=P, d_entropy=P,
+                  d_grad_entropy=P)
+
+REFUSED = [
+    ("embed", EMBED, [dict(n_ids=-1), dict(vocab=0), dict(dim=0), dict(n_ids=1 << 31), dict(vocab=1 << 31), dict(dim=(1 << 20) + 1),
+                      dict(table_stride=-1), dict(out_stride=7), dict(d_ids=0), dict(d_table=0), dict(d_out=0), dict(d_ids=P + 2),
+                      dict(d_table=P + 2), dict(d_out=P + 2), dict(d_out=P + 1, out_type="bf16")]),
+    ("embed_grad", EMBED_GRAD, [dict(n_ids=-1), dict(vocab=0), dict(dim=0), dict(n_ids=1 << 31), dict(vocab=1 << 31), dict(dim=(1 << 20) + 1),
+                                dict(out_stride=-1), dict(table_stride=7), dict(d_ids=0), dict(d_grad_out=0), dict(d_grad_table=0),
+                                dict(d_workspace=0), dict(d_workspace=P + 8), dict(workspace_bytes=255), dict(d_ids=P + 1),
+                                dict(d_grad_out=P + 2), dict(d_grad_table=P + 1, table_type="f16"), dict(n_ids=0, d_grad_table=0)]),
+    ("token_logprobs", SCORE, [dict(n_rows=-1), dict(vocab=0), dict(n_rows=1 << 31), dict(vocab=(1 << 30) + 1), dict(stride=-1),
+                               dict(scale=0.0), dict(scale=-1.0), dict(scale=math.inf), dict(scale=math.nan), dict(top_k=-1),
+                               dict(top_k=33), dict(top_k=0), dict(d_top_ids=0, d_top_logprobs=0), dict(d_logits=0), dict(d_targets=0),
+                               dict(d_logits=P + 2), dict(d_logits=P + 1, type="bf16"), dict(d_targets=P + 2), dict(d_lse=P + 1),
+                               dict(d_top_ids=P + 2)]),
+    ("token_logprobs_grad", SCORE_GRAD, [dict(n_rows=-1), dict(vocab=0), dict(n_rows=1 << 31), dict(vocab=(1 << 30) + 1), dict(stride=-1),
+                                         dict(grad_stride=9), dict(scale=0.0), dict(scale=math.nan), dict(d_logits=0), dict(d_lse=0),
+                                         dict(d_targets=0), dict(d_grad_logits=0), dict(d_entropy=0), dict(d_grad_logits=P + 2),
+                                         dict(d_logits=P + 1, type="f16"), dict(d_lse=P + 2), dict(stride=16, grad_stride=10)]),
+]
+
+
+@pytest.mark.parametrize("name,good,change", [(n, g, c) for n, g, cs in REFUSED for c in cs],
+                         ids=lambda v: v if isinstance(v, str) else ",".join(f"{k}={x}" for k, x in v.items()) if len(v) < 3 else "")
+def test_refused_arguments(host, name, good, change):
+    with pytest.raises(GtkError) as e:
+        getattr(host, name)(**{**good, **change})
+    assert e.value.code == 1 and len(str(e.value)) > 30
+
+
+@pytest.mark.parametrize("name,good", [(n, g) for n, g, _ in REFUSED])
+def test_host_only_handle_has_no_operators(host, name, good):
+    with pytest.raises(GtkError) as e:
+        getattr(host, name)(**good)
+    assert e.value.code == 6
+
+
+def test_unknown_types_and_null_handles(host):
+    lib = load_library()
+    assert lib.gtk_embed(host._h, P, 1, P, 3, 10, 8, 8, 1.0, P, 0, 8) == 1
+    assert lib.gtk_embed(host._h, P, 1, P, 0, 10, 8, 8, 1.0, P, -1, 8) == 1
+    assert lib.gtk_token_logprobs(host._h, P, 7, 1, 10, 10, 1.0, P, 0, P, None, None, None, None) == 1
+    assert lib.gtk_embed(None, P, 1, P, 0, 10, 8, 8, 1.0, P, 0, 8) == 1
+    assert lib.gtk_embed_grad_workspace(None, 1, 1, 1, None) == 1
+    assert lib.gtk_embed_grad_workspace(host._h, 1, 1, 1, None) == 1
+    with pytest.raises(GtkError):
+        host.embed_grad_workspace(1, 0, 1)
+
+
+def test_workspace_sizes(host):
+    """Enough for what the call keeps: sorted ids, and parts of sums; never beyond a small multiple of it."""
+    for n in (0, 1, 7, 4096, 131072, 1 << 22):
+        for vocab in (1, 257, 50257, 131072):
+            for dim in (1, 64, 777, 4096):
+                need = host.embed_grad_workspace(n, vocab, dim)
+                assert need >= 8 * n and need % 256 == 0
+                assert need < 64 * n + 4 * vocab + 48 * (1 << 20) + 64 * 8 * dim
+
+
+# ---------------------------------------------------------------------------------------------------- on the GPU
+@pytest.fixture(scope="module")
+def tok(native_built, merges_path):
+    import torch
+
+    t = Tokenizer(merges_path, 2048, 50, device=0)
+    t.set_stream(torch.cuda.current_stream().cuda_stream)
+    return t
+
+
+def dtype(name):
+    import torch
+
+    return {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}[name]
+
+
+def half_step(name):
+    import torch
+
+    return torch.finfo(dtype(name)).eps / 2
+
+
+def tiny(name):
+    """Half a step among the subnormals."""
+    import torch
+
+    fi = torch.finfo(dtype(name))
+    return fi.smallest_normal * fi.eps / 2
+
+
+def rows(values, name, stride=None, shift=0):
+    """The values (n x d) in an array of the type with a stride and a first element `shift` elements behind an aligned one;
+    what lies around holds a mark.  Returns (whole array, view)."""
+    import torch
+
+    n, d = values.shape
+    stride = d if stride is None else stride
+    whole = torch.full((n * stride + shift + 16,), 7.5, device="cuda", dtype=dtype(name))
+    view = whole[shift:].as_strided((n, d), (stride, 1))
+    view.copy_(values)
+    return whole, view
+
+
+def marks_untouched(whole, n, d, stride, shift):
+    import torch
+
+    keep = torch.ones_like(whole, dtype=torch.bool)
+    keep[shift:].as_strided((n, d), (stride, 1)).fill_(False)
+    return bool((whole[keep] == 7.5).all())
+
+
+def some_ids(seed, n, vocab, kind):
+    """int32 ids on the GPU: 'text' (id v about as often as 1 / v), 'one' (all the same), 'all' (every id once, shuffled),
+    'padded' (text with negative ids), 'wrong' (some >= vocab too)."""
+    import torch
+
+    g = torch.Generator().manual_seed(seed)
+    ids = (torch.exp(torch.rand(n, generator=g, dtype=torch.float64) * math.log(vocab + 1.0)) - 1).long().clamp(0, vocab - 1)
+    if kind == "one":
+        ids[:] = vocab // 2
+    if kind == "all":
+        ids = torch.randperm(max(n, vocab), generator=g)[:n] % vocab
+    if kind in ("padded", "wrong"):
+        ids[torch.rand(n, generator=g) < 0.3] = -1
+        ids[torch.rand(n, generator=g) < 0.05] = -(1 << 31)
+    if kind == "wrong":
+        ids[torch.rand(n, generator=g) < 0.1] = vocab
+        ids[torch.rand(n, generator=g) < 0.05] = (1 << 31) - 1
+    return ids.to(torch.int32).cuda()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("table_type", TYPES)
+@pytest.mark.parametrize("out_type", TYPES)
+@pytest.mark.parametrize("n,vocab,dim,ts,os,shift,kind", [
+    (1, 50257, 768, 768, 768, 0, "text"),
+    (1, 1, 1, 1, 1, 0, "one"),
+    (2, 300, 8, 16, 24, 0, "wrong"),
+    (33, 300, 100, 104, 128, 0, "padded"),       # rows aligned, their length no multiple of a pack
+    (257, 1000, 777, 777, 780, 1, "wrong"),
+    (100, 511, 1024, 1024, 1024, 1, "text"),     # packs would fit, the first element is not aligned
+    (65, 90, 4100, 4104, 4100, 0, "text"),
+    (4099, 5000, 256, 256, 256, 0, "padded"),
+    (50, 40, 64, 0, 64, 0, "text"),              # every row of the table is the same one
+])
+def test_embed(tok, table_type, out_type, n, vocab, dim, ts, os, shift, kind):
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(n + dim)
+    values = torch.randn(1 if ts == 0 else vocab, dim, generator=g, device="cuda")
+    _, table = rows(values, table_type, max(ts, dim), shift)
+    out_all, out = rows(torch.zeros(n, dim, device="cuda"), out_type, os, shift)
+    ids = some_ids(n, n, vocab, kind)
+    scale = 1.7
+    tok.embed(ids.data_ptr(), n, table.data_ptr(), table_type, vocab, dim, out.data_ptr(), out_type, scale=scale, table_stride=ts,
+              out_stride=os)
+    fine = (ids >= 0) & (ids < vocab)
+    want = table.double()[torch.zeros_like(ids) if ts == 0 else torch.where(fine, ids, torch.zeros_like(ids))]
+    want = want * float(np.float32(scale))
+    want = torch.where(fine[:, None], want, torch.zeros_like(want))
+    got = out.double()
+    assert bool((torch.isnan(got) == (ids >= vocab)[:, None]).all())
+    want = torch.where((ids >= vocab)[:, None], got, want)
+    # one product in 32 bits, one rounding to the type
+    err = (got - want).abs() - (want.abs() * (U + half_step(out_type) * (1 + U)) + tiny(out_type))
+    assert not bool((err > 0).any())
+    assert marks_untouched(out_all, n, dim, os, shift)
+
+
+@pytest.mark.gpu
+def test_embed_of_nothing(tok):
+    import torch
+
+    out = torch.full((8,), 3.0, device="cuda")
+    tok.embed(0, 0, 0, "f32", 10, 8, 0, "f32")
+    tok.embed(out.data_ptr(), 0, out.data_ptr(), "f32", 10, 8, out.data_ptr(), "f32")
+    assert bool((out == 3).all())
+
+
+def embed_grad(tok, ids, grad, grad_type, vocab, dim, table, table_type, spare=0, **more):
+    import torch
+
+    n = ids.numel()
+    need = tok.embed_grad_workspace(n, vocab, dim)
+    work = torch.full((need + spare,), 0xAB, device="cuda", dtype=torch.uint8)
+    tok.embed_grad(ids.data_ptr(), n, grad.data_ptr(), grad_type, vocab, dim, table.data_ptr(), table_type, work.data_ptr(), need, **more)
+    return work
+
+
+def check_embed_grad(ids, grad, vocab, dim, scale, base, got, table_type):
+    """Against the formula, with the bound that the number of summands gives."""
+    import torch
+
+    fine = (ids >= 0) & (ids < vocab)
+    at = ids[fine].long()
+    dy = grad.double()[fine]
+    scale = float(np.float32(scale))
+    total = torch.zeros(vocab, dim, device="cuda", dtype=torch.float64).index_add_(0, at, dy) * scale
+    size = torch.zeros(vocab, dim, device="cuda", dtype=torch.float64).index_add_(0, at, dy.abs()) * scale
+    count = torch.zeros(vocab, device="cuda", dtype=torch.float64).index_add_(0, at, torch.ones_like(at, dtype=torch.float64))
+    want = total if base is None else base.double() + total
+    # the sum, the product with scale, the base's addition, the rounding to the type
+    bound = size * (count[:, None] + 2) * U * 1.01 + want.abs() * (U + half_step(table_type) * 1.01) + tiny(table_type) + 1e-44
+    if base is not None:
+        bound = torch.where((count > 0)[:, None], bound, torch.zeros_like(bound))  # rows that no id points to are not touched
+    else:
+        assert bool((got[count == 0] == 0).all())
+    err = (got.double() - want).abs() - bound
+    assert not bool((err > 0).any()), float(err.max())
+
+
+GRAD_CASES = [
+    (1, 50257, 768, 768, 768, 0, "text"),
+    (1, 1, 1, 1, 1, 0, "one"),
+    (7, 300, 8, 16, 24, 0, "wrong"),
+    (33, 300, 100, 104, 128, 0, "padded"),
+    (600, 300, 100, 100, 100, 0, "one"),        # one sum over many units
+    (513, 1000, 777, 777, 780, 1, "wrong"),
+    (2048, 4096, 36, 40, 36, 0, "all"),
+    (2049, 257, 264, 264, 264, 0, "text"),
+    (5000, 70000, 64, 64, 72, 0, "padded"),     # ids beyond 16 bits
+    (9000, 600, 333, 333, 333, 0, "text"),
+    (40001, 50257, 96, 96, 96, 0, "text"),
+    (5000, 40, 64, 0, 64, 0, "text"),           # the same gradient for every token
+    (30, 300, 2050, 2056, 2056, 0, "text"),
+    (300, 12, 64, 64, 64, 0, "empty"),          # nothing but padding
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("grad_type,table_type", [("f32", "f32"), ("bf16", "f32"), ("bf16", "bf16"), ("f16", "f16"), ("f16", "f32")])
+@pytest.mark.parametrize("n,vocab,dim,gs,ts,shift,kind", GRAD_CASES)
+def test_embed_grad(tok, grad_type, table_type, n, vocab, dim, gs, ts, shift, kind, accumulate):
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(n + dim)
+    _, grad = rows(torch.randn(1 if gs == 0 else n, dim, generator=g, device="cuda"), grad_type, max(gs, dim), shift)
+    ids = some_ids(n, n, vocab, "text" if kind == "empty" else kind)
+    if kind == "empty":
+        ids.fill_(-1)
+    start = torch.randn(vocab, dim, generator=g, device="cuda")
+    whole, table = rows(start, table_type, ts, shift)
+    base = table.clone() if accumulate else None
+    embed_grad(tok, ids, grad, grad_type, vocab, dim, table, table_type, scale=0.75, accumulate=accumulate, out_stride=gs, table_stride=ts)
+    check_embed_grad(ids, grad.expand(n, dim) if gs == 0 else grad, vocab, dim, 0.75, base, table, table_type)
+    assert marks_untouched(whole, vocab, dim, ts, shift)
+    again_whole, again = rows(start, table_type, ts, shift)     # the same ids: the same bits
+    embed_grad(tok, ids, grad, grad_type, vocab, dim, again, table_type, scale=0.75, accumulate=accumulate, out_stride=gs, table_stride=ts)
+    assert torch.equal(again, table)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,vocab,dim", [(70000, 300, 64), (150000, 50257, 40), (300000, 200000, 24), (1 << 20, 1 << 19, 8)])
+@pytest.mark.parametrize("kind", ["text", "one", "all"])
+def test_embed_grad_of_many_tokens(tok, n, vocab, dim, kind):
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(n)
+    grad = torch.randn(n, dim, generator=g, device="cuda")
+    ids = some_ids(n, n, vocab, kind)
+    table = torch.empty(vocab, dim, device="cuda")
+    work = embed_grad(tok, ids, grad, "f32", vocab, dim, table, "f32", spare=4096)
+    check_embed_grad(ids, grad, vocab, dim, 1.0, None, table, "f32")
+    assert bool((work[-4096:] == 0xAB).all())
+
+
+@pytest.mark.gpu
+def test_embed_grad_of_nothing(tok):
+    import torch
+
+    table = torch.full((5, 24), 3.0, device="cuda")
+    tok.embed_grad(0, 0, 0, "f32", 5, 20, table.data_ptr(), "f32", 0, 0, accumulate=True, table_stride=24)
+    assert bool((table == 3).all())
+    tok.embed_grad(0, 0, 0, "f32", 5, 20, table.data_ptr(), "f32", 0, 0, table_stride=24)
+    assert bool((table[:, :20] == 0).all()) and bool((table[:, 20:] == 3).all())
+
+
+# ---------------------------------------------------------------------------------------------------- log probabilities
+def some_logits(seed, n, vocab, kind):
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    x = torch.randn(n, vocab, generator=g, device="cuda") * 3
+    if kind == "masked":             # rows with fewer and fewer columns left, the last with none
+        for r in range(n):
+            allowed = torch.rand(vocab, generator=g, device="cuda") < 0.5 ** (1 + r % 12)
+            x[r, ~allowed] = -math.inf
+        x[n - 1] = -math.inf
+    if kind == "lowest":             # masked with the type's lowest value; a whole row of it
+        x[:, ::2] = -65504.0
+        x[n // 2] = -65504.0
+    if kind == "ties":               # few different values, a constant row
+        x = x.round()
+        x[n // 2] = 1.0
+        x[0, ::3] = -0.0
+        x[0, 1::3] = 0.0
+    if kind == "peaked":             # far apart
+        x = x * 30
+    if kind == "rising":             # each column above the one before
+        x = torch.arange(vocab, device="cuda").float().expand(n, vocab) / 64
+    if kind == "crowded":            # the highest lie in columns that a few threads own
+        x[:, torch.arange(vocab, device="cuda") % 2048 < 160] += 40
+    return x
+
+
+def score(tok, x, name, targets, k, scale, stride):
+    import torch
+
+    n, vocab = x.shape
+    f = lambda *s: torch.full(s, 9.25, device="cuda")  # noqa: E731
+    lp, H, lse, ids, tops = f(n + 1), f(n + 1), f(n + 1), torch.full((n * k + 1,), 77, device="cuda", dtype=torch.int32), f(n * k + 1)
+    tok.token_logprobs(x.data_ptr(), name, n, vocab, targets.data_ptr(), lp.data_ptr(), H.data_ptr(), lse.data_ptr(), k,
+                       ids.data_ptr() if k else 0, tops.data_ptr() if k else 0, scale=scale, stride=stride)
+    for t in (lp, H, lse, tops):
+        assert float(t[-1]) == 9.25
+    assert int(ids[-1]) == 77
+    return lp[:-1], H[:-1], lse[:-1], ids[:-1].view(n, k), tops[:-1].view(n, k)
+
+
+def score_wanted(x, targets, k, scale):
+    """Formulas in 64 bits and bounds: lists (value, bound)."""
+    import torch
+
+    n, vocab = x.shape
+    scale = float(np.float32(scale))
+    raw = x.double()
+    top = raw.amax(1)
+    none = top == -math.inf
+    m = torch.where(none, torch.zeros_like(top), top)
+    y = (raw - m[:, None]) * scale
+    s = y.exp().sum(1)
+    log_s = s.log()
+    lse = m * scale + log_s
+    logp = y - log_s[:, None]            # not z - lse: around the lowest number 64 bits hold no log_s
+    logp[none] = -math.inf
+    p = logp.exp()
+    p[none] = 0
+    H = torch.where(p > 0, -p * logp, torch.zeros_like(p)).sum(1)
+    yy = torch.where(p > 0, p * y * y, torch.zeros_like(p)).sum(1)
+    # y: three roundings; 2^y: the approximation's 2^-22 and y's error; every thread adds at most vocab / 256 + 8 numbers, the threads' sums
+    # are joined in 13 steps with three roundings each, and a sum is rescaled (three roundings) once per new maximum of a
+    # thread, 24 at the outside for columns in any order but a rising one, where they are as many as the columns
+    steps = (vocab / 256 + 8) * 4 + 64
+    rel = steps * U + 2.0 ** -22 + 4 * U * H
+    lse_bound = rel + 2 * U * log_s.abs() + 2 * U * (m * scale).abs() + 2 * U * lse.abs()
+    H_bound = rel * (2 * H + 2) + 8 * U * yy + 4 * U * log_s.abs()
+    t = targets.long()
+    inside = (t >= 0) & (t < vocab)
+    lp = logp.gather(1, torch.where(inside, t, torch.zeros_like(t))[:, None])[:, 0]
+    yt = y.gather(1, torch.where(inside, t, torch.zeros_like(t))[:, None])[:, 0]
+    lp_bound = rel + 2 * U * log_s.abs() + 4 * U * torch.where(yt > -math.inf, yt.abs(), torch.zeros_like(yt))
+    lp = torch.where(none & inside, torch.full_like(lp, -math.inf), lp)
+    lp = torch.where(t < 0, torch.zeros_like(lp), torch.where(t >= vocab, torch.full_like(lp, math.nan), lp))
+    order = torch.sort(raw, dim=1, descending=True, stable=True)
+    best, ids = order.values[:, :k], order.indices[:, :k]
+    if vocab < k:
+        pad = torch.full((n, k - vocab), -1, device="cuda", dtype=ids.dtype)
+        best, ids = torch.cat([best, pad.double() * math.inf], 1), torch.cat([ids, pad], 1)
+    dead = best == -math.inf
+    ids = torch.where(dead, torch.full_like(ids, -1), ids)
+    tops = torch.where(dead, best, (best - m[:, None]) * scale - log_s[:, None])
+    bt = torch.where(dead, torch.zeros_like(best), (best - m[:, None]).abs() * scale)
+    tops_bound = (rel + 2 * U * log_s.abs())[:, None] + 4 * U * bt
+    lse = torch.where(none, torch.full_like(lse, -math.inf), lse)
+    return (lp, lp_bound), (H, H_bound), (lse, lse_bound), ids, (tops, tops_bound)
+
+
+def same(got, want, bound, what):
+    import torch
+
+    got = got.double()
+    assert bool((torch.isnan(got) == torch.isnan(want)).all()), what
+    fine = torch.isfinite(want)
+    assert bool((got[~fine & ~torch.isnan(want)] == want[~fine & ~torch.isnan(want)]).all()), what
+    bound = bound.expand_as(want)[fine]
+    err = (got[fine] - want[fine]).abs() - bound
+    assert not bool((err > 0).any()), (what, float(err.max()), float(bound.max()))
+
+
+SCORE_CASES = [
+    (1, 1, 1, 0, "plain"), (3, 2, 2, 0, "plain"), (1, 50257, 50257, 0, "plain"), (5, 31, 40, 1, "masked"), (9, 257, 257, 0, "plain"),
+    (20, 1000, 1000, 0, "masked"), (17, 1001, 1001, 1, "masked"), (4, 4099, 4104, 0, "ties"), (7, 8192, 8192, 0, "lowest"),
+    (3, 50257, 50304, 0, "masked"), (2, 50257, 50257, 1, "ties"), (6, 32003, 32003, 3, "peaked"), (2, 131072, 131072, 0, "plain"),
+    (2, 200001, 200001, 1, "masked"), (40, 3001, 3001, 0, "crowded"), (11, 50257, 50257, 0, "crowded"), (4, 9999, 9999, 0, "rising"),
+    (160, 777, 777, 0, "masked"), (400, 2053, 2056, 5, "ties"), (1300, 513, 513, 0, "plain"),
+]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("n,vocab,stride,shift,kind", SCORE_CASES)
+def test_token_logprobs(tok, name, n, vocab, stride, shift, kind):
+    import torch
+
+    _, x = rows(some_logits(n + vocab, n, vocab, kind), name, stride, shift)
+    if kind == "lowest":
+        lowest = torch.finfo(dtype(name)).min
+        x[x == torch.tensor(-65504.0).to(dtype(name)).item()] = lowest
+    targets = some_ids(vocab, n, vocab, "wrong" if n > 4 else "text")
+    for k, scale in ((0, 1.0), (1, 0.7), (20, 1.0), (32, 1.3)):
+        if kind == "lowest":
+            scale = min(scale, 1.0)      # 1.3 times the lowest number of 32 bits is none
+        lp, H, lse, ids, tops = score(tok, x, name, targets, k, scale, stride)
+        w_lp, w_H, w_lse, w_ids, w_tops = score_wanted(x, targets, k, scale)
+        assert torch.equal(ids.long(), w_ids), (k, scale)
+        same(lse, *w_lse, "lse")
+        same(lp, *w_lp, "logprob")
+        same(H, *w_H, "entropy")
+        same(tops, *w_tops, "top")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("vocab", [5, 1000, 50257])
+def test_rows_without_a_distribution(tok, vocab):
+    import torch
+
+    x = some_logits(1, 6, vocab, "plain")
+    x[1, vocab // 2] = math.nan
+    x[2, vocab - 1] = math.inf
+    x[3, 0] = math.nan
+    x[3, 1:] = -math.inf
+    x[4] = -math.inf
+    targets = torch.tensor([1, 0, 2, -1, 3, vocab], device="cuda", dtype=torch.int32)
+    lp, H, lse, ids, tops = score(tok, x, "f32", targets, 3, 1.0, vocab)
+    for r in (1, 2, 3):
+        assert math.isnan(lse[r]) and math.isnan(H[r]) and bool(torch.isnan(tops[r]).all()) and ids[r].tolist() == [-1] * 3
+    assert math.isnan(lp[1]) and math.isnan(lp[2]) and float(lp[3]) == 0 and math.isnan(lp[5])
+    assert float(lp[4]) == -math.inf and float(H[4]) == 0 and float(lse[4]) == -math.inf and ids[4].tolist() == [-1] * 3
+    for r in (0, 5):
+        assert bool(torch.isfinite(lse[r])) and (ids[r] >= 0).all()
+    g = torch.ones(6, device="cuda")
+    out = torch.full_like(x, 5.0)
+    tok.token_logprobs_grad(x.data_ptr(), "f32", 6, vocab, targets.data_ptr(), lse.data_ptr(), g.data_ptr(), out.data_ptr())
+    assert bool(torch.isnan(out[1]).all()) and bool((out[3:] == 0).all()) and bool(torch.isfinite(out[0]).all())
+
+
+@pytest.mark.gpu
+def test_outputs_that_are_not_wanted(tok):
+    import torch
+
+    x = some_logits(3, 5, 777, "plain")
+    targets = some_ids(3, 5, 777, "text")
+    lp, H, lse, ids, tops = score(tok, x, "f32", targets, 4, 1.0, 777)
+    one = torch.full((5,), 9.0, device="cuda")
+    tok.token_logprobs(x.data_ptr(), "f32", 5, 777, d_lse=one.data_ptr())
+    assert torch.equal(one, lse)
+    tok.token_logprobs(x.data_ptr(), "f32", 5, 777, d_entropy=one.data_ptr())
+    assert torch.equal(one, H)
+    tok.token_logprobs(x.data_ptr(), "f32", 5, 777, targets.data_ptr(), one.data_ptr())
+    assert torch.equal(one, lp)
+    few = torch.zeros(5, 4, device="cuda", dtype=torch.int32)
+    tok.token_logprobs(x.data_ptr(), "f32", 5, 777, top_k=4, d_top_ids=few.data_ptr())
+    assert torch.equal(few, ids)
+    some = torch.zeros(5, 4, device="cuda")
+    tok.token_logprobs(x.data_ptr(), "f32", 5, 777, top_k=4, d_top_logprobs=some.data_ptr())
+    assert torch.equal(some, tops)
+    tok.token_logprobs(0, "f32", 0, 777)
+    same_row = x[2:3]
+    tok.token_logprobs(same_row.data_ptr(), "f32", 5, 777, d_lse=one.data_ptr(), stride=0)
+    assert bool((one == lse[2]).all())
+
+
+def grad_wanted(x, targets, scale, g, e):
+    """The gradient in 64 bits and a bound on what 32 bits and the given statistics' own rounding make of it."""
+    import torch
+
+    n, vocab = x.shape
+    scale = float(np.float32(scale))
+    z = x.double() * scale
+    lse = torch.logsumexp(z, 1)
+    none = lse == -math.inf
+    safe = torch.where(none, torch.zeros_like(lse), lse)
+    logp = z - safe[:, None]
+    p = torch.where(none[:, None], torch.zeros_like(z), logp.exp())
+    logp = torch.where(p > 0, logp, torch.zeros_like(logp))
+    H = -(p * logp).sum(1)
+    t = targets.long()
+    inside = (t >= 0) & (t < vocab) & ~none
+    g = torch.where(inside, g.double(), torch.zeros_like(g.double())) if g is not None else torch.zeros(n, device="cuda", dtype=torch.float64)
+    here = (torch.arange(vocab, device="cuda")[None] == t[:, None]) & inside[:, None]
+    d = g[:, None] * (here.double() - p)
+    e = e.double() if e is not None else torch.zeros_like(g)
+    inner = logp + H[:, None]
+    d = d - e[:, None] * p * inner
+    err_z = 3 * U * logp.abs() + 2 * U * safe.abs()[:, None]
+    rel_p = err_z + 2.0 ** -22
+    bound = p * rel_p * (g[:, None].abs() + (e[:, None] * inner).abs()) + e[:, None].abs() * p * (err_z + 4 * U * H[:, None] + 4 * U * inner.abs())
+    # a p below 2^-126 (log p < -87) may count as 0: its whole part of the gradient, (|g| + |e (log p + H)|) p, is then missing
+    logp = torch.where(none[:, None], torch.zeros_like(z), z - safe[:, None]).clamp(min=-1000)
+    gone = p.clamp(max=2.0 ** -126) * (g[:, None].abs() + (e[:, None] * (logp + H[:, None])).abs())
+    bound = bound + gone + 4 * U * (g[:, None].abs() * (here.double() + p) + (e[:, None] * p * inner).abs())
+    return lse, H, d * scale, bound * scale
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("n,vocab,stride,shift,kind", [c for c in SCORE_CASES if c[4] != "lowest"])
+@pytest.mark.parametrize("parts", ["logprob", "entropy", "both"])
+def test_token_logprobs_grad(tok, name, n, vocab, stride, shift, kind, parts):
+    import torch
+
+    x_all, x = rows(some_logits(n + vocab, n, vocab, kind), name, stride, shift)
+    targets = some_ids(vocab, n, vocab, "wrong" if n > 4 else "text")
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    g = torch.randn(n, generator=gen, device="cuda") if parts != "entropy" else None
+    e = torch.randn(n, generator=gen, device="cuda") if parts != "logprob" else None
+    scale = 0.9
+    lse, H, want, bound = grad_wanted(x, targets, scale, g, e)
+    lse32, H32 = lse.float(), H.float()
+    bound = bound + want.abs() * half_step(name) * 1.01 + tiny(name) + 1e-36
+
+    def call(out, out_stride):
+        tok.token_logprobs_grad(x.data_ptr(), name, n, vocab, targets.data_ptr() if g is not None else 0, lse32.data_ptr(),
+                                g.data_ptr() if g is not None else 0, out.data_ptr(), H32.data_ptr() if e is not None else 0,
+                                e.data_ptr() if e is not None else 0, scale=scale, stride=stride, grad_stride=out_stride)
+
+    for out_stride, out_shift in ((stride, shift), (vocab + 3, 2), (stride, shift + 1)):
+        whole, out = rows(torch.zeros(n, vocab, device="cuda"), name, out_stride, out_shift)
+        call(out, out_stride)
+        same(out, want, bound, (out_stride, out_shift))
+        assert marks_untouched(whole, n, vocab, out_stride, out_shift)
+    if stride >= vocab:
+        call(x, stride)                                   # in place
+        same(x, want, bound, "in place")
+        assert marks_untouched(x_all, n, vocab, stride, shift)
+
+
+@pytest.mark.gpu
+def test_gradients_against_differences(tok):
+    """Central differences of the formulas in 64 bits: their own error is h^2 / 6 times third derivatives below 8 here, and
+    1e-16 / h of rounding times values below 4."""
+    import torch
+
+    n, vocab, scale = 4, 37, 0.8
+    x = some_logits(5, n, vocab, "plain")
+    targets = torch.tensor([0, 5, 36, -1], device="cuda", dtype=torch.int32)
+    g = torch.tensor([1.0, -0.5, 2.0, 3.0], device="cuda")
+    e = torch.tensor([0.5, 1.0, -1.0, 0.25], device="cuda")
+
+    def value(v):
+        z = v * float(np.float32(scale))
+        logp = z - torch.logsumexp(z, 1, keepdim=True)
+        lp = torch.where(targets >= 0, logp.gather(1, targets.clamp(min=0).long()[:, None])[:, 0], torch.zeros(n, device="cuda", dtype=torch.float64))
+        return g.double() * lp - e.double() * (logp.exp() * logp).sum(1)
+
+    h, want = 1e-4, torch.zeros(n, vocab, device="cuda", dtype=torch.float64)
+    for c in range(vocab):
+        d = torch.zeros_like(want)
+        d[:, c] = h
+        want[:, c] = (value(x.double() + d) - value(x.double() - d)) / (2 * h)
+    _, H, lse, _, _ = score(tok, x, "f32", targets, 0, scale, vocab)
+    out = torch.empty_like(x)
+    tok.token_logprobs_grad(x.data_ptr(), "f32", n, vocab, targets.data_ptr(), lse.data_ptr(), g.data_ptr(), out.data_ptr(), H.data_ptr(),
+                            e.data_ptr(), scale=scale)
+    _, _, _, bound = grad_wanted(x, targets, scale, g, e)
+    # the statistics come from the operator itself here: their error (of the order of 2^-20) counts too
+    assert bool(((out.double() - want).abs() <= bound + 2.0 ** -20 * 4 + 8 * h * h + 4e-16 / h * 4).all())
+
+
+# ---------------------------------------------------------------------------------------------------- as they are used
+@pytest.mark.gpu
+def test_from_text_to_gradients(native_built, merges_path):
+    """Text on the device -> ids -> rows -> logits of a tied table -> log probabilities and alternatives -> text; and back:
+    the gradient of the logits, and the table's from both its uses, against differentiation in 64 bits."""
+    import torch
+
+    import gputok_b200
+
+    t = Tokenizer(merges_path, 1 << 16, 50, device=0)
+    t.set_stream(torch.cuda.current_stream().cuda_stream)
+    vocab, dim = 50257, 64
+    data = gputok_b200.TextGen(3).text(3000)
+    d_bytes = torch.from_numpy(data.copy()).cuda()
+    d_off = torch.tensor([0, len(data)], dtype=torch.int64, device="cuda")
+    ids = torch.empty(len(data), dtype=torch.int32, device="cuda")
+    n, _, _ = t.encode_device(d_bytes.data_ptr(), len(data), d_off.data_ptr(), 1, ids.data_ptr(), len(data))
+    ids = ids[:n]
+    assert n > 300
+    g = torch.Generator(device="cuda").manual_seed(1)
+    table = torch.randn(vocab, dim, generator=g, device="cuda") * 0.3
+    mix = torch.randn(dim, dim, generator=g, device="cuda") * 0.3
+    x = torch.empty(n - 1, dim, device="cuda")
+    t.embed(ids.data_ptr(), n - 1, table.data_ptr(), "f32", vocab, dim, x.data_ptr(), "f32", scale=8.0)
+    hidden = (x.double() @ mix.double()).float()
+    logits = (hidden.double() @ table.double().T).float()
+    nxt = ids[1:].contiguous()
+    lp, H, lse, tops, top_lps = score(t, logits, "f32", nxt, 5, 1.0, vocab)
+    words = t.decode(tops.cpu().numpy().reshape(-1))
+    assert len(words) >= 5 * (n - 1)
+    assert t.decode(ids.cpu().numpy()) == data.tobytes()
+    w = torch.full((n - 1,), -1.0 / (n - 1), device="cuda")    # mean loss
+    t.token_logprobs_grad(logits.data_ptr(), "f32", n - 1, vocab, nxt.data_ptr(), lse.data_ptr(), w.data_ptr(), logits.data_ptr())
+    d_table = logits.double().T @ hidden.double()              # the head's part
+    d_x = ((logits.double() @ table.double()) @ mix.double().T).float()
+    d_table = d_table.float()
+    embed_grad(t, ids[:n - 1], d_x, "f32", vocab, dim, d_table, "f32", scale=8.0, accumulate=True)
+
+    T = table.double().requires_grad_()
+    z = (T[ids[:n - 1].long()] * 8.0 @ mix.double()) @ T.T
+    logp = torch.log_softmax(z, 1)
+    loss = -logp.gather(1, nxt.long()[:, None]).mean()
+    loss.backward()
+    assert abs(float(-lp.double().mean()) - float(loss)) < 1e-4
+    # f32 logits of size up to 60 are off by 2e-6, their probabilities by as much, sums of products with numbers below 60 of them
+    scale = float(T.grad.abs().max())
+    assert float((d_table.double() - T.grad).abs().max()) < 1e-4 * scale
+
+
+@pytest.mark.gpu
+def test_captured_and_replayed(native_built, merges_path):
+    """All four in one graph, replayed on other inputs in the same places; the handle's first calls of them."""
+    import torch
+
+    t = Tokenizer(merges_path, 2048, 50, device=0)
+    n, vocab, dim = 3000, 1000, 96
+    s = torch.cuda.Stream()
+    ids = some_ids(1, n, vocab, "padded")
+    table = torch.randn(vocab, dim, device="cuda")
+    out = torch.empty(n, dim, device="cuda")
+    grad = torch.empty(vocab, dim, device="cuda")
+    logits = some_logits(2, n, vocab, "plain")
+    lp, H, lse = (torch.empty(n, device="cuda") for _ in range(3))
+    top = torch.empty(n, 5, device="cuda", dtype=torch.int32)
+    w = torch.randn(n, device="cuda")
+    d_logits = torch.empty(n, vocab, device="cuda")
+    work = torch.empty(t.embed_grad_workspace(n, vocab, dim), device="cuda", dtype=torch.uint8)
+
+    def calls():
+        t.embed(ids.data_ptr(), n, table.data_ptr(), "f32", vocab, dim, out.data_ptr(), "f32")
+        t.token_logprobs(logits.data_ptr(), "f32", n, vocab, ids.data_ptr(), lp.data_ptr(), H.data_ptr(), lse.data_ptr(), 5, top.data_ptr())
+        t.token_logprobs_grad(logits.data_ptr(), "f32", n, vocab, ids.data_ptr(), lse.data_ptr(), w.data_ptr(), d_logits.data_ptr())
+        t.embed_grad(ids.data_ptr(), n, out.data_ptr(), "f32", vocab, dim, grad.data_ptr(), "f32", work.data_ptr(), work.numel())
+
+    torch.cuda.synchronize()
+    t.set_stream(s.cuda_stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        calls()
+    results = (out, grad, lp, H, lse, top, d_logits)
+    for seed in (4, 5):
+        ids.copy_(some_ids(seed, n, vocab, "padded"))
+        logits.copy_(some_logits(seed, n, vocab, "plain"))
+        work.fill_(0x55)
+        for r in results:
+            r.fill_(3)
+        graph.replay()
+        torch.cuda.synchronize()
+        got = [r.clone() for r in results]
+        for r in results:
+            r.fill_(4)
+        torch.cuda.synchronize()
+        calls()
+        torch.cuda.synchronize()
+        for a, b in zip(got, results):
+            assert torch.equal(a.nan_to_num(nan=-5.0), b.nan_to_num(nan=-5.0))
+        check_embed_grad(ids, out, vocab, dim, 1.0, None, grad, "f32")
+
+
+@pytest.mark.gpu
+def test_two_handles_on_two_streams(native_built, merges_path):
+    """Calls of two handles at once, each with its own workspace, give what they give alone."""
+    import torch
+
+    n, vocab, dim = 20000, 5000, 128
+    a, b = (Tokenizer(merges_path, 2048, 50, device=0) for _ in range(2))
+    sa, sb = torch.cuda.Stream(), torch.cuda.Stream()
+    a.set_stream(sa.cuda_stream)
+    b.set_stream(sb.cuda_stream)
+    sets = []
+    for t, seed in ((a, 1), (b, 2)):
+        ids = some_ids(seed, n, vocab, "text")
+        grad = torch.randn(n, dim, device="cuda")
+        sets.append((t, ids, grad, torch.empty(vocab, dim, device="cuda"),
+                     torch.empty(t.embed_grad_workspace(n, vocab, dim), device="cuda", dtype=torch.uint8)))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for t, ids, grad, out, work in sets:
+            t.embed_grad(ids.data_ptr(), n, grad.data_ptr(), "f32", vocab, dim, out.data_ptr(), "f32", work.data_ptr(), work.numel())
+    torch.cuda.synchronize()
+    for t, ids, grad, out, work in sets:
+        check_embed_grad(ids, grad, vocab, dim, 1.0, None, out, "f32")
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits(tok):
+    """A table and rows of logits whose last elements lie more than 2^32 elements behind the first."""
+    import torch
+
+    vocab, dim, n = 40, 16, 6
+    stride = 1 << 27
+    table = torch.empty(39 * stride + dim, device="cuda", dtype=torch.bfloat16)   # 10 GiB, hardly any of it touched
+    view = table.as_strided((vocab, dim), (stride, 1))
+    view.copy_(torch.randn(vocab, dim, device="cuda"))
+    ids = torch.tensor([39, 0, 38, 33, 39, 32], device="cuda", dtype=torch.int32)
+    out = torch.empty(n, dim, device="cuda")
+    tok.embed(ids.data_ptr(), n, view.data_ptr(), "bf16", vocab, dim, out.data_ptr(), "f32", table_stride=stride)
+    assert torch.equal(out, view[ids.long()].float())
+    grad = torch.randn(n, dim, device="cuda")
+    embed_grad(tok, ids, grad, "f32", vocab, dim, view, "bf16", table_stride=stride)
+    check_embed_grad(ids, grad, vocab, dim, 1.0, None, view, "bf16")
+    view.copy_(torch.randn(vocab, dim, device="cuda"))
+    targets = some_ids(1, vocab, dim, "text")
+    lp, H, lse, top, tops = score(tok, view, "bf16", targets, 3, 1.0, stride)
+    w_lp, w_H, w_lse, w_ids, w_tops = score_wanted(view, targets, 3, 1.0)
+    assert torch.equal(top.long(), w_ids)
+    same(lp, *w_lp, "logprob")
+    ones = torch.ones(vocab, device="cuda")
+    _, _, want, bound = grad_wanted(view, targets, 1.0, ones, None)
+    tok.token_logprobs_grad(view.data_ptr(), "bf16", vocab, dim, targets.data_ptr(), lse.data_ptr(), ones.data_ptr(), view.data_ptr(),
+                            stride=stride, grad_stride=stride)
+    same(view, want, bound + 2.0 ** -20 + want.abs() * half_step("bf16") * 1.01, "in place")
