@@ -71,6 +71,19 @@ cudaError_t launch(void (*kernel)(Formal...), dim3 grid, dim3 block, size_t smem
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<Formal>(args)...);
 }
 
+// the same in clusters of `cluster` blocks next to each other
+template <class... Formal, class... Args>
+cudaError_t launch_clusters(void (*kernel)(Formal...), dim3 grid, dim3 block, int cluster, cudaStream_t stream, Args&&... args)
+{
+  cudaLaunchAttribute attr{};
+  attr.id               = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = unsigned(cluster), attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid, cfg.blockDim = block, cfg.stream = stream;
+  cfg.attrs = &attr, cfg.numAttrs = cluster > 1 ? 1 : 0;
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Formal>(args)...);
+}
+
 // What a refused argument is reported with: a message, or nullptr when there is nothing to refuse.
 using Refusal = const char*;
 
