@@ -1,4 +1,6 @@
 // gtk_embed.cu -- embedding lookup with scaling, and its gradient by sorted tokens.
+#include <cooperative_groups.h>
+
 #include <algorithm>
 #include <cmath>
 
@@ -61,21 +63,24 @@ cudaError_t launch_embed(const gtk::HandleView& v, const int32_t* ids, int64_t n
 }
 
 // ------------------------------------------------------------------------------------------------ gradient
-// grad_table[v] = scale * sum of grad_out[i] over the i with ids[i] == v.  The ids are sorted (stable, by digits from the
-// lowest), which brings the rows of a sum next to each other in order of i.  The sorted positions are cut into units of
-// equal length; a row group walks a unit and keeps the running sum in registers.  A sum that begins and ends inside its
-// unit is stored right away; what a unit has of a sum that reaches over its ends goes to the workspace, and a last
-// kernel joins those parts from left to right.  Every sum is thus formed in an order that the ids alone decide.
-constexpr int kSortThreads = 512, kSortWarps = kSortThreads / 32;
-constexpr int kMaxDigitBits = 9;  // bins <= threads
+// grad_table[v] = scale * sum of grad_out[i] over the i with ids[i] == v, in three launches:
+//   k_embed_grad_sort   one cluster sorts the ids (stable, by digits from the lowest), which brings the rows of a sum next
+//                       to each other in order of i; the other CTAs meanwhile write the rows that no id points to
+//   k_embed_grad_sums   the sorted positions in blocks of equal length, a row group of threads per block; a sum is kept in
+//                       registers.  One that lies in a block or reaches over one boundary is its first block's alone; a
+//                       longer one is cut at the boundaries and its parts go to the workspace
+//   k_embed_grad_join   adds the parts of the long ones from left to right
+// Every sum is thus formed in an order that the ids alone decide.
+constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32, kSortCtas = 8;
+constexpr int kDigitBits = 8, kBins = 1 << kDigitBits;
 constexpr int64_t kMaxDim = int64_t(1) << 20;
 
 struct GradPlan {
-  int passes, digit_bits;
-  int rounds;         // a sort tile is rounds * kSortThreads ids
-  int64_t tiles;
-  int64_t unit_rows, units;
-  size_t at_pairs[2], at_counts, at_present, at_parts, bytes;
+  int passes;
+  int block_log2;   // sorted positions per block of k_embed_grad_sums
+  int64_t blocks;
+  int64_t pitch;    // 32-bit floats between rows of the parts
+  size_t at_pairs[2], at_long, at_parts, bytes;
 };
 
 int bits_of(int64_t x)
@@ -85,19 +90,18 @@ int bits_of(int64_t x)
   return b;
 }
 
+constexpr int kMinBlockLog2 = 3, kMaxBlockLog2 = 10;
+
 GradPlan grad_plan(int64_t n, int64_t vocab, int64_t dim)
 {
   GradPlan p{};
-  const int bits = std::max(1, bits_of(vocab));  // keys are 0 .. vocab, the last one stands for ids that take no part
-  p.passes       = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
-  p.digit_bits   = (bits + p.passes - 1) / p.passes;
-  p.rounds       = 4;
-  while (p.rounds < 32 && n > int64_t(64) * p.rounds * kSortThreads) p.rounds *= 2;
-  p.tiles = (n + int64_t(p.rounds) * kSortThreads - 1) / (int64_t(p.rounds) * kSortThreads);
-  // units: long enough that few sums are cut, short enough that their number times the columns fills the GPU
-  const int64_t most_units = std::max<int64_t>(64, (int64_t(4096) * 768) / dim);
-  p.unit_rows = std::max<int64_t>(8, (n + most_units - 1) / most_units);
-  p.units     = (n + p.unit_rows - 1) / p.unit_rows;
+  // keys are 0 .. vocab, the last one stands for ids that take no part
+  p.passes     = (bits_of(vocab) + kDigitBits - 1) / kDigitBits;
+  p.block_log2 = kMinBlockLog2;
+  // blocks as long as still leaves about 1.5 M columns of them: a dozen row groups of 768 columns per SM
+  while (p.block_log2 < kMaxBlockLog2 && (n >> (p.block_log2 + 1)) * dim >= int64_t(3) << 19) ++p.block_log2;
+  p.blocks    = (n + (int64_t(1) << p.block_log2) - 1) >> p.block_log2;
+  p.pitch     = (dim + 7) / 8 * 8;
   size_t at   = 0;
   auto room   = [&](size_t bytes) {
     const size_t here = at;
@@ -106,148 +110,212 @@ GradPlan grad_plan(int64_t n, int64_t vocab, int64_t dim)
   };
   p.at_pairs[0] = room(size_t(n) * sizeof(uint2));
   p.at_pairs[1] = room(size_t(n) * sizeof(uint2));
-  p.at_counts   = room(size_t(p.tiles) * (size_t(1) << p.digit_bits) * 4);
-  p.at_present  = room(size_t(vocab));
-  p.at_parts    = room(size_t(p.units) * 2 * size_t(dim) * 4);
+  p.at_long     = room(size_t(p.blocks + 1) * 4);
+  p.at_parts    = room(size_t(p.blocks) * 2 * size_t(p.pitch) * 4);
   p.bytes       = at;
   return p;
 }
 
-// what is sorted: the ids themselves in the first pass, {key, place} pairs in later ones
-struct SortInput {
+struct SortArgs {
   const int32_t* ids;
-  const uint2* pairs;
   int64_t n;
   uint32_t vocab;
-  __device__ uint2 at(int64_t i) const
+  int passes;
+  uint2 *pairs0, *pairs1;  // {key, place}: written by the first, third .. and by the second, fourth .. pass
+  uint32_t* long_sums;  // [0] how many, behind it the blocks in which they begin (k_embed_grad_sums)
+};
+
+struct SortShared {
+  uint32_t at[kSortWarps][kBins];
+  uint32_t total[kBins];
+  uint32_t warp_sum[kBins / 32];
+};
+
+// The ids of a CTA are a stretch of the whole, those of a warp a stretch of the CTA's; a pass counts the digits of every
+// stretch, turns the counts into places (digits in front, then stretches in front) and moves the pairs there.
+__device__ void sort_ids(const SortArgs& a, SortShared& S)
+{
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int cta         = int(cluster.block_rank());
+  const int64_t rounds  = (a.n + int64_t(kSortCtas) * kSortThreads - 1) / (int64_t(kSortCtas) * kSortThreads);
+  const int64_t first   = (int64_t(cta) * kSortWarps + warp) * rounds * 32;
+  const int64_t last    = min(a.n, first + rounds * 32);
+  const uint32_t lower  = (1u << lane) - 1u;
+  for (int pass = 0; pass < a.passes; ++pass) {
+    const int shift   = pass * kDigitBits;
+    const uint2* from = pass & 1 ? a.pairs0 : a.pairs1;
+    uint2* to         = pass & 1 ? a.pairs1 : a.pairs0;
+    auto load = [&](int64_t i) {
+      if (pass == 0) return make_uint2(min(uint32_t(__ldg(a.ids + i)), a.vocab), uint32_t(i));
+      return __ldcg(from + i);  // written by other SMs of the cluster
+    };
+    for (int b = lane; b < kBins; b += 32) S.at[warp][b] = 0;
+    __syncwarp();
+#pragma unroll 4
+    for (int64_t i = first + lane; i < last; i += 32) atomicAdd(&S.at[warp][(load(i).x >> shift) & (kBins - 1)], 1u);
+    __syncthreads();
+    if (tid < kBins) {
+      uint32_t sum = 0;
+#pragma unroll 8
+      for (int w = 0; w < kSortWarps; ++w) {
+        const uint32_t c = S.at[w][tid];
+        S.at[w][tid]     = sum;
+        sum += c;
+      }
+      S.total[tid] = sum;
+    }
+    cluster.sync();
+    uint32_t before = 0;
+    if (tid < kBins) {
+      uint32_t all = 0;
+#pragma unroll
+      for (int c = 0; c < kSortCtas; ++c) {
+        const uint32_t t = cluster.map_shared_rank(S.total, c)[tid];
+        before += c < cta ? t : 0u;
+        all += t;
+      }
+      uint32_t upto = all;
+#pragma unroll
+      for (int d = 1; d < 32; d *= 2) {
+        const uint32_t o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+        if (lane >= d) upto += o;
+      }
+      if (lane == 31) S.warp_sum[warp] = upto;
+      before += upto - all;
+    }
+    __syncthreads();
+    if (tid < kBins) {
+      for (int w = 0; w < warp; ++w) before += S.warp_sum[w];
+#pragma unroll 8
+      for (int w = 0; w < kSortWarps; ++w) S.at[w][tid] += before;
+    }
+    __syncthreads();
+#pragma unroll 2
+    for (int64_t i0 = first; i0 < last; i0 += 32) {
+      const int64_t i      = i0 + lane;
+      const bool here      = i < last;
+      const uint2 x        = here ? load(i) : make_uint2(0u, 0u);
+      const uint32_t digit = here ? (x.x >> shift) & uint32_t(kBins - 1) : 0xFFFFFFFFu;
+      const uint32_t peers = __match_any_sync(0xFFFFFFFFu, digit);
+      const uint32_t place = here ? S.at[warp][digit] + __popc(peers & lower) : 0u;
+      __syncwarp();
+      if (here && (peers >> lane) == 1u) S.at[warp][digit] = place + 1u;  // the last of the peers
+      __syncwarp();
+      if (here) to[place] = x;
+    }
+    cluster.sync();  // the pairs are where the next pass reads them; nobody reads S.total any more
+  }
+}
+
+// zeros over a row, however it lies
+template <class T>
+__device__ __forceinline__ void clear_row(T* row, int dim, int lane, int lanes)
+{
+  const int head = min(dim, int((16u - (uint32_t(reinterpret_cast<uintptr_t>(row)) & 15u)) % 16u / sizeof(T)));
+  constexpr int E = 16 / int(sizeof(T));
+  const int packs = (dim - head) / E;
+  uint4* body     = reinterpret_cast<uint4*>(row + head);
+  for (int p = lane; p < packs; p += lanes) body[p] = make_uint4(0u, 0u, 0u, 0u);
+  const T zero = gtk::from_float<T>(0.f);
+  for (int c = lane; c < dim - packs * E; c += lanes) row[c < head ? c : c + packs * E] = zero;
+}
+
+// The first cluster sorts, the CTAs behind it clear the rows that no id points to (accumulate == 0): each looks at all ids
+// for those of its own rows.
+template <class T>
+__global__ void __launch_bounds__(kSortThreads) __cluster_dims__(kSortCtas, 1, 1)
+k_embed_grad_sort(const SortArgs a, T* __restrict__ grad_table, int dim, int64_t table_stride)
+{
+  constexpr int kRowsAtOnce = sizeof(SortShared) / 4 * 32;
+  __shared__ union {
+    SortShared sort;
+    uint32_t used[kRowsAtOnce / 32];
+  } S;
+  if (blockIdx.x < kSortCtas) {
+    if (blockIdx.x == 0 && threadIdx.x == 0 && a.n > 0) a.long_sums[0] = 0;
+    if (a.n > 0) sort_ids(a, S.sort);
+    return;
+  }
+  const int64_t ctas = gridDim.x - kSortCtas, cta = blockIdx.x - kSortCtas;
+  const int64_t share = (a.vocab + ctas - 1) / ctas, end = min(int64_t(a.vocab), (cta + 1) * share);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  for (int64_t v0 = cta * share; v0 < end; v0 += kRowsAtOnce) {
+    const int rows = int(min(int64_t(kRowsAtOnce), end - v0));
+    for (int w = threadIdx.x; w < (rows + 31) / 32; w += kSortThreads) S.used[w] = 0;
+    __syncthreads();
+#pragma unroll 8
+    for (int64_t i = threadIdx.x; i < a.n; i += kSortThreads) {
+      const int64_t v = int64_t(__ldg(a.ids + i)) - v0;
+      if (v >= 0 && v < rows) {
+        const uint32_t bit = 1u << (v & 31);
+        if (!(S.used[v >> 5] & bit)) atomicOr(&S.used[v >> 5], bit);
+      }
+    }
+    __syncthreads();
+    for (int v = warp; v < rows; v += kSortWarps)
+      if (!(S.used[v >> 5] >> (v & 31) & 1u)) clear_row(grad_table + (v0 + v) * table_stride, dim, lane, 32);
+    __syncthreads();
+  }
+}
+
+// How a thread sees its V columns of a row, `valid` of them within the row.
+// Packs: rows start on 16-byte boundaries (or what V elements take), V = 8.
+// Words: 16-bit elements at any address, V = 2: the one or two aligned 32-bit words that hold them.  A word is read only
+// if an element of the row lies in it, so nothing is touched that the row does not share four bytes with.
+// Singles: 32-bit elements, V = 1.
+template <class T, int V>
+struct Columns {
+  static constexpr bool kWords = V == 2 && sizeof(T) == 2;
+  Pack<T, kWords ? 4 : V> raw;
+  uint32_t odd;
+  __device__ __forceinline__ void load(const T* p, int valid)
   {
-    if (pairs) return pairs[i];
-    const uint32_t id = uint32_t(ids[i]);
-    return make_uint2(min(id, vocab), uint32_t(i));
+    if constexpr (kWords) {
+      const uintptr_t at  = reinterpret_cast<uintptr_t>(p);
+      const uint32_t* w   = reinterpret_cast<const uint32_t*>(at & ~uintptr_t(3));
+      odd                 = uint32_t(at & 2) * 8;
+      uint32_t* r         = reinterpret_cast<uint32_t*>(&raw);
+      r[0]                = __ldg(w);
+      r[1]                = odd && valid > 1 ? __ldg(w + 1) : 0u;
+    } else if (valid >= V) {
+      raw = gtk::load_pack<T, V>(p);
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) raw.e[j] = j < valid ? p[j] : gtk::from_float<T>(0.f);
+    }
+  }
+  __device__ __forceinline__ void add_to(float (&sum)[V]) const
+  {
+    if constexpr (kWords) {
+      const uint32_t* r = reinterpret_cast<const uint32_t*>(&raw);
+      const uint32_t w  = __funnelshift_r(r[0], r[1], odd);
+      const T* e        = reinterpret_cast<const T*>(&w);
+      sum[0] += gtk::to_float(e[0]);
+      sum[1] += gtk::to_float(e[1]);  // beyond the row's end: never stored
+    } else {
+#pragma unroll
+      for (int j = 0; j < V; ++j) sum[j] += gtk::to_float(raw.e[j]);
+    }
   }
 };
 
-__global__ void __launch_bounds__(kSortThreads)
-k_digit_counts(SortInput in, int shift, int bins, int64_t tile, uint32_t* __restrict__ counts, uint8_t* __restrict__ present)
-{
-  __shared__ uint32_t s_count[1 << kMaxDigitBits];
-  for (int b = threadIdx.x; b < bins; b += kSortThreads) s_count[b] = 0;
-  if (present)
-    for (int64_t v = int64_t(blockIdx.x) * kSortThreads + threadIdx.x; v < in.vocab; v += int64_t(gridDim.x) * kSortThreads) present[v] = 0;
-  __syncthreads();
-  const int64_t from = blockIdx.x * tile, to = min(in.n, from + tile);
-  for (int64_t i = from + threadIdx.x; i < to; i += kSortThreads) atomicAdd(s_count + ((in.at(i).x >> shift) & (bins - 1)), 1u);
-  __syncthreads();
-  for (int b = threadIdx.x; b < bins; b += kSortThreads) counts[blockIdx.x * int64_t(bins) + b] = s_count[b];
-}
-
-template <int ROUNDS>
-__global__ void __launch_bounds__(kSortThreads)
-k_digit_scatter(SortInput in, int shift, int bins, const uint32_t* __restrict__ counts, uint2* __restrict__ out, uint8_t* __restrict__ present)
-{
-  __shared__ uint32_t s_at[kSortWarps][1 << kMaxDigitBits];
-  __shared__ uint32_t s_warp_sum[kSortWarps];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int b = lane; b < bins; b += 32) s_at[warp][b] = 0;
-  __syncwarp();
-  // places within the warp's own stretch of the tile
-  const int64_t first = int64_t(blockIdx.x) * (ROUNDS * kSortThreads) + warp * (ROUNDS * 32);
-  uint2 x[ROUNDS];
-  uint32_t place[ROUNDS];
-#pragma unroll
-  for (int r = 0; r < ROUNDS; ++r) {
-    const int64_t i = first + r * 32 + lane;
-    x[r]            = i < in.n ? in.at(i) : make_uint2(0u, 0u);
-  }
-#pragma unroll
-  for (int r = 0; r < ROUNDS; ++r) {
-    const bool here      = first + r * 32 + lane < in.n;
-    const uint32_t digit = here ? (x[r].x >> shift) & uint32_t(bins - 1) : 0xFFFFFFFFu;
-    const uint32_t peers = __match_any_sync(0xFFFFFFFFu, digit);
-    const uint32_t before = here ? s_at[warp][digit] : 0u;
-    place[r]              = before + __popc(peers & ((1u << lane) - 1u));
-    __syncwarp();
-    if (here && (peers >> lane) == 1u) s_at[warp][digit] = before + __popc(peers);  // the last of the peers
-    __syncwarp();
-  }
-  // where every bin of this tile begins: bins in front of it, and the same bin in the tiles in front
-  uint32_t total = 0, front = 0;
-  const int bin  = threadIdx.x;
-  if (bin < bins)
-    for (int64_t t = 0; t < gridDim.x; ++t) {
-      const uint32_t c = counts[t * bins + bin];
-      front += t < blockIdx.x ? c : 0u;
-      total += c;
-    }
-  uint32_t upto = total;
-#pragma unroll
-  for (int d = 1; d < 32; d *= 2) {
-    const uint32_t o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
-    if (lane >= d) upto += o;
-  }
-  if (lane == 31) s_warp_sum[warp] = upto;
-  __syncthreads();
-  if (bin < bins) {
-    uint32_t at = upto - total + front;
-    for (int w = 0; w < warp; ++w) at += s_warp_sum[w];
-    for (int w = 0; w < kSortWarps; ++w) {
-      const uint32_t c = s_at[w][bin];
-      s_at[w][bin]     = at;
-      at += c;
-    }
-  }
-  __syncthreads();
-#pragma unroll
-  for (int r = 0; r < ROUNDS; ++r)
-    if (first + r * 32 + lane < in.n) {
-      out[s_at[warp][(x[r].x >> shift) & uint32_t(bins - 1)] + place[r]] = x[r];
-      if (present && x[r].x < in.vocab) present[x[r].x] = 1;  // whoever writes it writes the same
-    }
-}
-
-// V columns of a row; valid < V at the end of a row that V does not divide
+// a finished sum to its row; packs: all V columns may be stored in one piece
 template <class T, int V>
-__device__ __forceinline__ void load_row(const T* p, int valid, float (&x)[V])
+__device__ __forceinline__ void store_sum(T* row, int valid, bool packs, float scale, bool accumulate, const float (&sum)[V])
 {
-  if (valid == V) {
-    const Pack<T, V> v = gtk::load_pack<T, V>(p);
-#pragma unroll
-    for (int j = 0; j < V; ++j) x[j] = gtk::to_float(v.e[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) x[j] = j < valid ? gtk::to_float(p[j]) : 0.f;
-  }
-}
-
-template <class T, int V>
-__device__ __forceinline__ void store_row(T* p, int valid, const float (&x)[V])
-{
-  if (valid == V) {
+  if (packs && valid >= V) {
     Pack<T, V> v;
+    if (accumulate) v = gtk::load_pack<T, V>(row);
 #pragma unroll
-    for (int j = 0; j < V; ++j) v.e[j] = gtk::from_float<T>(x[j]);
-    gtk::store_pack<T, V>(p, v);
+    for (int j = 0; j < V; ++j) v.e[j] = gtk::from_float<T>(accumulate ? fmaf(sum[j], scale, gtk::to_float(v.e[j])) : sum[j] * scale);
+    gtk::store_pack<T, V>(row, v);
   } else {
 #pragma unroll
     for (int j = 0; j < V; ++j)
-      if (j < valid) p[j] = gtk::from_float<T>(x[j]);
+      if (j < valid) row[j] = gtk::from_float<T>(accumulate ? fmaf(sum[j], scale, gtk::to_float(row[j])) : sum[j] * scale);
   }
-}
-
-// a finished sum to its row
-template <class T, int V>
-__device__ __forceinline__ void store_sum(T* row, int valid, float scale, bool accumulate, const float (&sum)[V])
-{
-  float y[V];
-  if (accumulate) {
-    load_row<T, V>(row, valid, y);
-#pragma unroll
-    for (int j = 0; j < V; ++j) y[j] = fmaf(sum[j], scale, y[j]);
-  } else {
-#pragma unroll
-    for (int j = 0; j < V; ++j) y[j] = sum[j] * scale;
-  }
-  store_row<T, V>(row, valid, y);
 }
 
 struct GradArgs {
@@ -255,99 +323,144 @@ struct GradArgs {
   int64_t n;
   uint32_t vocab;
   int dim;
-  int64_t unit_rows, units;
-  int64_t out_stride, table_stride;
+  int block_log2;
+  int64_t blocks;
+  int64_t out_stride, table_stride, pitch;
   float scale;
   bool accumulate;
-  float* parts;  // [units][2][dim]: of the sum that has begun in an earlier unit, of the one that goes on in the next
+  uint32_t* long_sums;
+  float* parts;  // [blocks][2][pitch]: of the long sum that begins further left, of the one that begins in the block
 };
 
 constexpr int kGradThreads = 256, kRowsInFlight = 8;
 
-template <class O, class T, int V>
-__global__ void __launch_bounds__(kGradThreads) k_embed_grad_units(const GradArgs a, const O* __restrict__ grad_out, T* __restrict__ grad_table)
+// first place in [from, to) whose key is not `key` (the keys are sorted and from there on >= key)
+__device__ __forceinline__ int end_of_key(const uint2* pairs, int from, int to, uint32_t key)
 {
-  const int64_t unit = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
-  const int c        = (blockIdx.y * blockDim.x + threadIdx.x) * V;
-  if (unit >= a.units || c >= a.dim) return;
-  const int valid     = min(V, a.dim - c);
-  const int64_t begin = unit * a.unit_rows, end = min(a.n, begin + a.unit_rows);
-  uint32_t key = __ldg(&a.pairs[begin].x);
-  bool from_before = begin > 0 && __ldg(&a.pairs[begin - 1].x) == key;
+  while (from < to) {
+    const int mid = (from + to) >> 1;
+    if (pairs[mid].x == key) from = mid + 1;
+    else to = mid;
+  }
+  return from;
+}
+
+template <class O, class T, int V>
+__global__ void __launch_bounds__(kGradThreads) k_embed_grad_sums(const GradArgs a, const O* __restrict__ grad_out, T* __restrict__ grad_table)
+{
+  extern __shared__ uint2 s_pairs[];  // [blockDim.y][2 * block]: the block's and the next one's
+  const int length    = 1 << a.block_log2;
+  const int64_t block = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
+  const int64_t begin = block << a.block_log2;
+  uint2* P            = s_pairs + threadIdx.y * 2 * length;
+  const int known     = int(max(int64_t(0), min(int64_t(2) * length, a.n - begin)));
+  for (int i = threadIdx.x; i < known; i += blockDim.x) P[i] = __ldg(a.pairs + begin + i);
+  __syncthreads();
+  const int c = (blockIdx.y * blockDim.x + threadIdx.x) * V;
+  if (known == 0 || c >= a.dim) return;
+  const int valid    = a.dim - c;
+  const int end      = min(length, known);
+  const uint32_t key0 = P[0].x;
+  // the sum that begins further left: skipped, or this block's part of a long one
+  bool from_left = begin > 0 && __ldg(&a.pairs[begin - 1].x) == key0;
+  int at = 0;
+  if (from_left) {
+    const bool is_long = (end < known && P[end].x == key0) || (begin > length && __ldg(&a.pairs[begin - length - 1].x) == key0);
+    if (!is_long) {
+      at        = end_of_key(P, 0, end, key0);
+      from_left = false;
+    }
+  }
+  if (at >= end) return;
+  // the sum that reaches over the end: to its end, or up to the boundary when it is a long one
+  const uint32_t key1 = P[end - 1].x;
+  int stop            = end;
+  bool to_right       = false;
+  if (end < known && P[end].x == key1 && !(from_left && key1 == key0)) {
+    to_right = begin + end + length < a.n && __ldg(&a.pairs[begin + end + length].x) == key1;
+    if (!to_right) stop = end_of_key(P, end, known, key1);
+    else if (key1 < a.vocab && c == 0) a.long_sums[1 + atomicAdd(a.long_sums, 1u)] = uint32_t(block);
+  }
+  uint32_t key = P[at].x;
   float sum[V] = {};
-  for (int64_t at = begin; at < end; at += kRowsInFlight) {
-    uint2 p[kRowsInFlight];
-    float x[kRowsInFlight][V];
+  auto finish  = [&](bool rest) {
+    if (from_left || rest) {
+      Pack<float, V> part;
 #pragma unroll
-    for (int k = 0; k < kRowsInFlight; ++k) p[k] = at + k < end ? __ldg(a.pairs + at + k) : make_uint2(a.vocab, 0u);
+      for (int j = 0; j < V; ++j) part.e[j] = sum[j];
+      gtk::store_pack<float, V>(a.parts + (block * 2 + (from_left ? 0 : 1)) * a.pitch + c, part);  // the pitch is a multiple of V
+    } else {
+      store_sum<T, V>(grad_table + int64_t(key) * a.table_stride + c, valid, V == 8, a.scale, a.accumulate, sum);
+    }
+    from_left = false;
+  };
+  for (; at < stop; at += kRowsInFlight) {
+    Columns<O, V> x[kRowsInFlight];
 #pragma unroll
     for (int k = 0; k < kRowsInFlight; ++k)
-      if (p[k].x < a.vocab) load_row<O, V>(grad_out + int64_t(p[k].y) * a.out_stride + c, valid, x[k]);
+      if (at + k < stop) x[k].load(grad_out + int64_t(P[at + k].y) * a.out_stride + c, valid);
 #pragma unroll
     for (int k = 0; k < kRowsInFlight; ++k) {
-      if (at + k >= end) break;
-      if (p[k].x != key) {
-        if (from_before) store_row<float, V>(a.parts + unit * 2 * a.dim + c, valid, sum);
-        else store_sum<T, V>(grad_table + int64_t(key) * a.table_stride + c, valid, a.scale, a.accumulate, sum);
-        from_before = false;
-        key         = p[k].x;
+      if (at + k >= stop) break;
+      const uint32_t now = P[at + k].x;
+      if (now != key) {
+        finish(false);
+        key = now;
 #pragma unroll
         for (int j = 0; j < V; ++j) sum[j] = 0.f;
       }
-      if (key >= a.vocab) return;  // sorted behind every sum
-#pragma unroll
-      for (int j = 0; j < V; ++j) sum[j] += x[k][j];
+      if (key >= a.vocab) return;  // ids that take no part, sorted behind all others
+      x[k].add_to(sum);
     }
   }
-  const bool goes_on = end < a.n && __ldg(&a.pairs[end].x) == key;
-  if (from_before) store_row<float, V>(a.parts + unit * 2 * a.dim + c, valid, sum);
-  else if (goes_on) store_row<float, V>(a.parts + (unit * 2 + 1) * a.dim + c, valid, sum);
-  else store_sum<T, V>(grad_table + int64_t(key) * a.table_stride + c, valid, a.scale, a.accumulate, sum);
+  finish(to_right);
 }
 
-// A block per unit in which a sum begins that goes on in the next.
+// The parts of a long sum, 128 columns at a time: each warp adds a run of parts, then the warps' sums are added in order.
 template <class T>
-__global__ void __launch_bounds__(kGradThreads) k_embed_grad_join(const GradArgs a, T* __restrict__ grad_table)
+__global__ void __launch_bounds__(kGradThreads) k_embed_grad_join(const GradArgs a, T* __restrict__ grad_table, bool packs)
 {
-  __shared__ int64_t s_units;
-  const int64_t unit  = blockIdx.x;
-  const int64_t begin = unit * a.unit_rows, end = min(a.n, begin + a.unit_rows);
-  if (end >= a.n) return;
-  const uint32_t key = a.pairs[end - 1].x;
-  if (key >= a.vocab || a.pairs[end].x != key) return;
-  if (a.pairs[begin].x == key && begin > 0 && a.pairs[begin - 1].x == key) return;  // begins further left
-  if (threadIdx.x < 32) {  // units behind this one that begin with the same key
-    int64_t more = 0;
+  constexpr int kWarps = kGradThreads / 32;
+  __shared__ float4 s_sum[kWarps][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int slabs     = (a.dim + 127) / 128;
+  const int64_t items = int64_t(a.long_sums[0]) * slabs;
+  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
+    const int64_t block = a.long_sums[1 + item / slabs];
+    const int c         = int(item % slabs) * 128 + lane * 4;
+    const uint32_t key  = a.pairs[((block + 1) << a.block_log2) - 1].x;
+    int64_t more = 0;  // blocks behind this one that begin with the same key
     for (;;) {
-      const int64_t u     = unit + 1 + more + threadIdx.x;
-      const uint32_t same = __ballot_sync(0xFFFFFFFFu, u < a.units && a.pairs[u * a.unit_rows].x == key);
+      const int64_t b     = block + 1 + more + lane;
+      const uint32_t same = __ballot_sync(0xFFFFFFFFu, b < a.blocks && a.pairs[b << a.block_log2].x == key);
       if (same != 0xFFFFFFFFu) {
         more += __ffs(~same) - 1;
         break;
       }
       more += 32;
     }
-    if (threadIdx.x == 0) s_units = more;
-  }
-  __syncthreads();
-  const int64_t more = s_units;
-  for (int c = threadIdx.x; c < a.dim; c += kGradThreads) {
-    float sum[1] = {a.parts[(unit * 2 + 1) * a.dim + c]};
+    const int64_t each = (more + 1 + kWarps - 1) / kWarps;
+    const int64_t from = warp * each, to = min(more + 1, from + each);
+    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (c < a.dim) {
 #pragma unroll 8
-    for (int64_t u = 1; u <= more; ++u) sum[0] += a.parts[(unit + u) * 2 * a.dim + c];
-    store_sum<T, 1>(grad_table + int64_t(key) * a.table_stride + c, 1, a.scale, a.accumulate, sum);
-  }
-}
-
-// zeros for the rows that no id points to
-template <class T, int V>
-__global__ void __launch_bounds__(kGradThreads)
-k_embed_grad_fill(const uint8_t* __restrict__ present, int64_t vocab, int dim, T* __restrict__ grad_table, int64_t table_stride)
-{
-  const float zero[V] = {};
-  for (int64_t v = int64_t(blockIdx.x) * blockDim.y + threadIdx.y; v < vocab; v += int64_t(gridDim.x) * blockDim.y) {
-    if (present && present[v]) continue;
-    for (int c = threadIdx.x * V; c < dim; c += blockDim.x * V) store_row<T, V>(grad_table + v * table_stride + c, min(V, dim - c), zero);
+      for (int64_t i = from; i < to; ++i) {  // part 0 is the one that begins in the block
+        const float4 x = *reinterpret_cast<const float4*>(a.parts + ((block + i) * 2 + (i == 0 ? 1 : 0)) * a.pitch + c);
+        sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+      }
+    }
+    s_sum[warp][lane] = sum;
+    __syncthreads();
+    if (warp == 0 && c < a.dim) {
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) {
+        const float4 x = s_sum[w][lane];
+        sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+      }
+      const float y[4] = {sum.x, sum.y, sum.z, sum.w};
+      store_sum<T, 4>(grad_table + int64_t(key) * a.table_stride + c, a.dim - c, packs, a.scale, a.accumulate, y);
+    }
+    __syncthreads();
   }
 }
 
@@ -366,40 +479,25 @@ template <class O, class T, int V>
 cudaError_t launch_embed_grad(const gtk::HandleView& v, const GradPlan& p, GradArgs a, const int32_t* ids, const void* grad_out,
                               void* grad_table, unsigned char* work)
 {
-  uint8_t* present = a.accumulate ? nullptr : work + p.at_present;
-  T* table         = static_cast<T*>(grad_table);
-  const unsigned tx = column_threads(a.dim, V), ty = kGradThreads / tx;
-  cudaError_t e     = cudaSuccess;
-  if (a.n > 0) {
-    SortInput in{ids, nullptr, a.n, a.vocab};
-    uint32_t* counts   = reinterpret_cast<uint32_t*>(work + p.at_counts);
-    const int bins     = 1 << p.digit_bits;
-    const int64_t tile = int64_t(p.rounds) * kSortThreads;
-    uint2* sorted      = nullptr;
-    for (int pass = 0; pass < p.passes && e == cudaSuccess; ++pass) {
-      const int shift = pass * p.digit_bits;
-      sorted          = reinterpret_cast<uint2*>(work + p.at_pairs[pass & 1]);
-      e = gtk::launch(k_digit_counts, dim3(unsigned(p.tiles)), dim3(kSortThreads), 0, v.stream, in, shift, bins, tile, counts,
-                      pass == 0 ? present : nullptr);
-      auto scatter = p.rounds == 4 ? k_digit_scatter<4> : p.rounds == 8 ? k_digit_scatter<8> : p.rounds == 16 ? k_digit_scatter<16>
-                                                                                                          : k_digit_scatter<32>;
-      if (e == cudaSuccess)
-        e = gtk::launch(scatter, dim3(unsigned(p.tiles)), dim3(kSortThreads), 0, v.stream, in, shift, bins, counts, sorted,
-                        pass == 0 ? present : nullptr);
-      in.pairs = sorted;
-    }
-    a.pairs = sorted;
-    if (e == cudaSuccess)
-      e = gtk::launch(k_embed_grad_units<O, T, V>, dim3(unsigned((p.units + ty - 1) / ty), unsigned((a.dim + tx * V - 1) / (tx * V))),
-                      dim3(tx, ty), 0, v.stream, a, static_cast<const O*>(grad_out), table);
-    if (e == cudaSuccess)
-      e = gtk::launch(k_embed_grad_join<T>, dim3(unsigned(p.units)), dim3(kGradThreads), 0, v.stream, a, table);
-  }
-  if (e == cudaSuccess && !a.accumulate) {
-    const int64_t blocks = std::min<int64_t>((a.vocab + ty - 1) / ty, int64_t(v.sm_count) * 8);
-    e = gtk::launch(k_embed_grad_fill<T, V>, dim3(unsigned(blocks)), dim3(tx, ty), 0, v.stream, a.n > 0 ? present : nullptr,
-                    int64_t(a.vocab), a.dim, table, a.table_stride);
-  }
+  T* table = static_cast<T*>(grad_table);
+  SortArgs s{ids, a.n, a.vocab, p.passes, reinterpret_cast<uint2*>(work + p.at_pairs[0]), reinterpret_cast<uint2*>(work + p.at_pairs[1]),
+             a.long_sums};
+  int64_t clear = 0;  // clusters that clear: one CTA per 64 KiB, as many as there are SMs
+  if (!a.accumulate)
+    clear = std::max<int64_t>(1, std::min<int64_t>(v.sm_count / kSortCtas, int64_t(a.vocab) * a.dim * int64_t(sizeof(T)) / (int64_t(kSortCtas) << 16)));
+  cudaError_t e = gtk::launch(k_embed_grad_sort<T>, dim3(unsigned((1 + clear) * kSortCtas)), dim3(kSortThreads), 0, v.stream, s, table, a.dim,
+                              a.table_stride);
+  if (e != cudaSuccess || a.n == 0) return e;
+  a.pairs = p.passes & 1 ? s.pairs0 : s.pairs1;
+  const unsigned tx = column_threads(a.dim, V), slabs = unsigned((a.dim + tx * V - 1) / (tx * V));
+  const unsigned pairs_bytes = unsigned(sizeof(uint2)) * 2u << a.block_log2;  // of a row group, 16 KiB at most
+  const unsigned ty = std::max(1u, std::min(kGradThreads / tx, 32768u / pairs_bytes));
+  e = gtk::launch(k_embed_grad_sums<O, T, V>, dim3(unsigned((p.blocks + ty - 1) / ty), slabs), dim3(tx, ty),
+                  ty * pairs_bytes, v.stream, a, static_cast<const O*>(grad_out), table);
+  // a sum is long when it holds a whole block
+  if (e == cudaSuccess && p.blocks > 2)
+    e = gtk::launch(k_embed_grad_join<T>, dim3(unsigned(std::min<int64_t>(p.blocks * ((a.dim + 127) / 128), int64_t(v.sm_count) * 8))),
+                    dim3(kGradThreads), 0, v.stream, a, table, V == 8);
   return e;
 }
 
@@ -480,14 +578,16 @@ extern "C" GTK_API int gtk_embed_grad(gtk_tokenizer* h, const int32_t* d_ids, in
   return gtk::run_operator(h, check, [&](const gtk::HandleView& v) -> cudaError_t {
     if (n_ids == 0 && accumulate) return cudaSuccess;
     const GradPlan p = grad_plan(n_ids, vocab, dim);
-    const GradArgs a{nullptr, n_ids, uint32_t(vocab), int(dim), p.unit_rows, p.units, out_stride, table_stride, scale, accumulate != 0,
-                     reinterpret_cast<float*>(static_cast<unsigned char*>(d_workspace) + p.at_parts)};
-    const bool packs = gtk::rows_aligned(d_grad_out, out_stride, out_type, 8) && gtk::rows_aligned(d_grad_table, table_stride, table_type, 8) &&
-                       dim % 4 == 0;  // the workspace's rows are dim 32-bit floats
+    unsigned char* work = static_cast<unsigned char*>(d_workspace);
+    const GradArgs a{nullptr, n_ids, uint32_t(vocab), int(dim), p.block_log2, p.blocks, out_stride, table_stride, p.pitch, scale, accumulate != 0,
+                     reinterpret_cast<uint32_t*>(work + p.at_long), reinterpret_cast<float*>(work + p.at_parts)};
+    const bool packs = gtk::rows_aligned(d_grad_out, out_stride, out_type, 8) && gtk::rows_aligned(d_grad_table, table_stride, table_type, 8);
     return gtk::with_type(out_type, [&](auto o) {
       return gtk::with_type(table_type, [&](auto t) {
-        auto f = packs ? launch_embed_grad<decltype(o), decltype(t), 8> : launch_embed_grad<decltype(o), decltype(t), 1>;
-        return f(v, p, a, d_ids, d_grad_out, d_grad_table, static_cast<unsigned char*>(d_workspace));
+        using O = decltype(o);
+        using T = decltype(t);
+        auto f  = packs ? launch_embed_grad<O, T, 8> : launch_embed_grad<O, T, sizeof(O) == 2 ? 2 : 1>;
+        return f(v, p, a, d_ids, d_grad_out, d_grad_table, work);
       });
     });
   });
