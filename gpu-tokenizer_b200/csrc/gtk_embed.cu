@@ -225,7 +225,7 @@ __device__ __forceinline__ void clear_row(T* row, int dim, int lane, int lanes)
 // The first cluster sorts, the CTAs behind it clear the rows that no id points to (accumulate == 0): each looks at all ids
 // for those of its own rows.
 template <class T>
-__global__ void __launch_bounds__(kSortThreads) __cluster_dims__(kSortCtas, 1, 1)
+__global__ void __launch_bounds__(kSortThreads, 2) __cluster_dims__(kSortCtas, 1, 1)
 k_embed_grad_sort(const SortArgs a, T* __restrict__ grad_table, int dim, int64_t table_stride)
 {
   constexpr int kRowsAtOnce = sizeof(SortShared) / 4 * 32;
@@ -332,7 +332,7 @@ struct GradArgs {
   float* parts;  // [blocks][2][pitch]: of the long sum that begins further left, of the one that begins in the block
 };
 
-constexpr int kGradThreads = 256, kRowsInFlight = 8;
+constexpr int kGradThreads = 256, kGradBlocksPerSm = 4;
 
 // first place in [from, to) whose key is not `key` (the keys are sorted and from there on >= key)
 __device__ __forceinline__ int end_of_key(const uint2* pairs, int from, int to, uint32_t key)
@@ -345,75 +345,89 @@ __device__ __forceinline__ int end_of_key(const uint2* pairs, int from, int to, 
   return from;
 }
 
-template <class O, class T, int V>
-__global__ void __launch_bounds__(kGradThreads) k_embed_grad_sums(const GradArgs a, const O* __restrict__ grad_out, T* __restrict__ grad_table)
+// Positions [at, stop) of the keys and places in P: sums of equal keys, each to finish(key, sum) when the key changes; the
+// rows are loaded kRowsInFlight at a time, whole packs of V columns where FULL.  Returns whether a last sum is left over.
+template <bool FULL, class O, int V, class Finish>
+__device__ __forceinline__ bool sum_rows(const uint2* P, int at, int stop, uint32_t vocab, const O* grad_out, int64_t stride, int valid,
+                                         uint32_t& key, float (&sum)[V], Finish&& finish)
 {
-  extern __shared__ uint2 s_pairs[];  // [blockDim.y][2 * block]: the block's and the next one's
-  const int length    = 1 << a.block_log2;
+  constexpr int kRowsInFlight = sizeof(Columns<O, V>) > 20 ? 4 : 8;
+  key = P[at].x;
+#pragma unroll
+  for (int j = 0; j < V; ++j) sum[j] = 0.f;
+  for (; at < stop; at += kRowsInFlight) {
+    Columns<O, V> x[kRowsInFlight];
+#pragma unroll
+    for (int k = 0; k < kRowsInFlight; ++k) x[k].load(grad_out + int64_t(P[min(at + k, stop - 1)].y) * stride, FULL ? V : valid);
+#pragma unroll
+    for (int k = 0; k < kRowsInFlight; ++k) {
+      if (at + k >= stop) break;
+      const uint32_t now = P[at + k].x;
+      if (now != key) {
+        finish(key, sum);
+        key = now;
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum[j] = 0.f;
+      }
+      if (key >= vocab) return false;  // ids that take no part, sorted behind all others
+      x[k].add_to(sum);
+    }
+  }
+  return true;
+}
+
+template <class O, class T, int V>
+__global__ void __launch_bounds__(kGradThreads, kGradBlocksPerSm) k_embed_grad_sums(const GradArgs a, const O* __restrict__ grad_out, T* __restrict__ grad_table)
+{
+  extern __shared__ uint2 s_pairs[];  // [blockDim.y][3 * block + 2]: the block's, its neighbours' and one more at each end
+  const int length    = 1 << a.block_log2, window = 3 * length + 2;
   const int64_t block = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
   const int64_t begin = block << a.block_log2;
-  uint2* P            = s_pairs + threadIdx.y * 2 * length;
-  const int known     = int(max(int64_t(0), min(int64_t(2) * length, a.n - begin)));
-  for (int i = threadIdx.x; i < known; i += blockDim.x) P[i] = __ldg(a.pairs + begin + i);
+  uint2* P            = s_pairs + threadIdx.y * window + length + 1;
+  for (int i = int(threadIdx.x) - length - 1; i <= 2 * length; i += blockDim.x)
+    P[i] = begin + i >= 0 && begin + i < a.n ? __ldg(a.pairs + begin + i) : make_uint2(0xFFFFFFFFu, 0u);  // beyond the ends: no key
   __syncthreads();
   const int c = (blockIdx.y * blockDim.x + threadIdx.x) * V;
-  if (known == 0 || c >= a.dim) return;
-  const int valid    = a.dim - c;
-  const int end      = min(length, known);
+  if (begin >= a.n || c >= a.dim) return;
+  const int valid     = a.dim - c;
+  const int end       = int(min(int64_t(length), a.n - begin));
   const uint32_t key0 = P[0].x;
   // the sum that begins further left: skipped, or this block's part of a long one
-  bool from_left = begin > 0 && __ldg(&a.pairs[begin - 1].x) == key0;
+  bool from_left = P[-1].x == key0;
   int at = 0;
-  if (from_left) {
-    const bool is_long = (end < known && P[end].x == key0) || (begin > length && __ldg(&a.pairs[begin - length - 1].x) == key0);
-    if (!is_long) {
-      at        = end_of_key(P, 0, end, key0);
-      from_left = false;
-    }
+  if (from_left && P[end].x != key0 && P[-length - 1].x != key0) {
+    at        = end_of_key(P, 0, end, key0);
+    from_left = false;
   }
   if (at >= end) return;
   // the sum that reaches over the end: to its end, or up to the boundary when it is a long one
   const uint32_t key1 = P[end - 1].x;
   int stop            = end;
   bool to_right       = false;
-  if (end < known && P[end].x == key1 && !(from_left && key1 == key0)) {
-    to_right = begin + end + length < a.n && __ldg(&a.pairs[begin + end + length].x) == key1;
-    if (!to_right) stop = end_of_key(P, end, known, key1);
+  if (P[end].x == key1 && !(from_left && key1 == key0)) {
+    to_right = P[2 * length].x == key1;
+    if (!to_right) stop = end_of_key(P, end, 2 * length, key1);
     else if (key1 < a.vocab && c == 0) a.long_sums[1 + atomicAdd(a.long_sums, 1u)] = uint32_t(block);
   }
-  uint32_t key = P[at].x;
-  float sum[V] = {};
-  auto finish  = [&](bool rest) {
-    if (from_left || rest) {
-      Pack<float, V> part;
+  uint32_t key;
+  float sum[V];
+  auto part = [&](int which, const float (&x)[V]) {
+    Pack<float, V> p;
 #pragma unroll
-      for (int j = 0; j < V; ++j) part.e[j] = sum[j];
-      gtk::store_pack<float, V>(a.parts + (block * 2 + (from_left ? 0 : 1)) * a.pitch + c, part);  // the pitch is a multiple of V
-    } else {
-      store_sum<T, V>(grad_table + int64_t(key) * a.table_stride + c, valid, V == 8, a.scale, a.accumulate, sum);
-    }
+    for (int j = 0; j < V; ++j) p.e[j] = x[j];
+    gtk::store_pack<float, V>(a.parts + (block * 2 + which) * a.pitch + c, p);  // the pitch is a multiple of V
+  };
+  auto finish = [&](uint32_t of, const float (&x)[V]) {
+    if (from_left) part(0, x);
+    else store_sum<T, V>(grad_table + int64_t(of) * a.table_stride + c, valid, V == 8, a.scale, a.accumulate, x);
     from_left = false;
   };
-  for (; at < stop; at += kRowsInFlight) {
-    Columns<O, V> x[kRowsInFlight];
-#pragma unroll
-    for (int k = 0; k < kRowsInFlight; ++k)
-      if (at + k < stop) x[k].load(grad_out + int64_t(P[at + k].y) * a.out_stride + c, valid);
-#pragma unroll
-    for (int k = 0; k < kRowsInFlight; ++k) {
-      if (at + k >= stop) break;
-      const uint32_t now = P[at + k].x;
-      if (now != key) {
-        finish(false);
-        key = now;
-#pragma unroll
-        for (int j = 0; j < V; ++j) sum[j] = 0.f;
-      }
-      if (key >= a.vocab) return;  // ids that take no part, sorted behind all others
-      x[k].add_to(sum);
-    }
-  }
-  finish(to_right);
+  const O* column = grad_out + c;
+  const bool rest = valid >= V ? sum_rows<true, O, V>(P, at, stop, a.vocab, column, a.out_stride, valid, key, sum, finish)
+                               : sum_rows<false, O, V>(P, at, stop, a.vocab, column, a.out_stride, valid, key, sum, finish);
+  if (!rest) return;
+  if (to_right) part(1, sum);
+  else finish(key, sum);
 }
 
 // The parts of a long sum, 128 columns at a time: each warp adds a run of parts, then the warps' sums are added in order.
@@ -430,14 +444,9 @@ __global__ void __launch_bounds__(kGradThreads) k_embed_grad_join(const GradArgs
     const int c         = int(item % slabs) * 128 + lane * 4;
     const uint32_t key  = a.pairs[((block + 1) << a.block_log2) - 1].x;
     int64_t more = 0;  // blocks behind this one that begin with the same key
-    for (;;) {
-      const int64_t b     = block + 1 + more + lane;
-      const uint32_t same = __ballot_sync(0xFFFFFFFFu, b < a.blocks && a.pairs[b << a.block_log2].x == key);
-      if (same != 0xFFFFFFFFu) {
-        more += __ffs(~same) - 1;
-        break;
-      }
-      more += 32;
+    for (int found = kGradThreads; found == kGradThreads; more += found) {
+      const int64_t b = block + 1 + more + threadIdx.x;
+      found           = __syncthreads_count(b < a.blocks && a.pairs[b << a.block_log2].x == key);
     }
     const int64_t each = (more + 1 + kWarps - 1) / kWarps;
     const int64_t from = warp * each, to = min(more + 1, from + each);
@@ -484,16 +493,16 @@ cudaError_t launch_embed_grad(const gtk::HandleView& v, const GradPlan& p, GradA
              a.long_sums};
   int64_t clear = 0;  // clusters that clear: one CTA per 64 KiB, as many as there are SMs
   if (!a.accumulate)
-    clear = std::max<int64_t>(1, std::min<int64_t>(v.sm_count / kSortCtas, int64_t(a.vocab) * a.dim * int64_t(sizeof(T)) / (int64_t(kSortCtas) << 16)));
+    clear = std::max<int64_t>(1, std::min<int64_t>(2 * v.sm_count / kSortCtas - 8, int64_t(a.vocab) * a.dim * int64_t(sizeof(T)) / (int64_t(kSortCtas) << 16)));
   cudaError_t e = gtk::launch(k_embed_grad_sort<T>, dim3(unsigned((1 + clear) * kSortCtas)), dim3(kSortThreads), 0, v.stream, s, table, a.dim,
                               a.table_stride);
   if (e != cudaSuccess || a.n == 0) return e;
   a.pairs = p.passes & 1 ? s.pairs0 : s.pairs1;
   const unsigned tx = column_threads(a.dim, V), slabs = unsigned((a.dim + tx * V - 1) / (tx * V));
-  const unsigned pairs_bytes = unsigned(sizeof(uint2)) * 2u << a.block_log2;  // of a row group, 16 KiB at most
-  const unsigned ty = std::max(1u, std::min(kGradThreads / tx, 32768u / pairs_bytes));
+  const unsigned pairs_bytes = unsigned(sizeof(uint2)) * ((3u << a.block_log2) + 2u);  // of a row group, 24 KiB at most
+  const unsigned ty = std::max(1u, std::min(kGradThreads / tx, 49152u / pairs_bytes));
   e = gtk::launch(k_embed_grad_sums<O, T, V>, dim3(unsigned((p.blocks + ty - 1) / ty), slabs), dim3(tx, ty),
-                  ty * pairs_bytes, v.stream, a, static_cast<const O*>(grad_out), table);
+                  size_t(ty) * pairs_bytes, v.stream, a, static_cast<const O*>(grad_out), table);
   // a sum is long when it holds a whole block
   if (e == cudaSuccess && p.blocks > 2)
     e = gtk::launch(k_embed_grad_join<T>, dim3(unsigned(std::min<int64_t>(p.blocks * ((a.dim + 127) / 128), int64_t(v.sm_count) * 8))),
