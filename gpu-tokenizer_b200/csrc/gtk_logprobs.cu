@@ -11,6 +11,8 @@
 
 namespace {
 
+using gtk::Two;
+
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr float kLn2 = 0.693147180559945309f, kLog2e = 1.44269504088896341f;
 
@@ -20,32 +22,6 @@ __device__ __forceinline__ float pow2(float y)
   float p;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(p) : "f"(y));
   return p;
-}
-
-// Two 32-bit floats that one instruction works on.
-struct Two {
-  uint64_t v;
-  Two() = default;
-  __device__ __forceinline__ Two(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi)); }
-  __device__ __forceinline__ void get(float& lo, float& hi) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
-};
-__device__ __forceinline__ Two operator+(Two a, Two b)
-{
-  Two d;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-  return d;
-}
-__device__ __forceinline__ Two operator*(Two a, Two b)
-{
-  Two d;
-  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-  return d;
-}
-__device__ __forceinline__ Two fma2(Two a, Two b, Two c)
-{
-  Two d;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-  return d;
 }
 
 // 16 bytes of a row: its elements as pairs of 32-bit floats, and their maximum (NaN only where all are).

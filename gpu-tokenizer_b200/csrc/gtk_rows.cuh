@@ -41,6 +41,32 @@ __device__ __forceinline__ Pack<T, V> load_pack(const T* p) { return *reinterpre
 template <class T, int V>
 __device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& v) { *reinterpret_cast<Pack<T, V>*>(p) = v; }
 
+// Two 32-bit floats that one instruction works on.
+struct Two {
+  uint64_t v;
+  Two() = default;
+  __device__ __forceinline__ Two(float lo, float hi) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(lo), "f"(hi)); }
+  __device__ __forceinline__ void get(float& lo, float& hi) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v)); }
+};
+__device__ __forceinline__ Two operator+(Two a, Two b)
+{
+  Two d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ Two operator*(Two a, Two b)
+{
+  Two d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+  return d;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c)
+{
+  Two d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return d;
+}
+
 // ------------------------------------------------------------------------------------------------ host side
 inline int element_size(int type) { return type == GTK_F32 ? 4 : 2; }
 inline bool known_type(int type) { return type == GTK_F32 || type == GTK_BF16 || type == GTK_F16; }
@@ -68,6 +94,10 @@ cudaError_t launch(void (*kernel)(Formal...), dim3 grid, dim3 block, size_t smem
 {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid, cfg.blockDim = block, cfg.dynamicSmemBytes = smem, cfg.stream = stream;
+  if (smem > (48 << 10)) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    if (e != cudaSuccess) return e;
+  }
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<Formal>(args)...);
 }
 
