@@ -75,12 +75,17 @@ constexpr int kOwnersLog2 = 7, kOwners = 1 << kOwnersLog2;  // CTAs of k_embed_g
 constexpr int kMaxDigitBits = 9;                            // a thread per bin at most
 constexpr int64_t kMaxDim = int64_t(1) << 20;
 
+// Of a block of tokens: the long sum that begins in it, and in how many blocks that has a part; parts == 0: none.
+struct LongSum {
+  uint32_t id, parts;
+};
+
 struct GradPlan {
   int passes, digit_bits;
   int block_log2;   // tokens per block of k_embed_grad_sums
   int64_t blocks;
   int64_t pitch;    // 32-bit floats between rows of the parts
-  size_t at_tokens[2], at_header, at_parts, bytes;
+  size_t at_tokens[2], at_long, at_parts, bytes;
 };
 
 int bits_of(int64_t x)
@@ -112,32 +117,29 @@ GradPlan grad_plan(int64_t n, int64_t vocab, int64_t dim)
   };
   p.at_tokens[0] = room(size_t(n) * sizeof(uint2));
   p.at_tokens[1] = room(size_t(n) * sizeof(uint2));
-  p.at_header    = room(size_t(p.blocks + 2) * 4);
+  p.at_long      = room(size_t(p.blocks) * sizeof(LongSum));
   p.at_parts     = room(size_t(p.blocks) * 2 * size_t(p.pitch) * 4);
   p.bytes        = at;
   return p;
 }
 
-// Written by k_embed_grad_sort and read by what follows.
-struct GradHeader {
-  uint32_t tokens;      // that take part
-  uint32_t long_sums;   // sums that k_embed_grad_sums has cut
-  uint32_t block[1];    // .. and the blocks in which they begin
-};
-
 struct SortArgs {
   const int32_t* ids;
   int64_t n;
   uint32_t vocab;
-  int passes, digit_bits;
+  int passes, digit_bits, block_log2;
   uint2 *tokens0, *tokens1;  // {id, place}: the grouped tokens end up in tokens0 after an even number of passes
-  GradHeader* header;
+  LongSum* long_sums;  // one per block
 };
+
+constexpr uint32_t kNoId = 0xFFFFFFFFu;  // ids are below 2^31
+constexpr int kListRoom  = 320;          // tokens of an owner that a warp finds in its part of the text
 
 struct SortShared {
   uint32_t at[kSortWarps][1 << kMaxDigitBits];
+  uint2 list[kSortWarps][kListRoom];
   uint32_t warp_sum[kSortWarps];
-  uint32_t lower[kSortWarps], mine[kSortWarps];
+  uint32_t lower[kSortWarps], mine[kSortWarps], valid[kSortWarps];
 };
 
 // The sum over the warps in front and over all of them, of a number that each warp has put into v.
@@ -152,27 +154,22 @@ __device__ __forceinline__ void over_warps(const uint32_t* v, int warp, uint32_t
   }
 }
 
-// One digit of a stable sort of the CTA's own `count` tokens.  Each warp takes a stretch of them, counts its digits, and
-// moves its tokens to the places that digits in front and stretches in front leave it.
-__device__ void sort_digit(const uint2* from, uint2* to, uint32_t count, int shift, int digit_bits, SortShared& S)
+// One digit of a stable sort of the CTA's own tokens, of which this warp has from[0 .. count) (each warp those behind the
+// warp in front).  Each warp counts its digits and moves its tokens to the places that digits in front and warps in front leave.
+__device__ void sort_digit(const uint2* from, uint32_t count, uint2* to, int shift, int digit_bits, SortShared& S)
 {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int bins         = 1 << digit_bits;
-  const uint32_t stretch = (count + kSortThreads - 1) / kSortThreads * 32;
-  const int warps        = int((count + stretch - 1) / stretch);  // that have any
-  const uint32_t first   = warp * stretch, last = min(count, first + stretch);
-  const uint32_t lower   = (1u << lane) - 1u;
-  if (warp < warps) {
-    for (int b = lane; b < bins; b += 32) S.at[warp][b] = 0;
-    __syncwarp();
+  const int bins       = 1 << digit_bits;
+  const uint32_t lower = (1u << lane) - 1u;
+  for (int b = lane; b < bins; b += 32) S.at[warp][b] = 0;
+  __syncwarp();
 #pragma unroll 4
-    for (uint32_t i = first + lane; i < last; i += 32) atomicAdd(&S.at[warp][(from[i].x >> shift) & (bins - 1)], 1u);
-  }
+  for (uint32_t i = lane; i < count; i += 32) atomicAdd(&S.at[warp][(from[i].x >> shift) & (bins - 1)], 1u);
   __syncthreads();
   uint32_t sum = 0;
   if (tid < bins) {
-#pragma unroll 4
-    for (int w = 0; w < warps; ++w) {
+#pragma unroll
+    for (int w = 0; w < kSortWarps; ++w) {
       const uint32_t c = S.at[w][tid];
       S.at[w][tid]     = sum;
       sum += c;
@@ -190,71 +187,116 @@ __device__ void sort_digit(const uint2* from, uint2* to, uint32_t count, int shi
     uint32_t front, all;
     over_warps(S.warp_sum, warp, front, all);
     front += upto - sum;
-#pragma unroll 4
-    for (int w = 0; w < warps; ++w) S.at[w][tid] += front;
+#pragma unroll
+    for (int w = 0; w < kSortWarps; ++w) S.at[w][tid] += front;
   }
   __syncthreads();
-  if (warp < warps) {
 #pragma unroll 2
-    for (uint32_t i0 = first; i0 < last; i0 += 32) {
-      const bool here      = i0 + lane < last;
-      const uint2 x        = here ? from[i0 + lane] : make_uint2(0u, 0u);
-      const uint32_t digit = here ? (x.x >> shift) & uint32_t(bins - 1) : 0xFFFFFFFFu;
-      const uint32_t peers = __match_any_sync(0xFFFFFFFFu, digit);
-      const uint32_t place = here ? S.at[warp][digit] + __popc(peers & lower) : 0u;
-      __syncwarp();
-      if (here && (peers >> lane) == 1u) S.at[warp][digit] = place + 1u;  // the last of the peers
-      __syncwarp();
-      if (here) to[place] = x;
-    }
+  for (uint32_t i0 = 0; i0 < count; i0 += 32) {
+    const bool here      = i0 + lane < count;
+    const uint2 x        = here ? from[i0 + lane] : make_uint2(0u, 0u);
+    const uint32_t digit = here ? (x.x >> shift) & uint32_t(bins - 1) : 0xFFFFFFFFu;
+    const uint32_t peers = __match_any_sync(0xFFFFFFFFu, digit);
+    const uint32_t place = here ? S.at[warp][digit] + __popc(peers & lower) : 0u;
+    __syncwarp();
+    if (here && (peers >> lane) == 1u) S.at[warp][digit] = place + 1u;  // the last of the peers
+    __syncwarp();
+    if (here) to[place] = x;
   }
   __syncthreads();
 }
 
+// f(is_mine[4], id[4], place of the first, lanes with any) for the ids of the warp's part, four per lane at a time.  Ids in front of the
+// array and behind it, which share 16 bytes with its ends, are nobody's.
+template <class F>
+__device__ __forceinline__ void scan_ids(const SortArgs& a, int warp, int lane, F&& f)
+{
+  const int64_t skip  = int64_t(reinterpret_cast<uintptr_t>(a.ids) & 15u) / 4;
+  const uint4* quads  = reinterpret_cast<const uint4*>(a.ids - skip);
+  const int64_t count = (a.n + skip + 3) / 4, each = ((count + kSortWarps - 1) / kSortWarps + 31) / 32 * 32;
+  const int64_t last  = min(count, (warp + 1) * each);
+  constexpr int kAhead = 4;
+  for (int64_t q0 = warp * each; q0 < last; q0 += 32 * kAhead) {
+    uint4 x[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) x[k] = q0 + k * 32 + lane < last ? __ldg(quads + q0 + k * 32 + lane) : make_uint4(kNoId, kNoId, kNoId, kNoId);
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k) {
+      const int64_t i = (q0 + k * 32 + lane) * 4 - skip;
+      uint32_t id[4]  = {x[k].x, x[k].y, x[k].z, x[k].w};
+      if (i < 0 || i + 4 > a.n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (i + j < 0 || i + j >= a.n) id[j] = kNoId;
+      f(id, i);
+    }
+  }
+}
+
 // CTA c owns the ids with id % kOwners == c: it looks at all ids, learns how many tokens lower owners have, which is where
-// its own go, writes them there in order and sorts them.  Nothing is waited for between CTAs.  Returns its share.
+// its own go, and sorts its own.  Nothing is waited for between CTAs.  Returns its share of the grouped tokens; behind the
+// last share are tokens of no id.
 __device__ void group_tokens(const SortArgs& a, SortShared& S, uint32_t& begin, uint32_t& count)
 {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t owner  = blockIdx.x;
-  const int64_t stretch = (a.n + kSortThreads - 1) / kSortThreads * 32;
-  const int64_t first   = min(a.n, warp * stretch), last = min(a.n, first + stretch);
-  uint32_t lower = 0, mine = 0;
-#pragma unroll 8
-  for (int64_t i = first + lane; i < last; i += 32) {
-    const uint32_t id = uint32_t(__ldg(a.ids + i)), of = id < a.vocab ? id & (kOwners - 1) : uint32_t(kOwners);
-    lower += of < owner;
-    mine += of == owner;
-  }
+  const uint32_t owner = blockIdx.x, lanes_below = (1u << lane) - 1u;
+  uint32_t lower = 0, valid = 0, mine = 0;
+  // the tokens of one step to to[], in order; returns how many
+  auto take = [&](const uint32_t (&id)[4], int64_t i, uint2* to, uint32_t room) {
+    uint32_t mask[4], total = 0, at = 0;
+    bool is_mine[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      is_mine[j] = id[j] < a.vocab && (id[j] & (kOwners - 1)) == owner;
+      mask[j]    = __ballot_sync(0xFFFFFFFFu, is_mine[j]);
+    }
+    if (!(mask[0] | mask[1] | mask[2] | mask[3])) return 0u;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      total += __popc(mask[j]);
+      at += __popc(mask[j] & lanes_below);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (is_mine[j]) {
+        if (at < room) to[at] = make_uint2(id[j], uint32_t(i + j));
+        ++at;
+      }
+    return total;
+  };
+  scan_ids(a, warp, lane, [&](const uint32_t (&id)[4], int64_t i) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      valid += id[j] < a.vocab;
+      lower += id[j] < a.vocab && (id[j] & (kOwners - 1)) < owner;
+    }
+    mine += take(id, i, S.list[warp] + mine, mine < kListRoom ? kListRoom - mine : 0u);
+  });
   lower = __reduce_add_sync(0xFFFFFFFFu, lower);
-  mine  = __reduce_add_sync(0xFFFFFFFFu, mine);
-  if (lane == 0) S.lower[warp] = lower, S.mine[warp] = mine;
-  __syncthreads();
-  uint32_t at;
+  valid = __reduce_add_sync(0xFFFFFFFFu, valid);
+  if (lane == 0) S.lower[warp] = lower, S.mine[warp] = mine, S.valid[warp] = valid;
+  const bool listed = !__syncthreads_or(mine > kListRoom);
+  uint32_t at, all;
+  over_warps(S.valid, warp, at, all);
   over_warps(S.lower, warp, at, begin);
   over_warps(S.mine, warp, at, count);
-  if (owner == kOwners - 1 && tid == 0) a.header->tokens = begin + count;
-  if (mine) {
-    uint2* to = a.tokens0 + begin + at;
-    for (int64_t i0 = first; i0 < last; i0 += 8 * 32) {
-      uint32_t id[8];
-#pragma unroll
-      for (int k = 0; k < 8; ++k) id[k] = i0 + k * 32 + lane < last ? uint32_t(__ldg(a.ids + i0 + k * 32 + lane)) : 0xFFFFFFFFu;
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const bool is_mine  = id[k] < a.vocab && (id[k] & (kOwners - 1)) == owner;
-        const uint32_t mask = __ballot_sync(0xFFFFFFFFu, is_mine);
-        if (!mask) continue;
-        if (is_mine) to[__popc(mask & ((1u << lane) - 1u))] = make_uint2(id[k], uint32_t(i0 + k * 32 + lane));
-        to += __popc(mask);
-      }
-    }
+  uint2* const last = a.passes & 1 ? a.tokens1 : a.tokens0;
+  for (int64_t i = int64_t(all) + int64_t(owner) * kSortThreads + tid; i < a.n; i += int64_t(kOwners) * kSortThreads) {
+    last[i] = make_uint2(kNoId, 0u);
+    if (i + 1 == a.n || ((i + 1) & ((1 << a.block_log2) - 1)) == 0) a.long_sums[i >> a.block_log2] = LongSum{kNoId, 0u};
   }
-  __syncthreads();
   if (count == 0) return;
-  for (int pass = 0; pass < a.passes; ++pass)
-    sort_digit((pass & 1 ? a.tokens1 : a.tokens0) + begin, (pass & 1 ? a.tokens0 : a.tokens1) + begin, count,
-               kOwnersLog2 + pass * a.digit_bits, a.digit_bits, S);
+  if (!listed) {
+    uint2* to = a.tokens0 + begin + at;
+    scan_ids(a, warp, lane, [&](const uint32_t (&id)[4], int64_t i) { to += take(id, i, to, 128u); });
+    __syncthreads();
+  }
+  const uint32_t stretch = (count + kSortThreads - 1) / kSortThreads * 32, first = min(count, warp * stretch), some = min(count - first, stretch);
+  for (int pass = 0; pass < a.passes; ++pass) {
+    const bool from_list = pass == 0 && listed;
+    sort_digit(from_list ? S.list[warp] : (pass & 1 ? a.tokens1 : a.tokens0) + begin + first, from_list ? mine : some,
+               (pass & 1 ? a.tokens0 : a.tokens1) + begin, kOwnersLog2 + pass * a.digit_bits, a.digit_bits, S);
+  }
 }
 
 // zeros over a row, however it lies
@@ -277,16 +319,33 @@ k_embed_grad_sort(const SortArgs a, T* __restrict__ grad_table, int dim, int64_t
   extern __shared__ uint4 s_raw[];
   SortShared& S = *reinterpret_cast<SortShared*>(s_raw);
   uint32_t begin = 0, count = 0;
-  if (a.n > 0) {
-    if (blockIdx.x == 0 && threadIdx.x == 0) a.header->long_sums = 0;
-    group_tokens(a, S, begin, count);
+  if (a.n > 0) group_tokens(a, S, begin, count);
+  const uint2* tokens = (a.passes & 1 ? a.tokens1 : a.tokens0) + begin;
+  // the blocks whose last token is this owner's: the sum that it belongs to is long when it reaches over the next boundary
+  // too, and begins in the block or further left
+  const int64_t length = int64_t(1) << a.block_log2, end = int64_t(begin) + count;
+  for (int64_t block = (begin >> a.block_log2) + threadIdx.x; block << a.block_log2 < end; block += kSortThreads) {
+    const int64_t last = min(((block + 1) << a.block_log2), a.n) - 1, third = (block + 2) << a.block_log2;
+    if (last >= end) continue;
+    const uint32_t id = tokens[last - begin].x;
+    LongSum L{id, 0u};
+    const int64_t left = (block << a.block_log2) - 1;
+    if (third < end && tokens[third - begin].x == id && !(left >= int64_t(begin) && tokens[left - begin].x == id)) {
+      int64_t from = third, to = end;  // the last place with the id is in [from, to)
+      while (to - from > 1) {
+        const int64_t mid = (from + to) / 2;
+        if (tokens[mid - begin].x == id) from = mid;
+        else to = mid;
+      }
+      L.parts = uint32_t((from >> a.block_log2) - block + 1);
+    }
+    a.long_sums[block] = L;
   }
   if (!clear) return;
   // the rows of this owner that have no token, as many at once as the shared memory has bits
-  uint32_t* used         = &S.at[0][0];
-  constexpr int kAtOnce  = sizeof(S.at) * 8;
-  const uint2* tokens    = (a.passes & 1 ? a.tokens1 : a.tokens0) + begin;
-  const int64_t rows     = (int64_t(a.vocab) - int64_t(blockIdx.x) + kOwners - 1) >> kOwnersLog2;
+  uint32_t* used        = &S.at[0][0];
+  constexpr int kAtOnce = sizeof(S.at) * 8;
+  const int64_t rows    = (int64_t(a.vocab) - int64_t(blockIdx.x) + kOwners - 1) >> kOwnersLog2;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int64_t r0 = 0; r0 < rows; r0 += kAtOnce) {
     const int here = int(min(int64_t(kAtOnce), rows - r0));
@@ -323,8 +382,9 @@ __device__ __forceinline__ void store_sum(T* row, int valid, bool packs, float s
 }
 
 struct GradArgs {
-  const uint2* tokens;  // grouped {id, place}
-  GradHeader* header;
+  const uint2* tokens;  // grouped {id, place}, those of no id behind them
+  int64_t n;
+  LongSum* long_sums;  // one per block
   int dim;
   int block_log2;
   int64_t out_stride, table_stride, pitch;
@@ -333,7 +393,6 @@ struct GradArgs {
   float* parts;  // [blocks][2][pitch]: of the long sum that begins further left, of the one that begins in the block
 };
 
-constexpr uint32_t kNoId = 0xFFFFFFFFu;
 constexpr int kChunk = 4, kChunks = 4;  // rows that are waited for together, and such chunks in flight
 
 __device__ __forceinline__ void copy16(uint32_t shared_at, const void* from)
@@ -345,126 +404,164 @@ template <int PENDING>
 __device__ __forceinline__ void await_chunks() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
 
 // first place in [from, to) whose id is not `id` (where one id follows another it does not come back)
-__device__ __forceinline__ int end_of_id(const uint2* tokens, int from, int to, uint32_t id)
+__device__ __forceinline__ int end_of_id(const uint32_t* ids, int from, int to, uint32_t id)
 {
   while (from < to) {
     const int mid = (from + to) >> 1;
-    if (tokens[mid].x == id) from = mid + 1;
+    if (ids[mid] == id) from = mid + 1;
     else to = mid;
   }
   return from;
 }
 
-// 16 bytes of a row, added to its columns' sums
-__device__ __forceinline__ void add_pack(const uint4& r, const float*, Two (&sum)[2])
+// how many of the places in front of `length` hold a token
+__device__ __forceinline__ int end_of_tokens(const uint32_t* ids, int length)
 {
-  sum[0] = sum[0] + Two(__uint_as_float(r.x), __uint_as_float(r.y));
-  sum[1] = sum[1] + Two(__uint_as_float(r.z), __uint_as_float(r.w));
-}
-template <class O>
-__device__ __forceinline__ void add_pack(const uint4& r, const O*, Two (&sum)[4])
-{
-  const O* e = reinterpret_cast<const O*>(&r);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) sum[j] = sum[j] + Two(gtk::to_float(e[2 * j]), gtk::to_float(e[2 * j + 1]));
+  int from = 0;
+  while (from < length) {
+    const int mid = (from + length) >> 1;
+    if (ids[mid] != kNoId) from = mid + 1;
+    else length = mid;
+  }
+  return from;
 }
 
-// the 16 bytes that begin `bytes` (a multiple of 2, below 16) behind the first of two packs
-__device__ __forceinline__ uint4 shifted(const uint4& a, const uint4& b, uint32_t bytes)
+// How a group's threads share the columns of a slab: a thread has kUnits units of kUnit neighbouring columns.
+// ALIGNED (rows of both arrays start where 16 bytes of grad_out's elements do): one unit, the 16 bytes that it copies itself.
+// Otherwise: four units of 32 bits each, 32 units apart, so that the threads of a warp read and store neighbouring words
+// however a row lies.
+template <class O, bool ALIGNED>
+struct Share {
+  static constexpr int kUnit  = (ALIGNED ? 16 : 4) / int(sizeof(O));
+  static constexpr int kUnits = ALIGNED ? 1 : 4;
+  static constexpr int kCount = kUnit * kUnits;
+};
+
+// sum[u * kUnit ..] += the thread's units of a staged row; `shift` bytes of its first piece belong to what lies in front of it.
+// Unless ALIGNED, `mine` counts 32-bit words and the units are kStep words apart.
+constexpr int kStep = 32;
+template <bool ALIGNED, class O>
+__device__ __forceinline__ void add_row(const uint4* row, int mine, uint32_t shift, Two (&sum)[16 / sizeof(O) / 2])
 {
-  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
-  if (bytes & 8)
-#pragma unroll
-    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
-  if (bytes & 4)
-#pragma unroll
-    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
-  const uint32_t half = (bytes & 2) * 8;
-  return make_uint4(__funnelshift_r(w[0], w[1], half), __funnelshift_r(w[1], w[2], half), __funnelshift_r(w[2], w[3], half),
-                    __funnelshift_r(w[3], w[4], half));
+  uint4 r;
+  if constexpr (ALIGNED) {
+    r = row[mine];
+  } else {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(row) + (shift >> 2) + mine;
+    r = make_uint4(w[0], w[kStep], w[2 * kStep], w[3 * kStep]);
+    if (sizeof(O) == 2 && (shift & 2)) {  // the same for the whole group: pairs of elements that lie in two words
+      r.x = __funnelshift_r(r.x, w[1], 16);
+      r.y = __funnelshift_r(r.y, w[kStep + 1], 16);
+      r.z = __funnelshift_r(r.z, w[2 * kStep + 1], 16);
+      r.w = __funnelshift_r(r.w, w[3 * kStep + 1], 16);
+    }
+  }
+  if constexpr (sizeof(O) == 4) {
+    sum[0] = sum[0] + Two(__uint_as_float(r.x), __uint_as_float(r.y));
+    sum[1] = sum[1] + Two(__uint_as_float(r.z), __uint_as_float(r.w));
+  } else {
+    sum[0] = sum[0] + gtk::word_pair(r.x, O{});
+    sum[1] = sum[1] + gtk::word_pair(r.y, O{});
+    sum[2] = sum[2] + gtk::word_pair(r.z, O{});
+    sum[3] = sum[3] + gtk::word_pair(r.w, O{});
+  }
 }
 
-// A group of threads (part of a warp, or the whole CTA) takes a block of tokens.  Every thread has the columns of 16 bytes and
-// copies its share of the rows to shared memory, up to kChunk * kChunks rows ahead.
-// ALIGNED: rows of both arrays start where 16 bytes of grad_out's elements do.  Otherwise a row's 16-byte pieces are copied as they lie
-// between 16-byte boundaries (the outer ones hold bytes of its neighbours, which nobody looks at) and a thread takes its
-// columns from two of them; sums go through shared memory to be stored by neighbouring threads side by side.
+// Shared memory of a group: the ring of 16-byte pieces (and one more: whoever takes words from the last piece looks into the
+// next one), the addresses of the rows and the ids of two blocks of tokens, and room for a chunk behind them.
+struct GroupShared {
+  int ring, tokens;
+  __host__ __device__ GroupShared(int group, int length) : ring((kChunk * kChunks * group + 1) * 16), tokens(2 * length + kChunk) {}
+  __host__ __device__ int bytes() const { return ring + (tokens * 12 + 15) / 16 * 16; }
+};
+
+// A group of threads (part of a warp, or the whole CTA) takes a block of tokens.  The rows come to shared memory in 16-byte pieces,
+// each thread copying one piece of every row, kChunk * kChunks rows ahead.  The pieces are those between 16-byte
+// boundaries: the outer ones may hold bytes of a row's neighbours, which nobody looks at.
 template <class O, class T, bool ALIGNED>
 __global__ void __launch_bounds__(kGradThreads) k_embed_grad_sums(const GradArgs a, const O* __restrict__ grad_out, T* __restrict__ grad_table)
 {
+  using S         = Share<O, ALIGNED>;
   constexpr int E = 16 / int(sizeof(O));
   extern __shared__ uint4 s_raw[];
-  const int group = blockDim.x, groups = blockDim.y, lane = threadIdx.x;
-  const int length = 1 << a.block_log2, window = 3 * length + 2;
-  // [groups][rows][group] pieces, [groups][group * E] sums unless ALIGNED, [groups][window] tokens
-  uint4* ring = s_raw + threadIdx.y * (kChunk * kChunks) * group;
-  float* sums = reinterpret_cast<float*>(s_raw + groups * (kChunk * kChunks) * group) + threadIdx.y * group * E;
-  uint2* P    = reinterpret_cast<uint2*>(s_raw + groups * group * (kChunk * kChunks + (ALIGNED ? 0 : E / 4))) + threadIdx.y * window + length + 1;
-  // the block's tokens, its neighbours' and one more at each end
-  const int64_t n     = a.header->tokens;
-  const int64_t block = int64_t(blockIdx.x) * groups + threadIdx.y;
-  const int64_t begin = block << a.block_log2;
-  for (int i = lane - length - 1; i <= 2 * length; i += group)
-    P[i] = begin + i >= 0 && begin + i < n ? __ldg(a.tokens + begin + i) : make_uint2(kNoId, 0u);  // ids are below 2^31
-  __syncthreads();
-  // the columns: from `first` on, `own` of them this thread's; `pieces` 16-byte pieces of a row, counted from the one with `first`
+  const int group = blockDim.x, lane = threadIdx.x;
+  const int length = 1 << a.block_log2;
+  const GroupShared shared(group, length);
+  unsigned char* base     = reinterpret_cast<unsigned char*>(s_raw) + threadIdx.y * shared.bytes();
+  const uint4* ring       = reinterpret_cast<const uint4*>(base);
+  uint64_t* address       = reinterpret_cast<uint64_t*>(base + shared.ring);
+  uint32_t* ids           = reinterpret_cast<uint32_t*>(address + shared.tokens);
+  // the columns: `width` from `first` on
   const int slab  = (ALIGNED ? group : group - 1) * E;
   const int first = blockIdx.y * slab, width = min(slab, a.dim - first);
-  const int c     = first + lane * E, own = max(0, min(E, first + width - c));
+  // the tokens of this block and the next, and one at either end of the block in front
+  const int64_t block = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
+  const int64_t begin = block << a.block_log2;
+  const uint32_t left = begin > 0 && begin < a.n ? __ldg(&a.tokens[begin - 1].x) : kNoId;
+  const uint32_t far_left = begin > length && begin < a.n ? __ldg(&a.tokens[begin - length - 1].x) : kNoId;
+  for (int i = lane; i < shared.tokens; i += group) {
+    const uint2 token = begin + i < a.n ? __ldg(a.tokens + begin + i) : make_uint2(kNoId, 0u);
+    ids[i]     = token.x;
+    address[i] = reinterpret_cast<uint64_t>(grad_out + first + int64_t(token.y) * a.out_stride);
+  }
+  __syncthreads();
   const uint32_t mask = group >= 32 ? 0xFFFFFFFFu : ((1u << group) - 1u) << (threadIdx.y * group & 31);
-  auto meet = [&] {
-    if (group > 32) __syncthreads();
-    else __syncwarp(mask);
-  };
   int at = 0, stop = 0;
   bool from_left = false, to_right = false;
-  if (begin < n) {
-    const int end      = int(min(int64_t(length), n - begin));
-    const uint32_t id0 = P[0].x, id1 = P[end - 1].x;
+  if (ids[0] != kNoId) {
+    const int end      = ids[length - 1] != kNoId ? length : end_of_tokens(ids, length);
+    const uint32_t id0 = ids[0], id1 = ids[end - 1];
     stop = end;
     // the sum that begins further left: skipped, or this block's part of a long one
-    from_left = P[-1].x == id0;
-    if (from_left && P[end].x != id0 && P[-length - 1].x != id0) {
-      at        = end_of_id(P, 0, end, id0);
+    from_left = left == id0;
+    if (from_left && ids[end] != id0 && far_left != id0) {
+      at        = end_of_id(ids, 0, end, id0);
       from_left = false;
     }
     // the sum that reaches over the end: to its end, or up to the boundary when it is a long one
-    if (at < end && P[end].x == id1 && !(from_left && id1 == id0)) {
-      to_right = P[2 * length].x == id1;
-      if (!to_right) stop = end_of_id(P, end, 2 * length, id1);
-      else if (c == 0) a.header->block[atomicAdd(&a.header->long_sums, 1u)] = uint32_t(block);
+    if (at < end && ids[end] == id1 && !(from_left && id1 == id0)) {
+      to_right = ids[2 * length] == id1;
+      if (!to_right) stop = end_of_id(ids, end, 2 * length, id1);
     }
   }
   if (at >= stop) return;  // the whole group
-  const uint32_t ring_at = uint32_t(__cvta_generic_to_shared(ring)) + lane * 16;
-  const char* column     = reinterpret_cast<const char*>(grad_out + first);
-  const int64_t row_bytes = a.out_stride * int64_t(sizeof(O));
-  const uint32_t width_bytes = uint32_t(width) * uint32_t(sizeof(O));
-  auto request = [&](int chunk) {
+  const uint32_t ring_at = uint32_t(__cvta_generic_to_shared(ring)) + lane * 16, width_bytes = uint32_t(width) * uint32_t(sizeof(O));
+  const uint32_t slot_bytes = group * 16, chunk_bytes = kChunk * slot_bytes;
+  uint32_t to = ring_at;  // where the next chunk goes
+  auto request = [&](int chunk) {  // rows of window places chunk * kChunk ..
 #pragma unroll
     for (int k = 0; k < kChunk; ++k) {
-      const int i = at + chunk * kChunk + k;
-      if (i < stop) {
-        const char* row      = column + int64_t(P[i].y) * row_bytes;
-        const uint32_t shift = ALIGNED ? 0u : uint32_t(reinterpret_cast<uintptr_t>(row)) & 15u;
-        if (uint32_t(lane) * 16u < shift + width_bytes) copy16(ring_at + ((chunk % kChunks) * kChunk + k) * group * 16, row - shift + lane * 16);
+      const int i = chunk * kChunk + k;
+      if (i >= at && i < stop) {
+        const uint64_t row   = address[i];
+        const uint32_t shift = ALIGNED ? 0u : uint32_t(row) & 15u;
+        if (uint32_t(lane) * 16u < shift + width_bytes) copy16(to + k * slot_bytes, reinterpret_cast<const char*>(row - shift) + lane * 16);
       }
     }
     end_chunk();
+    to = to + chunk_bytes == ring_at + kChunks * chunk_bytes ? ring_at : to + chunk_bytes;
   };
-  Two sum[E / 2];
+  // ALIGNED: the thread's own piece.  Otherwise words, those of a warp next to each other
+  const int mine = ALIGNED ? lane : (lane & ~31) * 4 + (lane & 31);
+  Two sum[S::kCount / 2];
+  auto each_unit = [&](auto&& f) {  // f(first column, columns within the row, the sums)
+    float x[S::kCount];
 #pragma unroll
-  for (int j = 0; j < E / 2; ++j) sum[j] = Two(0.f, 0.f);
-  auto store_part = [&](int which) {
-    if (!own) return;
-    float* to = a.parts + (block * 2 + which) * a.pitch + c;  // the pitch is a multiple of E
+    for (int j = 0; j < S::kCount / 2; ++j) sum[j].get(x[2 * j], x[2 * j + 1]);
 #pragma unroll
-    for (int j = 0; j < E / 2; j += 2) {
-      float4 v;
-      sum[j].get(v.x, v.y);
-      sum[j + 1].get(v.z, v.w);
-      *reinterpret_cast<float4*>(to + 2 * j) = v;
+    for (int u = 0; u < S::kUnits; ++u) {
+      const int c = (mine + u * kStep) * S::kUnit;
+      if (c < width) f(first + c, min(S::kUnit, width - c), x + u * S::kUnit);
     }
+  };
+  auto store_part = [&](int which) {
+    float* to_part = a.parts + (block * 2 + which) * a.pitch;
+    each_unit([&](int c, int, const float* x) {  // whole units: the pitch is a multiple of them
+      Pack<float, S::kUnit> p;
+#pragma unroll
+      for (int j = 0; j < S::kUnit; ++j) p.e[j] = x[j];
+      gtk::store_pack<float, S::kUnit>(to_part + c, p);
+    });
   };
   auto finish = [&](uint32_t id) {
     if (from_left) {
@@ -472,77 +569,77 @@ __global__ void __launch_bounds__(kGradThreads) k_embed_grad_sums(const GradArgs
       from_left = false;
       return;
     }
-    T* row = grad_table + int64_t(id) * a.table_stride;
-    float x[E];
-#pragma unroll
-    for (int j = 0; j < E / 2; ++j) sum[j].get(x[2 * j], x[2 * j + 1]);
-    if constexpr (ALIGNED) {
-      store_sum<T, E>(row + c, own, true, a.scale, a.accumulate, x);
-    } else {
-#pragma unroll
-      for (int j = 0; j < E; j += 4) *reinterpret_cast<float4*>(sums + lane * E + j) = make_float4(x[j], x[j + 1], x[j + 2], x[j + 3]);
-      meet();
-      for (int i = lane; i < width; i += group) store_sum<T, 1>(row + first + i, 1, true, a.scale, a.accumulate, sums + i);
-      meet();
-    }
+    T* row           = grad_table + int64_t(id) * a.table_stride;
+    const bool packs = ALIGNED || reinterpret_cast<uintptr_t>(row + first) % (sizeof(T) * S::kUnit) == 0;
+    each_unit([&](int c, int own, const float* x) { store_sum<T, S::kUnit>(row + c, own, packs, a.scale, a.accumulate, x); });
   };
+  int chunk = at / kChunk;
 #pragma unroll
-  for (int q = 0; q < kChunks - 1; ++q) request(q);
-  uint32_t id = P[at].x;
-  for (int chunk = 0; at + chunk * kChunk < stop; ++chunk) {
+  for (int q = 0; q < kChunks - 1; ++q) request(chunk + q);
+#pragma unroll
+  for (int j = 0; j < S::kCount / 2; ++j) sum[j] = Two(0.f, 0.f);
+  uint32_t id = ids[at];
+  const uint4* rows = ring;
+  for (; chunk * kChunk < stop; ++chunk) {
     await_chunks<kChunks - 2>();
-    if constexpr (!ALIGNED) meet();
+    if constexpr (!ALIGNED) {
+      if (group > 32) __syncthreads();
+      else __syncwarp(mask);
+    }
     request(chunk + kChunks - 1);  // over the chunk in front, which everybody has added
-    const uint4* rows = ring + (chunk % kChunks) * kChunk * group + lane;
+    uint32_t now[kChunk], shift[kChunk];
 #pragma unroll
     for (int k = 0; k < kChunk; ++k) {
-      const int i = at + chunk * kChunk + k;
-      if (i >= stop) break;
-      const uint2 token = P[i];
-      if (token.x != id) {
-        finish(id);
-        id = token.x;
+      now[k]   = ids[chunk * kChunk + k];
+      shift[k] = ALIGNED ? 0u : uint32_t(reinterpret_cast<const uint32_t*>(address)[2 * (chunk * kChunk + k)]) & 15u;
+    }
+    if (now[0] == id && now[kChunk - 1] == id) {  // all of one sum; what lies outside [at, stop) has other ids
 #pragma unroll
-        for (int j = 0; j < E / 2; ++j) sum[j] = Two(0.f, 0.f);
-      }
-      if constexpr (ALIGNED) {
-        add_pack(rows[k * group], static_cast<const O*>(nullptr), sum);
-      } else if (own) {
-        const uint32_t shift = (uint32_t(reinterpret_cast<uintptr_t>(column)) + token.y * uint32_t(row_bytes)) & 15u;
-        add_pack(shifted(rows[k * group], rows[k * group + 1], shift), static_cast<const O*>(nullptr), sum);
+      for (int k = 0; k < kChunk; ++k) add_row<ALIGNED, O>(rows + k * group, mine, shift[k], sum);
+    } else {
+#pragma unroll
+      for (int k = 0; k < kChunk; ++k) {
+        const int i = chunk * kChunk + k;
+        if (i < at || i >= stop) continue;
+        if (now[k] != id) {
+          finish(id);
+          id = now[k];
+#pragma unroll
+          for (int j = 0; j < S::kCount / 2; ++j) sum[j] = Two(0.f, 0.f);
+        }
+        add_row<ALIGNED, O>(rows + k * group, mine, shift[k], sum);
       }
     }
+    rows = rows + kChunk * group == ring + kChunks * kChunk * group ? ring : rows + kChunk * group;
   }
   if (to_right) store_part(1);
   else finish(id);
 }
 
 // The parts of a long sum, 128 columns at a time: each warp adds a run of parts, then the warps' sums are added in order.
+constexpr int kJoinThreads = 128;
 template <class T>
-__global__ void __launch_bounds__(kGradThreads) k_embed_grad_join(const GradArgs a, T* __restrict__ grad_table, bool packs)
+__global__ void __launch_bounds__(kJoinThreads) k_embed_grad_join(const GradArgs a, T* __restrict__ grad_table, bool packs)
 {
-  constexpr int kWarps = kGradThreads / 32;
+  constexpr int kWarps = kJoinThreads / 32;
   __shared__ float4 s_sum[kWarps][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t n     = a.header->tokens;
-  const int slabs     = (a.dim + 127) / 128;
-  const int64_t items = int64_t(a.header->long_sums) * slabs;
-  for (int64_t item = blockIdx.x; item < items; item += gridDim.x) {
-    const int64_t block = a.header->block[item / slabs];
-    const int c         = int(item % slabs) * 128 + lane * 4;
-    const uint32_t id   = a.tokens[((block + 1) << a.block_log2) - 1].x;
-    int64_t more = 0;  // blocks behind this one that begin with the same id
-    for (int found = kGradThreads; found == kGradThreads; more += found) {
-      const int64_t i = (block + 1 + more + threadIdx.x) << a.block_log2;
-      found           = __syncthreads_count(i < n && a.tokens[i].x == id);
-    }
-    const int64_t each = (more + 1 + kWarps - 1) / kWarps;
-    const int64_t from = warp * each, to = min(more + 1, from + each);
-    float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int c         = blockIdx.y * 128 + lane * 4;
+  const int64_t first = int64_t(blockIdx.x) * 32, blocks = (a.n + (int64_t(1) << a.block_log2) - 1) >> a.block_log2;
+  LongSum mine{kNoId, 0u};
+  if (first + lane < blocks) mine = a.long_sums[first + lane];
+  for (uint32_t some = __ballot_sync(0xFFFFFFFFu, mine.parts > 0); some; some &= some - 1) {  // the same for every warp
+    const int at = __ffs(some) - 1;
+    LongSum L;
+    L.id                = __shfl_sync(0xFFFFFFFFu, mine.id, at);
+    L.parts             = __shfl_sync(0xFFFFFFFFu, mine.parts, at);
+    const uint32_t each = (L.parts + kWarps - 1) / kWarps, from = min(L.parts, warp * each), to = min(L.parts, from + each);
+    const float* part   = a.parts + (first + at) * 2 * a.pitch + c;
+    float4 sum          = make_float4(0.f, 0.f, 0.f, 0.f);
     if (c < a.dim) {
 #pragma unroll 8
-      for (int64_t i = from; i < to; ++i) {  // part 0 is the one that begins in the block
-        const float4 x = *reinterpret_cast<const float4*>(a.parts + ((block + i) * 2 + (i == 0 ? 1 : 0)) * a.pitch + c);
+      for (uint32_t i = from; i < to; ++i) {  // part 0 is the one that begins in the block
+        const float4 x = *reinterpret_cast<const float4*>(part + (2 * int64_t(i) + (i == 0 ? 1 : 0)) * a.pitch);
         sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
       }
     }
@@ -555,7 +652,7 @@ __global__ void __launch_bounds__(kGradThreads) k_embed_grad_join(const GradArgs
         sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
       }
       const float y[4] = {sum.x, sum.y, sum.z, sum.w};
-      store_sum<T, 4>(grad_table + int64_t(id) * a.table_stride + c, a.dim - c, packs, a.scale, a.accumulate, y);
+      store_sum<T, 4>(grad_table + int64_t(L.id) * a.table_stride + c, a.dim - c, packs, a.scale, a.accumulate, y);
     }
     __syncthreads();
   }
@@ -566,29 +663,26 @@ cudaError_t launch_embed_grad(const gtk::HandleView& v, const GradPlan& p, GradA
                               const void* grad_out, void* grad_table, unsigned char* work)
 {
   T* table = static_cast<T*>(grad_table);
-  const SortArgs s{ids, n, uint32_t(vocab), p.passes, p.digit_bits, reinterpret_cast<uint2*>(work + p.at_tokens[0]),
-                   reinterpret_cast<uint2*>(work + p.at_tokens[1]), a.header};
+  const SortArgs s{ids, n, uint32_t(vocab), p.passes, p.digit_bits, p.block_log2, reinterpret_cast<uint2*>(work + p.at_tokens[0]),
+                   reinterpret_cast<uint2*>(work + p.at_tokens[1]), a.long_sums};
   cudaError_t e = gtk::launch(k_embed_grad_sort<T>, dim3(kOwners), dim3(kSortThreads), sizeof(SortShared), v.stream, s, table, a.dim,
                               a.table_stride, !a.accumulate);
   if (e != cudaSuccess || n == 0) return e;
   a.tokens = p.passes & 1 ? s.tokens1 : s.tokens0;
-  // threads of a group: a power of two below a warp, several groups in a CTA; else whole warps, a CTA's at most
+  // threads of a group: a power of two below a warp when each has 16 bytes of its own; else whole warps, a CTA's at most
   constexpr int E      = 16 / int(sizeof(O));
   const int64_t wanted = (a.dim + E - 1) / E + (ALIGNED ? 0 : 1);
-  unsigned group = 1;
-  if (wanted > 32) group = unsigned(std::min<int64_t>(kGradThreads, (wanted + 31) / 32 * 32));
-  else
-    while (group < wanted) group *= 2;
+  unsigned group = unsigned(std::min<int64_t>(kGradThreads, (wanted + 31) / 32 * 32));
+  while (ALIGNED && group <= 32 && group / 2 >= wanted) group /= 2;
   const unsigned columns = (ALIGNED ? group : group - 1) * E, slabs = unsigned((a.dim + columns - 1) / columns);
-  const size_t bytes     = size_t(group) * 16 * (kChunk * kChunks + (ALIGNED ? 0 : E / 4)) + sizeof(uint2) * ((size_t(3) << a.block_log2) + 2);
-  unsigned groups = group > 32 ? 1 : std::max(1u, 128 / group);
+  const size_t bytes     = size_t(GroupShared(int(group), 1 << a.block_log2).bytes());
+  unsigned groups = group > 32 ? 1 : 128 / group;
   while (groups > 1 && groups * bytes > kSharedMost) groups /= 2;
   e = gtk::launch(k_embed_grad_sums<O, T, ALIGNED>, dim3(unsigned((p.blocks + groups - 1) / groups), slabs), dim3(group, groups), groups * bytes,
                   v.stream, a, static_cast<const O*>(grad_out), table);
-  // a sum is long when it holds a whole block and more on both sides
-  if (e == cudaSuccess && p.blocks > 2)
-    e = gtk::launch(k_embed_grad_join<T>, dim3(unsigned(std::min<int64_t>(p.blocks * ((a.dim + 127) / 128), int64_t(v.sm_count) * 8))),
-                    dim3(kGradThreads), 0, v.stream, a, table, ALIGNED);
+  if (e == cudaSuccess && p.blocks > 2)  // a long sum begins in one block, fills the next and goes on
+    e = gtk::launch(k_embed_grad_join<T>, dim3(unsigned((p.blocks + 31) / 32), unsigned((a.dim + 127) / 128)), dim3(kJoinThreads), 0, v.stream, a,
+                    table, ALIGNED);
   return e;
 }
 
@@ -670,7 +764,7 @@ extern "C" GTK_API int gtk_embed_grad(gtk_tokenizer* h, const int32_t* d_ids, in
     if (n_ids == 0 && accumulate) return cudaSuccess;
     const GradPlan p = grad_plan(n_ids, vocab, dim);
     unsigned char* work = static_cast<unsigned char*>(d_workspace);
-    const GradArgs a{nullptr, reinterpret_cast<GradHeader*>(work + p.at_header), int(dim), p.block_log2, out_stride, table_stride, p.pitch,
+    const GradArgs a{nullptr, n_ids, reinterpret_cast<LongSum*>(work + p.at_long), int(dim), p.block_log2, out_stride, table_stride, p.pitch,
                      scale, accumulate != 0, reinterpret_cast<float*>(work + p.at_parts)};
     const bool aligned = gtk::rows_aligned(d_grad_out, out_stride, out_type, 8) && gtk::rows_aligned(d_grad_table, table_stride, table_type, 8);
     return gtk::with_type(out_type, [&](auto o) {

@@ -67,6 +67,14 @@ __device__ __forceinline__ Two fma2(Two a, Two b, Two c)
   return d;
 }
 
+// a 32-bit word's one or two elements as 32-bit floats
+__device__ __forceinline__ Two word_pair(uint32_t w, __nv_bfloat16) { return Two(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u)); }
+__device__ __forceinline__ Two word_pair(uint32_t w, __half)
+{
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
+  return Two(f.x, f.y);
+}
+
 // ------------------------------------------------------------------------------------------------ host side
 inline int element_size(int type) { return type == GTK_F32 ? 4 : 2; }
 inline bool known_type(int type) { return type == GTK_F32 || type == GTK_BF16 || type == GTK_F16; }
