@@ -395,14 +395,6 @@ struct GradArgs {
 
 constexpr int kChunk = 4, kChunks = 4;  // rows that are waited for together, and such chunks in flight
 
-__device__ __forceinline__ void copy16(uint32_t shared_at, const void* from)
-{
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared_at), "l"(from) : "memory");
-}
-__device__ __forceinline__ void end_chunk() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int PENDING>
-__device__ __forceinline__ void await_chunks() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
-
 // first place in [from, to) whose id is not `id` (where one id follows another it does not come back)
 __device__ __forceinline__ int end_of_id(const uint32_t* ids, int from, int to, uint32_t id)
 {
@@ -535,10 +527,10 @@ __global__ void __launch_bounds__(kGradThreads) k_embed_grad_sums(const GradArgs
       if (i >= at && i < stop) {
         const uint64_t row   = address[i];
         const uint32_t shift = ALIGNED ? 0u : uint32_t(row) & 15u;
-        if (uint32_t(lane) * 16u < shift + width_bytes) copy16(to + k * slot_bytes, reinterpret_cast<const char*>(row - shift) + lane * 16);
+        if (uint32_t(lane) * 16u < shift + width_bytes) gtk::copy16(to + k * slot_bytes, reinterpret_cast<const char*>(row - shift) + lane * 16);
       }
     }
-    end_chunk();
+    gtk::end_chunk();
     to = to + chunk_bytes == ring_at + kChunks * chunk_bytes ? ring_at : to + chunk_bytes;
   };
   // ALIGNED: the thread's own piece.  Otherwise words, those of a warp next to each other
@@ -581,7 +573,7 @@ __global__ void __launch_bounds__(kGradThreads) k_embed_grad_sums(const GradArgs
   uint32_t id = ids[at];
   const uint4* rows = ring;
   for (; chunk * kChunk < stop; ++chunk) {
-    await_chunks<kChunks - 2>();
+    gtk::await_chunks<kChunks - 2>();
     if constexpr (!ALIGNED) {
       if (group > 32) __syncthreads();
       else __syncwarp(mask);

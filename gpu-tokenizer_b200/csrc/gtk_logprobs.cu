@@ -4,6 +4,7 @@
 
 #include <cfloat>
 #include <cmath>
+#include <cstdlib>
 #include <initializer_list>
 #include <type_traits>
 
@@ -24,7 +25,7 @@ __device__ __forceinline__ float pow2(float y)
   return p;
 }
 
-// 16 bytes of a row: its elements as pairs of 32-bit floats, and their maximum (NaN only where all are).
+// 16 bytes of a row: its elements as pairs of 32-bit floats, and their maxima (NaN only where all are).
 template <class T>
 struct Pack16;
 template <>
@@ -37,15 +38,16 @@ struct Pack16<float> {
     x[0] = Two(__uint_as_float(r.x), __uint_as_float(r.y));
     x[1] = Two(__uint_as_float(r.z), __uint_as_float(r.w));
   }
-  template <int N>
-  static __device__ __forceinline__ float highest(const uint4 (&r)[N])
+  // maxima: one of the whole pack
+  using Max = float;
+  static constexpr int kHalves = 1;
+  static __device__ __forceinline__ Max lowest() { return -INFINITY; }
+  static __device__ __forceinline__ Max highest(const uint4& r)
   {
-    float m = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < N; ++i)
-      m = fmaxf(m, fmaxf(fmaxf(__uint_as_float(r[i].x), __uint_as_float(r[i].y)), fmaxf(__uint_as_float(r[i].z), __uint_as_float(r[i].w))));
-    return m;
+    return fmaxf(fmaxf(__uint_as_float(r.x), __uint_as_float(r.y)), fmaxf(__uint_as_float(r.z), __uint_as_float(r.w)));
   }
+  static __device__ __forceinline__ Max higher(Max a, Max b) { return fmaxf(a, b); }
+  static __device__ __forceinline__ float of(Max m, int) { return m; }
 };
 template <class T, class T2>
 struct Pack16Half {
@@ -61,14 +63,15 @@ struct Pack16Half {
       x[i]           = Two(f.x, f.y);
     }
   }
-  template <int N>
-  static __device__ __forceinline__ float highest(const uint4 (&r)[N])
+  // maxima: one of the even elements, one of the odd ones
+  using Max = T2;
+  static constexpr int kHalves = 2;
+  static __device__ __forceinline__ Max highest(const uint4& r) { return __hmax2(__hmax2(as(r.x), as(r.y)), __hmax2(as(r.z), as(r.w))); }
+  static __device__ __forceinline__ Max higher(Max a, Max b) { return __hmax2(a, b); }
+  static __device__ __forceinline__ float of(Max m, int half)
   {
-    T2 m = __hmax2(__hmax2(as(r[0].x), as(r[0].y)), __hmax2(as(r[0].z), as(r[0].w)));
-#pragma unroll
-    for (int i = 1; i < N; ++i) m = __hmax2(m, __hmax2(__hmax2(as(r[i].x), as(r[i].y)), __hmax2(as(r[i].z), as(r[i].w))));
     const float2 f = both(m);
-    return fmaxf(f.x, f.y);
+    return half ? f.y : f.x;
   }
 };
 template <>
@@ -77,11 +80,13 @@ template <>
 __device__ __forceinline__ float2 Pack16Half<__half, __half2>::both(__half2 w) { return __half22float2(w); }
 template <>
 struct Pack16<__nv_bfloat16> : Pack16Half<__nv_bfloat16, __nv_bfloat162> {
+  static __device__ __forceinline__ Max lowest() { return __float2bfloat162_rn(-INFINITY); }
   static constexpr uint32_t kMinusInf = 0xFF80FF80u;
   static constexpr int kLowestBit     = 16;
 };
 template <>
 struct Pack16<__half> : Pack16Half<__half, __half2> {
+  static __device__ __forceinline__ Max lowest() { return __float2half2_rn(-INFINITY); }
   static constexpr uint32_t kMinusInf = 0xFC00FC00u;
   static constexpr int kLowestBit     = 13;
 };
@@ -159,129 +164,177 @@ struct ScoreArgs {
 
 constexpr int kBatch = 4;              // packs that a thread has in flight
 constexpr int kMaxParts = 8;           // CTAs that share a row
-constexpr int kMostWinners = 64, kMostCandidates = 1024;
+// Sets that are read again and keys that are ranked at most; beyond that the way through ties and crowds is taken.  The keys of
+// all parts fit into one CTA's list.
+constexpr int kMostSets = 64, kMostKeys = 512, kMostKeysOfPart = kMostKeys / kMaxParts;
+static_assert(kMostKeysOfPart >= GTK_MAX_TOP, "a part's own top_k fit into its share");
 
 struct TopScratch {
-  uint64_t candidate[kMostCandidates];
+  uint64_t key[kMostKeys];
   uint64_t best[kWarps];
-  uint64_t top[GTK_MAX_TOP];  // of this CTA's part of the row, highest first, 0 where there is none
-  int winner[kThreads];
-  int winners, candidates;
+  int set[kThreads];  // thread << 8 | q << 4 | half
+  int sets, keys;
+  uint32_t bound;
 };
 
-// The top_k columns of packs [begin, end) and, for loose, of the elements outside the packs, to S.top.
-// Each thread knows the highest element `best` of the packs that it has read (begin + thread, and every kThreads-th from
-// there).  The top_k-th highest of those is a bound that at least top_k elements reach; threads whose best is below it
-// hold none of the top.  So the packs of about top_k threads are read again (from L2) and what reaches the bound is
-// ranked.  Where more threads than kMostWinners reach it, with equal numbers, the columns decide among those: the argument
-// holds for (value, column) too.
+// The highest value_key that at least `wanted` of the CTA's threads reach with `mine`, or a lower one that exactly so many
+// reach; 0 where fewer threads have any.
 template <class T>
-__device__ __forceinline__ void select_top(const RowParts<T>& row, int begin, int end, bool loose, int top_k, float best, TopScratch& S)
+__device__ __forceinline__ uint32_t find_bound(uint32_t mine, int wanted)
 {
-  constexpr int E = Pack16<T>::kElems;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const uint32_t mine = value_key(best);
-  uint32_t bound      = 0;
+  uint32_t bound = 0;
 #pragma unroll 1
   for (int bit = 31; bit >= Pack16<T>::kLowestBit; --bit) {
     const uint32_t higher = bound | 1u << bit;
-    if (__syncthreads_count(mine >= higher) >= top_k) bound = higher;
+    const int reach       = __syncthreads_count(mine >= higher);
+    if (reach >= wanted) bound = higher;
+    if (reach == wanted) break;
   }
+  // the low bits that are the same in all numbers of the type: ones below a negative one, see value_key
+  if (bound && !(bound & 0x80000000u)) bound |= (1u << Pack16<T>::kLowestBit) - 1u;
+  return bound;
+}
+
+// Leaves in S.key[0 .. S.keys), in any order, keys of packs [begin, end) and, for loose, of the elements outside the packs,
+// at most `most` of them, among which are all of the top_k highest that reach the bound.
+// A thread has read packs begin + thread, and every blockDim-th from there; of those that were q-th in their batch it knows the
+// highest elements best[q], and `mine` is the value_key of its highest of all.  Only packs of sets (a thread, a q, a half of the
+// elements) whose highest reaches the bound are read again, from L2.  That is about top_k sets, as long as numbers differ.
+// Where more than kMostSets reach it, the threads whose highest (by value, then by column) are the top_k highest of their
+// kind take the sets' place: what the others hold comes behind those.
+template <class T>
+__device__ __forceinline__ void collect_keys(const RowParts<T>& row, int begin, int end, bool loose, int top_k, int most, uint32_t bound, uint32_t mine,
+                                             const typename Pack16<T>::Max (&best)[kBatch], TopScratch& S)
+{
+  using P         = Pack16<T>;
+  constexpr int E = P::kElems;
+  const int tid = threadIdx.x, threads = blockDim.x, warp = tid >> 5, lane = tid & 31;
   uint64_t floor = uint64_t(bound) << 32;
-  if (tid == 0) S.winners = S.candidates = 0;
-  if (tid < top_k) S.top[tid] = 0;
-  bool wins = mine >= max(bound, 1u);
-  if (__syncthreads_count(wins) > kMostWinners && bound) {
+  if (tid == 0) S.sets = S.keys = 0;
+  __syncthreads();
+  if (mine && mine >= bound) {
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q)
+#pragma unroll
+      for (int half = 0; half < P::kHalves; ++half) {
+        const uint32_t key = value_key(P::of(best[q], half));
+        if (key && key >= bound) {
+          const int at = atomicAdd(&S.sets, 1);
+          if (at < kMostSets) S.set[at] = tid << 8 | q << 4 | half;
+        }
+      }
+  }
+  __syncthreads();
+  const bool by_set = S.sets <= kMostSets;
+  if (!by_set) {
+    bound        = max(bound, find_bound<T>(mine, top_k));
+    floor        = uint64_t(bound) << 32;
     uint64_t key = 0;  // the thread's highest with its column
-    if (mine >= bound)
-      for (int p = begin + tid; p < end && !key; p += kThreads) {
+    if (mine && mine >= bound)
+      for (int p = begin + tid; p < end && !key; p += threads) {
         const T* x = row.x + row.pack_column(p);
         for (int j = 0; j < E && !key; ++j)
-          if (gtk::to_float(x[j]) == best) key = rank_key(best, uint32_t(row.pack_column(p) + j));
+          if (value_key(gtk::to_float(x[j])) == mine) key = rank_key(gtk::to_float(x[j]), uint32_t(row.pack_column(p) + j));
       }
+    if (__syncthreads_count(key != 0) >= top_k) {
 #pragma unroll 1
-    for (int bit = 31; bit >= 0; --bit) {
-      const uint64_t higher = floor | 1u << bit;
-      if (__syncthreads_count(key >= higher) >= top_k) floor = higher;
+      for (int bit = 31; bit >= 0; --bit) {
+        const uint64_t higher = floor | 1u << bit;
+        if (__syncthreads_count(key >= higher) >= top_k) floor = higher;
+      }
     }
-    wins = key >= floor;
+    if (tid == 0) S.sets = 0;
+    __syncthreads();
+    if (key && key >= floor) S.set[atomicAdd(&S.sets, 1)] = tid << 8;
+    __syncthreads();
   }
-  if (wins) S.winner[atomicAdd(&S.winners, 1)] = tid;
-  __syncthreads();
-  const int each = (end - begin + kThreads - 1) / kThreads, pairs = S.winners * each;  // packs of the winners
-  auto offer = [&](uint64_t key) {
-    if (key < max(floor, uint64_t(1))) return;
-    const int at = atomicAdd(&S.candidates, 1);
-    if (at < kMostCandidates) S.candidate[at] = key;
-  };
-  const int loose_count = loose ? row.head + row.tail : 0;
-  for (int i = tid; i < pairs; i += kThreads) {
-    const int p = begin + S.winner[i / each] + i % each * kThreads;
-    if (p >= end) continue;
+  const int step = by_set ? kBatch * threads : threads;
+  const uint32_t each = uint32_t(max(1, (end - begin + step - 1) / step)), inverse = ~0u / each + 1u, packs = uint32_t(S.sets) * each;
+  const float reach = bound ? key_value(floor) : -INFINITY;
+  // f(key) for the elements of the i-th pack of the sets that reach the bound
+  auto each_key = [&](uint32_t i, auto&& f) {
+    const uint32_t at = each == 1 ? i : __umulhi(i, inverse);  // i / each: both are small
+    const int w = S.set[at], p = begin + (w >> 8) + (w >> 4 & 15) * threads + int(i - at * each) * step;
+    if (p >= end) return;
     const uint4 raw = __ldg(row.pack(p));
     const T* x      = reinterpret_cast<const T*>(&raw);
 #pragma unroll
-    for (int j = 0; j < E; ++j) offer(rank_key(gtk::to_float(x[j]), uint32_t(row.pack_column(p) + j)));
-  }
-  if (tid < loose_count) offer(rank_key(gtk::to_float(row.x[row.loose_column(tid)]), uint32_t(row.loose_column(tid))));
+    for (int j = 0; j < E; ++j)
+      if (gtk::to_float(x[j]) >= reach && (!by_set || P::kHalves == 1 || (j & 1) == (w & 1))) f(rank_key(gtk::to_float(x[j]), uint32_t(row.pack_column(p) + j)));
+  };
+  auto each_loose = [&](auto&& f) {
+    if (loose && tid < row.head + row.tail) f(rank_key(gtk::to_float(row.x[row.loose_column(tid)]), uint32_t(row.loose_column(tid))));
+  };
+  auto offer = [&](uint64_t key) {
+    if (key == 0 || key < floor) return;
+    const int at = atomicAdd(&S.keys, 1);
+    if (at < most) S.key[at] = key;
+  };
+#pragma unroll 1
+  for (uint32_t i = tid; i < packs; i += threads) each_key(i, offer);
+  each_loose(offer);
   __syncthreads();
-  const int n = S.candidates;
-  if (n <= kMostCandidates) {
-    for (int i = tid; i < n; i += kThreads) {
-      const uint64_t key = S.candidate[i];
-      int above          = 0;
-      for (int j = 0; j < n; ++j) above += S.candidate[j] > key;
-      if (above < top_k) S.top[above] = key;
-    }
-  } else {  // few threads own many of the highest: one after the other
-    uint64_t below = ~uint64_t(0);
-    for (int r = 0; r < top_k; ++r) {
-      uint64_t high = 0;
-      for (int i = tid; i < pairs; i += kThreads) {
-        const int p = begin + S.winner[i / each] + i % each * kThreads;
-        if (p >= end) continue;
-        const T* x = row.x + row.pack_column(p);
-        for (int j = 0; j < E; ++j) {
-          const uint64_t key = rank_key(gtk::to_float(x[j]), uint32_t(row.pack_column(p) + j));
-          if (key < below) high = max(high, key);
-        }
-      }
-      if (tid < loose_count) {
-        const uint64_t key = rank_key(gtk::to_float(row.x[row.loose_column(tid)]), uint32_t(row.loose_column(tid)));
-        if (key < below) high = max(high, key);
-      }
+  if (S.keys <= most) return;
+  // few sets hold many of the highest: one after the other
+  uint64_t below = ~uint64_t(0);
+  int found      = 0;
+#pragma unroll 1
+  for (; found < top_k; ++found) {
+    uint64_t high = 0;
+    auto look     = [&](uint64_t key) {
+      if (key < below) high = max(high, key);
+    };
+#pragma unroll 1
+    for (uint32_t i = tid; i < packs; i += threads) each_key(i, look);
+    each_loose(look);
 #pragma unroll
-      for (int d = 16; d; d >>= 1) high = max(high, uint64_t(__shfl_xor_sync(0xFFFFFFFFu, high, d)));
-      if (lane == 0) S.best[warp] = high;
-      __syncthreads();
-      for (int w = 0; w < kWarps; ++w) high = max(high, S.best[w]);
-      __syncthreads();
-      if (tid == 0) S.top[r] = high;
-      below = high;
-    }
+    for (int d = 16; d; d >>= 1) high = max(high, uint64_t(__shfl_xor_sync(0xFFFFFFFFu, high, d)));
+    if (lane == 0) S.best[warp] = high;
+    __syncthreads();
+    for (int w = 0; w < threads / 32; ++w) high = max(high, S.best[w]);
+    __syncthreads();
+    if (high == 0) break;
+    if (tid == 0) S.key[found] = high;
+    below = high;
   }
+  if (tid == 0) S.keys = found;
   __syncthreads();
+}
+
+// The top_k highest of S.key[0 .. n), each to put(place, key) by one thread, places that remain with key 0.
+template <class Put>
+__device__ __forceinline__ void rank_keys(const TopScratch& S, int n, int top_k, Put&& put)
+{
+#pragma unroll 1
+  for (int i = threadIdx.x; i < max(n, top_k); i += blockDim.x) {
+    const uint64_t key = i < n ? S.key[i] : 0u;
+    int above          = i < n ? 0 : i;  // nothing comes behind all that there is
+    if (i < n)
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) above += S.key[j] > key;
+    if (above < top_k) put(above, key);
+  }
 }
 
 struct NoScratch {};
 
-// A row's CTAs (a cluster when there are several) each stream their share of its packs once.
+// A row is streamed once, by a CTA of 64 .. kThreads threads or by a cluster of such CTAs that take a share of its packs each.
 template <class T, bool ENTROPY, bool TOP>
-__global__ void __launch_bounds__(kThreads) k_token_logprobs(const T* __restrict__ logits, const ScoreArgs a, int parts)
+__global__ void __launch_bounds__(kThreads, 5) k_token_logprobs(const T* __restrict__ logits, const ScoreArgs a, int parts)
 {
   namespace cg = cooperative_groups;
-  constexpr int E = Pack16<T>::kElems;
-  __shared__ float s_m[kWarps];
-  __shared__ float s_s[kWarps], s_t[kWarps];
+  using P         = Pack16<T>;
+  constexpr int E = P::kElems;
+  __shared__ float s_m[kWarps], s_s[kWarps], s_t[kWarps];
   __shared__ RowSum s_part;  // of this CTA, read by the row's first
   __shared__ typename std::conditional<TOP, TopScratch, NoScratch>::type s_top;
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int tid = threadIdx.x, threads = blockDim.x, warps = threads >> 5, warp = tid >> 5, lane = tid & 31;
   const int64_t r = blockIdx.x / unsigned(parts);
   const int part  = int(blockIdx.x % unsigned(parts));
   const RowParts<T> row(logits + r * a.stride, a.vocab);
   const int share = (row.packs + parts - 1) / parts;
   const int begin = min(row.packs, part * share), end = min(row.packs, begin + share);
-  const float k   = a.scale * kLog2e;
+  const float k = a.scale * kLog2e, nan = __int_as_float(0x7FC00000);
   int target      = -1;
   float at_target = 0.f;
   if (tid == 0 && part == 0 && a.logprob) {
@@ -292,30 +345,37 @@ __global__ void __launch_bounds__(kThreads) k_token_logprobs(const T* __restrict
   if (part == 0 && tid < row.head + row.tail) sum.add(gtk::to_float(row.x[row.loose_column(tid)]), k);
   Two s2(sum.s, 0.f), t2(sum.t, 0.f);
   const Two k2(k, k);
-  float best = -INFINITY;
-  for (int p0 = begin + tid; p0 < end; p0 += kBatch * kThreads) {
+  typename P::Max best[kBatch];
+#pragma unroll
+  for (int q = 0; q < kBatch; ++q) best[q] = P::lowest();
+  for (int p0 = begin + tid; p0 < end; p0 += kBatch * threads) {
     uint4 raw[kBatch];
 #pragma unroll
     for (int q = 0; q < kBatch; ++q) {
-      constexpr uint32_t w = Pack16<T>::kMinusInf;
-      raw[q] = p0 + q * kThreads < end ? __ldg(row.pack(p0 + q * kThreads)) : make_uint4(w, w, w, w);
+      constexpr uint32_t w = P::kMinusInf;
+      raw[q] = p0 + q * threads < end ? __ldg(row.pack(p0 + q * threads)) : make_uint4(w, w, w, w);
     }
-    const float high = Pack16<T>::highest(raw);
-    if (high > best) {
-      best = high;
-      if (high > sum.m) {
-        const float d = fmaxf((sum.m - high) * k, -1e4f), f = pow2(d);
-        const Two f2(f, f);
-        if (ENTROPY) t2 = fma2(s2, Two(d, d), t2) * f2;
-        s2    = s2 * f2;
-        sum.m = high;
-      }
+    typename P::Max all = P::highest(raw[0]);
+    if (TOP) best[0] = P::higher(best[0], all);
+#pragma unroll
+    for (int q = 1; q < kBatch; ++q) {
+      const typename P::Max m = P::highest(raw[q]);
+      if (TOP) best[q] = P::higher(best[q], m);
+      all = P::higher(all, m);
+    }
+    const float high = P::kHalves == 2 ? fmaxf(P::of(all, 0), P::of(all, 1)) : P::of(all, 0);
+    if (high > sum.m) {
+      const float d = fmaxf((sum.m - high) * k, -1e4f), f = pow2(d);
+      const Two f2(f, f);
+      if (ENTROPY) t2 = fma2(s2, Two(d, d), t2) * f2;
+      s2    = s2 * f2;
+      sum.m = high;
     }
     const Two m2(-sum.m, -sum.m);
 #pragma unroll
     for (int q = 0; q < kBatch; ++q) {
       Two x[E / 2];
-      Pack16<T>::pairs(raw[q], x);
+      P::pairs(raw[q], x);
 #pragma unroll
       for (int j = 0; j < E / 2; ++j) {
         float y0, y1;
@@ -345,56 +405,79 @@ __global__ void __launch_bounds__(kThreads) k_token_logprobs(const T* __restrict
   }
   if (lane == 0) s_m[warp] = sum.m, s_s[warp] = sum.s, s_t[warp] = sum.t;
   __syncthreads();
-  m = s_m[0];
-#pragma unroll
-  for (int w = 1; w < kWarps; ++w) m = fmaxf(m, s_m[w]);
   RowSum all;
-  all.m = m;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
+  all.m = s_m[0];
+  for (int w = 1; w < warps; ++w) all.m = fmaxf(all.m, s_m[w]);
+  for (int w = 0; w < warps; ++w) {
     RowSum o;
     o.m = s_m[w], o.s = s_s[w], o.t = s_t[w];
-    o.raise(m, k);
+    o.raise(all.m, k);
     all.s += o.s;
     all.t += o.t;
   }
-  if constexpr (TOP) select_top(row, begin, end, part == 0, a.top_k, best, s_top);
-  if (parts > 1) {
+  float log_sum = logf(all.s);  // -inf: nothing allowed, NaN: no distribution
+  auto put = [&](int place, uint64_t key) {  // an alternative of the row, once `all` is the whole row's
+    const bool broken = isnan(all.s);
+    if (a.top_ids) a.top_ids[r * a.top_k + place] = key && !broken ? int32_t(key_column(key)) : -1;
+    if (a.top_logprobs)
+      a.top_logprobs[r * a.top_k + place] = broken ? nan : key ? (key_value(key) - all.m) * a.scale - log_sum : -INFINITY;
+  };
+  uint32_t mine = 0, bound = 0;  // value_key of the thread's highest, and what the alternatives reach
+  if constexpr (TOP) {
+    typename P::Max over = best[0];
+#pragma unroll
+    for (int q = 1; q < kBatch; ++q) over = P::higher(over, best[q]);
+    mine = value_key(P::kHalves == 2 ? fmaxf(P::of(over, 0), P::of(over, 1)) : P::of(over, 0));
+    // at least top_k elements reach the top_k-th highest of the threads' own; with several parts, the lowest of the parts'
+    // (top_k / parts)-th highest
+    bound = find_bound<T>(mine, (a.top_k + parts - 1) / parts);
+  }
+  if (parts == 1) {
+    if constexpr (TOP) {
+      collect_keys(row, begin, end, true, a.top_k, kMostKeys, bound, mine, best, s_top);
+      rank_keys(s_top, s_top.keys, a.top_k, put);
+    }
+  } else {
     cg::cluster_group cluster = cg::this_cluster();
-    if (tid == 0) s_part = all;
+    if (tid == 0) {
+      s_part = all;
+      if constexpr (TOP) s_top.bound = bound;
+    }
     cluster.sync();
+    if constexpr (TOP) {
+      for (int c = 0; c < parts; ++c) bound = min(bound, cluster.map_shared_rank(&s_top, c)->bound);
+      collect_keys(row, begin, end, part == 0, a.top_k, kMostKeysOfPart, bound, mine, best, s_top);
+      cluster.sync();
+    }
     if (part == 0) {
-      for (int c = 1; c < parts; ++c) m = fmaxf(m, cluster.map_shared_rank(&s_part, c)->m);
       RowSum joined;
-      joined.m = m;
+      joined.m = all.m;
+      for (int c = 1; c < parts; ++c) joined.m = fmaxf(joined.m, cluster.map_shared_rank(&s_part, c)->m);
       for (int c = 0; c < parts; ++c) {
         RowSum o = *cluster.map_shared_rank(&s_part, c);
-        o.raise(m, k);
+        o.raise(joined.m, k);
         joined.s += o.s;
         joined.t += o.t;
       }
-      all = joined;
+      all     = joined;
+      log_sum = logf(all.s);
       if constexpr (TOP) {
-        // at most kMaxParts * GTK_MAX_TOP = kThreads keys, one per thread
-        uint64_t key = 0;
-        if (tid < parts * a.top_k) key = cluster.map_shared_rank(&s_top, tid / a.top_k)->top[tid % a.top_k];
-        s_top.candidate[tid] = key;
+        int n = s_top.keys;
+        for (int c = 1; c < parts; ++c) {
+          const TopScratch* other = cluster.map_shared_rank(&s_top, c);
+          const int more          = other->keys;
+          for (int i = tid; i < more; i += threads) s_top.key[n + i] = other->key[i];
+          n += more;
+        }
         __syncthreads();
-        if (tid < a.top_k) s_top.top[tid] = 0;
-        __syncthreads();
-        int above = 0;
-        for (int j = 0; j < parts * a.top_k; ++j) above += s_top.candidate[j] > key;
-        if (key && above < a.top_k) s_top.top[above] = key;
-        __syncthreads();
+        rank_keys(s_top, n, a.top_k, put);
       }
     }
     cluster.sync();  // nobody leaves while its shared memory is read
     if (part != 0) return;
   }
-  const float log_sum = logf(all.s);  // -inf: nothing allowed, NaN: no distribution
-  const bool none = all.s == 0.f, broken = isnan(all.s);
-  const float nan = __int_as_float(0x7FC00000);
   if (tid == 0) {
+    const bool none = all.s == 0.f, broken = isnan(all.s);
     if (a.logprob) {
       float lp = target < 0 ? 0.f : nan;
       if (target >= 0 && target < a.vocab && !broken) lp = none ? -INFINITY : (at_target - all.m) * a.scale - log_sum;
@@ -403,29 +486,32 @@ __global__ void __launch_bounds__(kThreads) k_token_logprobs(const T* __restrict
     if (a.entropy) a.entropy[r] = none ? 0.f : broken ? nan : fmaxf(log_sum - kLn2 * all.t / all.s, 0.f);
     if (a.lse) a.lse[r] = none ? -INFINITY : broken ? nan : fmaf(all.m, a.scale, log_sum);
   }
-  if constexpr (TOP) {
-    if (tid < a.top_k) {
-      const uint64_t key = broken ? 0 : s_top.top[tid];
-      if (a.top_ids) a.top_ids[r * a.top_k + tid] = key ? int32_t(key_column(key)) : -1;
-      if (a.top_logprobs) a.top_logprobs[r * a.top_k + tid] = broken ? nan : key ? (key_value(key) - all.m) * a.scale - log_sum : -INFINITY;
-    }
-  }
 }
 
-// How many CTAs share a row: few rows are split until the GPU has a few CTAs per SM.
-int row_parts(int64_t rows, int64_t bytes, int sm_count)
+// How many CTAs share a row, and how many threads they have.  Few rows are split, as long as a CTA keeps 12 KiB and there is an SM for
+// each (for two, of rows from 160 KiB on).  Rows in numbers take fewer threads each, so that more of them are under way
+// while others are at their ends.
+struct Teams {
+  int parts, threads;
+};
+Teams teams_for(int64_t rows, int64_t bytes, int sm_count)
 {
-  int parts = 1;
-  while (parts < kMaxParts && rows * parts * 2 <= int64_t(sm_count) * 2 && bytes / (parts * 2) >= 8192) parts *= 2;
-  return parts;
+  Teams t{1, kThreads};
+  const int64_t room = int64_t(sm_count) * (bytes >= (160 << 10) ? 2 : 1);
+  while (t.parts < kMaxParts && rows * t.parts * 2 <= room && bytes / (t.parts * 2) >= (12 << 10)) t.parts *= 2;
+  if (rows > int64_t(sm_count) * 5 || (bytes <= (24 << 10) && rows > int64_t(sm_count) * 3 / 2)) t.threads = 128;
+  if (bytes <= (24 << 10) && rows > int64_t(sm_count) * 8) t.threads = 64;
+  return t;
 }
 
 template <class T, bool ENTROPY, bool TOP>
 cudaError_t launch_logprobs(const gtk::HandleView& v, const void* logits, int64_t n_rows, const ScoreArgs& a)
 {
-  const int parts = row_parts(n_rows, int64_t(a.vocab) * int64_t(sizeof(T)), v.sm_count);
-  return gtk::launch_clusters(k_token_logprobs<T, ENTROPY, TOP>, dim3(unsigned(n_rows * parts)), dim3(kThreads), parts, v.stream,
-                              static_cast<const T*>(logits), a, parts);
+  Teams t = teams_for(n_rows, int64_t(a.vocab) * int64_t(sizeof(T)), v.sm_count);
+  if (const char* e = getenv("GTK_PARTS")) t.parts = atoi(e);
+  if (const char* e = getenv("GTK_TEAM")) t.threads = atoi(e);
+  return gtk::launch_clusters(k_token_logprobs<T, ENTROPY, TOP>, dim3(unsigned(n_rows * t.parts)), dim3(unsigned(t.threads)), t.parts, 0, v.stream,
+                              static_cast<const T*>(logits), a, t.parts);
 }
 
 struct ScoreGradArgs {

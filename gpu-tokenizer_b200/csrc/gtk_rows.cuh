@@ -41,6 +41,16 @@ __device__ __forceinline__ Pack<T, V> load_pack(const T* p) { return *reinterpre
 template <class T, int V>
 __device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& v) { *reinterpret_cast<Pack<T, V>*>(p) = v; }
 
+// Copies of 16 bytes to shared memory that a thread does not wait for: begun, closed as a chunk, and awaited until at most PENDING of
+// its own chunks are under way.
+__device__ __forceinline__ void copy16(uint32_t shared_at, const void* from)
+{
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(shared_at), "l"(from) : "memory");
+}
+__device__ __forceinline__ void end_chunk() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int PENDING>
+__device__ __forceinline__ void await_chunks() { asm volatile("cp.async.wait_group %0;" ::"n"(PENDING) : "memory"); }
+
 // Two 32-bit floats that one instruction works on.
 struct Two {
   uint64_t v;
@@ -111,13 +121,13 @@ cudaError_t launch(void (*kernel)(Formal...), dim3 grid, dim3 block, size_t smem
 
 // the same in clusters of `cluster` blocks next to each other
 template <class... Formal, class... Args>
-cudaError_t launch_clusters(void (*kernel)(Formal...), dim3 grid, dim3 block, int cluster, cudaStream_t stream, Args&&... args)
+cudaError_t launch_clusters(void (*kernel)(Formal...), dim3 grid, dim3 block, int cluster, size_t smem, cudaStream_t stream, Args&&... args)
 {
   cudaLaunchAttribute attr{};
   attr.id               = cudaLaunchAttributeClusterDimension;
   attr.val.clusterDim.x = unsigned(cluster), attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid, cfg.blockDim = block, cfg.stream = stream;
+  cfg.gridDim = grid, cfg.blockDim = block, cfg.dynamicSmemBytes = smem, cfg.stream = stream;
   cfg.attrs = &attr, cfg.numAttrs = cluster > 1 ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, kernel, static_cast<Formal>(args)...);
 }
