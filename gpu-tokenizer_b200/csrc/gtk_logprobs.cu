@@ -4,7 +4,6 @@
 
 #include <cfloat>
 #include <cmath>
-#include <cstdlib>
 #include <initializer_list>
 #include <type_traits>
 
@@ -445,32 +444,44 @@ __global__ void __launch_bounds__(kThreads, 5) k_token_logprobs(const T* __restr
     }
     cluster.sync();
     if constexpr (TOP) {
-      for (int c = 0; c < parts; ++c) bound = min(bound, cluster.map_shared_rank(&s_top, c)->bound);
+      // lane c asks part c, here and below: reads of other CTAs' shared memory take long, one after the other too long
+      bound = __reduce_min_sync(0xFFFFFFFFu, lane < parts ? cluster.map_shared_rank(&s_top, lane)->bound : bound);
       collect_keys(row, begin, end, part == 0, a.top_k, kMostKeysOfPart, bound, mine, best, s_top);
       cluster.sync();
     }
     if (part == 0) {
-      RowSum joined;
-      joined.m = all.m;
-      for (int c = 1; c < parts; ++c) joined.m = fmaxf(joined.m, cluster.map_shared_rank(&s_part, c)->m);
-      for (int c = 0; c < parts; ++c) {
-        RowSum o = *cluster.map_shared_rank(&s_part, c);
-        o.raise(joined.m, k);
-        joined.s += o.s;
-        joined.t += o.t;
+      RowSum o;
+      int keys = 0;
+      if (lane < parts) {
+        o = *cluster.map_shared_rank(&s_part, lane);
+        if constexpr (TOP) keys = cluster.map_shared_rank(&s_top, lane)->keys;
       }
-      all     = joined;
+      all.m = o.m;
+#pragma unroll
+      for (int d = kMaxParts / 2; d; d >>= 1) all.m = fmaxf(all.m, __shfl_xor_sync(0xFFFFFFFFu, all.m, d));
+      all.m = __shfl_sync(0xFFFFFFFFu, all.m, 0);
+      o.raise(all.m, k);
+#pragma unroll
+      for (int d = kMaxParts / 2; d; d >>= 1) {
+        o.s += __shfl_xor_sync(0xFFFFFFFFu, o.s, d);
+        o.t += __shfl_xor_sync(0xFFFFFFFFu, o.t, d);
+      }
+      all.s   = __shfl_sync(0xFFFFFFFFu, o.s, 0);
+      all.t   = __shfl_sync(0xFFFFFFFFu, o.t, 0);
       log_sum = logf(all.s);
-      if constexpr (TOP) {
-        int n = s_top.keys;
-        for (int c = 1; c < parts; ++c) {
-          const TopScratch* other = cluster.map_shared_rank(&s_top, c);
-          const int more          = other->keys;
-          for (int i = tid; i < more; i += threads) s_top.key[n + i] = other->key[i];
-          n += more;
+      if constexpr (TOP) {  // the others' keys behind its own
+        int upto = keys;
+#pragma unroll
+        for (int d = 1; d < kMaxParts; d *= 2) {
+          const int more = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+          if (lane >= d) upto += more;
+        }
+        for (int c = 1 + warp; c < parts; c += warps) {
+          const int count = __shfl_sync(0xFFFFFFFFu, keys, c), at = __shfl_sync(0xFFFFFFFFu, upto, c) - count;
+          for (int i = lane; i < count; i += 32) s_top.key[at + i] = cluster.map_shared_rank(&s_top, c)->key[i];
         }
         __syncthreads();
-        rank_keys(s_top, n, a.top_k, put);
+        rank_keys(s_top, __shfl_sync(0xFFFFFFFFu, upto, parts - 1), a.top_k, put);
       }
     }
     cluster.sync();  // nobody leaves while its shared memory is read
@@ -507,9 +518,7 @@ Teams teams_for(int64_t rows, int64_t bytes, int sm_count)
 template <class T, bool ENTROPY, bool TOP>
 cudaError_t launch_logprobs(const gtk::HandleView& v, const void* logits, int64_t n_rows, const ScoreArgs& a)
 {
-  Teams t = teams_for(n_rows, int64_t(a.vocab) * int64_t(sizeof(T)), v.sm_count);
-  if (const char* e = getenv("GTK_PARTS")) t.parts = atoi(e);
-  if (const char* e = getenv("GTK_TEAM")) t.threads = atoi(e);
+  const Teams t = teams_for(n_rows, int64_t(a.vocab) * int64_t(sizeof(T)), v.sm_count);
   return gtk::launch_clusters(k_token_logprobs<T, ENTROPY, TOP>, dim3(unsigned(n_rows * t.parts)), dim3(unsigned(t.threads)), t.parts, 0, v.stream,
                               static_cast<const T*>(logits), a, t.parts);
 }
@@ -630,7 +639,7 @@ cudaError_t launch_logprobs_grad(const gtk::HandleView& v, const void* logits, v
   const bool alike = (reinterpret_cast<uintptr_t>(logits) - reinterpret_cast<uintptr_t>(grad)) % 16 == 0 &&
                      (n_rows == 1 || (a.stride - a.grad_stride) * int64_t(sizeof(T)) % 16 == 0);
   const int64_t batches = (a.vocab + kBatch * kThreads * Pack16<T>::kElems - 1) / (kBatch * kThreads * Pack16<T>::kElems);
-  const int parts = int(std::max<int64_t>(1, std::min<int64_t>(batches, int64_t(v.sm_count) * 8 / n_rows)));
+  const int parts = int(std::max<int64_t>(1, std::min<int64_t>(batches, int64_t(v.sm_count) * 32 / n_rows)));
   return gtk::launch(alike ? k_token_logprobs_grad<T, ENTROPY> : k_token_logprobs_grad_plain<T, ENTROPY>, dim3(unsigned(n_rows * parts)),
                      dim3(kThreads), 0, v.stream, static_cast<const T*>(logits), static_cast<T*>(grad), a, parts);
 }
