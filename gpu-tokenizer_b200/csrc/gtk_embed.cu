@@ -10,54 +10,131 @@ using gtk::Pack;
 using gtk::Two;
 
 // ------------------------------------------------------------------------------------------------ lookup
-// out[i] = scale * table[ids[i]].  A block's threads are split into row groups of 1 << group_log2; a group copies a row
-// in packs of V elements, four loads in flight per thread.
+// out[i] = scale * table[ids[i]].  A block's threads are split into groups of 1 << group_log2; a group copies ROWS rows at a time, so
+// that the wait for an id and then for its row is shared by several.
+// V = 8: rows of both arrays start where 8 elements may be moved at once.  V = 2: any rows, two columns at a time.
 constexpr int kEmbedThreads = 256;
 
-template <class T, class O, int V>
+// Two neighbouring elements at any address.  16-bit ones come in the one or two aligned 32-bit words that hold them; a word
+// is read only if a wanted element lies in it.
+template <class T>
+__device__ __forceinline__ uint2 load_two(const T* p, bool second)
+{
+  if constexpr (sizeof(T) == 4) {
+    return make_uint2(__ldg(reinterpret_cast<const uint32_t*>(p)), second ? __ldg(reinterpret_cast<const uint32_t*>(p) + 1) : 0u);
+  } else {
+    const uint32_t* w = reinterpret_cast<const uint32_t*>(reinterpret_cast<uintptr_t>(p) & ~uintptr_t(3));
+    const bool odd    = reinterpret_cast<uintptr_t>(p) & 2;
+    return make_uint2(__ldg(w), odd && second ? __ldg(w + 1) : 0u);
+  }
+}
+template <class T>
+__device__ __forceinline__ void two_floats(uint2 raw, const T* p, float& a, float& b)
+{
+  if constexpr (sizeof(T) == 4) a = __uint_as_float(raw.x), b = __uint_as_float(raw.y);
+  else gtk::word_pair(__funnelshift_r(raw.x, raw.y, uint32_t(reinterpret_cast<uintptr_t>(p) & 2) * 8), T{}).get(a, b);
+}
+template <class O>
+__device__ __forceinline__ void store_two(O* p, bool second, float a, float b)
+{
+  Pack<O, 2> y;
+  y.e[0] = gtk::from_float<O>(a), y.e[1] = gtk::from_float<O>(b);
+  if (second && reinterpret_cast<uintptr_t>(p) % sizeof(y) == 0) {
+    gtk::store_pack<O, 2>(p, y);
+  } else {
+    p[0] = y.e[0];
+    if (second) p[1] = y.e[1];
+  }
+}
+
+template <class T, class O, int V, int ROWS>
 __global__ void __launch_bounds__(kEmbedThreads)
 k_embed(const int32_t* __restrict__ ids, int64_t n, const T* __restrict__ table, int vocab, int dim, int64_t table_stride,
         float scale, O* __restrict__ out, int64_t out_stride, int group_log2)
 {
   const int group = 1 << group_log2, lane = threadIdx.x & (group - 1);
-  const int64_t i = int64_t(blockIdx.x) * (kEmbedThreads >> group_log2) + (threadIdx.x >> group_log2);
-  if (i >= n) return;
-  const int id = __ldg(ids + i);
-  O* to        = out + i * out_stride;
-  if (uint32_t(id) >= uint32_t(vocab)) {
-    const O fill = gtk::from_float<O>(id < 0 ? 0.f : __int_as_float(0x7FC00000));
-    for (int c = lane; c < dim; c += group) to[c] = fill;
-    return;
+  const int64_t first = (int64_t(blockIdx.x) * (kEmbedThreads >> group_log2) + (threadIdx.x >> group_log2)) * ROWS;
+  int id[ROWS];
+  const T* from[ROWS];
+  O* to[ROWS];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) id[r] = first + r < n ? __ldg(ids + first + r) : -1;
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const bool has = uint32_t(id[r]) < uint32_t(vocab);
+    from[r]        = has ? table + int64_t(id[r]) * table_stride : nullptr;
+    to[r]          = out + (first + r) * out_stride;
+    if (!has && first + r < n) {
+      const O fill = gtk::from_float<O>(id[r] < 0 ? 0.f : __int_as_float(0x7FC00000));
+      for (int c = lane; c < dim; c += group) to[r][c] = fill;
+    }
   }
-  const T* from   = table + int64_t(id) * table_stride;
-  const int packs = dim / V;
-  for (int u0 = lane; u0 < packs; u0 += 4 * group) {
-    Pack<T, V> x[4];
+  if constexpr (V == 8) {
+    constexpr int kAhead = ROWS == 1 ? 4 : sizeof(T) == 2 ? 2 : 1;
+    const int packs      = dim / V;
+    for (int u0 = lane; u0 < packs; u0 += kAhead * group) {
+      Pack<T, V> x[ROWS][kAhead];
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (u0 + k * group < packs) x[k] = gtk::load_pack<T, V>(from + int64_t(u0 + k * group) * V);
+      for (int r = 0; r < ROWS; ++r)
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-      if (u0 + k * group < packs) {
-        Pack<O, V> y;
+        for (int k = 0; k < kAhead; ++k)
+          if (from[r] && u0 + k * group < packs) x[r][k] = gtk::load_pack<T, V>(from[r] + (u0 + k * group) * V);
 #pragma unroll
-        for (int j = 0; j < V; ++j) y.e[j] = gtk::from_float<O>(gtk::to_float(x[k].e[j]) * scale);
-        gtk::store_pack<O, V>(to + int64_t(u0 + k * group) * V, y);
-      }
+      for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k)
+          if (from[r] && u0 + k * group < packs) {
+            Pack<O, V> y;
+#pragma unroll
+            for (int j = 0; j < V; ++j) y.e[j] = gtk::from_float<O>(gtk::to_float(x[r][k].e[j]) * scale);
+            gtk::store_pack<O, V>(to[r] + (u0 + k * group) * V, y);
+          }
+    }
+    for (int c = packs * V + lane; c < dim; c += group)
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r)
+        if (from[r]) to[r][c] = gtk::from_float<O>(gtk::to_float(from[r][c]) * scale);
+  } else {
+    constexpr int kAhead = 4;
+    const int pairs      = (dim + 1) / 2;
+    for (int u0 = lane; u0 < pairs; u0 += kAhead * group) {
+      uint2 x[ROWS][kAhead];
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          const int c = (u0 + k * group) * 2;
+          if (from[r] && c < dim) x[r][k] = load_two(from[r] + c, c + 1 < dim);
+        }
+#pragma unroll
+      for (int r = 0; r < ROWS; ++r)
+#pragma unroll
+        for (int k = 0; k < kAhead; ++k) {
+          const int c = (u0 + k * group) * 2;
+          if (from[r] && c < dim) {
+            float a, b;
+            two_floats(x[r][k], from[r] + c, a, b);
+            store_two(to[r] + c, c + 1 < dim, a * scale, b * scale);
+          }
+        }
+    }
   }
-  for (int c = packs * V + lane; c < dim; c += group) to[c] = gtk::from_float<O>(gtk::to_float(from[c]) * scale);
 }
 
 template <class T, class O, int V>
 cudaError_t launch_embed(const gtk::HandleView& v, const int32_t* ids, int64_t n, const void* table, int64_t vocab, int64_t dim,
                          int64_t table_stride, float scale, void* out, int64_t out_stride)
 {
-  const int64_t packs = std::max<int64_t>(1, dim / V);
-  int group_log2 = 5;  // a warp per row, more for rows of more than four packs a lane
-  while (group_log2 < 8 && (int64_t(4) << group_log2) < packs) ++group_log2;
-  const int64_t rows = kEmbedThreads >> group_log2;
-  return gtk::launch(k_embed<T, O, V>, dim3(unsigned((n + rows - 1) / rows)), dim3(kEmbedThreads), 0, v.stream, ids, n,
-                     static_cast<const T*>(table), int(vocab), int(dim), table_stride, scale, static_cast<O*>(out), out_stride,
+  // Few rows: a thread for every unit of a row.  Many: a quarter as many and two rows at once when they are packs (32768 rows of 1024
+  // bf16: 18.1 us, one row at once 19.0, four 24.8; 100000 rows of 256: 14.8, with a lane for every pack 34.4), a warp and one
+  // row when they are pairs (30000 rows of 1601 bf16: 43 us, two rows at once 49).
+  const int64_t units = (dim + (V == 8 ? 7 : 1)) / V;
+  const bool many     = n >= int64_t(v.sm_count) * 64;
+  int group_log2      = 0;
+  while (group_log2 < (many ? 5 : 8) && (int64_t(many ? 4 : 1) << group_log2) < units) ++group_log2;
+  const int64_t rows = (kEmbedThreads >> group_log2) * (many && V == 8 ? 2 : 1);
+  return gtk::launch(many && V == 8 ? k_embed<T, O, V, 2> : k_embed<T, O, V, 1>, dim3(unsigned((n + rows - 1) / rows)), dim3(kEmbedThreads), 0,
+                     v.stream, ids, n, static_cast<const T*>(table), int(vocab), int(dim), table_stride, scale, static_cast<O*>(out), out_stride,
                      group_log2);
 }
 
@@ -709,7 +786,7 @@ extern "C" GTK_API int gtk_embed(gtk_tokenizer* h, const int32_t* d_ids, int64_t
     const bool packs = gtk::rows_aligned(d_table, table_stride, table_type, 8) && gtk::rows_aligned(d_out, out_stride, out_type, 8);
     return gtk::with_type(table_type, [&](auto t) {
       return gtk::with_type(out_type, [&](auto o) {
-        auto f = packs ? launch_embed<decltype(t), decltype(o), 8> : launch_embed<decltype(t), decltype(o), 1>;
+        auto f = packs ? launch_embed<decltype(t), decltype(o), 8> : launch_embed<decltype(t), decltype(o), 2>;
         return f(v, d_ids, n_ids, d_table, vocab, dim, table_stride, scale, d_out, out_stride);
       });
     });
