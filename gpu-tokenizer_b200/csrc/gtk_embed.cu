@@ -1,6 +1,7 @@
 // gtk_embed.cu -- embedding lookup with scaling, and its gradient by sorted tokens.
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 
 #include "gtk_rows.cuh"
 
@@ -184,6 +185,7 @@ GradPlan grad_plan(int64_t n, int64_t vocab, int64_t dim)
   p.block_log2   = kMinBlockLog2;
   // blocks as long as still leaves about 1.5 M columns of them: a dozen row groups of 768 columns per SM
   while (p.block_log2 < kMaxBlockLog2 && (n >> (p.block_log2 + 1)) * dim >= int64_t(3) << 19) ++p.block_log2;
+  if (getenv("GTK_BL")) p.block_log2 = atoi(getenv("GTK_BL"));
   p.blocks    = (n + (int64_t(1) << p.block_log2) - 1) >> p.block_log2;
   p.pitch     = (dim + 7) / 8 * 8;
   size_t at   = 0;
@@ -545,8 +547,8 @@ struct GroupShared {
 };
 
 // A group of threads (part of a warp, or the whole CTA) takes a block of tokens.  The rows come to shared memory in 16-byte pieces,
-// each thread copying one piece of every row, kChunk * kChunks rows ahead.  The pieces are those between 16-byte
-// boundaries: the outer ones may hold bytes of a row's neighbours, which nobody looks at.
+// a warp copying a row, kChunk * kChunks rows ahead.  The pieces are those between 16-byte boundaries: the outer ones may
+// hold bytes of a row's neighbours, which nobody looks at.
 template <class O, class T, bool ALIGNED>
 __global__ void __launch_bounds__(kGradThreads) k_embed_grad_sums(const GradArgs a, const O* __restrict__ grad_out, T* __restrict__ grad_table)
 {
@@ -594,43 +596,53 @@ __global__ void __launch_bounds__(kGradThreads) k_embed_grad_sums(const GradArgs
     }
   }
   if (at >= stop) return;  // the whole group
-  const uint32_t ring_at = uint32_t(__cvta_generic_to_shared(ring)) + lane * 16, width_bytes = uint32_t(width) * uint32_t(sizeof(O));
-  const uint32_t slot_bytes = group * 16, chunk_bytes = kChunk * slot_bytes;
+  const uint32_t width_bytes = uint32_t(width) * uint32_t(sizeof(O)), slot_bytes = group * 16, chunk_bytes = kChunk * slot_bytes;
+  const uint32_t ring_at = uint32_t(__cvta_generic_to_shared(ring));
   uint32_t to = ring_at;  // where the next chunk goes
-  auto request = [&](int chunk) {  // rows of window places chunk * kChunk ..
-#pragma unroll
-    for (int k = 0; k < kChunk; ++k) {
+  // The rows of window places chunk * kChunk ..: each is one warp's to copy, or the group's when that is smaller.
+  const int warps = max(1, group >> 5), copier = group > 32 ? lane & 31 : lane, copiers = min(group, 32);
+  auto request = [&](int chunk) {
+    for (int k = lane >> 5; k < kChunk; k += warps) {
       const int i = chunk * kChunk + k;
-      if (i >= at && i < stop) {
-        const uint64_t row   = address[i];
-        const uint32_t shift = ALIGNED ? 0u : uint32_t(row) & 15u;
-        if (uint32_t(lane) * 16u < shift + width_bytes) gtk::copy16(to + k * slot_bytes, reinterpret_cast<const char*>(row - shift) + lane * 16);
-      }
+      if (i < at || i >= stop) continue;
+      const uint64_t row    = address[i];
+      const uint32_t shift  = ALIGNED ? 0u : uint32_t(row) & 15u;
+      const char* from      = reinterpret_cast<const char*>(row - shift) + copier * 16;
+      const uint32_t slot   = to + k * slot_bytes + copier * 16;
+      const int pieces      = int((shift + width_bytes + 15u) >> 4) - copier;
+#pragma unroll
+      for (int p = 0; p < kGradThreads; p += 32)
+        if (p < pieces) gtk::copy16(slot + p * 16, from + p * 16);
+        else break;
     }
     gtk::end_chunk();
     to = to + chunk_bytes == ring_at + kChunks * chunk_bytes ? ring_at : to + chunk_bytes;
   };
   // ALIGNED: the thread's own piece.  Otherwise words, those of a warp next to each other
   const int mine = ALIGNED ? lane : (lane & ~31) * 4 + (lane & 31);
+  // the thread's columns from the first of the slab: unit u begins at own + u * kStep units and has valid(u) of them in the row
+  const int own  = mine * S::kUnit;
+  auto valid     = [&](int u) { return max(0, min(S::kUnit, width - own - u * kStep * S::kUnit)); };
+  uint32_t whole = 0, some = 0;
+#pragma unroll
+  for (int u = 0; u < S::kUnits; ++u) {
+    whole |= (valid(u) == S::kUnit ? 1u : 0u) << u;
+    some |= (valid(u) > 0 ? 1u : 0u) << u;
+  }
   Two sum[S::kCount / 2];
-  auto each_unit = [&](auto&& f) {  // f(first column, columns within the row, the sums)
+  auto store_part = [&](int which) {
+    float* to_part = a.parts + (block * 2 + which) * a.pitch + first + own;
     float x[S::kCount];
 #pragma unroll
     for (int j = 0; j < S::kCount / 2; ++j) sum[j].get(x[2 * j], x[2 * j + 1]);
 #pragma unroll
-    for (int u = 0; u < S::kUnits; ++u) {
-      const int c = (mine + u * kStep) * S::kUnit;
-      if (c < width) f(first + c, min(S::kUnit, width - c), x + u * S::kUnit);
-    }
-  };
-  auto store_part = [&](int which) {
-    float* to_part = a.parts + (block * 2 + which) * a.pitch;
-    each_unit([&](int c, int, const float* x) {  // whole units: the pitch is a multiple of them
-      Pack<float, S::kUnit> p;
+    for (int u = 0; u < S::kUnits; ++u)
+      if (some >> u & 1u) {  // whole units: the pitch is a multiple of them
+        Pack<float, S::kUnit> p;
 #pragma unroll
-      for (int j = 0; j < S::kUnit; ++j) p.e[j] = x[j];
-      gtk::store_pack<float, S::kUnit>(to_part + c, p);
-    });
+        for (int j = 0; j < S::kUnit; ++j) p.e[j] = x[u * S::kUnit + j];
+        gtk::store_pack<float, S::kUnit>(to_part + u * kStep * S::kUnit, p);
+      }
   };
   auto finish = [&](uint32_t id) {
     if (from_left) {
@@ -638,9 +650,38 @@ __global__ void __launch_bounds__(kGradThreads) k_embed_grad_sums(const GradArgs
       from_left = false;
       return;
     }
-    T* row           = grad_table + int64_t(id) * a.table_stride;
-    const bool packs = ALIGNED || reinterpret_cast<uintptr_t>(row + first) % (sizeof(T) * S::kUnit) == 0;
-    each_unit([&](int c, int own, const float* x) { store_sum<T, S::kUnit>(row + c, own, packs, a.scale, a.accumulate, x); });
+    T* row           = grad_table + int64_t(id) * a.table_stride + first + own;
+    const bool packs = ALIGNED || reinterpret_cast<uintptr_t>(row) % (sizeof(T) * S::kUnit) == 0;
+    float x[S::kCount];
+    const Two scale(a.scale, a.scale);
+#pragma unroll
+    for (int j = 0; j < S::kCount / 2; ++j) (sum[j] * scale).get(x[2 * j], x[2 * j + 1]);
+#pragma unroll
+    for (int u = 0; u < S::kUnits; ++u) {
+      T* unit = row + u * kStep * S::kUnit;
+      if (packs && (whole >> u & 1u)) {
+        Pack<T, S::kUnit> y;
+        if (a.accumulate) {
+          const Pack<T, S::kUnit> old = gtk::load_pack<T, S::kUnit>(unit);
+          float z[S::kCount];
+#pragma unroll
+          for (int j = 0; j < S::kCount / 2; ++j) sum[j].get(z[2 * j], z[2 * j + 1]);
+#pragma unroll
+          for (int j = 0; j < S::kUnit; ++j) x[u * S::kUnit + j] = fmaf(z[u * S::kUnit + j], a.scale, gtk::to_float(old.e[j]));
+        }
+#pragma unroll
+        for (int j = 0; j < S::kUnit; ++j) y.e[j] = gtk::from_float<T>(x[u * S::kUnit + j]);
+        gtk::store_pack<T, S::kUnit>(unit, y);
+      } else {
+        float z[S::kCount];
+#pragma unroll
+        for (int j = 0; j < S::kCount / 2; ++j) sum[j].get(z[2 * j], z[2 * j + 1]);
+        const int here = whole >> u & 1u ? S::kUnit : some >> u & 1u ? (ALIGNED ? valid(u) : 1) : 0;
+#pragma unroll
+        for (int j = 0; j < S::kUnit; ++j)
+          if (j < here) unit[j] = gtk::from_float<T>(a.accumulate ? fmaf(z[u * S::kUnit + j], a.scale, gtk::to_float(unit[j])) : x[u * S::kUnit + j]);
+      }
+    }
   };
   int chunk = at / kChunk;
 #pragma unroll
@@ -651,10 +692,8 @@ __global__ void __launch_bounds__(kGradThreads) k_embed_grad_sums(const GradArgs
   const uint4* rows = ring;
   for (; chunk * kChunk < stop; ++chunk) {
     gtk::await_chunks<kChunks - 2>();
-    if constexpr (!ALIGNED) {
-      if (group > 32) __syncthreads();
-      else __syncwarp(mask);
-    }
+    if (group > 32) __syncthreads();
+    else __syncwarp(mask);
     request(chunk + kChunks - 1);  // over the chunk in front, which everybody has added
     uint32_t now[kChunk], shift[kChunk];
 #pragma unroll
