@@ -142,10 +142,10 @@ cudaError_t launch_embed(const gtk::HandleView& v, const int32_t* ids, int64_t n
 // ------------------------------------------------------------------------------------------------ gradient
 // grad_table[v] = scale * sum of grad_out[i] over the i with ids[i] == v, in three launches:
 //   k_embed_grad_sort   groups the tokens by id, which brings the rows of a sum next to each other in order of i, and
-//                       writes the rows that no id points to
-//   k_embed_grad_sums   the grouped tokens in blocks of equal length, a row group of threads per block; a sum is kept in
-//                       registers.  One that lies in a block or reaches over one boundary is its first block's alone; a
-//                       longer one is cut at the boundaries and its parts go to the workspace
+//                       clears the rows that no id points to
+//   k_embed_grad_sums   the grouped tokens in blocks of equal length, a group of threads per block; a sum is kept in registers.
+//                       One that lies in a block or reaches over one boundary is its first block's alone; a longer one is cut
+//                       at the boundaries and its parts go to the workspace
 //   k_embed_grad_join   adds the parts of the long ones from left to right
 // Every sum is thus formed in an order that the ids alone decide.
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
@@ -174,7 +174,7 @@ int bits_of(int64_t x)
 }
 
 constexpr size_t kSharedMost = 96 << 10;  // of a CTA
-constexpr int kMinBlockLog2 = 3, kMaxBlockLog2 = 10;
+constexpr int kMinBlockLog2 = 3, kMaxBlockLog2 = 9;
 
 GradPlan grad_plan(int64_t n, int64_t vocab, int64_t dim)
 {
@@ -212,25 +212,27 @@ struct SortArgs {
 };
 
 constexpr uint32_t kNoId = 0xFFFFFFFFu;  // ids are below 2^31
-constexpr int kListRoom  = 320;          // tokens of an owner that a warp finds in its part of the text
+constexpr int kListRoom  = 600;          // tokens of an owner that a warp finds in its part of the text
 
 struct SortShared {
   uint32_t at[kSortWarps][1 << kMaxDigitBits];
   uint2 list[kSortWarps][kListRoom];
   uint32_t warp_sum[kSortWarps];
-  uint32_t lower[kSortWarps], mine[kSortWarps], valid[kSortWarps];
+  uint32_t lower[kSortWarps], mine[kSortWarps];
 };
 
 // The sum over the warps in front and over all of them, of a number that each warp has put into v.
-__device__ __forceinline__ void over_warps(const uint32_t* v, int warp, uint32_t& front, uint32_t& all)
+__device__ __forceinline__ void over_warps(const uint32_t* v, int warp, int lane, uint32_t& front, uint32_t& all)
 {
-  front = all = 0;
+  const uint32_t mine = v[lane];  // kSortWarps == 32
+  uint32_t upto       = mine;
 #pragma unroll
-  for (int w = 0; w < kSortWarps; ++w) {
-    const uint32_t x = v[w];
-    front += w < warp ? x : 0u;
-    all += x;
+  for (int d = 1; d < 32; d *= 2) {
+    const uint32_t o = __shfl_up_sync(0xFFFFFFFFu, upto, d);
+    if (lane >= d) upto += o;
   }
+  front = __shfl_sync(0xFFFFFFFFu, upto - mine, warp);
+  all   = __shfl_sync(0xFFFFFFFFu, upto, 31);
 }
 
 // One digit of a stable sort of the CTA's own tokens, of which this warp has from[0 .. count) (each warp those behind the
@@ -242,17 +244,23 @@ __device__ void sort_digit(const uint2* from, uint32_t count, uint2* to, int shi
   const uint32_t lower = (1u << lane) - 1u;
   for (int b = lane; b < bins; b += 32) S.at[warp][b] = 0;
   __syncwarp();
+  // The lanes of one digit are counted by the last of them: a frequent id would have them wait for each other at one address.
+  auto peers_of = [&](uint32_t digit) { return __match_any_sync(0xFFFFFFFFu, digit); };
 #pragma unroll 4
-  for (uint32_t i = lane; i < count; i += 32) atomicAdd(&S.at[warp][(from[i].x >> shift) & (bins - 1)], 1u);
+  for (uint32_t i0 = 0; i0 < count; i0 += 32) {
+    const bool here      = i0 + lane < count;
+    const uint32_t digit = here ? (from[i0 + lane].x >> shift) & uint32_t(bins - 1) : 0xFFFFFFFFu;
+    const uint32_t peers = peers_of(digit);
+    if (here && (peers >> lane) == 1u) S.at[warp][digit] += __popc(peers);
+    __syncwarp();
+  }
   __syncthreads();
-  uint32_t sum = 0;
+  uint32_t counts[kSortWarps], sum = 0;
   if (tid < bins) {
 #pragma unroll
-    for (int w = 0; w < kSortWarps; ++w) {
-      const uint32_t c = S.at[w][tid];
-      S.at[w][tid]     = sum;
-      sum += c;
-    }
+    for (int w = 0; w < kSortWarps; ++w) counts[w] = S.at[w][tid];
+#pragma unroll
+    for (int w = 0; w < kSortWarps; ++w) sum += counts[w];
   }
   uint32_t upto = sum;
 #pragma unroll
@@ -262,12 +270,15 @@ __device__ void sort_digit(const uint2* from, uint32_t count, uint2* to, int shi
   }
   if (lane == 31) S.warp_sum[warp] = upto;
   __syncthreads();
+  uint32_t at, all;
+  over_warps(S.warp_sum, warp, lane, at, all);
+  at += upto - sum;
   if (tid < bins) {
-    uint32_t front, all;
-    over_warps(S.warp_sum, warp, front, all);
-    front += upto - sum;
 #pragma unroll
-    for (int w = 0; w < kSortWarps; ++w) S.at[w][tid] += front;
+    for (int w = 0; w < kSortWarps; ++w) {
+      S.at[w][tid] = at;
+      at += counts[w];
+    }
   }
   __syncthreads();
 #pragma unroll 2
@@ -275,7 +286,7 @@ __device__ void sort_digit(const uint2* from, uint32_t count, uint2* to, int shi
     const bool here      = i0 + lane < count;
     const uint2 x        = here ? from[i0 + lane] : make_uint2(0u, 0u);
     const uint32_t digit = here ? (x.x >> shift) & uint32_t(bins - 1) : 0xFFFFFFFFu;
-    const uint32_t peers = __match_any_sync(0xFFFFFFFFu, digit);
+    const uint32_t peers = peers_of(digit);
     const uint32_t place = here ? S.at[warp][digit] + __popc(peers & lower) : 0u;
     __syncwarp();
     if (here && (peers >> lane) == 1u) S.at[warp][digit] = place + 1u;  // the last of the peers
@@ -319,21 +330,15 @@ __device__ void group_tokens(const SortArgs& a, SortShared& S, uint32_t& begin, 
 {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t owner = blockIdx.x, lanes_below = (1u << lane) - 1u;
-  uint32_t lower = 0, valid = 0, mine = 0;
+  uint32_t lower = 0, mine = 0;
   // the tokens of one step to to[], in order; returns how many
-  auto take = [&](const uint32_t (&id)[4], int64_t i, uint2* to, uint32_t room) {
-    uint32_t mask[4], total = 0, at = 0;
-    bool is_mine[4];
+  auto take = [&](const uint32_t (&id)[4], const bool (&is_mine)[4], int64_t i, uint2* to, uint32_t room) {
+    uint32_t total = 0, at = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      is_mine[j] = id[j] < a.vocab && (id[j] & (kOwners - 1)) == owner;
-      mask[j]    = __ballot_sync(0xFFFFFFFFu, is_mine[j]);
-    }
-    if (!(mask[0] | mask[1] | mask[2] | mask[3])) return 0u;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      total += __popc(mask[j]);
-      at += __popc(mask[j] & lanes_below);
+      const uint32_t mask = __ballot_sync(0xFFFFFFFFu, is_mine[j]);
+      total += __popc(mask);
+      at += __popc(mask & lanes_below);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j)
@@ -344,30 +349,38 @@ __device__ void group_tokens(const SortArgs& a, SortShared& S, uint32_t& begin, 
     return total;
   };
   scan_ids(a, warp, lane, [&](const uint32_t (&id)[4], int64_t i) {
+    bool is_mine[4];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      valid += id[j] < a.vocab;
-      lower += id[j] < a.vocab && (id[j] & (kOwners - 1)) < owner;
+      const uint32_t of = id[j] < a.vocab ? id[j] & (kOwners - 1) : uint32_t(kOwners);
+      lower += of < owner;
+      is_mine[j] = of == owner;
     }
-    mine += take(id, i, S.list[warp] + mine, mine < kListRoom ? kListRoom - mine : 0u);
+    if (__any_sync(0xFFFFFFFFu, is_mine[0] | is_mine[1] | is_mine[2] | is_mine[3]))
+      mine += take(id, is_mine, i, S.list[warp] + mine, mine < kListRoom ? kListRoom - mine : 0u);
   });
   lower = __reduce_add_sync(0xFFFFFFFFu, lower);
-  valid = __reduce_add_sync(0xFFFFFFFFu, valid);
-  if (lane == 0) S.lower[warp] = lower, S.mine[warp] = mine, S.valid[warp] = valid;
+  if (lane == 0) S.lower[warp] = lower, S.mine[warp] = mine;
   const bool listed = !__syncthreads_or(mine > kListRoom);
-  uint32_t at, all;
-  over_warps(S.valid, warp, at, all);
-  over_warps(S.lower, warp, at, begin);
-  over_warps(S.mine, warp, at, count);
-  uint2* const last = a.passes & 1 ? a.tokens1 : a.tokens0;
-  for (int64_t i = int64_t(all) + int64_t(owner) * kSortThreads + tid; i < a.n; i += int64_t(kOwners) * kSortThreads) {
-    last[i] = make_uint2(kNoId, 0u);
-    if (i + 1 == a.n || ((i + 1) & ((1 << a.block_log2) - 1)) == 0) a.long_sums[i >> a.block_log2] = LongSum{kNoId, 0u};
+  uint32_t at;
+  over_warps(S.lower, warp, lane, at, begin);
+  over_warps(S.mine, warp, lane, at, count);
+  if (owner == kOwners - 1) {  // behind the last share
+    uint2* const last = a.passes & 1 ? a.tokens1 : a.tokens0;
+    for (int64_t i = int64_t(begin) + count + tid; i < a.n; i += kSortThreads) {
+      last[i] = make_uint2(kNoId, 0u);
+      if (i + 1 == a.n || ((i + 1) & ((1 << a.block_log2) - 1)) == 0) a.long_sums[i >> a.block_log2] = LongSum{kNoId, 0u};
+    }
   }
   if (count == 0) return;
   if (!listed) {
     uint2* to = a.tokens0 + begin + at;
-    scan_ids(a, warp, lane, [&](const uint32_t (&id)[4], int64_t i) { to += take(id, i, to, 128u); });
+    scan_ids(a, warp, lane, [&](const uint32_t (&id)[4], int64_t i) {
+      bool is_mine[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) is_mine[j] = id[j] < a.vocab && (id[j] & (kOwners - 1)) == owner;
+      to += take(id, is_mine, i, to, 128u);
+    });
     __syncthreads();
   }
   const uint32_t stretch = (count + kSortThreads - 1) / kSortThreads * 32, first = min(count, warp * stretch), some = min(count - first, stretch);
@@ -428,16 +441,17 @@ k_embed_grad_sort(const SortArgs a, T* __restrict__ grad_table, int dim, int64_t
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   for (int64_t r0 = 0; r0 < rows; r0 += kAtOnce) {
     const int here = int(min(int64_t(kAtOnce), rows - r0));
+    __syncthreads();
     for (int w = threadIdx.x; w < (here + 31) / 32; w += kSortThreads) used[w] = 0;
     __syncthreads();
+#pragma unroll 4
     for (uint32_t i = threadIdx.x; i < count; i += kSortThreads) {
       const int64_t r = int64_t(tokens[i].x >> kOwnersLog2) - r0;
-      if (r >= 0 && r < here && (i == 0 || tokens[i - 1].x != tokens[i].x)) atomicOr(used + (r >> 5), 1u << (r & 31));
+      if (r >= 0 && r < here && !(used[r >> 5] >> (r & 31) & 1u)) atomicOr(used + (r >> 5), 1u << (r & 31));
     }
     __syncthreads();
     for (int r = warp; r < here; r += kSortWarps)
       if (!(used[r >> 5] >> (r & 31) & 1u)) clear_row(grad_table + (((r0 + r) << kOwnersLog2) + blockIdx.x) * table_stride, dim, lane, 32);
-    __syncthreads();
   }
 }
 
@@ -563,6 +577,7 @@ __global__ void __launch_bounds__(kGradThreads) k_embed_grad_sums(const GradArgs
   uint64_t* address       = reinterpret_cast<uint64_t*>(base + shared.ring);
   uint32_t* ids           = reinterpret_cast<uint32_t*>(address + shared.tokens);
   // the columns: `width` from `first` on
+  gtk::await_kernel();
   const int slab  = (ALIGNED ? group : group - 1) * E;
   const int first = blockIdx.y * slab, width = min(slab, a.dim - first);
   // the tokens of this block and the next, and one at either end of the block in front
@@ -724,8 +739,9 @@ __global__ void __launch_bounds__(kGradThreads) k_embed_grad_sums(const GradArgs
   else finish(id);
 }
 
-// The parts of a long sum, 128 columns at a time: each warp adds a run of parts, then the warps' sums are added in order.
-constexpr int kJoinThreads = 128;
+// The parts of long sums, 128 columns at a time: a warp per sum; those of more than kJoinAlone parts are all warps' work, each adds
+// a run of parts, then the warps' sums are added in order.
+constexpr int kJoinThreads = 128, kJoinBlocks = 16, kJoinAlone = 32;
 template <class T>
 __global__ void __launch_bounds__(kJoinThreads) k_embed_grad_join(const GradArgs a, T* __restrict__ grad_table, bool packs)
 {
@@ -733,34 +749,53 @@ __global__ void __launch_bounds__(kJoinThreads) k_embed_grad_join(const GradArgs
   __shared__ float4 s_sum[kWarps][32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int c         = blockIdx.y * 128 + lane * 4;
-  const int64_t first = int64_t(blockIdx.x) * 32, blocks = (a.n + (int64_t(1) << a.block_log2) - 1) >> a.block_log2;
+  const int64_t first = int64_t(blockIdx.x) * kJoinBlocks, blocks = (a.n + (int64_t(1) << a.block_log2) - 1) >> a.block_log2;
+  gtk::await_kernel();
   LongSum mine{kNoId, 0u};
-  if (first + lane < blocks) mine = a.long_sums[first + lane];
-  for (uint32_t some = __ballot_sync(0xFFFFFFFFu, mine.parts > 0); some; some &= some - 1) {  // the same for every warp
-    const int at = __ffs(some) - 1;
-    LongSum L;
-    L.id                = __shfl_sync(0xFFFFFFFFu, mine.id, at);
-    L.parts             = __shfl_sync(0xFFFFFFFFu, mine.parts, at);
-    const uint32_t each = (L.parts + kWarps - 1) / kWarps, from = min(L.parts, warp * each), to = min(L.parts, from + each);
-    const float* part   = a.parts + (first + at) * 2 * a.pitch + c;
-    float4 sum          = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (c < a.dim) {
-#pragma unroll 8
-      for (uint32_t i = from; i < to; ++i) {  // part 0 is the one that begins in the block
-        const float4 x = *reinterpret_cast<const float4*>(part + (2 * int64_t(i) + (i == 0 ? 1 : 0)) * a.pitch);
-        sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
+  if (lane < kJoinBlocks && first + lane < blocks) mine = a.long_sums[first + lane];
+  auto add_parts = [&](int at, uint32_t from, uint32_t to) {  // part 0 is the one that begins in the block
+    const float* part = a.parts + (first + at) * 2 * a.pitch + c;
+    float4 sum        = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (c < a.dim)
+      for (uint32_t i0 = from; i0 < to; i0 += 8) {
+        float4 x[8];
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k) {
+          const uint32_t i = min(i0 + k, to - 1);
+          x[k]             = __ldcg(reinterpret_cast<const float4*>(part + (2 * int64_t(i) + (i == 0 ? 1 : 0)) * a.pitch));
+        }
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k)
+          if (i0 + k < to) sum.x += x[k].x, sum.y += x[k].y, sum.z += x[k].z, sum.w += x[k].w;
       }
-    }
-    s_sum[warp][lane] = sum;
+    return sum;
+  };
+  auto store = [&](uint32_t id, const float4& sum) {
+    const float y[4] = {sum.x, sum.y, sum.z, sum.w};
+    if (c < a.dim) store_sum<T, 4>(grad_table + int64_t(id) * a.table_stride + c, a.dim - c, packs, a.scale, a.accumulate, y);
+  };
+  // the same for every warp
+  const uint32_t few = __ballot_sync(0xFFFFFFFFu, mine.parts > 0 && mine.parts <= kJoinAlone), many = __ballot_sync(0xFFFFFFFFu, mine.parts > kJoinAlone);
+  int turn = 0;
+  for (uint32_t some = few; some; some &= some - 1, ++turn) {
+    const int at         = __ffs(some) - 1;
+    const uint32_t id    = __shfl_sync(0xFFFFFFFFu, mine.id, at), parts = __shfl_sync(0xFFFFFFFFu, mine.parts, at);
+    if (turn % kWarps == warp) store(id, add_parts(at, 0, parts));
+  }
+  for (uint32_t some = many; some; some &= some - 1) {
+    const int at        = __ffs(some) - 1;
+    const uint32_t id   = __shfl_sync(0xFFFFFFFFu, mine.id, at), parts = __shfl_sync(0xFFFFFFFFu, mine.parts, at);
+    const uint32_t each = (parts + kWarps - 1) / kWarps, from = min(parts, warp * each);
+    float4 sum          = add_parts(at, from, min(parts, from + each));
+    s_sum[warp][lane]   = sum;
     __syncthreads();
-    if (warp == 0 && c < a.dim) {
+    if (warp == 0) {
 #pragma unroll
       for (int w = 1; w < kWarps; ++w) {
         const float4 x = s_sum[w][lane];
         sum.x += x.x, sum.y += x.y, sum.z += x.z, sum.w += x.w;
       }
-      const float y[4] = {sum.x, sum.y, sum.z, sum.w};
-      store_sum<T, 4>(grad_table + int64_t(L.id) * a.table_stride + c, a.dim - c, packs, a.scale, a.accumulate, y);
+      store(id, sum);
     }
     __syncthreads();
   }
@@ -777,20 +812,20 @@ cudaError_t launch_embed_grad(const gtk::HandleView& v, const GradPlan& p, GradA
                               a.table_stride, !a.accumulate);
   if (e != cudaSuccess || n == 0) return e;
   a.tokens = p.passes & 1 ? s.tokens1 : s.tokens0;
-  // threads of a group: a power of two below a warp when each has 16 bytes of its own; else whole warps, a CTA's at most
+  // threads of a group: a power of two from 8 on below a warp when each has 16 bytes of its own; else whole warps, a CTA's at most
   constexpr int E      = 16 / int(sizeof(O));
   const int64_t wanted = (a.dim + E - 1) / E + (ALIGNED ? 0 : 1);
   unsigned group = unsigned(std::min<int64_t>(kGradThreads, (wanted + 31) / 32 * 32));
-  while (ALIGNED && group <= 32 && group / 2 >= wanted) group /= 2;
+  while (ALIGNED && group <= 32 && group > 8 && group / 2 >= wanted) group /= 2;
   const unsigned columns = (ALIGNED ? group : group - 1) * E, slabs = unsigned((a.dim + columns - 1) / columns);
   const size_t bytes     = size_t(GroupShared(int(group), 1 << a.block_log2).bytes());
   unsigned groups = group > 32 ? 1 : 128 / group;
-  while (groups > 1 && groups * bytes > kSharedMost) groups /= 2;
-  e = gtk::launch(k_embed_grad_sums<O, T, ALIGNED>, dim3(unsigned((p.blocks + groups - 1) / groups), slabs), dim3(group, groups), groups * bytes,
+  while (groups * group > 32 && groups > 1 && groups * bytes > kSharedMost) groups /= 2;
+  e = gtk::launch_behind(k_embed_grad_sums<O, T, ALIGNED>, dim3(unsigned((p.blocks + groups - 1) / groups), slabs), dim3(group, groups), groups * bytes,
                   v.stream, a, static_cast<const O*>(grad_out), table);
   if (e == cudaSuccess && p.blocks > 2)  // a long sum begins in one block, fills the next and goes on
-    e = gtk::launch(k_embed_grad_join<T>, dim3(unsigned((p.blocks + 31) / 32), unsigned((a.dim + 127) / 128)), dim3(kJoinThreads), 0, v.stream, a,
-                    table, ALIGNED);
+    e = gtk::launch_behind(k_embed_grad_join<T>, dim3(unsigned((p.blocks + kJoinBlocks - 1) / kJoinBlocks), unsigned((a.dim + 127) / 128)),
+                    dim3(kJoinThreads), 0, v.stream, a, table, ALIGNED);
   return e;
 }
 

@@ -41,6 +41,9 @@ __device__ __forceinline__ Pack<T, V> load_pack(const T* p) { return *reinterpre
 template <class T, int V>
 __device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& v) { *reinterpret_cast<Pack<T, V>*>(p) = v; }
 
+// Everything that the kernels in front of this one in the stream have written is there afterwards (gtk::launch_behind).
+__device__ __forceinline__ void await_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // Copies of 16 bytes to shared memory that a thread does not wait for: begun, closed as a chunk, and awaited until at most PENDING of
 // its own chunks are under way.
 __device__ __forceinline__ void copy16(uint32_t shared_at, const void* from)
@@ -112,6 +115,24 @@ cudaError_t launch(void (*kernel)(Formal...), dim3 grid, dim3 block, size_t smem
 {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid, cfg.blockDim = block, cfg.dynamicSmemBytes = smem, cfg.stream = stream;
+  if (smem > (48 << 10)) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
+    if (e != cudaSuccess) return e;
+  }
+  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Formal>(args)...);
+}
+
+// the same for a kernel that begins with await_kernel(): its blocks may take their places while the kernel in front of it
+// in the stream is still ending
+template <class... Formal, class... Args>
+cudaError_t launch_behind(void (*kernel)(Formal...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args&&... args)
+{
+  cudaLaunchAttribute attr{};
+  attr.id                                         = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid, cfg.blockDim = block, cfg.dynamicSmemBytes = smem, cfg.stream = stream;
+  cfg.attrs = &attr, cfg.numAttrs = 1;
   if (smem > (48 << 10)) {
     const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
     if (e != cudaSuccess) return e;
