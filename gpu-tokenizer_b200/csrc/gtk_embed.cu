@@ -1,7 +1,6 @@
 // gtk_embed.cu -- embedding lookup with scaling, and its gradient by sorted tokens.
 #include <algorithm>
 #include <cmath>
-#include <cstdlib>
 
 #include "gtk_rows.cuh"
 
@@ -174,7 +173,7 @@ int bits_of(int64_t x)
 }
 
 constexpr size_t kSharedMost = 96 << 10;  // of a CTA
-constexpr int kMinBlockLog2 = 3, kMaxBlockLog2 = 9;
+constexpr int kMinBlockLog2 = 3, kMaxBlockLog2 = 10;
 
 GradPlan grad_plan(int64_t n, int64_t vocab, int64_t dim)
 {
@@ -183,9 +182,11 @@ GradPlan grad_plan(int64_t n, int64_t vocab, int64_t dim)
   p.passes       = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
   p.digit_bits   = (bits + p.passes - 1) / p.passes;
   p.block_log2   = kMinBlockLog2;
-  // blocks as long as still leaves about 1.5 M columns of them: a dozen row groups of 768 columns per SM
-  while (p.block_log2 < kMaxBlockLog2 && (n >> (p.block_log2 + 1)) * dim >= int64_t(3) << 19) ++p.block_log2;
-  if (getenv("GTK_BL")) p.block_log2 = atoi(getenv("GTK_BL"));
+  // Blocks of up to 64 tokens: as long as they leave some 600 000 columns of blocks, so that all SMs have work, and longer where there
+  // were more than 4096 of them, for the parts of the most frequent id's sum are added one after the other.  Longer
+  // ones only where the parts would take more than 32 MiB.
+  while (p.block_log2 < 6 && ((n >> (p.block_log2 + 1)) * dim >= 600000 || n >> p.block_log2 > 4096)) ++p.block_log2;
+  while (p.block_log2 < kMaxBlockLog2 && (n >> p.block_log2) * dim * 8 > (int64_t(32) << 20)) ++p.block_log2;
   p.blocks    = (n + (int64_t(1) << p.block_log2) - 1) >> p.block_log2;
   p.pitch     = (dim + 7) / 8 * 8;
   size_t at   = 0;
@@ -296,8 +297,8 @@ __device__ void sort_digit(const uint2* from, uint32_t count, uint2* to, int shi
   __syncthreads();
 }
 
-// f(is_mine[4], id[4], place of the first, lanes with any) for the ids of the warp's part, four per lane at a time.  Ids in front of the
-// array and behind it, which share 16 bytes with its ends, are nobody's.
+// f(id[4], place of the first) for the ids of the warp's part, four per lane at a time.  Ids in front of the array and behind
+// it, which share 16 bytes with its ends, are kNoId.
 template <class F>
 __device__ __forceinline__ void scan_ids(const SortArgs& a, int warp, int lane, F&& f)
 {
@@ -310,11 +311,12 @@ __device__ __forceinline__ void scan_ids(const SortArgs& a, int warp, int lane, 
     uint4 x[kAhead];
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) x[k] = q0 + k * 32 + lane < last ? __ldg(quads + q0 + k * 32 + lane) : make_uint4(kNoId, kNoId, kNoId, kNoId);
+    const bool edge = q0 * 4 < skip || (q0 + 32 * kAhead) * 4 - skip > a.n;  // the same for the warp
 #pragma unroll
     for (int k = 0; k < kAhead; ++k) {
       const int64_t i = (q0 + k * 32 + lane) * 4 - skip;
       uint32_t id[4]  = {x[k].x, x[k].y, x[k].z, x[k].w};
-      if (i < 0 || i + 4 > a.n)
+      if (edge)
 #pragma unroll
         for (int j = 0; j < 4; ++j)
           if (i + j < 0 || i + j >= a.n) id[j] = kNoId;
@@ -323,6 +325,22 @@ __device__ __forceinline__ void scan_ids(const SortArgs& a, int warp, int lane, 
   }
 }
 
+// Four ids' owners in the bytes of a word (those that take no part count as the last one's), and from them, as bit 7 of each
+// byte, whose owner is lower or this one: bytes below 128 neither borrow from nor carry into their neighbours here.
+struct Owners {
+  uint32_t of;
+  __device__ __forceinline__ Owners(const uint32_t (&id)[4], uint32_t vocab)
+  {
+    uint32_t x[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) x[j] = id[j] < vocab ? id[j] : uint32_t(kOwners - 1);
+    of = __byte_perm(__byte_perm(x[0], x[1], 0x0040), __byte_perm(x[2], x[3], 0x0040), 0x5410) & 0x7F7F7F7Fu;
+  }
+  __device__ __forceinline__ uint32_t below(uint32_t owner4) const { return ~((of | 0x80808080u) - owner4) & 0x80808080u; }
+  __device__ __forceinline__ uint32_t equal(uint32_t owner4) const { return ~((of ^ owner4) + 0x7F7F7F7Fu) & 0x80808080u; }
+};
+static_assert(kOwners == 128, "an owner is seven bits of a byte");
+
 // CTA c owns the ids with id % kOwners == c: it looks at all ids, learns how many tokens lower owners have, which is where
 // its own go, and sorts its own.  Nothing is waited for between CTAs.  Returns its share of the grouped tokens; behind the
 // last share are tokens of no id.
@@ -330,34 +348,42 @@ __device__ void group_tokens(const SortArgs& a, SortShared& S, uint32_t& begin, 
 {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const uint32_t owner = blockIdx.x, lanes_below = (1u << lane) - 1u;
+  const uint32_t owner4 = owner * 0x01010101u;
   uint32_t lower = 0, mine = 0;
-  // the tokens of one step to to[], in order; returns how many
-  auto take = [&](const uint32_t (&id)[4], const bool (&is_mine)[4], int64_t i, uint2* to, uint32_t room) {
+  // The tokens of one step that are this owner's to to[], in order; returns how many.
+  auto take = [&](const uint32_t (&id)[4], const Owners& o, int64_t i, uint2* to, uint32_t room) {
+    uint32_t bits = o.equal(owner4);
+    if (owner == kOwners - 1)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (id[j] >= a.vocab) bits &= ~(0x80u << 8 * j);
+    const uint32_t lanes = __ballot_sync(0xFFFFFFFFu, bits != 0);
+    if (!lanes) return 0u;
+    if (!__any_sync(0xFFFFFFFFu, bits & (bits - 1))) {  // one per lane at most
+      const uint32_t at = __popc(lanes & lanes_below);
+      const int j       = __clz(__brev(bits)) >> 3;
+      if (bits && at < room) to[at] = make_uint2(j == 0 ? id[0] : j == 1 ? id[1] : j == 2 ? id[2] : id[3], uint32_t(i + j));
+      return uint32_t(__popc(lanes));
+    }
     uint32_t total = 0, at = 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const uint32_t mask = __ballot_sync(0xFFFFFFFFu, is_mine[j]);
+      const uint32_t mask = __ballot_sync(0xFFFFFFFFu, bits >> (8 * j + 7) & 1u);
       total += __popc(mask);
       at += __popc(mask & lanes_below);
     }
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (is_mine[j]) {
+      if (bits >> (8 * j + 7) & 1u) {
         if (at < room) to[at] = make_uint2(id[j], uint32_t(i + j));
         ++at;
       }
     return total;
   };
   scan_ids(a, warp, lane, [&](const uint32_t (&id)[4], int64_t i) {
-    bool is_mine[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t of = id[j] < a.vocab ? id[j] & (kOwners - 1) : uint32_t(kOwners);
-      lower += of < owner;
-      is_mine[j] = of == owner;
-    }
-    if (__any_sync(0xFFFFFFFFu, is_mine[0] | is_mine[1] | is_mine[2] | is_mine[3]))
-      mine += take(id, is_mine, i, S.list[warp] + mine, mine < kListRoom ? kListRoom - mine : 0u);
+    const Owners o(id, a.vocab);
+    lower += __popc(o.below(owner4));
+    mine += take(id, o, i, S.list[warp] + mine, mine < kListRoom ? kListRoom - mine : 0u);
   });
   lower = __reduce_add_sync(0xFFFFFFFFu, lower);
   if (lane == 0) S.lower[warp] = lower, S.mine[warp] = mine;
@@ -375,12 +401,7 @@ __device__ void group_tokens(const SortArgs& a, SortShared& S, uint32_t& begin, 
   if (count == 0) return;
   if (!listed) {
     uint2* to = a.tokens0 + begin + at;
-    scan_ids(a, warp, lane, [&](const uint32_t (&id)[4], int64_t i) {
-      bool is_mine[4];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) is_mine[j] = id[j] < a.vocab && (id[j] & (kOwners - 1)) == owner;
-      to += take(id, is_mine, i, to, 128u);
-    });
+    scan_ids(a, warp, lane, [&](const uint32_t (&id)[4], int64_t i) { to += take(id, Owners(id, a.vocab), i, to, 128u); });
     __syncthreads();
   }
   const uint32_t stretch = (count + kSortThreads - 1) / kSortThreads * 32, first = min(count, warp * stretch), some = min(count - first, stretch);
@@ -415,7 +436,7 @@ k_embed_grad_sort(const SortArgs a, T* __restrict__ grad_table, int dim, int64_t
   const uint2* tokens = (a.passes & 1 ? a.tokens1 : a.tokens0) + begin;
   // the blocks whose last token is this owner's: the sum that it belongs to is long when it reaches over the next boundary
   // too, and begins in the block or further left
-  const int64_t length = int64_t(1) << a.block_log2, end = int64_t(begin) + count;
+  const int64_t end = int64_t(begin) + count;
   for (int64_t block = (begin >> a.block_log2) + threadIdx.x; block << a.block_log2 < end; block += kSortThreads) {
     const int64_t last = min(((block + 1) << a.block_log2), a.n) - 1, third = (block + 2) << a.block_log2;
     if (last >= end) continue;
@@ -486,7 +507,7 @@ struct GradArgs {
   float* parts;  // [blocks][2][pitch]: of the long sum that begins further left, of the one that begins in the block
 };
 
-constexpr int kChunk = 4, kChunks = 4;  // rows that are waited for together, and such chunks in flight
+constexpr int kChunk = 4, kChunks = 3;  // rows that are waited for together, and such chunks in flight
 
 // first place in [from, to) whose id is not `id` (where one id follows another it does not come back)
 __device__ __forceinline__ int end_of_id(const uint32_t* ids, int from, int to, uint32_t id)
@@ -741,7 +762,7 @@ __global__ void __launch_bounds__(kGradThreads) k_embed_grad_sums(const GradArgs
 
 // The parts of long sums, 128 columns at a time: a warp per sum; those of more than kJoinAlone parts are all warps' work, each adds
 // a run of parts, then the warps' sums are added in order.
-constexpr int kJoinThreads = 128, kJoinBlocks = 16, kJoinAlone = 32;
+constexpr int kJoinThreads = 256, kJoinBlocks = 16, kJoinAlone = 32;
 template <class T>
 __global__ void __launch_bounds__(kJoinThreads) k_embed_grad_join(const GradArgs a, T* __restrict__ grad_table, bool packs)
 {
