@@ -689,35 +689,27 @@ __global__ void __launch_bounds__(kGradThreads) k_embed_grad_sums(const GradArgs
     T* row           = grad_table + int64_t(id) * a.table_stride + first + own;
     const bool packs = ALIGNED || reinterpret_cast<uintptr_t>(row) % (sizeof(T) * S::kUnit) == 0;
     float x[S::kCount];
-    const Two scale(a.scale, a.scale);
+    if (whole == (1u << S::kUnits) - 1u && !a.accumulate) {  // nearly all threads, nearly always
+      const Two scale(a.scale, a.scale);
 #pragma unroll
-    for (int j = 0; j < S::kCount / 2; ++j) (sum[j] * scale).get(x[2 * j], x[2 * j + 1]);
+      for (int j = 0; j < S::kCount / 2; ++j) (sum[j] * scale).get(x[2 * j], x[2 * j + 1]);
 #pragma unroll
-    for (int u = 0; u < S::kUnits; ++u) {
-      T* unit = row + u * kStep * S::kUnit;
-      if (packs && (whole >> u & 1u)) {
+      for (int u = 0; u < S::kUnits; ++u) {
+        T* unit = row + u * kStep * S::kUnit;
         Pack<T, S::kUnit> y;
-        if (a.accumulate) {
-          const Pack<T, S::kUnit> old = gtk::load_pack<T, S::kUnit>(unit);
-          float z[S::kCount];
-#pragma unroll
-          for (int j = 0; j < S::kCount / 2; ++j) sum[j].get(z[2 * j], z[2 * j + 1]);
-#pragma unroll
-          for (int j = 0; j < S::kUnit; ++j) x[u * S::kUnit + j] = fmaf(z[u * S::kUnit + j], a.scale, gtk::to_float(old.e[j]));
-        }
 #pragma unroll
         for (int j = 0; j < S::kUnit; ++j) y.e[j] = gtk::from_float<T>(x[u * S::kUnit + j]);
-        gtk::store_pack<T, S::kUnit>(unit, y);
-      } else {
-        float z[S::kCount];
+        if (packs) gtk::store_pack<T, S::kUnit>(unit, y);
+        else
 #pragma unroll
-        for (int j = 0; j < S::kCount / 2; ++j) sum[j].get(z[2 * j], z[2 * j + 1]);
-        const int here = whole >> u & 1u ? S::kUnit : some >> u & 1u ? (ALIGNED ? valid(u) : 1) : 0;
-#pragma unroll
-        for (int j = 0; j < S::kUnit; ++j)
-          if (j < here) unit[j] = gtk::from_float<T>(a.accumulate ? fmaf(z[u * S::kUnit + j], a.scale, gtk::to_float(unit[j])) : x[u * S::kUnit + j]);
+          for (int j = 0; j < S::kUnit; ++j) unit[j] = y.e[j];
       }
+      return;
     }
+#pragma unroll
+    for (int j = 0; j < S::kCount / 2; ++j) sum[j].get(x[2 * j], x[2 * j + 1]);
+#pragma unroll
+    for (int u = 0; u < S::kUnits; ++u) store_sum<T, S::kUnit>(row + u * kStep * S::kUnit, valid(u), packs, a.scale, a.accumulate, x + u * S::kUnit);
   };
   int chunk = at / kChunk;
 #pragma unroll
