@@ -153,7 +153,7 @@ constexpr int kMaxDigitBits = 9;                            // a thread per bin 
 constexpr int64_t kMaxDim = int64_t(1) << 20;
 
 // Of a block of tokens: the long sum that begins in it, and in how many blocks that has a part; parts == 0: none.
-struct LongSum {
+struct alignas(8) LongSum {
   uint32_t id, parts;
 };
 
@@ -604,10 +604,10 @@ __global__ void __launch_bounds__(kGradThreads) k_embed_grad_sums(const GradArgs
   // the tokens of this block and the next, and one at either end of the block in front
   const int64_t block = int64_t(blockIdx.x) * blockDim.y + threadIdx.y;
   const int64_t begin = block << a.block_log2;
-  const uint32_t left = begin > 0 && begin < a.n ? __ldg(&a.tokens[begin - 1].x) : kNoId;
-  const uint32_t far_left = begin > length && begin < a.n ? __ldg(&a.tokens[begin - length - 1].x) : kNoId;
+  const uint32_t left = begin > 0 && begin < a.n ? __ldcg(&a.tokens[begin - 1].x) : kNoId;
+  const uint32_t far_left = begin > length && begin < a.n ? __ldcg(&a.tokens[begin - length - 1].x) : kNoId;
   for (int i = lane; i < shared.tokens; i += group) {
-    const uint2 token = begin + i < a.n ? __ldg(a.tokens + begin + i) : make_uint2(kNoId, 0u);
+    const uint2 token = begin + i < a.n ? __ldcg(a.tokens + begin + i) : make_uint2(kNoId, 0u);
     ids[i]     = token.x;
     address[i] = reinterpret_cast<uint64_t>(grad_out + first + int64_t(token.y) * a.out_stride);
   }
@@ -765,7 +765,10 @@ __global__ void __launch_bounds__(kJoinThreads) k_embed_grad_join(const GradArgs
   const int64_t first = int64_t(blockIdx.x) * kJoinBlocks, blocks = (a.n + (int64_t(1) << a.block_log2) - 1) >> a.block_log2;
   gtk::await_kernel();
   LongSum mine{kNoId, 0u};
-  if (lane < kJoinBlocks && first + lane < blocks) mine = a.long_sums[first + lane];
+  if (lane < kJoinBlocks && first + lane < blocks) {
+    const uint2 x = __ldcg(reinterpret_cast<const uint2*>(a.long_sums + first + lane));
+    mine          = LongSum{x.x, x.y};
+  }
   auto add_parts = [&](int at, uint32_t from, uint32_t to) {  // part 0 is the one that begins in the block
     const float* part = a.parts + (first + at) * 2 * a.pitch + c;
     float4 sum        = make_float4(0.f, 0.f, 0.f, 0.f);

@@ -41,7 +41,8 @@ __device__ __forceinline__ Pack<T, V> load_pack(const T* p) { return *reinterpre
 template <class T, int V>
 __device__ __forceinline__ void store_pack(T* p, const Pack<T, V>& v) { *reinterpret_cast<Pack<T, V>*>(p) = v; }
 
-// Everything that the kernels in front of this one in the stream have written is there afterwards (gtk::launch_behind).
+// Everything that the kernels in front of this one in the stream have written is there afterwards (gtk::launch_behind).  It is
+// read with loads that the compiler leaves behind this one and that the first-level cache has no part in (__ldcg, not __ldg).
 __device__ __forceinline__ void await_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Copies of 16 bytes to shared memory that a thread does not wait for: begun, closed as a chunk, and awaited until at most PENDING of

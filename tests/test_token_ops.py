@@ -742,3 +742,91 @@ def test_offsets_beyond_32_bits(tok):
     tok.token_logprobs_grad(view.data_ptr(), "bf16", vocab, dim, targets.data_ptr(), lse.data_ptr(), ones.data_ptr(), view.data_ptr(),
                             stride=stride, grad_stride=stride)
     same(view, want, bound + 2.0 ** -20 + want.abs() * half_step("bf16") * 1.01, "in place")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shift", [0, 1, 2, 3])
+@pytest.mark.parametrize("n", [1, 2, 3, 4, 5, 127, 1023, 1025, 70001])
+def test_ids_at_any_address(tok, n, shift):
+    """The ids are read sixteen bytes at a time: first and last ones that share these with strangers."""
+    import torch
+
+    vocab, dim = 500, 12
+    whole = torch.full((n + 16,), 3, device="cuda", dtype=torch.int32)   # strangers that would be ids
+    ids = whole[shift + 4:shift + 4 + n]
+    ids.copy_(some_ids(n, n, vocab, "padded"))
+    grad = torch.randn(n, dim, device="cuda")
+    table = torch.empty(vocab, dim, device="cuda")
+    embed_grad(tok, ids, grad, "f32", vocab, dim, table, "f32")
+    check_embed_grad(ids, grad, vocab, dim, 1.0, None, table, "f32")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim", [24, 23, 136])
+@pytest.mark.parametrize("n", [700, 5000, 40000, 150000])
+def test_sums_of_every_length(tok, n, dim):
+    """Ids that occur once, twice, .. and the rest on one id, so that sums begin and end at all places of the blocks that the
+    tokens are dealt with in."""
+    import torch
+
+    counts, left = [], n
+    while left > 0:
+        counts.append(min(left, 1 + len(counts) % 150))
+        left -= counts[-1]
+    vocab = len(counts) + 200
+    g = torch.Generator().manual_seed(n)
+    ids = torch.repeat_interleave(torch.randperm(vocab, generator=g)[:len(counts)], torch.tensor(counts))
+    ids = ids[torch.randperm(n, generator=g)].to(torch.int32).cuda()
+    for name in ("f32", "bf16"):
+        _, grad = rows(torch.randn(n, dim, device="cuda"), name)
+        table = torch.empty(vocab, dim, device="cuda")
+        embed_grad(tok, ids, grad, name, vocab, dim, table, "f32")
+        check_embed_grad(ids, grad, vocab, dim, 1.0, None, table, "f32")
+        base = table.clone()
+        embed_grad(tok, ids, grad, name, vocab, dim, table, "f32", accumulate=True)
+        check_embed_grad(ids, grad, vocab, dim, 1.0, base, table, "f32")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("n,vocab,stride,shift,kind", [
+    (800, 9001, 9001, 0, "masked"), (1500, 7001, 7001, 1, "ties"), (900, 12288, 12288, 0, "crowded"), (2000, 100, 104, 0, "masked"),
+    (760, 20011, 20016, 0, "lowest"), (30, 70001, 70001, 0, "rising"), (64, 100003, 100003, 1, "ties"), (12, 131072, 131072, 0, "crowded"),
+])
+def test_token_logprobs_of_other_shapes(tok, name, n, vocab, stride, shift, kind):
+    """More rows than a wave of CTAs, and rows that several CTAs share, against the same bounds."""
+    import torch
+
+    _, x = rows(some_logits(n + vocab, n, vocab, kind), name, stride, shift)
+    if kind == "lowest":
+        x[x == torch.tensor(-65504.0).to(dtype(name)).item()] = torch.finfo(dtype(name)).min
+    targets = some_ids(vocab, n, vocab, "wrong")
+    for k in (0, 3, 32):
+        lp, H, lse, ids, tops = score(tok, x, name, targets, k, 1.0, stride)
+        w_lp, w_H, w_lse, w_ids, w_tops = score_wanted(x, targets, k, 1.0)
+        assert torch.equal(ids.long(), w_ids), k
+        same(lse, *w_lse, "lse")
+        same(lp, *w_lp, "logprob")
+        same(H, *w_H, "entropy")
+        same(tops, *w_tops, "top")
+
+
+@pytest.mark.gpu
+def test_the_same_bits_every_time(tok):
+    import torch
+
+    n, vocab, dim = 30000, 20000, 200
+    ids = some_ids(3, n, vocab, "padded")
+    grad = torch.randn(n, dim, device="cuda")
+    first = None
+    for _ in range(4):
+        table = torch.empty(vocab, dim, device="cuda")
+        embed_grad(tok, ids, grad, "f32", vocab, dim, table, "f32")
+        first = table if first is None else first
+        assert torch.equal(first, table)
+    x = some_logits(9, 300, vocab, "ties")
+    targets = some_ids(9, 300, vocab, "text")
+    want = score(tok, x, "f32", targets, 20, 0.7, vocab)
+    for _ in range(4):
+        for a, b in zip(want, score(tok, x, "f32", targets, 20, 0.7, vocab)):
+            assert torch.equal(a, b)
