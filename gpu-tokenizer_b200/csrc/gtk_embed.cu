@@ -125,13 +125,15 @@ template <class T, class O, int V>
 cudaError_t launch_embed(const gtk::HandleView& v, const int32_t* ids, int64_t n, const void* table, int64_t vocab, int64_t dim,
                          int64_t table_stride, float scale, void* out, int64_t out_stride)
 {
-  // Few rows: a thread for every unit of a row.  Many: a quarter as many and two rows at once when they are packs (32768 rows of 1024
-  // bf16: 18.1 us, one row at once 19.0, four 24.8; 100000 rows of 256: 14.8, with a lane for every pack 34.4), a warp and one
-  // row when they are pairs (30000 rows of 1601 bf16: 43 us, two rows at once 49).
+  // Lanes for a row: a quarter as many as it has units, a warp at most; more, up to one per unit, while that keeps the GPU's threads
+  // from being used up (2048 rows of 1024 bf16: 2.5 us with 32 lanes, 3.3 with 128; 64 rows of 768: 2.1 and 1.9).  Many rows
+  // of packs go two at once (32768 rows of 1024 bf16: 18.1 us, one at once 19.0, four 24.8; 100000 rows of 256: 14.8, with a lane
+  // for every pack 34.4), of pairs one (30000 rows of 1601 bf16: 43 us, two 49).
   const int64_t units = (dim + (V == 8 ? 7 : 1)) / V;
   const bool many     = n >= int64_t(v.sm_count) * 64;
   int group_log2      = 0;
-  while (group_log2 < (many ? 5 : 8) && (int64_t(many ? 4 : 1) << group_log2) < units) ++group_log2;
+  while (group_log2 < 5 && (int64_t(4) << group_log2) < units) ++group_log2;
+  while (group_log2 < 8 && (int64_t(1) << group_log2) < units && n << (group_log2 + 1) <= int64_t(v.sm_count) * 512) ++group_log2;
   const int64_t rows = (kEmbedThreads >> group_log2) * (many && V == 8 ? 2 : 1);
   return gtk::launch(many && V == 8 ? k_embed<T, O, V, 2> : k_embed<T, O, V, 1>, dim3(unsigned((n + rows - 1) / rows)), dim3(kEmbedThreads), 0,
                      v.stream, ids, n, static_cast<const T*>(table), int(vocab), int(dim), table_stride, scale, static_cast<O*>(out), out_stride,
