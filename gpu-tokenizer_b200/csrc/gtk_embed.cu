@@ -12,7 +12,9 @@ using gtk::Two;
 // ------------------------------------------------------------------------------------------------ lookup
 // out[i] = scale * table[ids[i]].  A block's threads are split into groups of 1 << group_log2; a group copies ROWS rows at a time, so
 // that the wait for an id and then for its row is shared by several.
-// V = 8: rows of both arrays start where 8 elements may be moved at once.  V = 2: any rows, two columns at a time.
+// V = 8: rows of both arrays start where 8 elements may be moved at once.  V = 2: any rows, two columns at a time, but where both
+// types have 16 bits the 16 bytes between two boundaries of the output come from two such pieces of the table (30000 rows of
+// 1601 bf16: 37 us a call, in pairs 45; 20000 rows of 333 f32, which are 14.4 that way, are left at 12.3 in pairs).
 constexpr int kEmbedThreads = 256;
 
 // Two neighbouring elements at any address.  16-bit ones come in the one or two aligned 32-bit words that hold them; a word
@@ -44,6 +46,58 @@ __device__ __forceinline__ void store_two(O* p, bool second, float a, float b)
   } else {
     p[0] = y.e[0];
     if (second) p[1] = y.e[1];
+  }
+}
+
+// the 16 bytes that begin `bytes` (below 16, and even) behind the first of two pieces
+__device__ __forceinline__ uint4 shifted(const uint4& a, const uint4& b, uint32_t bytes)
+{
+  uint32_t w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+  if (bytes & 8)
+#pragma unroll
+    for (int i = 0; i < 6; ++i) w[i] = w[i + 2];
+  if (bytes & 4)
+#pragma unroll
+    for (int i = 0; i < 5; ++i) w[i] = w[i + 1];
+  const uint32_t half = (bytes & 2) * 8;
+  return make_uint4(__funnelshift_r(w[0], w[1], half), __funnelshift_r(w[1], w[2], half), __funnelshift_r(w[2], w[3], half),
+                    __funnelshift_r(w[3], w[4], half));
+}
+
+// A row of any alignment to one of any other, both of 16-bit types.  A piece of 16 bytes is read only if a wanted
+// element lies in it.
+template <class T, class O>
+__device__ __forceinline__ void copy_row(const T* from, O* to, int dim, float scale, int lane, int group)
+{
+  constexpr int E = 16 / int(sizeof(O)), kAhead = 4;
+  const int head  = min(dim, int((16u - (uint32_t(reinterpret_cast<uintptr_t>(to)) & 15u)) % 16u / sizeof(O)));
+  const int packs = (dim - head) / E;
+  const uintptr_t at    = reinterpret_cast<uintptr_t>(from + head);
+  const uint32_t shift  = uint32_t(at & 15);  // the same for all packs
+  const uint4* pieces   = reinterpret_cast<const uint4*>(at - shift);
+  uint4* out            = reinterpret_cast<uint4*>(to + head);
+  for (int p0 = lane; p0 < packs; p0 += kAhead * group) {
+    uint4 a[kAhead], b[kAhead];
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (p0 + k * group < packs) {
+        a[k] = __ldg(pieces + p0 + k * group);
+        b[k] = shift ? __ldg(pieces + p0 + k * group + 1) : make_uint4(0u, 0u, 0u, 0u);
+      }
+#pragma unroll
+    for (int k = 0; k < kAhead; ++k)
+      if (p0 + k * group < packs) {
+        const uint4 raw = shifted(a[k], b[k], shift);
+        const T* x      = reinterpret_cast<const T*>(&raw);
+        Pack<O, E> y;
+#pragma unroll
+        for (int j = 0; j < E; ++j) y.e[j] = gtk::from_float<O>(gtk::to_float(x[j]) * scale);
+        out[p0 + k * group] = *reinterpret_cast<const uint4*>(&y);
+      }
+  }
+  for (int i = lane; i < dim - packs * E; i += group) {
+    const int c = i < head ? i : i + packs * E;
+    to[c]       = gtk::from_float<O>(gtk::to_float(__ldg(from + c)) * scale);
   }
 }
 
@@ -94,6 +148,10 @@ k_embed(const int32_t* __restrict__ ids, int64_t n, const T* __restrict__ table,
 #pragma unroll
       for (int r = 0; r < ROWS; ++r)
         if (from[r]) to[r][c] = gtk::from_float<O>(gtk::to_float(from[r][c]) * scale);
+  } else if constexpr (sizeof(T) + sizeof(O) == 4) {
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r)
+      if (from[r]) copy_row(from[r], to[r], dim, scale, lane, group);
   } else {
     constexpr int kAhead = 4;
     const int pairs      = (dim + 1) / 2;
@@ -128,8 +186,8 @@ cudaError_t launch_embed(const gtk::HandleView& v, const int32_t* ids, int64_t n
   // Lanes for a row: a quarter as many as it has units, a warp at most; more, up to one per unit, while that keeps the GPU's threads
   // from being used up (2048 rows of 1024 bf16: 2.5 us with 32 lanes, 3.3 with 128; 64 rows of 768: 2.1 and 1.9).  Many rows
   // of packs go two at once (32768 rows of 1024 bf16: 18.1 us, one at once 19.0, four 24.8; 100000 rows of 256: 14.8, with a lane
-  // for every pack 34.4), of pairs one (30000 rows of 1601 bf16: 43 us, two 49).
-  const int64_t units = (dim + (V == 8 ? 7 : 1)) / V;
+  // for every pack 34.4), others one.
+  const int64_t units = V == 2 && sizeof(T) + sizeof(O) == 4 ? (dim * int64_t(sizeof(O)) + 15) / 16 : (dim + V - 1) / V;
   const bool many     = n >= int64_t(v.sm_count) * 64;
   int group_log2      = 0;
   while (group_log2 < 5 && (int64_t(4) << group_log2) < units) ++group_log2;
