@@ -10,7 +10,9 @@ using gtk::Pack;
 using gtk::Two;
 
 // ------------------------------------------------------------------------------------------------ lookup
-// out[i] = scale * table[ids[i]].  A block's threads are split into groups of 1 << group_log2; a group copies ROWS rows at a time, so
+// out[i] = scale * table[ids[i]], a product in 32 bits and one rounding.  Each row is read once and written once, so memory bounds
+// it: 32768 rows of 1024 bf16 take 18.3 us, 74 % of the measured copy rate over the bytes that differ; a few rows are a
+// launch and two waits behind one another, for the id and for the row (1.7 us).  A block's threads are split into groups of 1 << group_log2; a group copies ROWS rows at a time, so
 // that the wait for an id and then for its row is shared by several.
 // V = 8: rows of both arrays start where 8 elements may be moved at once.  V = 2: any rows, two columns at a time, but where both
 // types have 16 bits the 16 bytes between two boundaries of the output come from two such pieces of the table (30000 rows of
@@ -206,9 +208,17 @@ cudaError_t launch_embed(const gtk::HandleView& v, const int32_t* ids, int64_t n
 //                       One that lies in a block or reaches over one boundary is its first block's alone; a longer one is cut
 //                       at the boundaries and its parts go to the workspace
 //   k_embed_grad_join   adds the parts of the long ones from left to right
-// Every sum is thus formed in an order that the ids alone decide.
+// Every sum is thus formed in an order that the ids alone decide, in 32 bits, and rounded once.  A row of grad_out is read once and a
+// row of grad_table written once: that traffic is the floor, and the grouping, which the rows wait for, is what comes on top.
+// 32768 tokens of 768 bf16 to 50257 rows of f32: 57 us (28, 20 and 6.5 of the three; the last two begin while their predecessor
+// ends, which takes 4 us off), at the copy rate 32.  4096 tokens: 42 us, nearly all of it the 154 MB of zeros.  131072 tokens: 108
+// (43, 50, 14), at the copy rate 55.
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
-constexpr int kOwnersLog2 = 7, kOwners = 1 << kOwnersLog2;  // CTAs of k_embed_grad_sort
+// CTAs of k_embed_grad_sort, one to an SM.  All of them read all ids, from the second-level cache: no CTA waits for another and one
+// launch does it all, while up to some 100 000 ids the clearing of rows hides it (32768 tokens: 28 us, of which the zeros alone
+// take 24).  Beyond, the reading shows: 1M tokens, 350 us.  An id that a large part of the tokens has is one CTA's work:
+// 32768 tokens of which half have one id take 41 us here, all of them 82.
+constexpr int kOwnersLog2 = 7, kOwners = 1 << kOwnersLog2;
 constexpr int kMaxDigitBits = 9;                            // a thread per bin at most
 constexpr int64_t kMaxDim = int64_t(1) << 20;
 
@@ -242,10 +252,12 @@ GradPlan grad_plan(int64_t n, int64_t vocab, int64_t dim)
   p.passes       = (bits + kMaxDigitBits - 1) / kMaxDigitBits;
   p.digit_bits   = (bits + p.passes - 1) / p.passes;
   p.block_log2   = kMinBlockLog2;
-  // Blocks of up to 64 tokens: as long as they leave some 600 000 columns of blocks, so that all SMs have work, and longer where there
-  // were more than 4096 of them, for the parts of the most frequent id's sum are added one after the other.  Longer
-  // ones only where the parts would take more than 32 MiB.
-  while (p.block_log2 < 6 && ((n >> (p.block_log2 + 1)) * dim >= 600000 || n >> p.block_log2 > 4096)) ++p.block_log2;
+  // Blocks of 8 to 32 tokens: as long as they leave some 600 000 columns of blocks, so that all SMs have work (sums and join of 4096
+  // tokens of 768: 12 us with 8, 15 with 32, 20 with 64; of 131072 tokens of 1601: 175, 115, 115), and longer, up to 64, where
+  // there were more than 4096 of them, for the parts of the most frequent id's sum are added one after the other (131072 tokens of
+  // 64: 33 us with 8, 23 with 32, 34 with 64).  Longer ones only where the parts would take more than 32 MiB.
+  while (p.block_log2 < 5 && (n >> (p.block_log2 + 1)) * dim >= 600000) ++p.block_log2;
+  while (p.block_log2 < 6 && n >> p.block_log2 > 4096) ++p.block_log2;
   while (p.block_log2 < kMaxBlockLog2 && (n >> p.block_log2) * dim * 8 > (int64_t(32) << 20)) ++p.block_log2;
   p.blocks    = (n + (int64_t(1) << p.block_log2) - 1) >> p.block_log2;
   p.pitch     = (dim + 7) / 8 * 8;
@@ -567,7 +579,9 @@ struct GradArgs {
   float* parts;  // [blocks][2][pitch]: of the long sum that begins further left, of the one that begins in the block
 };
 
-constexpr int kChunk = 4, kChunks = 3;  // rows that are waited for together, and such chunks in flight
+// Rows that are waited for together, and such chunks in flight (131072 rows of 1601 bf16: 4 and 3 102 us, 4 and 2 108, 4 and 4 109,
+// 2 and 4 106, 8 and 3 131: what shared memory a group takes is taken from the number of groups).
+constexpr int kChunk = 4, kChunks = 3;
 
 // first place in [from, to) whose id is not `id` (where one id follows another it does not come back)
 __device__ __forceinline__ int end_of_id(const uint32_t* ids, int from, int to, uint32_t id)
@@ -641,7 +655,9 @@ struct GroupShared {
   __host__ __device__ int bytes() const { return ring + (tokens * 12 + 15) / 16 * 16; }
 };
 
-// A group of threads (part of a warp, or the whole CTA) takes a block of tokens.  The rows come to shared memory in 16-byte pieces,
+// A group of threads (part of a warp, or the whole CTA) takes a block of tokens.  One addition per element read: memory bounds it
+// (131072 rows of 1601 bf16, any alignment, 100 us: 4.2 TB/s over the rows; 131072 of 768 bf16 50 us: 4.0 TB/s; the ids of
+// a real text repeat, so the rows come in no order).  The rows come to shared memory in 16-byte pieces,
 // a warp copying a row, kChunk * kChunks rows ahead.  The pieces are those between 16-byte boundaries: the outer ones may
 // hold bytes of a row's neighbours, which nobody looks at.
 template <class O, class T, bool ALIGNED>
@@ -812,7 +828,7 @@ __global__ void __launch_bounds__(kGradThreads) k_embed_grad_sums(const GradArgs
   else finish(id);
 }
 
-// The parts of long sums, 128 columns at a time: a warp per sum; those of more than kJoinAlone parts are all warps' work, each adds
+// The parts of long sums (32768 tokens of a text-like distribution: 6.5 us, 131072: 14), 128 columns at a time: a warp per sum; those of more than kJoinAlone parts are all warps' work, each adds
 // a run of parts, then the warps' sums are added in order.
 constexpr int kJoinThreads = 256, kJoinBlocks = 16, kJoinAlone = 32;
 template <class T>

@@ -641,7 +641,10 @@ __global__ void __launch_bounds__(kThreads) k_token_logprobs_grad(const T* logit
   }
 }
 
-// The same where logits and gradient lie differently against 16-byte boundaries: element by element (2.5 times the time).
+// The same where logits and gradient lie differently against 16-byte boundaries: element by element, with
+// kPlainBatch loads in flight (2048 rows of 50257 bf16: 100 us, one load at a time 228, in packs where they lie alike 69; f32 143
+// and 134).
+constexpr int kPlainBatch = 8;
 template <class T, bool ENTROPY>
 __global__ void __launch_bounds__(kThreads) k_token_logprobs_grad_plain(const T* logits, T* grad, const ScoreGradArgs a, int parts)
 {
@@ -650,8 +653,17 @@ __global__ void __launch_bounds__(kThreads) k_token_logprobs_grad_plain(const T*
   const T* x      = logits + r * a.stride;
   T* to           = grad + r * a.grad_stride;
   const GradRow<T, ENTROPY> R(a, r);
-  for (int64_t c = part * kThreads + threadIdx.x; c < a.vocab; c += int64_t(parts) * kThreads)
-    to[c] = gtk::from_float<T>(R.nothing ? 0.f : R.of(gtk::to_float(x[c]), int(c)));
+  for (int64_t c0 = int64_t(part) * kPlainBatch * kThreads + threadIdx.x; c0 < a.vocab; c0 += int64_t(parts) * kPlainBatch * kThreads) {
+    T raw[kPlainBatch];
+#pragma unroll
+    for (int q = 0; q < kPlainBatch; ++q)
+      if (c0 + q * kThreads < a.vocab) raw[q] = x[c0 + q * kThreads];
+#pragma unroll
+    for (int q = 0; q < kPlainBatch; ++q) {
+      const int64_t c = c0 + q * kThreads;
+      if (c < a.vocab) to[c] = gtk::from_float<T>(R.nothing ? 0.f : R.of(gtk::to_float(raw[q]), int(c)));
+    }
+  }
 }
 
 template <class T, bool ENTROPY>
