@@ -7,9 +7,9 @@
 //
 // All of it is bound by memory, and just so: an element costs one exponential (16 a clock and SM) and some four further
 // instructions.  Measured against a copy (6.45 TB/s):
-//   8192 rows of 50257 bf16     130 us, 98 %; back to back for a second 155 us: at 1000 W the SMs run at 1.65 GHz, and 412 M
-//                               exponentials alone then take 105 us
-//   4096 rows of the same, f32  131 us, 97 %; with entropy 134; with 20 alternatives 168
+//   8192 rows of 50257 bf16     130 us, 98 %, with 20 alternatives 176; back to back for a second 150 us: at 1000 W the SMs run at
+//                               1.6 GHz, and 412 M exponentials alone then take 108 us
+//   4096 rows of the same, f32  123 us, 104 %, with entropy 124; with 20 alternatives 156
 //   gradient of 8192 rows       259 us, 98 %
 //   one row                     4 us without alternatives, 9 with 20 of them and entropy: phases that wait for each other
 #include <cooperative_groups.h>
@@ -334,9 +334,18 @@ struct NoScratch {};
 // What keeps memory busy here is many CTAs at different places of their rows, so registers are few and a CTA ends with its
 // row.  8192 rows of 50257 bf16 took 186 us with CTAs that stay and have the next row's first batch in registers, 147 us with a
 // ring of batches in shared memory that runs on into the next row, 138 us as it is but with 256 threads, 130 us with 128.
+// Alternatives cost a row its end: the bound and the packs that are read again take some 5 us, in which the CTA asks for
+// nothing (8192 rows of 8192 bf16: 29 us without, 43 with one, 52 with 20).
+// CTAs of kThreads per SM that registers are shared out for.  With 4 and 5, us: 8192 rows
+// of 50257 bf16 130 and 133, 4096 of them with entropy 80 and 76, with entropy and five alternatives 95 and 90; 999 of f32 with these
+// 40 and 45, 8192 rows of 8192 f32 with five alternatives 64 and 60.
 template <class T, bool ENTROPY, bool TOP>
-__global__ void __launch_bounds__(kThreads, 5) k_token_logprobs(const T* __restrict__ logits, const ScoreArgs a, int parts)
+constexpr int kResident = (sizeof(T) == 2 ? TOP || ENTROPY : TOP && !ENTROPY) ? 5 : 4;
+
+template <class T, bool ENTROPY, bool TOP, bool SPLIT>
+__global__ void __launch_bounds__(kThreads, kResident<T, ENTROPY, TOP>) k_token_logprobs(const T* __restrict__ logits, const ScoreArgs a, int n_parts)
 {
+  const int parts = SPLIT ? n_parts : 1;
   namespace cg = cooperative_groups;
   using P         = Pack16<T>;
   constexpr int E = P::kElems;
@@ -363,13 +372,7 @@ __global__ void __launch_bounds__(kThreads, 5) k_token_logprobs(const T* __restr
   typename P::Max best[kBatch];
 #pragma unroll
   for (int q = 0; q < kBatch; ++q) best[q] = P::lowest();
-  for (int p0 = begin + tid; p0 < end; p0 += kBatch * threads) {
-    uint4 raw[kBatch];
-#pragma unroll
-    for (int q = 0; q < kBatch; ++q) {
-      constexpr uint32_t w = P::kMinusInf;
-      raw[q] = p0 + q * threads < end ? __ldg(row.pack(p0 + q * threads)) : make_uint4(w, w, w, w);
-    }
+  auto take = [&](const uint4 (&raw)[kBatch]) {
     typename P::Max all = P::highest(raw[0]);
     if (TOP) best[0] = P::higher(best[0], all);
 #pragma unroll
@@ -400,7 +403,31 @@ __global__ void __launch_bounds__(kThreads, 5) k_token_logprobs(const T* __restr
         if (ENTROPY) t2 = fma2(p, Two(fmaxf(y0, -1e4f), fmaxf(y1, -1e4f)), t2);
       }
     }
-  }
+  };
+  int p0 = begin + tid;
+  // Whole batches by code of their own: 999 rows of f32 take 34 us, 41 with packs asked for one by one in all batches, 4096 of bf16
+  // with alternatives 84 and 95.  Parts of a row have few batches, which would wait for both codes to come in (one row: 4.6 us
+  // and 4.2).
+  if constexpr (!SPLIT)
+    for (; p0 < end - (kBatch - 1) * threads; p0 += kBatch * threads) {
+      uint4 raw[kBatch];
+#pragma unroll
+      for (int q = 0; q < kBatch; ++q) raw[q] = __ldg(row.pack(p0 + q * threads));
+      take(raw);
+    }
+  auto take_some = [&]() {
+    uint4 raw[kBatch];
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) {
+      constexpr uint32_t w = P::kMinusInf;
+      raw[q] = p0 + q * threads < end ? __ldg(row.pack(p0 + q * threads)) : make_uint4(w, w, w, w);
+    }
+    take(raw);
+  };
+  if constexpr (SPLIT)
+    for (; p0 < end; p0 += kBatch * threads) take_some();
+  else if (p0 < end)
+    take_some();
   {
     float lo, hi;
     s2.get(lo, hi);
@@ -447,7 +474,7 @@ __global__ void __launch_bounds__(kThreads, 5) k_token_logprobs(const T* __restr
     // (top_k / parts)-th highest
     bound = find_bound<T>(mine, (a.top_k + parts - 1) / parts);
   }
-  if (parts == 1) {
+  if constexpr (!SPLIT) {
     if constexpr (TOP) {
       collect_keys(row, begin, end, true, a.top_k, kMostKeys, bound, mine, best, s_top);
       rank_keys(s_top, s_top.keys, a.top_k, put);
@@ -539,7 +566,8 @@ template <class T, bool ENTROPY, bool TOP>
 cudaError_t launch_logprobs(const gtk::HandleView& v, const void* logits, int64_t n_rows, const ScoreArgs& a)
 {
   const Teams t = teams_for(n_rows, int64_t(a.vocab) * int64_t(sizeof(T)), v.sm_count);
-  return gtk::launch_clusters(k_token_logprobs<T, ENTROPY, TOP>, dim3(unsigned(n_rows * t.parts)), dim3(unsigned(t.threads)), t.parts, 0, v.stream,
+  auto kernel   = t.parts > 1 ? k_token_logprobs<T, ENTROPY, TOP, true> : k_token_logprobs<T, ENTROPY, TOP, false>;
+  return gtk::launch_clusters(kernel, dim3(unsigned(n_rows * t.parts)), dim3(unsigned(t.threads)), t.parts, 0, v.stream,
                               static_cast<const T*>(logits), a, t.parts);
 }
 
