@@ -706,13 +706,14 @@ cudaError_t launch_logprobs_grad(const gtk::HandleView& v, const void* logits, v
 }
 
 constexpr int64_t kMaxVocab = int64_t(1) << 30, kMaxRows = (int64_t(1) << 31) - 1;
+constexpr float kMaxScale = 1e38f;  // times log2(e) it is a number too
 
 gtk::Refusal refuse_sizes(int type, int64_t n_rows, int64_t vocab, int64_t stride, float scale)
 {
   if (!gtk::known_type(type)) return "unknown element type";
   if (n_rows < 0 || vocab <= 0 || stride < 0) return "n_rows and stride must be >= 0, vocab > 0";
   if (n_rows > kMaxRows || vocab > kMaxVocab) return "n_rows of 2^31 and more, or vocab beyond 2^30";
-  if (!(scale > 0.f) || std::isinf(scale)) return "scale must be a finite number > 0";
+  if (!(scale > 0.f && scale <= kMaxScale)) return "scale must be a number > 0, 1e38 at most";
   return nullptr;
 }
 

@@ -332,7 +332,7 @@ GTK_API int gtk_embed_grad(gtk_tokenizer* h, const int32_t* d_ids, int64_t n_ids
 #define GTK_MAX_TOP 32
 
 /* Row r of d_logits (vocab elements) stands for the distribution p_j = exp(scale * x_j - lse), lse = log sum_j
- * exp(scale * x_j); scale > 0 is the inverse temperature.  Outputs, 32-bit floats, NULL for those that are not wanted
+ * exp(scale * x_j); scale, above 0 and at most 1e38, is the inverse temperature.  Outputs, 32-bit floats, NULL for those that are not wanted
  * (d_targets may be NULL when d_logprob is):
  *   d_logprob[r]             log p of d_targets[r]; 0 where that is negative, NaN where it is >= vocab
  *   d_entropy[r]             -sum_j p_j log p_j
@@ -341,8 +341,8 @@ GTK_API int gtk_embed_grad(gtk_tokenizer* h, const int32_t* d_ids, int64_t n_ids
  *                            first (int32, rows back to back), and
  *   d_top_logprobs[r][..]    their log p.  Columns at -inf are no alternatives: places that remain hold -1 and -inf
  * A row of nothing but -inf (every id masked) has lse -inf, log p -inf, entropy 0 and no alternatives.  A row that holds
- * a NaN or +inf has NaN everywhere (a negative target's 0 excepted) and no alternatives.  n_rows < 2^31,
- * vocab <= 2^30, 0 <= top_k <= GTK_MAX_TOP. */
+ * a NaN or +inf has NaN everywhere (a negative target's 0 excepted) and no alternatives.  Differences between a row's
+ * logits that no 32-bit float holds count as infinite.  n_rows < 2^31, vocab <= 2^30, 0 <= top_k <= GTK_MAX_TOP. */
 GTK_API int gtk_token_logprobs(gtk_tokenizer* h, const void* d_logits, int type, int64_t n_rows, int64_t vocab,
                                int64_t stride, float scale, const int32_t* d_targets, int top_k, float* d_logprob,
                                float* d_entropy, float* d_lse, int32_t* d_top_ids, float* d_top_logprobs);

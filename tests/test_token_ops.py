@@ -830,3 +830,78 @@ def test_the_same_bits_every_time(tok):
     for _ in range(4):
         for a, b in zip(want, score(tok, x, "f32", targets, 20, 0.7, vocab)):
             assert torch.equal(a, b)
+
+
+def test_scales_that_32_bits_do_not_hold(host):
+    for scale in (1.1e38, 3e38, 5e-324):
+        for name, good in (("token_logprobs", SCORE), ("token_logprobs_grad", SCORE_GRAD)):
+            with pytest.raises(GtkError) as e:
+                getattr(host, name)(**good, scale=scale)
+            assert e.value.code == 1
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("scale", [1e-38, 1e-20, 1e20, 1e38])
+def test_scales_at_the_ends(tok, scale):
+    """Logits of which the scale makes numbers around one."""
+    import torch
+
+    n, vocab = 6, 3001
+    x = torch.randn(n, vocab, device="cuda") * 3
+    x = (x.double() / scale).float() if scale > 1 else x * (0.1 / scale if scale > 1e-30 else 1e37)
+    targets = some_ids(2, n, vocab, "text")
+    lp, H, lse, ids, tops = score(tok, x, "f32", targets, 9, scale, vocab)
+    w_lp, w_H, w_lse, w_ids, w_tops = score_wanted(x, targets, 9, scale)
+    # the scale's product with log2(e), and logits below 2^-126, have their own steps: 2^-149 each, of numbers down to 1e-38
+    more = 2.0 ** -149 / min(scale, 1e-37) * 16
+    assert torch.equal(ids.long(), w_ids)
+    same(lse, w_lse[0], w_lse[1] + more, "lse")
+    same(lp, w_lp[0], w_lp[1] + more, "logprob")
+    same(H, w_H[0], w_H[1] + more, "entropy")
+
+
+@pytest.mark.gpu
+def test_rows_of_many_millions(tok):
+    """Rows that a CTA reads in more than 4096 batches, all rows being the same one, and one that CTAs share."""
+    import torch
+
+    vocab, k = 40_000_003, 20
+    g = torch.Generator(device="cuda").manual_seed(5)
+    x = (torch.randn(vocab, generator=g, device="cuda") * 0.25).to(torch.bfloat16)
+    places = torch.randperm(vocab, generator=g, device="cuda")[:k]
+    x[places] = torch.arange(2, 2 + k, device="cuda").to(torch.bfloat16)
+    raw = x.double()
+    lse = float(torch.logsumexp(raw, 0))
+    p = (raw - lse).exp()
+    H = float(-(p * (raw - lse)).sum())
+    bound = (vocab / 256 + 8) * 4 * U + 2.0 ** -20           # see score_wanted
+    for n in (1, 150):
+        f = lambda *s: torch.zeros(*s, device="cuda")  # noqa: E731
+        lp, entropy, got_lse, top = f(n), f(n), f(n), torch.zeros(n, k, device="cuda", dtype=torch.int32)
+        targets = torch.full((n,), vocab - 1, device="cuda", dtype=torch.int32)
+        tok.token_logprobs(x.data_ptr(), "bf16", n, vocab, targets.data_ptr(), lp.data_ptr(), entropy.data_ptr(), got_lse.data_ptr(), k,
+                           top.data_ptr(), stride=0)
+        assert torch.equal(top.long(), places.flip(0).expand(n, k))
+        assert bool(((got_lse.double() - lse).abs() < bound + 4 * U * lse).all())
+        assert bool(((lp.double() - (float(raw[-1]) - lse)).abs() < bound + 8 * U * lse).all())
+        assert bool(((entropy.double() - H).abs() < bound * (2 * H + 2) + 4 * U * lse).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", TYPES)
+def test_gradient_of_one_row_for_all(tok, name):
+    """Logits with a stride of zero, which is not the gradient's."""
+    import torch
+
+    n, vocab = 700, 300
+    ids = some_ids(4, n, vocab, "padded")
+    _, x = rows(torch.randn(1, vocab, device="cuda"), name)
+    g = torch.randn(n, device="cuda")
+    lse, H, want, bound = grad_wanted(x.expand(n, vocab), ids, 1.0, g, None)
+    lse32 = lse.float()
+    for stride in (vocab, vocab + 4, vocab + 5):
+        whole, grad = rows(torch.zeros(n, vocab, device="cuda"), name, stride)
+        tok.token_logprobs_grad(x.data_ptr(), name, n, vocab, ids.data_ptr(), lse32.data_ptr(), g.data_ptr(), grad.data_ptr(), stride=0,
+                                grad_stride=stride)
+        same(grad, want, bound + want.abs() * half_step(name) * 1.01 + tiny(name) + 1e-36, "grad")
+        assert marks_untouched(whole, n, vocab, stride, 0)
