@@ -7,11 +7,11 @@
 //
 // All of it is bound by memory, and just so: an element costs one exponential (16 a clock and SM) and some four further
 // instructions.  Measured against a copy (6.45 TB/s):
-//   8192 rows of 50257 bf16     130 us, 98 %, with 20 alternatives 176; back to back for a second 150 us: at 1000 W the SMs run at
+//   8192 rows of 50257 bf16     130 us, 98 %, with 20 alternatives 167; back to back for a second 150 us: at 1000 W the SMs run at
 //                               1.6 GHz, and 412 M exponentials alone then take 108 us
-//   4096 rows of the same, f32  123 us, 104 %, with entropy 124; with 20 alternatives 156
+//   4096 rows of the same, f32  121 us, 105 %, with entropy 123; with 20 alternatives 154
 //   gradient of 8192 rows       259 us, 98 %
-//   one row                     4 us without alternatives, 9 with 20 of them and entropy: phases that wait for each other
+//   one row                     4 us without alternatives, 8.4 with 20 of them and entropy: phases that wait for each other
 #include <cooperative_groups.h>
 
 #include <cfloat>
@@ -184,7 +184,7 @@ struct TopScratch {
   uint64_t key[kMostKeys];
   uint64_t best[kWarps];
   int set[kThreads];  // thread << 8 | q << 4 | half
-  int sets, keys;
+  int sets, keys, crowded;
   uint32_t bound;
 };
 
@@ -221,6 +221,7 @@ __device__ __forceinline__ void collect_keys(const RowParts<T>& row, int begin, 
   constexpr int E = P::kElems;
   const int tid = threadIdx.x, threads = blockDim.x, warp = tid >> 5, lane = tid & 31;
   uint64_t floor = uint64_t(bound) << 32;
+  __syncthreads();  // all have seen collect_few's keys
   if (tid == 0) S.sets = S.keys = 0;
   __syncthreads();
   if (mine && mine >= bound) {
@@ -313,6 +314,65 @@ __device__ __forceinline__ void collect_keys(const RowParts<T>& row, int begin, 
   __syncthreads();
 }
 
+// The same where the sets that reach the bound are few in each warp, which then reads its own ones again and waits for no other
+// (with the list of all warps at once one row took 9.1 us, now 8.4, 8192 rows of 50257 bf16 with 20 alternatives 171, now 167): false
+// where they are not, or hold too many keys.  S.keys and S.crowded are 0 before.
+template <class T>
+__device__ __forceinline__ bool collect_few(const RowParts<T>& row, int begin, int end, bool loose, int most, uint32_t bound,
+                                            const typename Pack16<T>::Max (&best)[kBatch], TopScratch& S)
+{
+  using P         = Pack16<T>;
+  constexpr int E = P::kElems;
+  const int tid = threadIdx.x, threads = blockDim.x, warp = tid >> 5, lane = tid & 31;
+  const int room     = kThreads * 32 / threads;
+  int* const set     = S.set + warp * room;
+  const uint64_t floor = uint64_t(bound) << 32;
+  const float reach  = bound ? key_value(floor) : -FLT_MAX;  // -inf is no alternative
+  auto offer = [&](float x, int column) {
+    const int at = atomicAdd(&S.keys, 1);
+    if (at < most) S.key[at] = rank_key(x, uint32_t(column));
+  };
+  int sets = 0;
+#pragma unroll
+  for (int q = 0; q < kBatch; ++q)
+#pragma unroll
+    for (int half = 0; half < P::kHalves; ++half) {
+      const bool reaches  = P::of(best[q], half) >= reach;
+      const uint32_t some = __ballot_sync(0xFFFFFFFFu, reaches);
+      const int at        = sets + __popc(some & ((1u << lane) - 1u));
+      if (reaches && at < room) set[at] = tid << 8 | q << 4 | half;
+      sets += __popc(some);
+    }
+  __syncwarp();
+  if (sets > room) {
+    if (lane == 0) S.crowded = 1;
+  } else {
+    // as many threads to the packs of a set as there are for all, and each looks at two packs at a time (8192 rows of 50257 bf16 with 20
+    // alternatives 167 us; one at a time by eight threads 170, four at a time 182, for want of registers)
+    const int share_log2 = sets > 1 ? max(0, 5 - (32 - __clz(sets - 1))) : 5, stride = kBatch * threads << share_log2;
+    auto look            = [&](const uint4& raw, int p, int half) {
+      const T* x = reinterpret_cast<const T*>(&raw);
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (gtk::to_float(x[j]) >= reach && (P::kHalves == 1 || (j & 1) == half)) offer(gtk::to_float(x[j]), row.pack_column(p) + j);
+    };
+    for (int i = lane >> share_log2; i < sets; i += 32 >> share_log2) {
+      const int w = set[i];
+      for (int p = begin + (w >> 8) + ((w >> 4 & 15) + kBatch * (lane & ((1 << share_log2) - 1))) * threads; p < end; p += 2 * stride) {
+        const uint4 one = __ldg(row.pack(p)), two = __ldg(row.pack(p + stride < end ? p + stride : p));
+        look(one, p, w & 1);
+        if (p + stride < end) look(two, p + stride, w & 1);
+      }
+    }
+  }
+  if (loose && tid < row.head + row.tail) {
+    const float x = gtk::to_float(row.x[row.loose_column(tid)]);
+    if (x >= reach) offer(x, row.loose_column(tid));
+  }
+  __syncthreads();
+  return !S.crowded && S.keys <= most;
+}
+
 // The top_k highest of S.key[0 .. n), each to put(place, key) by one thread, places that remain with key 0.
 template <class Put>
 __device__ __forceinline__ void rank_keys(const TopScratch& S, int n, int top_k, Put&& put)
@@ -334,8 +394,8 @@ struct NoScratch {};
 // What keeps memory busy here is many CTAs at different places of their rows, so registers are few and a CTA ends with its
 // row.  8192 rows of 50257 bf16 took 186 us with CTAs that stay and have the next row's first batch in registers, 147 us with a
 // ring of batches in shared memory that runs on into the next row, 138 us as it is but with 256 threads, 130 us with 128.
-// Alternatives cost a row its end: the bound and the packs that are read again take some 5 us, in which the CTA asks for
-// nothing (8192 rows of 8192 bf16: 29 us without, 43 with one, 52 with 20).
+// Alternatives cost a row its end: the bound and the packs that are read again are waits one after another, in which the CTA asks
+// for nothing else (8192 rows of 8192 bf16: 29 us without, 37 with one, 47 with 20).
 // CTAs of kThreads per SM that registers are shared out for.  With 4 and 5, us: 8192 rows
 // of 50257 bf16 130 and 133, 4096 of them with entropy 80 and 76, with entropy and five alternatives 95 and 90; 999 of f32 with these
 // 40 and 45, 8192 rows of 8192 f32 with five alternatives 64 and 60.
@@ -446,6 +506,8 @@ __global__ void __launch_bounds__(kThreads, kResident<T, ENTROPY, TOP>) k_token_
     if (ENTROPY) sum.t += __shfl_xor_sync(0xFFFFFFFFu, sum.t, d);
   }
   if (lane == 0) s_m[warp] = sum.m, s_s[warp] = sum.s, s_t[warp] = sum.t;
+  if constexpr (TOP)
+    if (tid == 0) s_top.keys = s_top.crowded = 0;
   __syncthreads();
   RowSum all;
   all.m = s_m[0];
@@ -476,7 +538,8 @@ __global__ void __launch_bounds__(kThreads, kResident<T, ENTROPY, TOP>) k_token_
   }
   if constexpr (!SPLIT) {
     if constexpr (TOP) {
-      collect_keys(row, begin, end, true, a.top_k, kMostKeys, bound, mine, best, s_top);
+      if (!collect_few(row, begin, end, true, kMostKeys, bound, best, s_top))
+        collect_keys(row, begin, end, true, a.top_k, kMostKeys, bound, mine, best, s_top);
       rank_keys(s_top, s_top.keys, a.top_k, put);
     }
   } else {
@@ -489,7 +552,8 @@ __global__ void __launch_bounds__(kThreads, kResident<T, ENTROPY, TOP>) k_token_
     if constexpr (TOP) {
       // lane c asks part c, here and below: reads of other CTAs' shared memory take long, one after the other too long
       bound = __reduce_min_sync(0xFFFFFFFFu, lane < parts ? cluster.map_shared_rank(&s_top, lane)->bound : bound);
-      collect_keys(row, begin, end, part == 0, a.top_k, kMostKeysOfPart, bound, mine, best, s_top);
+      if (!collect_few(row, begin, end, part == 0, kMostKeysOfPart, bound, best, s_top))
+        collect_keys(row, begin, end, part == 0, a.top_k, kMostKeysOfPart, bound, mine, best, s_top);
       cluster.sync();
     }
     if (part == 0) {
