@@ -317,7 +317,7 @@ __device__ __forceinline__ void collect_keys(const RowParts<T>& row, int begin, 
 // The same where the sets that reach the bound are few in each warp, which then reads its own ones again and waits for no other
 // (with the list of all warps at once one row took 9.1 us, now 8.4, 8192 rows of 50257 bf16 with 20 alternatives 171, now 167): false
 // where they are not, or hold too many keys.  S.keys and S.crowded are 0 before.
-template <class T>
+template <int LOOK, class T>
 __device__ __forceinline__ bool collect_few(const RowParts<T>& row, int begin, int end, bool loose, int most, uint32_t bound,
                                             const typename Pack16<T>::Max (&best)[kBatch], TopScratch& S)
 {
@@ -347,8 +347,7 @@ __device__ __forceinline__ bool collect_few(const RowParts<T>& row, int begin, i
   if (sets > room) {
     if (lane == 0) S.crowded = 1;
   } else {
-    // as many threads to the packs of a set as there are for all, and each looks at two packs at a time (8192 rows of 50257 bf16 with 20
-    // alternatives 167 us; one at a time by eight threads 170, four at a time 182, for want of registers)
+    // as many threads to the packs of a set as there are for all, and each looks at LOOK packs at a time
     const int share_log2 = sets > 1 ? max(0, 5 - (32 - __clz(sets - 1))) : 5, stride = kBatch * threads << share_log2;
     auto look            = [&](const uint4& raw, int p, int half) {
       const T* x = reinterpret_cast<const T*>(&raw);
@@ -358,10 +357,13 @@ __device__ __forceinline__ bool collect_few(const RowParts<T>& row, int begin, i
     };
     for (int i = lane >> share_log2; i < sets; i += 32 >> share_log2) {
       const int w = set[i];
-      for (int p = begin + (w >> 8) + ((w >> 4 & 15) + kBatch * (lane & ((1 << share_log2) - 1))) * threads; p < end; p += 2 * stride) {
-        const uint4 one = __ldg(row.pack(p)), two = __ldg(row.pack(p + stride < end ? p + stride : p));
-        look(one, p, w & 1);
-        if (p + stride < end) look(two, p + stride, w & 1);
+      for (int p = begin + (w >> 8) + ((w >> 4 & 15) + kBatch * (lane & ((1 << share_log2) - 1))) * threads; p < end; p += LOOK * stride) {
+        uint4 raw[LOOK];
+#pragma unroll
+        for (int q = 0; q < LOOK; ++q) raw[q] = __ldg(row.pack(p + q * stride < end ? p + q * stride : p));
+#pragma unroll
+        for (int q = 0; q < LOOK; ++q)
+          if (p + q * stride < end) look(raw[q], p + q * stride, w & 1);
       }
     }
   }
@@ -402,10 +404,16 @@ struct NoScratch {};
 template <class T, bool ENTROPY, bool TOP>
 constexpr int kResident = (sizeof(T) == 2 ? TOP || ENTROPY : TOP && !ENTROPY) ? 5 : 4;
 
+// Packs that a thread reads again at a time.  8192 rows of 50257 bf16 with 20 alternatives: 167 us with two, 170 with one, 182 with four, for
+// want of registers; where there are more of them, 4096 rows of f32 with entropy too: 154 with four, 162 with two.
+template <class T, bool ENTROPY, bool TOP>
+constexpr int kLookAgain = kResident<T, ENTROPY, TOP> == 4 ? 4 : 2;
+
 template <class T, bool ENTROPY, bool TOP, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, kResident<T, ENTROPY, TOP>) k_token_logprobs(const T* __restrict__ logits, const ScoreArgs a, int n_parts)
 {
-  const int parts = SPLIT ? n_parts : 1;
+  const int parts     = SPLIT ? n_parts : 1;
+  constexpr int kLook = kLookAgain<T, ENTROPY, TOP>;
   namespace cg = cooperative_groups;
   using P         = Pack16<T>;
   constexpr int E = P::kElems;
@@ -538,7 +546,7 @@ __global__ void __launch_bounds__(kThreads, kResident<T, ENTROPY, TOP>) k_token_
   }
   if constexpr (!SPLIT) {
     if constexpr (TOP) {
-      if (!collect_few(row, begin, end, true, kMostKeys, bound, best, s_top))
+      if (!collect_few<kLook>(row, begin, end, true, kMostKeys, bound, best, s_top))
         collect_keys(row, begin, end, true, a.top_k, kMostKeys, bound, mine, best, s_top);
       rank_keys(s_top, s_top.keys, a.top_k, put);
     }
@@ -552,7 +560,7 @@ __global__ void __launch_bounds__(kThreads, kResident<T, ENTROPY, TOP>) k_token_
     if constexpr (TOP) {
       // lane c asks part c, here and below: reads of other CTAs' shared memory take long, one after the other too long
       bound = __reduce_min_sync(0xFFFFFFFFu, lane < parts ? cluster.map_shared_rank(&s_top, lane)->bound : bound);
-      if (!collect_few(row, begin, end, part == 0, kMostKeysOfPart, bound, best, s_top))
+      if (!collect_few<kLook>(row, begin, end, part == 0, kMostKeysOfPart, bound, best, s_top))
         collect_keys(row, begin, end, part == 0, a.top_k, kMostKeysOfPart, bound, mine, best, s_top);
       cluster.sync();
     }
