@@ -210,7 +210,8 @@ __device__ __forceinline__ uint32_t find_bound(uint32_t mine, int wanted)
 // at most `most` of them, among which are all of the top_k highest that reach the bound.
 // A thread has read packs begin + thread, and every blockDim-th from there; of those that were q-th in their batch it knows the
 // highest elements best[q], and `mine` is the value_key of its highest of all.  Only packs of sets (a thread, a q, a half of the
-// elements) whose highest reaches the bound are read again, from L2.  That is about top_k sets, as long as numbers differ.
+// elements) whose highest reaches the bound are read again, from L2.  That is about top_k sets, as long as numbers differ, and then
+// collect_few has answered already: this is the way of rows with ties and crowds.
 // Where more than kMostSets reach it, the threads whose highest (by value, then by column) are the top_k highest of their
 // kind take the sets' place: what the others hold comes behind those.
 template <class T>
@@ -261,12 +262,11 @@ __device__ __forceinline__ void collect_keys(const RowParts<T>& row, int begin, 
     __syncthreads();
   }
   const int step = by_set ? kBatch * threads : threads;
-  const uint32_t each = uint32_t(max(1, (end - begin + step - 1) / step)), inverse = ~0u / each + 1u, packs = uint32_t(S.sets) * each;
-  const bool short_ones = each > 1 && each < 4096;  // then kMostSets * each * each < 2^32, and the product below is exact
+  const uint32_t each = uint32_t(max(1, (end - begin + step - 1) / step)), packs = uint32_t(S.sets) * each;
   const float reach = bound ? key_value(floor) : -INFINITY;
   // f(key) for the elements of the i-th pack of the sets that reach the bound
   auto each_key = [&](uint32_t i, auto&& f) {
-    const uint32_t at = short_ones ? __umulhi(i, inverse) : i / each;
+    const uint32_t at = i / each;
     const int w = S.set[at], p = begin + (w >> 8) + (w >> 4 & 15) * threads + int(i - at * each) * step;
     if (p >= end) return;
     const uint4 raw = __ldg(row.pack(p));
