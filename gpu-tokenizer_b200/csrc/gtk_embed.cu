@@ -2,10 +2,12 @@
 #include <algorithm>
 #include <cmath>
 
+#include "gtk_long_sums.hpp"
 #include "gtk_rows.cuh"
 
 namespace {
 
+using gtk::LongSum;
 using gtk::Pack;
 using gtk::Two;
 
@@ -221,11 +223,6 @@ constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 constexpr int kOwnersLog2 = 7, kOwners = 1 << kOwnersLog2;
 constexpr int kMaxDigitBits = 9;                            // a thread per bin at most
 constexpr int64_t kMaxDim = int64_t(1) << 20;
-
-// Of a block of tokens: the long sum that begins in it, and in how many blocks that has a part; parts == 0: none.
-struct alignas(8) LongSum {
-  uint32_t id, parts;
-};
 
 struct GradPlan {
   int passes, digit_bits;
@@ -523,26 +520,9 @@ k_embed_grad_sort(const SortArgs a, T* __restrict__ grad_table, int dim, int64_t
   uint32_t begin = 0, count = 0;
   if (a.n > 0) group_tokens(a, S, begin, count);
   const uint2* tokens = (a.passes & 1 ? a.tokens1 : a.tokens0) + begin;
-  // the blocks whose last token is this owner's: the sum that it belongs to is long when it reaches over the next boundary
-  // too, and begins in the block or further left
-  const int64_t end = int64_t(begin) + count;
-  for (int64_t block = (begin >> a.block_log2) + threadIdx.x; block << a.block_log2 < end; block += kSortThreads) {
-    const int64_t last = min(((block + 1) << a.block_log2), a.n) - 1, third = (block + 2) << a.block_log2;
-    if (last >= end) continue;
-    const uint32_t id = tokens[last - begin].x;
-    LongSum L{id, 0u};
-    const int64_t left = (block << a.block_log2) - 1;
-    if (third < end && tokens[third - begin].x == id && !(left >= int64_t(begin) && tokens[left - begin].x == id)) {
-      int64_t from = third, to = end;  // the last place with the id is in [from, to)
-      while (to - from > 1) {
-        const int64_t mid = (from + to) / 2;
-        if (tokens[mid - begin].x == id) from = mid;
-        else to = mid;
-      }
-      L.parts = uint32_t((from >> a.block_log2) - block + 1);
-    }
-    a.long_sums[block] = L;
-  }
+  gtk::each_long_sum(
+      begin, int64_t(begin) + count, a.n, a.block_log2, threadIdx.x, kSortThreads, [&](int64_t place) { return tokens[place - begin].x; },
+      [&](int64_t block, const LongSum& L) { a.long_sums[block] = L; });
   if (!clear) return;
   // the rows of this owner that have no token, as many at once as the shared memory has bits
   uint32_t* used        = &S.at[0][0];

@@ -90,6 +90,84 @@ def test_workspace_sizes(host):
                 assert need < 64 * n + 4 * vocab + 48 * (1 << 20) + 64 * 8 * dim
 
 
+LONG_SUMS = r"""
+#include "gtk_long_sums.hpp"
+#include <algorithm>
+#include <cstdio>
+#include <cstdlib>
+#include <random>
+#include <vector>
+
+// Owners of ids by id % 8 on tokens grouped by owner, then id, those of no id last: every place that is asked about and every block
+// that is put, from all owners' threads.
+int main()
+{
+  std::mt19937 rng(7);
+  long outside = 0, twice = 0, missing = 0, wrong = 0, owners_without = 0;
+  for (int round = 0; round < 20000; ++round) {
+    const int log2 = 1 + int(rng() % 3), vocab = 1 + int(rng() % 40), none = int(rng() % 3 ? 0 : rng() % 9);
+    const int64_t kept = rng() % 90, n = kept + none;
+    const int kinds = 1 + int(rng() % vocab);
+    std::vector<uint32_t> ids(n, 0xFFFFFFFFu);
+    for (int64_t i = 0; i < kept; ++i) ids[i] = rng() % kinds;
+    std::sort(ids.begin(), ids.begin() + kept, [](uint32_t a, uint32_t b) { return a % 8 != b % 8 ? a % 8 < b % 8 : a < b; });
+    const int64_t blocks = (n + (1 << log2) - 1) >> log2;
+    std::vector<int> puts(blocks, 0);
+    std::vector<gtk::LongSum> got(blocks, gtk::LongSum{0, 99});
+    for (int64_t i = kept; i < n; ++i)  // the blocks that end behind the last share
+      if (i + 1 == n || (i + 1) % (1 << log2) == 0) ++puts[i >> log2], got[i >> log2] = gtk::LongSum{0xFFFFFFFFu, 0};
+    int64_t begin = 0;
+    for (uint32_t owner = 0; owner < 8; ++owner) {
+      int64_t end = begin;
+      while (end < kept && ids[end] % 8 == owner) ++end;
+      owners_without += begin == end;
+      for (int thread = 0; thread < 4; ++thread)
+        gtk::each_long_sum(
+            begin, end, n, log2, thread, 4,
+            [&](int64_t place) {
+              if (place < begin || place >= end) ++outside;
+              return place < 0 || place >= n ? 0u : ids[place];
+            },
+            [&](int64_t block, const gtk::LongSum& L) {
+              if (block < 0 || block >= blocks) return void(++outside);
+              ++puts[block];
+              got[block] = L;
+            });
+      begin = end;
+    }
+    std::vector<uint32_t> parts(blocks, 0);
+    for (int64_t s = 0; s < kept;) {
+      int64_t e = s;
+      while (e < kept && ids[e] == ids[s]) ++e;
+      const int64_t a = s >> log2, b = (e - 1) >> log2;
+      if (b >= a + 2) parts[a] = uint32_t(b - a + 1);
+      s = e;
+    }
+    for (int64_t b = 0; b < blocks; ++b) {
+      twice += puts[b] > 1, missing += puts[b] == 0;
+      const int64_t last = std::min((b + 1) << log2, n) - 1;
+      wrong += puts[b] && (got[b].parts != parts[b] || (parts[b] && got[b].id != ids[last]));
+    }
+  }
+  std::printf("outside=%ld twice=%ld missing=%ld wrong=%ld\n", outside, twice, missing, wrong);
+  return owners_without > 1000 ? 0 : 1;
+}
+"""
+
+
+def test_long_sums_are_found_by_one_owner_from_its_own_tokens(tmp_path):
+    """What k_embed_grad_sort does to find the sums that are cut into parts, run on the CPU: no owner looks at another's tokens, which
+    that one may be moving, and each block's entry is one owner's, those without tokens included."""
+    import os
+    import subprocess
+
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "gpu-tokenizer_b200", "csrc")
+    (tmp_path / "t.cpp").write_text(LONG_SUMS)
+    subprocess.run(["g++", "-O1", "-std=c++17", "-I", csrc, "t.cpp", "-o", "t"], cwd=tmp_path, check=True)
+    run = subprocess.run([str(tmp_path / "t")], capture_output=True, text=True, timeout=120)
+    assert run.returncode == 0 and run.stdout == "outside=0 twice=0 missing=0 wrong=0\n", run.stdout
+
+
 # ---------------------------------------------------------------------------------------------------- on the GPU
 @pytest.fixture(scope="module")
 def tok(native_built, merges_path):
@@ -295,6 +373,21 @@ def test_embed_grad_of_many_tokens(tok, n, vocab, dim, kind):
     work = embed_grad(tok, ids, grad, "f32", vocab, dim, table, "f32", spare=4096)
     check_embed_grad(ids, grad, vocab, dim, 1.0, None, table, "f32")
     assert bool((work[-4096:] == 0xAB).all())
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 13, 101, 1003])
+@pytest.mark.parametrize("dim", [16, 23])
+def test_embed_grad_with_owners_that_have_no_token(tok, n, dim):
+    """All ids in the lowest of the 128 residue classes that the tokens are dealt out by; no whole number of blocks."""
+    import torch
+
+    vocab = 1000
+    ids = (some_ids(n, n, 7, "text") * 128 + some_ids(n + 1, n, 5, "text")).clamp(max=vocab - 1).to(torch.int32)
+    grad = torch.randn(n, dim, device="cuda")
+    table = torch.full((vocab, dim), 3.0, device="cuda")
+    embed_grad(tok, ids, grad, "f32", vocab, dim, table, "f32")
+    check_embed_grad(ids, grad, vocab, dim, 1.0, None, table, "f32")
 
 
 @pytest.mark.gpu
