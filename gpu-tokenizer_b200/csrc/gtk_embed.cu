@@ -239,7 +239,7 @@ int bits_of(int64_t x)
   return b;
 }
 
-constexpr size_t kSharedMost = 96 << 10;  // of a CTA
+constexpr size_t kSharedGroups = 96 << 10;  // of a CTA, where it has the choice of fewer groups
 constexpr int kMinBlockLog2 = 3, kMaxBlockLog2 = 10;
 
 GradPlan grad_plan(int64_t n, int64_t vocab, int64_t dim)
@@ -909,7 +909,7 @@ cudaError_t launch_embed_grad(const gtk::HandleView& v, const GradPlan& p, GradA
   const unsigned columns = (ALIGNED ? group : group - 1) * E, slabs = unsigned((a.dim + columns - 1) / columns);
   const size_t bytes     = size_t(GroupShared(int(group), 1 << a.block_log2).bytes());
   unsigned groups = group > 32 ? 1 : 128 / group;
-  while (groups * group > 32 && groups > 1 && groups * bytes > kSharedMost) groups /= 2;
+  while (groups * group > 32 && groups > 1 && groups * bytes > kSharedGroups) groups /= 2;
   e = gtk::launch_behind(k_embed_grad_sums<O, T, ALIGNED>, dim3(unsigned((p.blocks + groups - 1) / groups), slabs), dim3(group, groups), groups * bytes,
                   v.stream, a, static_cast<const O*>(grad_out), table);
   if (e == cudaSuccess && p.blocks > 2)  // a long sum begins in one block, fills the next and goes on

@@ -111,16 +111,23 @@ cudaError_t with_type(int type, F&& f)
   }
 }
 
+// A kernel whose calls want more than the usual 48 KiB of dynamic shared memory is allowed all that a CTA can have, whatever this
+// call wants: the limit belongs to the kernel on the device, and another thread's call of another size, under another handle's lock,
+// must not find it lowered between the two calls here.
+constexpr int kSharedMost = 227 << 10;
+template <class... Formal>
+cudaError_t allow_shared(void (*kernel)(Formal...), size_t smem)
+{
+  return smem > (48 << 10) ? cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSharedMost) : cudaSuccess;
+}
+
 template <class... Formal, class... Args>
 cudaError_t launch(void (*kernel)(Formal...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args&&... args)
 {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid, cfg.blockDim = block, cfg.dynamicSmemBytes = smem, cfg.stream = stream;
-  if (smem > (48 << 10)) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
-    if (e != cudaSuccess) return e;
-  }
-  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Formal>(args)...);
+  const cudaError_t e = allow_shared(kernel, smem);
+  return e != cudaSuccess ? e : cudaLaunchKernelEx(&cfg, kernel, static_cast<Formal>(args)...);
 }
 
 // the same for a kernel that begins with await_kernel(): its blocks may take their places while the kernel in front of it
@@ -134,11 +141,8 @@ cudaError_t launch_behind(void (*kernel)(Formal...), dim3 grid, dim3 block, size
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = grid, cfg.blockDim = block, cfg.dynamicSmemBytes = smem, cfg.stream = stream;
   cfg.attrs = &attr, cfg.numAttrs = 1;
-  if (smem > (48 << 10)) {
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, int(smem));
-    if (e != cudaSuccess) return e;
-  }
-  return cudaLaunchKernelEx(&cfg, kernel, static_cast<Formal>(args)...);
+  const cudaError_t e = allow_shared(kernel, smem);
+  return e != cudaSuccess ? e : cudaLaunchKernelEx(&cfg, kernel, static_cast<Formal>(args)...);
 }
 
 // the same in clusters of `cluster` blocks next to each other

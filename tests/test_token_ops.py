@@ -998,3 +998,46 @@ def test_gradient_of_one_row_for_all(tok, name):
                                 grad_stride=stride)
         same(grad, want, bound + want.abs() * half_step(name) * 1.01 + tiny(name) + 1e-36, "grad")
         assert marks_untouched(whole, n, vocab, stride, 0)
+
+
+@pytest.mark.gpu
+def test_two_threads_with_calls_of_different_sizes(native_built, merges_path):
+    """A handle for each of two threads on one device, whose calls want different amounts of shared memory, above 48 KiB all of
+    them: 2048 columns of 16 bits, sums in blocks of 8, 16 and 32 tokens."""
+    import threading
+
+    import torch
+
+    vocab, dim = 300, 2048
+    handles = [Tokenizer(merges_path, 2048, 50, device=0) for _ in range(2)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    work = [[], []]
+    for i, sizes in enumerate(((2048,), (32768, 8192))):
+        handles[i].set_stream(streams[i].cuda_stream)
+        for n in sizes:
+            grad = torch.randn(n, dim, device="cuda").to(torch.bfloat16)
+            work[i].append((some_ids(n, n, vocab, "text"), grad, torch.empty(vocab, dim, device="cuda"),
+                            torch.empty(handles[i].embed_grad_workspace(n, vocab, dim), device="cuda", dtype=torch.uint8)))
+    torch.cuda.synchronize()
+    start, failed = threading.Barrier(2), []
+
+    def run(i):
+        try:
+            start.wait()
+            for _ in range(2000 // len(work[i])):
+                for ids, grad, table, space in work[i]:
+                    handles[i].embed_grad(ids.data_ptr(), ids.numel(), grad.data_ptr(), "bf16", vocab, dim, table.data_ptr(), "f32",
+                                          space.data_ptr(), space.numel())
+        except Exception as e:  # noqa: BLE001
+            failed.append(e)
+
+    threads = [threading.Thread(target=run, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not failed, failed
+    for i in range(2):
+        for ids, grad, table, _ in work[i]:
+            check_embed_grad(ids, grad, vocab, dim, 1.0, None, table, "f32")
