@@ -185,6 +185,7 @@ int run_operator(gtk_tokenizer* h, Check&& check, Launches&& launches) noexcept
     if (e == cudaSuccess) e = launches(v);
     if (before >= 0 && before != v.device) cudaSetDevice(before);
     if (e != cudaSuccess) {
+      cudaGetLastError();  // reported here: the thread's next call, which asks for the last error behind its launches, has its own
       *v.last_error = std::string("launch: ") + cudaGetErrorString(e);
       return GTK_ERR_CUDA;
     }

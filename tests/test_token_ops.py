@@ -1041,3 +1041,37 @@ def test_two_threads_with_calls_of_different_sizes(native_built, merges_path):
     for i in range(2):
         for ids, grad, table, _ in work[i]:
             check_embed_grad(ids, grad, vocab, dim, 1.0, None, table, "f32")
+
+
+@pytest.mark.gpu
+def test_a_failed_launch_is_the_calls_own(native_built, merges_path, oracle, novel):
+    """A launch that CUDA refuses on the host (on the legacy stream while a stream that waits for it is being captured) is reported
+    by its call, and by no later one."""
+    import ctypes
+
+    import torch
+
+    t = Tokenizer(merges_path, 2048, 50, device=0)
+    t.set_stream(0)
+    ids = torch.tensor([3, 1], device="cuda", dtype=torch.int32)
+    table, out = torch.randn(10, 8, device="cuda"), torch.full((2, 8), 5.0, device="cuda")
+    torch.cuda.synchronize()
+    want, _, _, _ = t.encode(novel[:5000])
+    runtime = ctypes.CDLL("libcudart.so.12")         # another copy of the runtime than the one that the library holds
+    stream, graph = ctypes.c_void_p(), ctypes.c_void_p()
+    assert runtime.cudaStreamCreate(ctypes.byref(stream)) == 0
+    assert runtime.cudaStreamBeginCapture(stream, 2) == 0
+    try:
+        with pytest.raises(GtkError) as e:
+            t.embed(ids.data_ptr(), 2, table.data_ptr(), "f32", 10, 8, out.data_ptr(), "f32")
+    finally:
+        runtime.cudaStreamEndCapture(stream, ctypes.byref(graph))
+        if graph:
+            runtime.cudaGraphDestroy(graph)
+        runtime.cudaStreamDestroy(stream)
+        runtime.cudaGetLastError()
+    assert e.value.code == 3 and "launch" in str(e.value)
+    got, _, _, _ = t.encode(novel[:5000])
+    assert np.array_equal(got, want)
+    t.embed(ids.data_ptr(), 2, table.data_ptr(), "f32", 10, 8, out.data_ptr(), "f32")
+    assert torch.equal(out, table[ids.long()])
