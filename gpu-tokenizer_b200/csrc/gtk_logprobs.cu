@@ -667,7 +667,7 @@ struct GradRow {
     e   = ENTROPY ? __ldg(a.grad_entropy + r) * -scale : 0.f;
     H   = ENTROPY ? __ldg(a.entropy + r) : 0.f;
     lse = __ldg(a.lse + r);
-    nothing = lse == -INFINITY || (t < 0 && !ENTROPY);
+    nothing = lse == -INFINITY || (g == 0.f && e == 0.f);  // whatever the row holds: padding may be NaN, and 0 * NaN is no zero
   }
   __device__ __forceinline__ float of(float x, int column) const
   {

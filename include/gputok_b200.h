@@ -351,7 +351,7 @@ GTK_API int gtk_token_logprobs(gtk_tokenizer* h, const void* d_logits, int type,
  *   grad_logits[r][j] = scale * (g * ([j == t] - p_j) - e * p_j * (log p_j + entropy[r]))
  * d_lse and d_entropy are what gtk_token_logprobs has given for the same logits and scale.  d_grad_entropy may be NULL
  * (then d_entropy is not read), and so may d_grad_logprob (then d_targets is not read).  A row whose target is negative
- * or >= vocab has g = 0; rows that neither part reaches, and rows of nothing but -inf, get zeros whatever they hold.
+ * or >= vocab has g = 0; rows with g = 0 and e = 0, and rows of nothing but -inf, get zeros whatever they hold.
  * d_grad_logits has the type of the logits and may be d_logits itself with the same stride; no other overlap. */
 GTK_API int gtk_token_logprobs_grad(gtk_tokenizer* h, const void* d_logits, int type, int64_t n_rows, int64_t vocab,
                                     int64_t stride, float scale, const int32_t* d_targets, const float* d_lse,

@@ -1075,3 +1075,37 @@ def test_a_failed_launch_is_the_calls_own(native_built, merges_path, oracle, nov
     assert np.array_equal(got, want)
     t.embed(ids.data_ptr(), 2, table.data_ptr(), "f32", 10, 8, out.data_ptr(), "f32")
     assert torch.equal(out, table[ids.long()])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("vocab,shift", [(1000, 0), (4099, 0), (4099, 1)])
+def test_rows_that_no_gradient_reaches(tok, name, vocab, shift):
+    """Rows with both parts of their gradient zero (a loss mask, padding) get zeros whatever they and their statistics hold;
+    a zero of one part alone takes nothing from the other."""
+    import torch
+
+    n, nan = 6, math.nan
+    _, x = rows(some_logits(3, n, vocab, "plain"), name)
+    targets = torch.tensor([1, 2, 3, -1, vocab, 4], device="cuda", dtype=torch.int32)
+    g = torch.tensor([0.0, -0.0, 0.0, 3.0, nan, 1.0], device="cuda")
+    e = torch.tensor([0.0, 0.0, 0.5, 0.0, -0.0, 0.0], device="cuda")
+    lse, H, want, bound = grad_wanted(x, targets, 1.0, g, e)
+    lse, H = lse.float(), H.float()
+    for r in (1, 3, 4):                # what the padding of a batch may hold
+        x[r] = nan
+        x[r, ::2] = math.inf
+        lse[r] = H[r] = nan
+    bound = bound + want.abs() * half_step(name) * 1.01 + tiny(name) + 1e-36
+    none = torch.tensor([0, 1, 3, 4], device="cuda")
+    for entropy in (True, False):
+        whole, out = rows(torch.ones(n, vocab, device="cuda"), name, vocab, shift)
+        tok.token_logprobs_grad(x.data_ptr(), name, n, vocab, targets.data_ptr(), lse.data_ptr(), g.data_ptr(), out.data_ptr(),
+                                H.data_ptr() if entropy else 0, e.data_ptr() if entropy else 0)
+        assert bool((out[none] == 0).all()), entropy
+        assert marks_untouched(whole, n, vocab, vocab, shift)
+        same(out[5:], want[5:], bound[5:], "log probability alone")
+        if entropy:
+            same(out[2:3], want[2:3], bound[2:3], "entropy alone")
+        else:
+            assert bool((out[2] == 0).all())
