@@ -3,7 +3,8 @@
 //
 // With k = scale * log2(e), m a row's maximum and y_j = (x_j - m) k:  S = sum 2^y_j,  lse = scale m + ln S,
 // log p_t = scale (x_t - m) - ln S,  H = ln S - ln 2 (sum 2^y_j y_j) / S.  Both sums are formed in one pass with the maximum so
-// far and moved when that rises.  dx_j = scale (g ([j = t] - p_j) - e p_j (log p_j + H)) needs lse and H only.
+// far and moved when that rises.  dx_j = scale (g ([j = t] - p_j) - e p_j (log p_j + H)) needs lse and H only, where 32 bits of lse
+// still hold ln S.
 //
 // All of it is bound by memory, and just so: an element costs one exponential (16 a clock and SM) and some four further
 // instructions.  Measured against a copy (6.45 TB/s):
@@ -651,27 +652,100 @@ struct ScoreGradArgs {
   const float *lse, *entropy, *grad_logprob, *grad_entropy;
 };
 
-// d = scale * (g * ([j == t] - p) - e * p * (log p + H)), log p = scale * x - lse.  Every element is read and written once, by
+// From this size on lse no longer does for p = exp(scale * x - lse): it is scale * m + ln S rounded to 32 bits, off by up to 2^-24 of itself,
+// and that is the relative error of p (7.6e-6 below 256, a 64th of what rounding to fp16 costs).  A row filled with the lowest number of
+// its type, which is how many a mask is written, keeps nothing of ln S at all, and scale * m may be beyond 32 bits where ln S is a small
+// number.  Such rows are summed again from their logits, as k_token_logprobs has done it, which costs a second reading by one CTA
+// (8192 rows of 50257 bf16 262 us, all far 362; 4096 of f32 273 and 379; one row 6.1 and 16.4): the limit is above the 100 or so that the
+// logits of models in use lie around.
+constexpr float kFarLse = 256.f;
+
+// The highest of a row and the sum of 2^((x - highest) k), by all threads of a CTA.
+template <class T>
+__device__ __noinline__ float2 sum_row(const T* x, int vocab, float k)
+{
+  using P         = Pack16<T>;
+  constexpr int E = P::kElems;
+  __shared__ float s_m[kWarps], s_s[kWarps];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const RowParts<T> row(x, vocab);
+  RowSum sum;
+  if (tid < row.head + row.tail) sum.add(gtk::to_float(row.x[row.loose_column(tid)]), k);
+  for (int p0 = tid; p0 < row.packs; p0 += kBatch * kThreads) {
+    uint4 raw[kBatch];
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) {
+      constexpr uint32_t w = P::kMinusInf;
+      raw[q] = p0 + q * kThreads < row.packs ? *row.pack(p0 + q * kThreads) : make_uint4(w, w, w, w);
+    }
+#pragma unroll
+    for (int q = 0; q < kBatch; ++q) {
+      const typename P::Max all = P::highest(raw[q]);
+      const float high          = P::kHalves == 2 ? fmaxf(P::of(all, 0), P::of(all, 1)) : P::of(all, 0);
+      if (high > sum.m) sum.raise(high, k);
+      Two pairs[E / 2];
+      P::pairs(raw[q], pairs);
+#pragma unroll
+      for (int j = 0; j < E / 2; ++j) {
+        float x0, x1;
+        pairs[j].get(x0, x1);
+        sum.s += pow2((x0 - sum.m) * k) + pow2((x1 - sum.m) * k);
+      }
+    }
+  }
+  float high = sum.m;
+#pragma unroll
+  for (int d = 16; d; d >>= 1) high = fmaxf(high, __shfl_xor_sync(0xFFFFFFFFu, high, d));
+  sum.raise(high, k);
+#pragma unroll
+  for (int d = 16; d; d >>= 1) sum.s += __shfl_xor_sync(0xFFFFFFFFu, sum.s, d);
+  if (lane == 0) s_m[warp] = sum.m, s_s[warp] = sum.s;
+  __syncthreads();
+  float m = s_m[0];
+  for (int w = 1; w < kWarps; ++w) m = fmaxf(m, s_m[w]);
+  float s = 0.f;
+  for (int w = 0; w < kWarps; ++w) {
+    RowSum o;
+    o.m = s_m[w], o.s = s_s[w];
+    o.raise(m, k);
+    s += o.s;
+  }
+  return make_float2(m, s);
+}
+
+// d = scale * (g * ([j == t] - p) - e * p * (log p + H)), log p = scale * (x - m) - log_sum.  With m = 0 and log_sum = lse in all rows but
+// far ones, where sum_again() finds both.  Every element is read and written once, by
 // the same thread, so that grad may be logits.  A row's elements are shared by `parts` CTAs: as many as it has batches, up to 32 CTAs
-// per SM in all (1021 rows of 32003 fp16 with entropy: 25 us, with up to 8 28 us; 2000 of them 42 and 46).
+// per SM in all (1021 rows of 32003 fp16 with entropy: 25 us, with up to 8 28 us; 2000 of them 42 and 46).  A far row is its first CTA's
+// alone, which has read all of it before it writes.
 template <class T, bool ENTROPY>
 struct GradRow {
-  float scale, lse, g, e, H;
+  float scale, m, log_sum, g, e, H;
   int t;
-  bool nothing;
-  __device__ GradRow(const ScoreGradArgs& a, int64_t r) : scale(a.scale)
+  bool nothing, far;
+  __device__ GradRow(const ScoreGradArgs& a, int64_t r) : scale(a.scale), m(0.f)
   {
     t   = a.grad_logprob ? __ldg(a.targets + r) : -1;
     if (t >= a.vocab) t = -1;
     g   = t >= 0 ? __ldg(a.grad_logprob + r) * -scale : 0.f;
     e   = ENTROPY ? __ldg(a.grad_entropy + r) * -scale : 0.f;
     H   = ENTROPY ? __ldg(a.entropy + r) : 0.f;
-    lse = __ldg(a.lse + r);
-    nothing = lse == -INFINITY || (g == 0.f && e == 0.f);  // whatever the row holds: padding may be NaN, and 0 * NaN is no zero
+    log_sum = __ldg(a.lse + r);
+    // Whatever the row holds: padding may be NaN, and 0 * NaN is no zero.  Up to a scale of 1 no number becomes -inf: all are masked
+    nothing = (g == 0.f && e == 0.f) || (log_sum == -INFINITY && scale <= 1.f);
+    far     = !nothing && fabsf(log_sum) >= kFarLse;
   }
+  // for a far row, by all threads of a CTA
+  __device__ __forceinline__ void sum_again(const T* x, int vocab)
+  {
+    const float2 found = sum_row(x, vocab, scale * kLog2e);
+    m = found.x, log_sum = logf(found.y);
+    nothing = found.y == 0.f;
+  }
+  template <bool NEAR = false>  // NEAR: m is known to be 0
   __device__ __forceinline__ float of(float x, int column) const
   {
-    const float z = fmaf(x, scale, -lse), p = pow2(z * kLog2e);
+    const float z = fmaf(NEAR ? x : x - m, scale, -log_sum), p = pow2(z * kLog2e);
     const float d = p * (ENTROPY ? fmaf(e, fmaxf(z, -1e4f) + H, g) : g);
     return column == t ? d - g : d;
   }
@@ -685,19 +759,23 @@ __global__ void __launch_bounds__(kThreads) k_token_logprobs_grad(const T* logit
   const int part  = int(blockIdx.x % unsigned(parts)), tid = threadIdx.x;
   const RowParts<T> row(logits + r * a.stride, a.vocab);
   T* to = grad + r * a.grad_stride;
-  const GradRow<T, ENTROPY> R(a, r);
+  GradRow<T, ENTROPY> R(a, r);
+  if (R.far) {
+    if (part != 0) return;
+    R.sum_again(row.x, a.vocab);
+  }
   if (part == 0 && tid < row.head + row.tail) {
     const int c = row.loose_column(tid);
     to[c]       = gtk::from_float<T>(R.nothing ? 0.f : R.of(gtk::to_float(row.x[c]), c));
   }
-  const int share = (row.packs + parts - 1) / parts;
+  const int share = R.far ? row.packs : (row.packs + parts - 1) / parts;
   const int begin = part * share, end = min(row.packs, begin + share);
   uint4* out = reinterpret_cast<uint4*>(to + row.head);
   if (R.nothing) {
     for (int p = begin + tid; p < end; p += kThreads) out[p] = make_uint4(0u, 0u, 0u, 0u);
     return;
   }
-  const Two scale2(R.scale, R.scale), lse2(-R.lse, -R.lse), log2e2(kLog2e, kLog2e), g2(R.g, R.g), e2(R.e, R.e), H2(R.H, R.H);
+  const Two scale2(R.scale, R.scale), m2(-R.m, -R.m), log_sum2(-R.log_sum, -R.log_sum), log2e2(kLog2e, kLog2e), g2(R.g, R.g), e2(R.e, R.e), H2(R.H, R.H);
   for (int p0 = begin + tid; p0 < end; p0 += kBatch * kThreads) {
     uint4 raw[kBatch];
 #pragma unroll
@@ -713,7 +791,7 @@ __global__ void __launch_bounds__(kThreads) k_token_logprobs_grad(const T* logit
       const int at = R.t - row.pack_column(p);
 #pragma unroll
       for (int j = 0; j < E / 2; ++j) {
-        const Two z = fma2(x[j], scale2, lse2);
+        const Two z = fma2(x[j] + m2, scale2, log_sum2);
         float y0, y1;
         (z * log2e2).get(y0, y1);
         const Two p2(pow2(y0), pow2(y1));
@@ -742,7 +820,7 @@ __global__ void __launch_bounds__(kThreads) k_token_logprobs_grad(const T* logit
 }
 
 // The same where logits and gradient lie differently against 16-byte boundaries: element by element, with
-// kPlainBatch loads in flight (2048 rows of 50257 bf16: 100 us, one load at a time 228, in packs where they lie alike 69; f32 143
+// kPlainBatch loads in flight (2048 rows of 50257 bf16: 95 us, one load at a time 228, in packs where they lie alike 69; f32 143
 // and 134).
 constexpr int kPlainBatch = 8;
 template <class T, bool ENTROPY>
@@ -752,17 +830,25 @@ __global__ void __launch_bounds__(kThreads) k_token_logprobs_grad_plain(const T*
   const int part  = int(blockIdx.x % unsigned(parts));
   const T* x      = logits + r * a.stride;
   T* to           = grad + r * a.grad_stride;
-  const GradRow<T, ENTROPY> R(a, r);
-  for (int64_t c0 = int64_t(part) * kPlainBatch * kThreads + threadIdx.x; c0 < a.vocab; c0 += int64_t(parts) * kPlainBatch * kThreads) {
-    T raw[kPlainBatch];
+  GradRow<T, ENTROPY> R(a, r);
+  auto all = [&](auto near, int first, int step) {
+    for (int64_t c0 = int64_t(first) * kPlainBatch * kThreads + threadIdx.x; c0 < a.vocab; c0 += int64_t(step) * kPlainBatch * kThreads) {
+      T raw[kPlainBatch];
 #pragma unroll
-    for (int q = 0; q < kPlainBatch; ++q)
-      if (c0 + q * kThreads < a.vocab) raw[q] = x[c0 + q * kThreads];
+      for (int q = 0; q < kPlainBatch; ++q)
+        if (c0 + q * kThreads < a.vocab) raw[q] = x[c0 + q * kThreads];
 #pragma unroll
-    for (int q = 0; q < kPlainBatch; ++q) {
-      const int64_t c = c0 + q * kThreads;
-      if (c < a.vocab) to[c] = gtk::from_float<T>(R.nothing ? 0.f : R.of(gtk::to_float(raw[q]), int(c)));
+      for (int q = 0; q < kPlainBatch; ++q) {
+        const int64_t c = c0 + q * kThreads;
+        if (c < a.vocab) to[c] = gtk::from_float<T>(R.nothing ? 0.f : R.template of<decltype(near)::value>(gtk::to_float(raw[q]), int(c)));
+      }
     }
+  };
+  if (!R.far) {
+    all(std::true_type{}, part, parts);
+  } else if (part == 0) {
+    R.sum_again(x, a.vocab);
+    all(std::false_type{}, 0, 1);
   }
 }
 

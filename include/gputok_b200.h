@@ -349,7 +349,10 @@ GTK_API int gtk_token_logprobs(gtk_tokenizer* h, const void* d_logits, int type,
 
 /* The gradient of sum_r grad_logprob[r] * logprob[r] + grad_entropy[r] * entropy[r] with respect to the logits:
  *   grad_logits[r][j] = scale * (g * ([j == t] - p_j) - e * p_j * (log p_j + entropy[r]))
- * d_lse and d_entropy are what gtk_token_logprobs has given for the same logits and scale.  d_grad_entropy may be NULL
+ * d_lse and d_entropy are what gtk_token_logprobs has given for the same logits and scale.  p_j is formed from d_lse, whose 32
+ * bits are off by up to 2^-24 of itself, and p_j by as much of p_j; rows whose d_lse is 256 or more in size (logits with a large common
+ * part, a mask of the type's lowest value in every column) have their sum formed again, to the precision of
+ * gtk_token_logprobs, by a second reading.  d_grad_entropy may be NULL
  * (then d_entropy is not read), and so may d_grad_logprob (then d_targets is not read).  A row whose target is negative
  * or >= vocab has g = 0; rows with g = 0 and e = 0, and rows of nothing but -inf, get zeros whatever they hold.
  * d_grad_logits has the type of the logits and may be d_logits itself with the same stride; no other overlap. */

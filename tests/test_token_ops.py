@@ -1109,3 +1109,95 @@ def test_rows_that_no_gradient_reaches(tok, name, vocab, shift):
             same(out[2:3], want[2:3], bound[2:3], "entropy alone")
         else:
             assert bool((out[2] == 0).all())
+
+
+def far_logits(seed, n, vocab, name, kind):
+    """Rows whose log of the sum is large next to what tells their logits apart, in values of the type."""
+    import torch
+
+    t = dtype(name)
+    x = some_logits(seed, n, vocab, "plain")
+    if kind == "lowest":               # masked with the type's lowest value, every third row all of it
+        x = x.to(t)
+        x[:, ::2] = torch.finfo(t).min
+        x[::3] = torch.finfo(t).min
+        return x
+    if kind == "highest":              # every third row at the other end, scale times which is no 32-bit number; one of -inf
+        x = x.to(t)
+        x[::3] = torch.finfo(t).max
+        x[1::3] = torch.finfo(t).min
+        x[1, ::3] = -math.inf
+        x[n - 1] = -math.inf
+        return x
+    if kind == "masked":
+        x[:, 1::3] = -math.inf
+        x[n // 2] = -math.inf
+    return (x + {"up": 3e4, "masked": -2e4, "down": -1e3}[kind]).to(t)
+
+
+def grad_from_maximum(x, targets, scale, g, e, H, H_err):
+    """grad_wanted() with log p_j = scale (x_j - m) - ln S in 64 bits, and a bound that is relative to p: of lse only what
+    the header allows, 2^-24 of it below 256."""
+    import torch
+
+    n, vocab = x.shape
+    scale = float(np.float32(scale))
+    raw = x.double()
+    top = raw.amax(1)
+    none = top == -math.inf
+    m = torch.where(none, torch.zeros_like(top), top)
+    y = (raw - m[:, None]) * scale
+    log_s = torch.where(none, torch.zeros_like(top), y.exp().sum(1).log())
+    logp = y - log_s[:, None]
+    p = torch.where(none[:, None], torch.zeros_like(y), logp.exp())
+    y = y.clamp(min=-1e4)
+    logp = logp.clamp(min=-1e4)
+    lse = m * scale + log_s
+    t = targets.long()
+    inside = (t >= 0) & (t < vocab) & ~none
+    zero = torch.zeros(n, device="cuda", dtype=torch.float64)
+    g = zero if g is None else torch.where(inside, g.double(), zero)
+    e = zero if e is None else e.double()
+    here = (torch.arange(vocab, device="cuda")[None] == t[:, None]) & inside[:, None]
+    inner = logp + H.double()[:, None]
+    d = g[:, None] * (here.double() - p) - e[:, None] * p * inner
+    # S as in score_wanted(); y and log p: a rounding of the difference, one of the product, one of the sum, and ln S's own three
+    steps = (vocab / 256 + 8) * 4 + 64
+    of_sum = steps * U + 2.0 ** -22 + 4 * U * (-(p * logp).sum(1)) + 3 * U * log_s.abs()
+    of_lse = torch.where(lse.abs() < 256, 2 * U * lse.abs(), zero)
+    err_z = (of_sum + of_lse)[:, None] + U * (2 * y.abs() + 3 * logp.abs())
+    size = g[:, None].abs() + (e[:, None] * inner).abs()
+    bound = p * (err_z + 2.0 ** -22) * size + e[:, None].abs() * p * (err_z + H_err[:, None] + 4 * U * inner.abs())
+    bound = bound + p.clamp(max=2.0 ** -126) * (g[:, None].abs() + e[:, None].abs() * (inner.abs() + 1)) + 4 * U * (g[:, None].abs() * (here.double() + p) + (e[:, None] * p * inner).abs())
+    return d * scale, bound * scale
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("kind,scale", [("lowest", 1.0), ("lowest", 0.7), ("lowest", 1.3), ("highest", 1.3), ("up", 1.0), ("masked", 0.9), ("down", 1.0)])
+@pytest.mark.parametrize("n,vocab,stride,shift", [(3, 1000, 1000, 0), (5, 50257, 50257, 0), (7, 8193, 8200, 3), (700, 2053, 2056, 1), (2, 5, 5, 0)])
+def test_gradient_where_the_sum_is_far_from_the_logits(tok, name, kind, scale, n, vocab, stride, shift):
+    """The gradient from the statistics that token_logprobs gives for the same rows: 32 bits of lse say little about them."""
+    import torch
+
+    x_all, x = rows(far_logits(n + vocab, n, vocab, name, kind), name, stride, shift)
+    targets = some_ids(vocab, n, vocab, "wrong" if n > 4 else "text")
+    gen = torch.Generator(device="cuda").manual_seed(n)
+    g, e = torch.randn(n, generator=gen, device="cuda"), torch.randn(n, generator=gen, device="cuda")
+    _, H, lse, _, _ = score(tok, x, name, targets, 0, scale, stride)
+    H_err = score_wanted(x, targets, 0, scale)[1][1]
+    before = x.clone()
+    for entropy in (False, True):
+        want, bound = grad_from_maximum(before, targets, scale, g, e if entropy else None, H, H_err)
+        bound = bound + want.abs() * half_step(name) * 1.01 + tiny(name) + 1e-36
+        more = dict(d_entropy=H.data_ptr(), d_grad_entropy=e.data_ptr()) if entropy else {}
+        for out_stride, out_shift in ((stride, shift), (stride + 1, shift + 1)):
+            whole, out = rows(torch.ones(n, vocab, device="cuda"), name, out_stride, out_shift)
+            tok.token_logprobs_grad(x.data_ptr(), name, n, vocab, targets.data_ptr(), lse.data_ptr(), g.data_ptr(), out.data_ptr(), scale=scale,
+                                    stride=stride, grad_stride=out_stride, **more)
+            same(out, want, bound, (entropy, out_stride))
+            assert marks_untouched(whole, n, vocab, out_stride, out_shift)
+    tok.token_logprobs_grad(x.data_ptr(), name, n, vocab, targets.data_ptr(), lse.data_ptr(), g.data_ptr(), x.data_ptr(), scale=scale, stride=stride,
+                            grad_stride=stride, **more)
+    same(x, want, bound, "in place")
+    assert marks_untouched(x_all, n, vocab, stride, shift)
