@@ -2,6 +2,7 @@
 #include <algorithm>
 #include <cmath>
 
+#include "gtk_checked.cuh"
 #include "gtk_long_sums.hpp"
 #include "gtk_rows.cuh"
 
@@ -324,7 +325,7 @@ __device__ void sort_digit(const uint2* from, uint32_t count, uint2* to, int shi
     const bool here      = i0 + lane < count;
     const uint32_t digit = here ? (from[i0 + lane].x >> shift) & uint32_t(bins - 1) : 0xFFFFFFFFu;
     const uint32_t peers = peers_of(digit);
-    if (here && (peers >> lane) == 1u) S.at[warp][digit] += __popc(peers);
+    if (here && (peers >> lane) == 1u && GTK_IN(digit, 1 << kMaxDigitBits, 200)) S.at[warp][digit] += __popc(peers);
     __syncwarp();
   }
   __syncthreads();
@@ -364,7 +365,7 @@ __device__ void sort_digit(const uint2* from, uint32_t count, uint2* to, int shi
     __syncwarp();
     if (here && (peers >> lane) == 1u) S.at[warp][digit] = place + 1u;  // the last of the peers
     __syncwarp();
-    if (here) to[place] = x;
+    if (here && GTK_IN(place, all, 201)) to[place] = x;
   }
   __syncthreads();
 }
@@ -422,8 +423,8 @@ __device__ void group_tokens(const SortArgs& a, SortShared& S, uint32_t& begin, 
   const uint32_t owner = blockIdx.x, lanes_below = (1u << lane) - 1u;
   const uint32_t owner4 = owner * 0x01010101u;
   uint32_t lower = 0, mine = 0;
-  // The tokens of one step that are this owner's to to[], in order; returns how many.
-  auto take = [&](const uint32_t (&id)[4], const Owners& o, int64_t i, uint2* to, uint32_t room) {
+  // The tokens of one step that are this owner's to to[], in order, as far as there is room; returns how many.
+  auto take = [&](const uint32_t (&id)[4], const Owners& o, int64_t i, uint2* to, uint32_t room, const uint2* whole, int64_t size) {
     uint32_t bits = o.equal(owner4);
     if (owner == kOwners - 1)
 #pragma unroll
@@ -434,7 +435,7 @@ __device__ void group_tokens(const SortArgs& a, SortShared& S, uint32_t& begin, 
     if (!__any_sync(0xFFFFFFFFu, bits & (bits - 1))) {  // one per lane at most
       const uint32_t at = __popc(lanes & lanes_below);
       const int j       = __clz(__brev(bits)) >> 3;
-      if (bits && at < room) to[at] = make_uint2(j == 0 ? id[0] : j == 1 ? id[1] : j == 2 ? id[2] : id[3], uint32_t(i + j));
+      if (bits && at < room && GTK_IN(to + at - whole, size, 202)) to[at] = make_uint2(j == 0 ? id[0] : j == 1 ? id[1] : j == 2 ? id[2] : id[3], uint32_t(i + j));
       return uint32_t(__popc(lanes));
     }
     uint32_t total = 0, at = 0;
@@ -447,7 +448,7 @@ __device__ void group_tokens(const SortArgs& a, SortShared& S, uint32_t& begin, 
 #pragma unroll
     for (int j = 0; j < 4; ++j)
       if (bits >> (8 * j + 7) & 1u) {
-        if (at < room) to[at] = make_uint2(id[j], uint32_t(i + j));
+        if (at < room && GTK_IN(to + at - whole, size, 203)) to[at] = make_uint2(id[j], uint32_t(i + j));
         ++at;
       }
     return total;
@@ -455,7 +456,7 @@ __device__ void group_tokens(const SortArgs& a, SortShared& S, uint32_t& begin, 
   scan_ids(a, warp, lane, [&](const uint32_t (&id)[4], int64_t i) {
     const Owners o(id, a.vocab);
     lower += __popc(o.below(owner4));
-    mine += take(id, o, i, S.list[warp] + mine, mine < kListRoom ? kListRoom - mine : 0u);
+    mine += take(id, o, i, S.list[warp] + mine, mine < kListRoom ? kListRoom - mine : 0u, S.list[warp], kListRoom);
   });
   lower = __reduce_add_sync(0xFFFFFFFFu, lower);
   if (lane == 0) S.lower[warp] = lower, S.mine[warp] = mine;
@@ -473,19 +474,20 @@ __device__ void group_tokens(const SortArgs& a, SortShared& S, uint32_t& begin, 
   if (count == 0) return;
   if (!listed) {
     uint2* to = a.tokens0 + begin + at;
-    scan_ids(a, warp, lane, [&](const uint32_t (&id)[4], int64_t i) { to += take(id, Owners(id, a.vocab), i, to, 128u); });
+    scan_ids(a, warp, lane, [&](const uint32_t (&id)[4], int64_t i) { to += take(id, Owners(id, a.vocab), i, to, 128u, a.tokens0, a.n); });
     __syncthreads();
   }
   if (listed && count <= kRankMost) {  // each token's place is the number of those in front of it
     uint64_t* const keys = reinterpret_cast<uint64_t*>(S.at);
-    for (uint32_t k = lane; k < mine; k += 32) keys[at + k] = uint64_t(S.list[warp][k].x) << 32 | S.list[warp][k].y;
+    for (uint32_t k = lane; k < mine; k += 32)
+      if (GTK_IN(at + k, kRankMost, 204)) keys[at + k] = uint64_t(S.list[warp][k].x) << 32 | S.list[warp][k].y;
     __syncthreads();
     if (tid < int(count)) {
       const uint64_t key = keys[tid];
       uint32_t place     = 0;
 #pragma unroll 8
       for (uint32_t k = 0; k < count; ++k) place += keys[k] < key;
-      (a.passes & 1 ? a.tokens1 : a.tokens0)[begin + place] = make_uint2(uint32_t(key >> 32), uint32_t(key));
+      if (GTK_IN(place, count, 205)) (a.passes & 1 ? a.tokens1 : a.tokens0)[begin + place] = make_uint2(uint32_t(key >> 32), uint32_t(key));
     }
     __syncthreads();
     return;
@@ -521,8 +523,11 @@ k_embed_grad_sort(const SortArgs a, T* __restrict__ grad_table, int dim, int64_t
   if (a.n > 0) group_tokens(a, S, begin, count);
   const uint2* tokens = (a.passes & 1 ? a.tokens1 : a.tokens0) + begin;
   gtk::each_long_sum(
-      begin, int64_t(begin) + count, a.n, a.block_log2, threadIdx.x, kSortThreads, [&](int64_t place) { return tokens[place - begin].x; },
-      [&](int64_t block, const LongSum& L) { a.long_sums[block] = L; });
+      begin, int64_t(begin) + count, a.n, a.block_log2, threadIdx.x, kSortThreads,
+      [&](int64_t place) { return GTK_IN(place - begin, count, 206) ? tokens[place - begin].x : kNoId; },
+      [&](int64_t block, const LongSum& L) {
+        if (GTK_IN(block, (a.n + (int64_t(1) << a.block_log2) - 1) >> a.block_log2, 207)) a.long_sums[block] = L;
+      });
   if (!clear) return;
   // the rows of this owner that have no token, as many at once as the shared memory has bits
   uint32_t* used        = &S.at[0][0];
@@ -537,11 +542,11 @@ k_embed_grad_sort(const SortArgs a, T* __restrict__ grad_table, int dim, int64_t
 #pragma unroll 4
     for (uint32_t i = threadIdx.x; i < count; i += kSortThreads) {
       const int64_t r = int64_t(tokens[i].x >> kOwnersLog2) - r0;
-      if (r >= 0 && r < here && !(used[r >> 5] >> (r & 31) & 1u)) atomicOr(used + (r >> 5), 1u << (r & 31));
+      if (r >= 0 && r < here && GTK_IN(r >> 5, kSortWarps << kMaxDigitBits, 208) && !(used[r >> 5] >> (r & 31) & 1u)) atomicOr(used + (r >> 5), 1u << (r & 31));
     }
     __syncthreads();
     for (int r = warp; r < here; r += kSortWarps)
-      if (!(used[r >> 5] >> (r & 31) & 1u)) clear_row(grad_table + (((r0 + r) << kOwnersLog2) + blockIdx.x) * table_stride, dim, lane, 32);
+      if (!(used[r >> 5] >> (r & 31) & 1u) && GTK_IN(((r0 + r) << kOwnersLog2) + blockIdx.x, a.vocab, 209)) clear_row(grad_table + (((r0 + r) << kOwnersLog2) + blockIdx.x) * table_stride, dim, lane, 32);
   }
 }
 
@@ -567,6 +572,7 @@ __device__ __forceinline__ void store_sum(T* row, int valid, bool packs, float s
 struct GradArgs {
   const uint2* tokens;  // grouped {id, place}, those of no id behind them
   int64_t n;
+  uint32_t vocab;
   LongSum* long_sums;  // one per block
   int dim;
   int block_log2;
@@ -680,7 +686,8 @@ __global__ void __launch_bounds__(kGradThreads) k_embed_grad_sums(const GradArgs
   const uint32_t left = begin > 0 && begin < a.n ? __ldcg(&a.tokens[begin - 1].x) : kNoId;
   const uint32_t far_left = begin > length && begin < a.n ? __ldcg(&a.tokens[begin - length - 1].x) : kNoId;
   for (int i = lane; i < shared.tokens; i += group) {
-    const uint2 token = begin + i < a.n ? __ldcg(a.tokens + begin + i) : make_uint2(kNoId, 0u);
+    uint2 token = begin + i < a.n ? __ldcg(a.tokens + begin + i) : make_uint2(kNoId, 0u);
+    if (!GTK_IN(token.y, a.n, 210)) token = make_uint2(kNoId, 0u);
     ids[i]     = token.x;
     address[i] = reinterpret_cast<uint64_t>(grad_out + first + int64_t(token.y) * a.out_stride);
   }
@@ -713,7 +720,7 @@ __global__ void __launch_bounds__(kGradThreads) k_embed_grad_sums(const GradArgs
   auto request = [&](int chunk) {
     for (int k = lane >> 5; k < kChunk; k += warps) {
       const int i = chunk * kChunk + k;
-      if (i < at || i >= stop) continue;
+      if (i < at || i >= stop || !GTK_IN(i, shared.tokens, 211)) continue;
       const uint64_t row    = address[i];
       const uint32_t shift  = ALIGNED ? 0u : uint32_t(row) & 15u;
       const char* from      = reinterpret_cast<const char*>(row - shift) + copier * 16;
@@ -721,7 +728,7 @@ __global__ void __launch_bounds__(kGradThreads) k_embed_grad_sums(const GradArgs
       const int pieces      = int((shift + width_bytes + 15u) >> 4) - copier;
 #pragma unroll
       for (int p = 0; p < kGradThreads; p += 32)
-        if (p < pieces) gtk::copy16(slot + p * 16, from + p * 16);
+        if (p < pieces && GTK_IN(to + k * slot_bytes + (copier + p) * 16 - ring_at, kChunk * kChunks * group * 16, 212) && GTK_IN(copier + p, group, 213)) gtk::copy16(slot + p * 16, from + p * 16);
         else break;
     }
     gtk::end_chunk();
@@ -746,7 +753,8 @@ __global__ void __launch_bounds__(kGradThreads) k_embed_grad_sums(const GradArgs
     for (int j = 0; j < S::kCount / 2; ++j) sum[j].get(x[2 * j], x[2 * j + 1]);
 #pragma unroll
     for (int u = 0; u < S::kUnits; ++u)
-      if (some >> u & 1u) {  // whole units: the pitch is a multiple of them
+      if ((some >> u & 1u) && GTK_IN(first + own + u * kStep * S::kUnit + S::kUnit - 1, a.pitch, 214) &&
+          GTK_IN(block << a.block_log2, a.n, 215)) {  // whole units: the pitch is a multiple of them
         Pack<float, S::kUnit> p;
 #pragma unroll
         for (int j = 0; j < S::kUnit; ++j) p.e[j] = x[u * S::kUnit + j];
@@ -759,6 +767,7 @@ __global__ void __launch_bounds__(kGradThreads) k_embed_grad_sums(const GradArgs
       from_left = false;
       return;
     }
+    if (!GTK_IN(id, a.vocab, 216)) return;
     T* row           = grad_table + int64_t(id) * a.table_stride + first + own;
     const bool packs = ALIGNED || reinterpret_cast<uintptr_t>(row) % (sizeof(T) * S::kUnit) == 0;
     float x[S::kCount];
@@ -791,7 +800,7 @@ __global__ void __launch_bounds__(kGradThreads) k_embed_grad_sums(const GradArgs
   for (int j = 0; j < S::kCount / 2; ++j) sum[j] = Two(0.f, 0.f);
   uint32_t id = ids[at];
   const uint4* rows = ring;
-  for (; chunk * kChunk < stop; ++chunk) {
+  for (; chunk * kChunk < stop && GTK_IN(chunk * kChunk + kChunk - 1, shared.tokens, 217); ++chunk) {
     gtk::await_chunks<kChunks - 2>();
     if (group > 32) __syncthreads();
     else __syncwarp(mask);
@@ -851,7 +860,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_embed_grad_join(const GradArgs
 #pragma unroll
         for (uint32_t k = 0; k < 8; ++k) {
           const uint32_t i = min(i0 + k, to - 1);
-          x[k]             = __ldcg(reinterpret_cast<const float4*>(part + (2 * int64_t(i) + (i == 0 ? 1 : 0)) * a.pitch));
+          if (GTK_IN(first + at + i, blocks, 218)) x[k]             = __ldcg(reinterpret_cast<const float4*>(part + (2 * int64_t(i) + (i == 0 ? 1 : 0)) * a.pitch));
         }
 #pragma unroll
         for (uint32_t k = 0; k < 8; ++k)
@@ -861,7 +870,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_embed_grad_join(const GradArgs
   };
   auto store = [&](uint32_t id, const float4& sum) {
     const float y[4] = {sum.x, sum.y, sum.z, sum.w};
-    if (c < a.dim) store_sum<T, 4>(grad_table + int64_t(id) * a.table_stride + c, a.dim - c, packs, a.scale, a.accumulate, y);
+    if (c < a.dim && GTK_IN(id, a.vocab, 219)) store_sum<T, 4>(grad_table + int64_t(id) * a.table_stride + c, a.dim - c, packs, a.scale, a.accumulate, y);
   };
   // the same for every warp
   const uint32_t few = __ballot_sync(0xFFFFFFFFu, mine.parts > 0 && mine.parts <= kJoinAlone), many = __ballot_sync(0xFFFFFFFFu, mine.parts > kJoinAlone);
@@ -996,7 +1005,7 @@ extern "C" GTK_API int gtk_embed_grad(gtk_tokenizer* h, const int32_t* d_ids, in
     if (n_ids == 0 && accumulate) return cudaSuccess;
     const GradPlan p = grad_plan(n_ids, vocab, dim);
     unsigned char* work = static_cast<unsigned char*>(d_workspace);
-    const GradArgs a{nullptr, n_ids, reinterpret_cast<LongSum*>(work + p.at_long), int(dim), p.block_log2, out_stride, table_stride, p.pitch,
+    const GradArgs a{nullptr, n_ids, uint32_t(vocab), reinterpret_cast<LongSum*>(work + p.at_long), int(dim), p.block_log2, out_stride, table_stride, p.pitch,
                      scale, accumulate != 0, reinterpret_cast<float*>(work + p.at_parts)};
     const bool aligned = gtk::rows_aligned(d_grad_out, out_stride, out_type, 8) && gtk::rows_aligned(d_grad_table, table_stride, table_type, 8);
     return gtk::with_type(out_type, [&](auto o) {
@@ -1009,3 +1018,8 @@ extern "C" GTK_API int gtk_embed_grad(gtk_tokenizer* h, const int32_t* d_ids, in
     });
   });
 }
+
+#ifdef GTK_CHECKED
+cudaError_t gtk::embed_check_words(int sum[4], bool reset) { return add_check_words(sum, reset); }
+cudaError_t gtk::embed_check_selftest() { return check_selftest(299); }
+#endif

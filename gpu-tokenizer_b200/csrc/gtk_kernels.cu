@@ -20,6 +20,7 @@
 // by latency and issue throughput, so there is no tensor-core code.
 // Kernels report trouble through a status word and never trap; every loop is
 // bounded.  -DGTK_CHECKED adds range checks on every data-dependent index.
+#include "gtk_checked.cuh"
 #include "gtk_device.cuh"
 #include "gtk_table.hpp"
 
@@ -30,28 +31,6 @@
 namespace gtk {
 namespace {
 
-
-// Checked build (-DGTK_CHECKED): every index into shared memory, the lane scratch, the staging buffer and the
-// per-chunk / per-unit arrays that is computed from data is compared with its limit before it is used.  A
-// violation is recorded (first failing check, offending value, limit, number of violations) and the access is
-// skipped, so a wrong index shows up as a report, never as a fault; read the record with
-// gtk_debug_check_words.  Without the flag the checks compile to nothing.
-#ifdef GTK_CHECKED
-__device__ int g_check_words[4];
-__device__ __noinline__ bool check_failed(int id, long long value, long long limit)
-{
-  if (atomicAdd(&g_check_words[3], 1) == 0) {
-    g_check_words[0] = id;
-    g_check_words[1] = int(value);
-    g_check_words[2] = int(limit);
-  }
-  return false;
-}
-#define GTK_IN(value, limit, id) \
-  ((static_cast<unsigned long long>(value) < static_cast<unsigned long long>(limit)) || check_failed((id), (long long)(value), (long long)(limit)))
-#else
-#define GTK_IN(value, limit, id) true
-#endif
 
 constexpr uint32_t NONE = 0xFFFFu;  // pair not mergeable
 constexpr uint32_t SEL  = 0xFFFEu;  // pair selected for the current pass
@@ -1968,28 +1947,17 @@ int launch_encode_small(const EncodeBuffers& b, const DeviceTable& t, cudaStream
 #ifdef GTK_CHECKED
 // Checked build only: the record of index checks that failed since the last reset ([0] id of the first failing
 // check, [1] its value, [2] its limit, [3] number of failures), plus a self-test of the mechanism: a kernel
-// evaluates one check that must fail and skips the guarded store.
-__global__ void k_check_selftest(int* sink)
-{
-  const int bad = 5 + int(threadIdx.x);
-  if (GTK_IN(bad, 4, 99)) sink[bad] = 1;
-}
-
+// evaluates one check that must fail and skips the guarded store (selftest 1 in this file, 2 gtk_embed.cu, 3 gtk_logprobs.cu).
 extern "C" __attribute__((visibility("default"))) int gtk_debug_check_words(int out[4], int reset, int selftest)
 {
-  if (selftest) {
-    int* sink = nullptr;
-    if (cudaMalloc(&sink, 64) != cudaSuccess) return -1;
-    k_check_selftest<<<1, 1>>>(sink);
-    cudaDeviceSynchronize();
-    cudaFree(sink);
-  }
-  if (cudaDeviceSynchronize() != cudaSuccess) return -1;
-  if (cudaMemcpyFromSymbol(out, g_check_words, sizeof(int) * 4) != cudaSuccess) return -1;
-  if (reset) {
-    const int z[4] = {0, 0, 0, 0};
-    cudaMemcpyToSymbol(g_check_words, z, sizeof(z));
-  }
+  cudaError_t e = cudaSuccess;
+  if (selftest == 1) e = check_selftest(99);
+  if (selftest == 2) e = gtk::embed_check_selftest();
+  if (selftest == 3) e = gtk::logprobs_check_selftest();
+  if (e != cudaSuccess || cudaDeviceSynchronize() != cudaSuccess) return -1;
+  for (int i = 0; i < 4; ++i) out[i] = 0;
+  for (auto add : {add_check_words, gtk::embed_check_words, gtk::logprobs_check_words})
+    if (add(out, reset != 0) != cudaSuccess) return -1;
   return 0;
 }
 #endif

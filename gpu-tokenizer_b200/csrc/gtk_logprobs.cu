@@ -20,6 +20,7 @@
 #include <initializer_list>
 #include <type_traits>
 
+#include "gtk_checked.cuh"
 #include "gtk_rows.cuh"
 
 namespace {
@@ -234,7 +235,7 @@ __device__ __forceinline__ void collect_keys(const RowParts<T>& row, int begin, 
         const uint32_t key = value_key(P::of(best[q], half));
         if (key && key >= bound) {
           const int at = atomicAdd(&S.sets, 1);
-          if (at < kMostSets) S.set[at] = tid << 8 | q << 4 | half;
+          if (at < kMostSets && GTK_IN(at, kThreads, 300)) S.set[at] = tid << 8 | q << 4 | half;
         }
       }
   }
@@ -259,7 +260,10 @@ __device__ __forceinline__ void collect_keys(const RowParts<T>& row, int begin, 
     }
     if (tid == 0) S.sets = 0;
     __syncthreads();
-    if (key && key >= floor) S.set[atomicAdd(&S.sets, 1)] = tid << 8;
+    if (key && key >= floor) {
+      const int at = atomicAdd(&S.sets, 1);
+      if (GTK_IN(at, kThreads, 301)) S.set[at] = tid << 8;
+    }
     __syncthreads();
   }
   const int step = by_set ? kBatch * threads : threads;
@@ -268,8 +272,9 @@ __device__ __forceinline__ void collect_keys(const RowParts<T>& row, int begin, 
   // f(key) for the elements of the i-th pack of the sets that reach the bound
   auto each_key = [&](uint32_t i, auto&& f) {
     const uint32_t at = i / each;
+    if (!GTK_IN(at, kThreads, 302)) return;
     const int w = S.set[at], p = begin + (w >> 8) + (w >> 4 & 15) * threads + int(i - at * each) * step;
-    if (p >= end) return;
+    if (p >= end || !GTK_IN(p, row.packs, 303)) return;
     const uint4 raw = __ldg(row.pack(p));
     const T* x      = reinterpret_cast<const T*>(&raw);
 #pragma unroll
@@ -282,7 +287,7 @@ __device__ __forceinline__ void collect_keys(const RowParts<T>& row, int begin, 
   auto offer = [&](uint64_t key) {
     if (key == 0 || key < floor) return;
     const int at = atomicAdd(&S.keys, 1);
-    if (at < most) S.key[at] = key;
+    if (at < most && GTK_IN(at, kMostKeys, 304)) S.key[at] = key;
   };
 #pragma unroll 1
   for (uint32_t i = tid; i < packs; i += threads) each_key(i, offer);
@@ -308,7 +313,7 @@ __device__ __forceinline__ void collect_keys(const RowParts<T>& row, int begin, 
     for (int w = 0; w < threads / 32; ++w) high = max(high, S.best[w]);
     __syncthreads();
     if (high == 0) break;
-    if (tid == 0) S.key[found] = high;
+    if (tid == 0 && GTK_IN(found, kMostKeysOfPart, 305)) S.key[found] = high;
     below = high;
   }
   if (tid == 0) S.keys = found;
@@ -331,7 +336,7 @@ __device__ __forceinline__ bool collect_few(const RowParts<T>& row, int begin, i
   const float reach  = bound ? key_value(floor) : -FLT_MAX;  // -inf is no alternative
   auto offer = [&](float x, int column) {
     const int at = atomicAdd(&S.keys, 1);
-    if (at < most) S.key[at] = rank_key(x, uint32_t(column));
+    if (at < most && GTK_IN(at, kMostKeys, 306)) S.key[at] = rank_key(x, uint32_t(column));
   };
   int sets = 0;
 #pragma unroll
@@ -341,7 +346,7 @@ __device__ __forceinline__ bool collect_few(const RowParts<T>& row, int begin, i
       const bool reaches  = P::of(best[q], half) >= reach;
       const uint32_t some = __ballot_sync(0xFFFFFFFFu, reaches);
       const int at        = sets + __popc(some & ((1u << lane) - 1u));
-      if (reaches && at < room) set[at] = tid << 8 | q << 4 | half;
+      if (reaches && at < room && GTK_IN(set + at - S.set, kThreads, 307)) set[at] = tid << 8 | q << 4 | half;
       sets += __popc(some);
     }
   __syncwarp();
@@ -357,11 +362,13 @@ __device__ __forceinline__ bool collect_few(const RowParts<T>& row, int begin, i
         if (gtk::to_float(x[j]) >= reach && (P::kHalves == 1 || (j & 1) == half)) offer(gtk::to_float(x[j]), row.pack_column(p) + j);
     };
     for (int i = lane >> share_log2; i < sets; i += 32 >> share_log2) {
+      if (!GTK_IN(set + i - S.set, kThreads, 308)) break;
       const int w = set[i];
       for (int p = begin + (w >> 8) + ((w >> 4 & 15) + kBatch * (lane & ((1 << share_log2) - 1))) * threads; p < end; p += LOOK * stride) {
         uint4 raw[LOOK];
 #pragma unroll
-        for (int q = 0; q < LOOK; ++q) raw[q] = __ldg(row.pack(p + q * stride < end ? p + q * stride : p));
+        for (int q = 0; q < LOOK; ++q)
+          if (GTK_IN(p + q * stride < end ? p + q * stride : p, row.packs, 309)) raw[q] = __ldg(row.pack(p + q * stride < end ? p + q * stride : p));
 #pragma unroll
         for (int q = 0; q < LOOK; ++q)
           if (p + q * stride < end) look(raw[q], p + q * stride, w & 1);
@@ -382,12 +389,12 @@ __device__ __forceinline__ void rank_keys(const TopScratch& S, int n, int top_k,
 {
 #pragma unroll 1
   for (int i = threadIdx.x; i < max(n, top_k); i += blockDim.x) {
-    const uint64_t key = i < n ? S.key[i] : 0u;
+    const uint64_t key = i < n && GTK_IN(i, kMostKeys, 310) ? S.key[i] : 0u;
     int above          = i < n ? 0 : i;  // nothing comes behind all that there is
     if (i < n)
 #pragma unroll 4
       for (int j = 0; j < n; ++j) above += S.key[j] > key;
-    if (above < top_k) put(above, key);
+    if (above < top_k && GTK_IN(above, top_k, 311)) put(above, key);
   }
 }
 
@@ -531,6 +538,7 @@ __global__ void __launch_bounds__(kThreads, kResident<T, ENTROPY, TOP>) k_token_
   float log_sum = logf(all.s);  // -inf: nothing allowed, NaN: no distribution
   auto put = [&](int place, uint64_t key) {  // an alternative of the row, once `all` is the whole row's
     const bool broken = isnan(all.s);
+    if (key && !GTK_IN(key_column(key), a.vocab, 312)) return;
     if (a.top_ids) a.top_ids[r * a.top_k + place] = key && !broken ? int32_t(key_column(key)) : -1;
     if (a.top_logprobs)
       a.top_logprobs[r * a.top_k + place] = broken ? nan : key ? (key_value(key) - all.m) * a.scale - log_sum : -INFINITY;
@@ -594,7 +602,8 @@ __global__ void __launch_bounds__(kThreads, kResident<T, ENTROPY, TOP>) k_token_
         }
         for (int c = 1 + warp; c < parts; c += warps) {
           const int count = __shfl_sync(0xFFFFFFFFu, keys, c), at = __shfl_sync(0xFFFFFFFFu, upto, c) - count;
-          for (int i = lane; i < count; i += 32) s_top.key[at + i] = cluster.map_shared_rank(&s_top, c)->key[i];
+          for (int i = lane; i < count; i += 32)
+            if (GTK_IN(at + i, kMostKeys, 313) && GTK_IN(i, kMostKeysOfPart, 314)) s_top.key[at + i] = cluster.map_shared_rank(&s_top, c)->key[i];
         }
         __syncthreads();
         rank_keys(s_top, __shfl_sync(0xFFFFFFFFu, upto, parts - 1), a.top_k, put);
@@ -809,7 +818,7 @@ __global__ void __launch_bounds__(kThreads) k_token_logprobs_grad(const T* logit
         y.e[2 * j + 1] = gtk::from_float<T>(d1);
       }
       if (uint32_t(at) < uint32_t(E)) {  // the target's own element
-        const float d = R.of(gtk::to_float(row.x[R.t]), R.t);
+        const float d = GTK_IN(R.t, a.vocab, 315) ? R.of(gtk::to_float(row.x[R.t]), R.t) : 0.f;
 #pragma unroll
         for (int j = 0; j < E; ++j)
           if (j == at) y.e[j] = gtk::from_float<T>(d);
@@ -938,3 +947,8 @@ extern "C" GTK_API int gtk_token_logprobs_grad(gtk_tokenizer* h, const void* d_l
     });
   });
 }
+
+#ifdef GTK_CHECKED
+cudaError_t gtk::logprobs_check_words(int sum[4], bool reset) { return add_check_words(sum, reset); }
+cudaError_t gtk::logprobs_check_selftest() { return check_selftest(399); }
+#endif

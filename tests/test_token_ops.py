@@ -1201,3 +1201,26 @@ def test_gradient_where_the_sum_is_far_from_the_logits(tok, name, kind, scale, n
                             grad_stride=stride, **more)
     same(x, want, bound, "in place")
     assert marks_untouched(x_all, n, vocab, stride, shift)
+
+
+@pytest.mark.gpu
+def test_checked_build_of_the_operators(native_built):
+    """The library with index checks (-DGTK_CHECKED) through the small cases of this file, in a process of its own: no check of an
+    index may fail.  Before that a check in either source file is made to fail, and is reported with its number, value and limit."""
+    import os
+    import subprocess
+    import sys
+
+    from gputok_b200.capi import checked_library_path
+
+    path = checked_library_path()
+    probe = ("import ctypes,sys; lib=ctypes.CDLL(sys.argv[1]); w=(ctypes.c_int*4)()\n"
+             "for t in (2, 3, 0): print(lib.gtk_debug_check_words(w, 1, t), *w)")
+    out = subprocess.run([sys.executable, "-c", probe, path], capture_output=True, text=True, timeout=300)
+    assert out.stdout.split("\n")[:3] == ["0 299 5 4 1", "0 399 5 4 1", "0 0 0 0 0"], out.stdout + out.stderr
+    chosen = ("(test_embed or test_sums or test_ids or owners or two_handles or captured or token_logprobs or rows_without or far_from or "
+              "no_gradient) and not checked")
+    run = subprocess.run([sys.executable, "-m", "pytest", os.path.abspath(__file__), "-m", "gpu", "-x", "-q", "-s", "-k", chosen],
+                         capture_output=True, text=True, timeout=1500, env=dict(os.environ, GPUTOK_B200_LIBRARY=path))
+    assert run.returncode == 0, run.stdout[-3000:] + run.stderr[-2000:]
+    assert "CHECKED_BUILD rc=0 failures=0" in run.stdout, run.stdout[-2000:]
