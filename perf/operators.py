@@ -90,15 +90,20 @@ def draw(rng):
 
 
 @functools.lru_cache(maxsize=None)
-def _tokenizer():
+def _tokenizer_on(device, stream):
     for p in (ROOT, os.path.join(ROOT, "gpu-tokenizer_b200")):
         if p not in sys.path:
             sys.path.insert(0, p)
     import gputok_b200
 
-    tok = gputok_b200.Tokenizer(os.path.join(ROOT, "tests", "golden", "gpt2_merges.txt"), device=torch.cuda.current_device())
-    tok.set_stream(torch.cuda.current_stream().cuda_stream)
+    tok = gputok_b200.Tokenizer(os.path.join(ROOT, "tests", "golden", "gpt2_merges.txt"), device=device)
+    tok.set_stream(stream)
     return tok
+
+
+def _tokenizer():
+    """The handle for torch's current device and stream, which a state's inputs are made on and its passes run on."""
+    return _tokenizer_on(torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream)
 
 
 def _ids(g, n, vocab, padded):
