@@ -1224,3 +1224,42 @@ def test_checked_build_of_the_operators(native_built):
                          capture_output=True, text=True, timeout=1500, env=dict(os.environ, GPUTOK_B200_LIBRARY=path))
     assert run.returncode == 0, run.stdout[-3000:] + run.stderr[-2000:]
     assert "CHECKED_BUILD rc=0 failures=0" in run.stdout, run.stdout[-2000:]
+
+
+@pytest.mark.gpu
+def test_measured_cases_follow_the_current_stream(native_built):
+    """perf/operators.py: what is prepared under a stream runs on it, behind what the stream has in front, and goes into a graph that
+    is captured from it, whichever stream was the first."""
+    import importlib.util
+    import os
+
+    import torch
+
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "perf", "operators.py")
+    spec = importlib.util.spec_from_file_location("perf_operators", path)
+    ops = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(ops)
+    ops.own = True
+    case = dict(ops._embed("embed", 200, 1000, 64, "f32", "f32"), name="small")
+    first = ops.prepare(case, 1)
+    ops.run(first)
+    torch.cuda.synchronize()
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        state = ops.prepare(case, 2)
+        ops.run(state).fill_(0)
+        torch.cuda._sleep(50_000_000)            # some 25 ms
+        state["table"].mul_(2)
+        out = ops.run(state)
+        got = out.clone()
+    torch.cuda.synchronize()
+    want = state["table"][state["ids"].long()]
+    assert torch.equal(got, want)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        ops.run(state)
+    state["table"].mul_(2)
+    out.fill_(0)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want * 2)
