@@ -360,6 +360,39 @@ def test_embed_grad(tok, grad_type, table_type, n, vocab, dim, gs, ts, shift, ki
     assert torch.equal(again, table)
 
 
+def run_embed_grad(tok, grad_type, table_type, n, vocab, dim, gs, ts, shift, kind, accumulate):
+    import torch
+
+    g = torch.Generator(device="cuda").manual_seed(n + dim)
+    _, grad = rows(torch.randn(1 if gs == 0 else n, dim, generator=g, device="cuda"), grad_type, max(gs, dim), shift)
+    ids = some_ids(n, n, vocab, "text" if kind == "empty" else kind)
+    if kind == "empty":
+        ids.fill_(-1)
+    whole, table = rows(torch.randn(vocab, dim, generator=g, device="cuda"), table_type, ts, shift)
+    base = table.clone() if accumulate else None
+    embed_grad(tok, ids, grad, grad_type, vocab, dim, table, table_type, scale=0.75, accumulate=accumulate, out_stride=gs, table_stride=ts)
+    check_embed_grad(ids, grad.expand(n, dim) if gs == 0 else grad, vocab, dim, 0.75, base, table, table_type)
+    assert marks_untouched(whole, vocab, dim, ts, shift)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("grad_type,table_type", [("f32", "bf16"), ("f32", "f16"), ("bf16", "f16"), ("f16", "bf16")])
+@pytest.mark.parametrize("n,vocab,dim,gs,ts,shift,kind", GRAD_CASES)
+def test_embed_grad_of_mixed_types(tok, grad_type, table_type, n, vocab, dim, gs, ts, shift, kind, accumulate):
+    run_embed_grad(tok, grad_type, table_type, n, vocab, dim, gs, ts, shift, kind, accumulate)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("accumulate", [False, True])
+@pytest.mark.parametrize("grad_type,table_type", [("f32", "f32"), ("bf16", "f32"), ("f16", "f16"), ("f32", "bf16")])
+@pytest.mark.parametrize("kind", ["one", "text", "wrong"])
+@pytest.mark.parametrize("dim,shift", [(2051, 1), (4099, 1), (4099, 3), (1021, 0), (4104, 0), (8200, 0)])
+def test_embed_grad_of_several_slabs(tok, grad_type, table_type, kind, dim, shift, accumulate):
+    """More columns than a CTA takes at once, at any alignment, with sums of one block, of two and of many."""
+    run_embed_grad(tok, grad_type, table_type, 523, 150, dim, dim, dim + (8 if shift == 0 else 5), shift, kind, accumulate)
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("n,vocab,dim", [(70000, 300, 64), (150000, 50257, 40), (300000, 200000, 24), (1 << 20, 1 << 19, 8)])
 @pytest.mark.parametrize("kind", ["text", "one", "all"])
