@@ -198,7 +198,10 @@ cudaError_t launch_embed(const gtk::HandleView& v, const int32_t* ids, int64_t n
   while (group_log2 < 5 && (int64_t(4) << group_log2) < units) ++group_log2;
   while (group_log2 < 8 && (int64_t(1) << group_log2) < units && n << (group_log2 + 1) <= int64_t(v.sm_count) * 512) ++group_log2;
   const int64_t rows = (kEmbedThreads >> group_log2) * (many && V == 8 ? 2 : 1);
-  return gtk::launch(many && V == 8 ? k_embed<T, O, V, 2> : k_embed<T, O, V, 1>, dim3(unsigned((n + rows - 1) / rows)), dim3(kEmbedThreads), 0,
+  auto kernel        = k_embed<T, O, V, 1>;
+  if constexpr (V == 8)
+    if (many) kernel = k_embed<T, O, V, 2>;
+  return gtk::launch(kernel, dim3(unsigned((n + rows - 1) / rows)), dim3(kEmbedThreads), 0,
                      v.stream, ids, n, static_cast<const T*>(table), int(vocab), int(dim), table_stride, scale, static_cast<O*>(out), out_stride,
                      group_log2);
 }
