@@ -1455,6 +1455,8 @@ cudaError_t wait_for_word(volatile const int32_t* word, int32_t seq, cudaStream_
   return cudaSuccess;
 }
 
+std::mutex* handle_mutex(gtk_tokenizer* h) { return h ? &h->mu : nullptr; }
+
 bool handle_view(gtk_tokenizer* h, HandleView* out)
 {
   if (!h || !out) return false;
@@ -1465,7 +1467,6 @@ bool handle_view(gtk_tokenizer* h, HandleView* out)
   out->wide = h->wide;
   out->low_id_map = (h->device >= 0 && h->id_space == GTK_IDS_GPT2) ? h->d_low_map.as<uint16_t>() : nullptr;
   out->pinned_words = h->device >= 0 ? h->h_totals.as<int32_t>() + 8 : nullptr;
-  out->mu = &h->mu;
   out->last_error = &h->last_error;
   return true;
 }

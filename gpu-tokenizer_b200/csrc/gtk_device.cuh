@@ -168,10 +168,10 @@ struct HandleView {
   const uint16_t* low_id_map;  // nullptr, or the 256-entry remap of ids < 256 (GPT-2 id space selected)
   bool wide;                   // table beyond 16 bits (the allocation-free kernel is 16-bit only)
   int32_t* pinned_words;  // 8 ints of page-locked host memory owned by the handle
-  std::mutex* mu;
   std::string* last_error;
 };
-bool handle_view(gtk_tokenizer* h, HandleView* out);
+std::mutex* handle_mutex(gtk_tokenizer* h);  // nullptr for no handle
+bool handle_view(gtk_tokenizer* h, HandleView* out);  // under that mutex: another thread may be selecting a stream
 // waits for a kernel's last store, the call number, in page-locked memory; an error when the stream fails or goes idle without it
 cudaError_t wait_for_word(volatile const int32_t* word, int32_t seq, cudaStream_t stream);
 

@@ -970,10 +970,11 @@ extern "C" GTK_API int gtk_embed(gtk_tokenizer* h, const int32_t* d_ids, int64_t
 
 extern "C" GTK_API int gtk_embed_grad_workspace(gtk_tokenizer* h, int64_t n_ids, int64_t vocab, int64_t dim, size_t* workspace_bytes)
 {
-  gtk::HandleView v;
-  if (!gtk::handle_view(h, &v)) return GTK_ERR_INVALID_ARG;
+  if (!h) return GTK_ERR_INVALID_ARG;
   try {
-    std::lock_guard<std::mutex> lock(*v.mu);
+    std::lock_guard<std::mutex> lock(*gtk::handle_mutex(h));
+    gtk::HandleView v;
+    gtk::handle_view(h, &v);
     const gtk::Refusal why = !workspace_bytes ? "workspace_bytes is null" : refuse_sizes(n_ids, vocab, dim);
     if (why) {
       *v.last_error = why;

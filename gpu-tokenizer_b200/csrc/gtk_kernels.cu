@@ -2182,9 +2182,10 @@ extern "C" GTK_API int gtk_encode_chunks_noalloc(gtk_tokenizer* h, const uint8_t
                                                  const int64_t* d_chunk_offsets, int64_t n_chunks,
                                                  int32_t max_chunk_bytes, int32_t* d_out_ids, int32_t* d_out_counts)
 {
+  if (!h) return GTK_ERR_INVALID_ARG;
+  std::lock_guard<std::mutex> lock(*gtk::handle_mutex(h));
   gtk::HandleView v;
-  if (!gtk::handle_view(h, &v)) return GTK_ERR_INVALID_ARG;
-  std::lock_guard<std::mutex> lock(*v.mu);
+  gtk::handle_view(h, &v);
   auto fail = [&](int code, const std::string& msg) {
     *v.last_error = msg;
     return code;

@@ -166,11 +166,11 @@ using Refusal = const char*;
 template <class Check, class Launches>
 int run_operator(gtk_tokenizer* h, Check&& check, Launches&& launches) noexcept
 {
-  HandleView v;
-  if (!handle_view(h, &v)) return GTK_ERR_INVALID_ARG;
+  if (!h) return GTK_ERR_INVALID_ARG;
   try {
-    std::lock_guard<std::mutex> lock(*v.mu);
-    handle_view(h, &v);  // the stream as it is under the lock
+    std::lock_guard<std::mutex> lock(*handle_mutex(h));
+    HandleView v;
+    handle_view(h, &v);
     if (const Refusal why = check()) {
       *v.last_error = why;
       return GTK_ERR_INVALID_ARG;
