@@ -406,22 +406,26 @@ struct NoScratch {};
 // ring of batches in shared memory that runs on into the next row, 138 us as it is but with 256 threads, 130 us with 128.
 // Alternatives cost a row its end: the bound and the packs that are read again are waits one after another, in which the CTA asks
 // for nothing else (8192 rows of 8192 bf16: 29 us without, 37 with one, 47 with 20).
-// CTAs of kThreads per SM that registers are shared out for.  With 4 and 5, us: 8192 rows
-// of 50257 bf16 130 and 133, 4096 of them with entropy 80 and 76, with entropy and five alternatives 95 and 90; 999 of f32 with these
-// 40 and 45, 8192 rows of 8192 f32 with five alternatives 64 and 60.
-template <class T, bool ENTROPY, bool TOP>
-constexpr int kResident = (sizeof(T) == 2 ? TOP || ENTROPY : TOP && !ENTROPY) ? 5 : 4;
+// CTAs of kThreads per SM that registers are shared out for.  With 4 and 5, us: 8192 rows of 50257 bf16 130 and 133, 4096 of them with
+// entropy 80 and 76, with entropy and five alternatives 95 and 90; 999 of f32 with these 40 and 45, 8192 rows of 8192 f32 with
+// five alternatives 64 and 60.  fp16, whose conversions want more registers: 4096 rows of 50257 with entropy 72.5 and 73.6, with
+// entropy and 20 alternatives 98.6 and 97.8, with 20 alternatives alone 96.7 and 101 (spilled).  Parts of rows, of which an SM has two
+// at most: 74 rows of 50257 fp16 with entropy 10.4 and 12.4, with 20 alternatives too 14.4 and 16.4, bf16 14.5 and 16.4.
+template <class T, bool ENTROPY, bool TOP, bool SPLIT>
+constexpr int kResident =
+    !SPLIT && (sizeof(T) == 4 ? TOP && !ENTROPY : ENTROPY || (TOP && std::is_same<T, __nv_bfloat16>::value)) ? 5 : 4;
 
 // Packs that a thread reads again at a time.  8192 rows of 50257 bf16 with 20 alternatives: 167 us with two, 170 with one, 182 with four, for
-// want of registers; where there are more of them, 4096 rows of f32 with entropy too: 154 with four, 162 with two.
-template <class T, bool ENTROPY, bool TOP>
-constexpr int kLookAgain = kResident<T, ENTROPY, TOP> == 4 ? 4 : 2;
+// want of registers; 4096 of fp16 111 with two, 115 with four.  Where there are more of them, 4096 rows of f32 with entropy too: 154 with
+// four, 162 with two; 16 rows of f32 in parts: 14.4 and 16.4.
+template <class T, bool ENTROPY, bool SPLIT>
+constexpr int kLookAgain = SPLIT || (sizeof(T) == 4 && ENTROPY) ? 4 : 2;
 
 template <class T, bool ENTROPY, bool TOP, bool SPLIT>
-__global__ void __launch_bounds__(kThreads, kResident<T, ENTROPY, TOP>) k_token_logprobs(const T* __restrict__ logits, const ScoreArgs a, int n_parts)
+__global__ void __launch_bounds__(kThreads, kResident<T, ENTROPY, TOP, SPLIT>) k_token_logprobs(const T* __restrict__ logits, const ScoreArgs a, int n_parts)
 {
   const int parts     = SPLIT ? n_parts : 1;
-  constexpr int kLook = kLookAgain<T, ENTROPY, TOP>;
+  constexpr int kLook = kLookAgain<T, ENTROPY, SPLIT>;
   namespace cg = cooperative_groups;
   using P         = Pack16<T>;
   constexpr int E = P::kElems;
