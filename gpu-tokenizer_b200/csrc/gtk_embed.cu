@@ -216,13 +216,13 @@ cudaError_t launch_embed(const gtk::HandleView& v, const int32_t* ids, int64_t n
 //   k_embed_grad_join   adds the parts of the long ones from left to right
 // Every sum is thus formed in an order that the ids alone decide, in 32 bits, and rounded once.  A row of grad_out is read once and a
 // row of grad_table written once: that traffic is the floor, and the grouping, which the rows wait for, is what comes on top.
-// 32768 tokens of 768 bf16 to 50257 rows of f32: 57 us (28, 20 and 6.5 of the three; the last two begin while their predecessor
+// 32768 tokens of 768 bf16 to 50257 rows of f32: 57 us (30, 20 and 6.6 of the three; the last two begin while their predecessor
 // ends, which takes 4 us off), at the copy rate 32.  4096 tokens: 42 us, nearly all of it the 154 MB of zeros.  131072 tokens: 108
 // (43, 50, 14), at the copy rate 55.
 constexpr int kSortThreads = 1024, kSortWarps = kSortThreads / 32;
 // CTAs of k_embed_grad_sort, one to an SM.  All of them read all ids, from the second-level cache: no CTA waits for another and one
-// launch does it all, while up to some 100 000 ids the clearing of rows hides it (32768 tokens: 28 us, of which the zeros alone
-// take 24).  Beyond, the reading shows: 1M tokens, 350 us.  An id that a large part of the tokens has is one CTA's work:
+// launch does it all, while up to some 100 000 ids the clearing of rows hides it (32768 tokens and 154 MB of table: 30 us, without
+// clearing 11.4, clearing all of it without a token 26.7).  Beyond, the reading shows: 1M tokens, 350 us.  An id that a large part of the tokens has is one CTA's work:
 // 32768 tokens of which half have one id take 41 us here, all of them 82.
 constexpr int kOwnersLog2 = 7, kOwners = 1 << kOwnersLog2;
 constexpr int kMaxDigitBits = 9;                            // a thread per bin at most

@@ -297,6 +297,9 @@ GTK_API int gtk_encode_chunks_noalloc(gtk_tokenizer* h, const uint8_t* d_bytes, 
  *   - strides count elements between the starts of neighbouring rows.  An input's may be anything >= 0 (0: every row is
  *     the same one), an output's must be >= the row's length; what lies between an output's rows is left alone.
  *     Pointers must be aligned to their elements, no more; rows that start on multiples of 16 bytes are fastest;
+ *   - arrays may be read in whole pieces of 16 bytes, aligned to 16: up to 15 bytes in front of an input's first element and behind
+ *     its last one, in the same 16 bytes as that.  Nothing is made of them, and nothing outside the outputs is written;
+ *   - an output overlaps no input and no other output, unless it is said below that it may;
  *   - they are queued on the handle's stream (gtk_set_stream) and return without waiting, allocate nothing and may be
  *     captured into a CUDA graph (select the stream before the capture begins).  Only arguments that the host can see
  *     are reported; they are looked at before anything else, on host-only handles too.  The calling thread's current
