@@ -27,9 +27,10 @@ TEXTGEN = os.path.join(HERE, "libgtk_textgen.so")
 PYMOD = os.path.join(HERE, "gputok_gpu" + (sysconfig.get_config_var("EXT_SUFFIX") or ".so"))
 CLI = os.path.join(HERE, "gpu_tokenizer_blockbpe")
 
-CUDA_SOURCES = [os.path.join(CSRC, f) for f in ("gtk_kernels.cu", "gtk_api.cu", "gtk_embed.cu", "gtk_logprobs.cu", "gtk_table.cpp")]
+CUDA_SOURCES = [os.path.join(CSRC, f) for f in ("gtk_kernels.cu", "gtk_api.cu", "gtk_embed.cu", "gtk_logprobs.cu", "gtk_paged.cu",
+                                                "gtk_sample.cu", "gtk_table.cpp")]
 CUDA_DEPENDENCIES = CUDA_SOURCES + [os.path.join(CSRC, f) for f in (
-    "gtk_device.cuh", "gtk_tile.cuh", "gtk_rows.cuh", "gtk_checked.cuh", "gtk_long_sums.hpp", "gtk_table.hpp", "gtk_crew.hpp")] + [os.path.join(INCLUDE, "gputok_b200.h")]
+    "gtk_device.cuh", "gtk_tile.cuh", "gtk_rows.cuh", "gtk_logits.cuh", "gtk_checked.cuh", "gtk_long_sums.hpp", "gtk_table.hpp", "gtk_crew.hpp")] + [os.path.join(INCLUDE, "gputok_b200.h")]
 
 NVCC_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
               "-Xcompiler", "-fPIC,-fvisibility=hidden", "-shared", "-t", "0"]

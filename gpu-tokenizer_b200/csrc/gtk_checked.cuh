@@ -4,7 +4,8 @@
 // computed from data is compared with its limit before it is used.  A violation is recorded (first failing check, offending
 // value, limit, number of violations) and the access is skipped, so a wrong index shows up as a report, never as a fault; read the
 // record with gtk_debug_check_words.  Without the flag the checks compile to nothing.  Each source file has a record of its
-// own; the checks' numbers are below 100 in gtk_kernels.cu, 200 to 299 in gtk_embed.cu, 300 to 399 in gtk_logprobs.cu.
+// own; the checks' numbers are below 100 in gtk_kernels.cu, 200 to 299 in gtk_embed.cu, 300 to 399 in gtk_logprobs.cu,
+// 400 to 499 in gtk_paged.cu, 500 to 599 in gtk_sample.cu.
 #pragma once
 #ifdef GTK_CHECKED
 #include <cuda_runtime.h>
@@ -60,6 +61,10 @@ cudaError_t embed_check_words(int sum[4], bool reset);
 cudaError_t embed_check_selftest();
 cudaError_t logprobs_check_words(int sum[4], bool reset);
 cudaError_t logprobs_check_selftest();
+cudaError_t paged_check_words(int sum[4], bool reset);
+cudaError_t paged_check_selftest();
+cudaError_t sample_check_words(int sum[4], bool reset);
+cudaError_t sample_check_selftest();
 }  // namespace gtk
 #else
 #define GTK_IN(value, limit, id) true

@@ -1947,16 +1947,19 @@ int launch_encode_small(const EncodeBuffers& b, const DeviceTable& t, cudaStream
 #ifdef GTK_CHECKED
 // Checked build only: the record of index checks that failed since the last reset ([0] id of the first failing
 // check, [1] its value, [2] its limit, [3] number of failures), plus a self-test of the mechanism: a kernel
-// evaluates one check that must fail and skips the guarded store (selftest 1 in this file, 2 gtk_embed.cu, 3 gtk_logprobs.cu).
+// evaluates one check that must fail and skips the guarded store (selftest 1 in this file, 2 gtk_embed.cu, 3 gtk_logprobs.cu,
+// 4 gtk_paged.cu, 5 gtk_sample.cu).
 extern "C" __attribute__((visibility("default"))) int gtk_debug_check_words(int out[4], int reset, int selftest)
 {
   cudaError_t e = cudaSuccess;
   if (selftest == 1) e = check_selftest(99);
   if (selftest == 2) e = gtk::embed_check_selftest();
   if (selftest == 3) e = gtk::logprobs_check_selftest();
+  if (selftest == 4) e = gtk::paged_check_selftest();
+  if (selftest == 5) e = gtk::sample_check_selftest();
   if (e != cudaSuccess || cudaDeviceSynchronize() != cudaSuccess) return -1;
   for (int i = 0; i < 4; ++i) out[i] = 0;
-  for (auto add : {add_check_words, gtk::embed_check_words, gtk::logprobs_check_words})
+  for (auto add : {add_check_words, gtk::embed_check_words, gtk::logprobs_check_words, gtk::paged_check_words, gtk::sample_check_words})
     if (add(out, reset != 0) != cudaSuccess) return -1;
   return 0;
 }

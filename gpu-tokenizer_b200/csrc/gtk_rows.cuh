@@ -1,4 +1,4 @@
-// gtk_rows.cuh -- what the operators on rows of numbers share (gtk_embed.cu, gtk_logprobs.cu): element types,
+// gtk_rows.cuh -- what the operators on rows of numbers share (gtk_embed.cu, gtk_logprobs.cu, gtk_sample.cu, gtk_paged.cu): element types,
 // vector loads and stores, and the frame of their entry points.
 #pragma once
 #include <cuda_bf16.h>

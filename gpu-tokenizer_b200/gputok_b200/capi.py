@@ -90,6 +90,9 @@ def load_library() -> C.CDLL:
     lib.gtk_embed_grad.argtypes = [vp, vp, i64, vp, C.c_int, i64, f32, i64, i64, vp, C.c_int, i64, C.c_int, vp, C.c_size_t]
     lib.gtk_token_logprobs.argtypes = [vp, vp, C.c_int, i64, i64, i64, f32, vp, C.c_int, vp, vp, vp, vp, vp]
     lib.gtk_token_logprobs_grad.argtypes = [vp, vp, C.c_int, i64, i64, i64, f32, vp, vp, vp, vp, vp, vp, i64]
+    lib.gtk_sample.argtypes = [vp, vp, C.c_int, i64, i64, i64, vp, vp, vp, vp, vp, vp, vp]
+    lib.gtk_block_tables.argtypes = [vp, vp, vp, i64, C.c_int, vp, i64, i64, vp, i64, vp, vp]
+    lib.gtk_slot_map.argtypes = [vp, vp, vp, i64, C.c_int, vp, i64, i64, vp, i64, vp, vp, vp, vp]
     lib.gtk_pinned_alloc.argtypes = [C.c_size_t]
     lib.gtk_pinned_alloc.restype = vp
     lib.gtk_pinned_free.argtypes = [vp]
@@ -343,6 +346,30 @@ class Tokenizer:
                                                       vocab if stride is None else stride, scale, d_targets, d_lse, d_entropy,
                                                       d_grad_logprob, d_grad_entropy, d_grad_logits,
                                                       vocab if grad_stride is None else grad_stride))
+
+    # ------------------------------------------------------------------ a step of generation
+    def sample(self, d_logits: int, type: str, n_rows: int, vocab: int, d_uniform: int, d_ids: int, d_logprob: int = 0,
+               d_temperature: int = 0, d_top_k: int = 0, d_top_p: int = 0, d_min_p: int = 0, stride: int | None = None) -> None:
+        """An id drawn from every row of logits by the row's random number (float64 in [0, 1), negative: no request), with the
+        row's temperature (0: the highest logit), top-k, top-p and min-p, and the log probability that it was drawn with."""
+        self._check(self._lib.gtk_sample(self._h, d_logits, ELEMENT_TYPES[type], n_rows, vocab, vocab if stride is None else stride,
+                                         d_uniform, d_temperature, d_top_k, d_top_p, d_min_p, d_ids, d_logprob))
+
+    def block_tables(self, d_old_lengths: int, d_new_lengths: int, n_requests: int, block_tokens: int, d_tables: int, columns: int,
+                     d_queue: int, queue_capacity: int, d_state: int, d_state_out: int, table_stride: int | None = None) -> None:
+        """Takes the blocks that requests grow by from the queue into their rows of the table, and gives back those they lose.
+        ``d_state``: int64[3], places taken from and given to the queue so far, and (out) what is missing."""
+        self._check(self._lib.gtk_block_tables(self._h, d_old_lengths, d_new_lengths, n_requests, block_tokens, d_tables, columns,
+                                               columns if table_stride is None else table_stride, d_queue, queue_capacity, d_state,
+                                               d_state_out))
+
+    def slot_map(self, d_old_lengths: int, d_new_lengths: int, n_requests: int, block_tokens: int, d_tables: int, columns: int,
+                 capacity: int, d_slots: int, d_offsets: int, d_positions: int = 0, d_requests: int = 0, d_state: int = 0,
+                 table_stride: int | None = None) -> None:
+        """Slot in the cache, position and request of every new token, requests one after another, and where each begins."""
+        self._check(self._lib.gtk_slot_map(self._h, d_old_lengths, d_new_lengths, n_requests, block_tokens, d_tables, columns,
+                                           columns if table_stride is None else table_stride, d_state, capacity, d_slots, d_positions,
+                                           d_requests, d_offsets))
 
     # ------------------------------------------------------------------ decode
     def decode(self, ids) -> bytes:

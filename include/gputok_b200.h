@@ -364,6 +364,66 @@ GTK_API int gtk_token_logprobs_grad(gtk_tokenizer* h, const void* d_logits, int 
                                     const float* d_entropy, const float* d_grad_logprob, const float* d_grad_entropy,
                                     void* d_grad_logits, int64_t grad_stride);
 
+/* ---------------------------------------------------------------------------------------------------------------
+ * A step of generation around a model: where requests' tokens lie in a cache of blocks, and which ids come next (no
+ * counterpart in the reference, compare_generation_quality.py:418-459 leaves both to a framework).  What is said above
+ * of the operators on a model's arrays holds for these three as well.
+ * ------------------------------------------------------------------------------------------------------------- */
+
+/* Largest vocabulary that gtk_sample takes. */
+#define GTK_MAX_SAMPLE_VOCAB (1 << 20)
+
+/* Draws an id from every row of d_logits (vocab elements).  With m the row's highest logit, T its temperature and the
+ * columns ranked by logit, of equal ones the lower first:
+ *   the first d_top_k[r] columns stay (<= 0, or as many as there are: all); logits of -inf never do;
+ *   of these the fewest first ones whose weights exp((x_j - m) / T) reach d_top_p[r] of their sum (>= 1: all, <= 0: one);
+ *   of these the ones with exp((x_j - m) / T) >= d_min_p[r] (<= 0: all, > 1: as 1);
+ * and d_ids[r] is the lowest column at which the sum of the weights that are left, taken in the order of columns, exceeds
+ * d_uniform[r] times their whole sum.  d_logprob[r] is the logarithm of the drawn column's weight over that sum.  Any of
+ * d_temperature (then 1), d_top_k, d_top_p, d_min_p (then all) and d_logprob may be NULL.  Which columns stay and which one is
+ * drawn is decided as in 64-bit arithmetic, and does not depend on the run.
+ *   T == 0              the highest logit, of equal ones the lowest column, with log probability 0
+ *   d_uniform[r] < 0    no request: id -1, log probability 0, the row is not looked at
+ *   d_uniform[r] >= 1   the last column that is left
+ *   a row of -inf       id -1, log probability -inf
+ *   a row with a NaN or +inf, a NaN limit or random number, a negative, infinite or NaN temperature: id -1, log probability NaN
+ * n_rows < 2^31, vocab <= GTK_MAX_SAMPLE_VOCAB. */
+GTK_API int gtk_sample(gtk_tokenizer* h, const void* d_logits, int type, int64_t n_rows, int64_t vocab, int64_t stride,
+                       const double* d_uniform, const float* d_temperature, const int32_t* d_top_k, const float* d_top_p,
+                       const float* d_min_p, int32_t* d_ids, float* d_logprob);
+
+/* A step of n_requests requests that have d_old_lengths[r] tokens in a cache of blocks of block_tokens tokens and will have
+ * d_new_lengths[r].  Row r of d_tables holds the request's blocks, token j's in column j / block_tokens; columns behind its
+ * blocks mean nothing.  Rows that grow take the blocks they lack, those that shrink (to 0: the request is over) give back
+ * what they no longer need and keep the entries as they were.  A negative length is no request: its row is left alone.
+ * Free blocks wait in d_queue, a ring of queue_capacity places: d_state[0] blocks have been taken from it so far, d_state[1]
+ * given to it, the next one to take is at place d_state[0] % queue_capacity, the next one given goes to place d_state[1] %
+ * queue_capacity.  Requests take and give in their order, and each in the order of columns; what is given back in a
+ * step cannot be taken in the same.  d_state_out (int64[3]) receives both counts after the step and its status; it may be
+ * d_state itself, or another array, and then the step may be queued again from the same state.  Status:
+ *   0     done
+ *   > 0   so many blocks are missing
+ *   -1    a request has, or would have, more blocks than `columns`
+ *   -2    the queue cannot be: a negative count, more blocks in it, or more after the step, than it has places
+ * Unless it is 0 nothing is taken, given or written, but for the counts as they were.  n_requests, columns and queue_capacity
+ * < 2^31, block_tokens <= 2^20. */
+GTK_API int gtk_block_tables(gtk_tokenizer* h, const int32_t* d_old_lengths, const int32_t* d_new_lengths, int64_t n_requests,
+                             int block_tokens, int32_t* d_tables, int64_t columns, int64_t table_stride, int32_t* d_queue,
+                             int64_t queue_capacity, const int64_t* d_state, int64_t* d_state_out);
+
+/* Where the tokens that a step brings go: request r has those at positions d_old_lengths[r] .. d_new_lengths[r] - 1 (none
+ * where it shrinks, or a length is negative), and they lie one request behind the other, as in the ids of a batch:
+ *   d_offsets[r]      where request r's begin (int64[n_requests + 1], the last is the number of all)
+ *   d_slots[i]        table entry * block_tokens + position % block_tokens (int64); -1 where the entry is negative or
+ *                     the position is beyond `columns`
+ *   d_positions[i]    the token's position, d_requests[i] its request (both may be NULL)
+ * for i < capacity; places from d_offsets[n_requests] on get -1 in all three, tokens beyond capacity are left out.  d_state
+ * may be NULL, or gtk_block_tables' d_state_out: after a step that was not done (a status other than 0) no request has
+ * tokens here, so that nothing goes to blocks that it does not hold.  n_requests, columns and capacity < 2^31. */
+GTK_API int gtk_slot_map(gtk_tokenizer* h, const int32_t* d_old_lengths, const int32_t* d_new_lengths, int64_t n_requests,
+                         int block_tokens, const int32_t* d_tables, int64_t columns, int64_t table_stride, const int64_t* d_state,
+                         int64_t capacity, int64_t* d_slots, int32_t* d_positions, int32_t* d_requests, int64_t* d_offsets);
+
 /* Page-locked host memory for inputs (cudaHostAlloc / cudaFreeHost). */
 GTK_API void* gtk_pinned_alloc(size_t bytes);
 GTK_API void  gtk_pinned_free(void* p);
