@@ -3,6 +3,11 @@
 // With m a row's maximum and w_j = exp((x_j - m) / T), columns ranked by logit, of equal ones the lower first: the first K = top_k are
 // looked at; of these the fewest whose weights reach top_p of their sum; of these those with w_j >= min_p.  The id is the first
 // column, in the order of columns, at which the sum of the weights that are left exceeds u times the whole of it.
+//
+// A row is read once.  Its weights are summed in 32 bits, by sections of neighbouring columns, and every decision that hangs on such a
+// sum is held against a bound of its error (Row::error); where a border lies within the bound the row is summed again in 64 bits.
+#include <cooperative_groups.h>
+
 #include <climits>
 #include <cmath>
 
@@ -11,13 +16,22 @@
 
 namespace {
 
+namespace cg = cooperative_groups;
 using gtk::key_column;
 using gtk::key_value;
+using gtk::Pack16;
+using gtk::pow2;
 using gtk::rank_key;
+using gtk::Two;
 using gtk::value_key;
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kSection = 1024, kMostSections = 1024;  // columns whose sums are kept, and how many of those a row has at most
+constexpr int kMaxParts = 8;     // CTAs that share a row
+constexpr int kSection  = 1024;  // columns whose sum is kept, neighbours of each other, one warp's at a time
+constexpr int kSets     = 4;     // sets of its columns that a thread knows the highest of
+constexpr int kBins     = 256;
+constexpr int kMostKeys = 1024;  // columns that are ranked at most
+constexpr float kLow    = -0x1p60f;
 
 struct SampleArgs {
   int vocab;
@@ -29,175 +43,765 @@ struct SampleArgs {
   float* logprob;
 };
 
+// What a row's request wants.
+struct Limits {
+  double u;
+  float t, p, least;
+  int k;
+  double inverse;  // of the temperature, 1 for 0
+  __device__ Limits(const SampleArgs& a, int64_t r)
+  {
+    u     = __ldg(a.uniform + r);
+    if (u > 1.0) u = 1.0;
+    t     = a.temperature ? __ldg(a.temperature + r) : 1.f;
+    p     = a.top_p ? __ldg(a.top_p + r) : 1.f;
+    least = a.min_p ? fminf(__ldg(a.min_p + r), 1.f) : 0.f;
+    if (a.min_p && isnan(__ldg(a.min_p + r))) least = NAN;
+    k = a.top_k ? __ldg(a.top_k + r) : 0;
+    if (k <= 0 || k >= a.vocab) k = INT_MAX;
+    if (t == 0.f) k = 1;
+    inverse = t == 0.f ? 1.0 : 1.0 / double(t);
+  }
+  __device__ bool broken() const { return !(t >= 0.f && t < INFINITY) || isnan(p) || isnan(least) || isnan(u); }
+  __device__ bool cut_by_mass() const { return p < 1.f && t > 0.f; }
+  __device__ bool all() const { return k == INT_MAX && !cut_by_mass() && !(least > 0.f); }
+};
+
+// What the threads of a CTA tell each other, and the columns that are ranked.
 struct Scratch {
-  double section[kMostSections];
+  uint64_t key[kMostKeys];
+  double weight[kMostKeys];
+  uint32_t order[kMostKeys];  // before: sets, by warps
   double mass[kWarps];
   int count[kWarps];
+  float top[kWarps], low[kWarps];
+  int hist[kBins], bins[kBins];  // of this CTA, of all that share the row
   double at, total;
-  int column;
+  int column, keys, left;
+  bool sure;
+  float part_top, part_low;
+  double part_sum;
 };
+
+// A row as the packs of 16 bytes that it touches; what lies in them outside of it counts as -inf.
+template <class T>
+struct Row {
+  static constexpr int E = Pack16<T>::kElems, kPacks = kSection / (32 * E);
+  const uint4* base;
+  int vocab, lead, packs, sections;
+  __device__ Row(const T* x, int vocab_) : vocab(vocab_)
+  {
+    lead     = int((uint32_t(reinterpret_cast<uintptr_t>(x)) & 15u) / sizeof(T));
+    base     = reinterpret_cast<const uint4*>(x - lead);
+    packs    = (lead + vocab + E - 1) / E;
+    sections = (packs + 32 * kPacks - 1) / (32 * kPacks);
+  }
+  __device__ __forceinline__ int column(int p) const { return p * E - lead; }
+  __device__ __forceinline__ uint4 load(int p) const
+  {
+    constexpr uint32_t w = Pack16<T>::kMinusInf;
+    if (p >= packs) return make_uint4(w, w, w, w);
+    uint4 raw = __ldg(base + p);
+    if (p == 0 || p == packs - 1) {
+      T* e = reinterpret_cast<T*>(&raw);
+#pragma unroll
+      for (int j = 0; j < E; ++j)
+        if (uint32_t(column(p) + j) >= uint32_t(vocab)) e[j] = gtk::from_float<T>(-INFINITY);
+    }
+    return raw;
+  }
+  __device__ __forceinline__ float value(int c) const
+  {
+    return gtk::to_float(reinterpret_cast<const T*>(base)[lead + c]);
+  }
+  // The first and the last pack are in no such section.
+  __device__ __forceinline__ bool whole(int s) const { return s > 0 && (s + 1) * 32 * kPacks < packs; }
+  // Of the sum of 32-bit weights, in any part of the row and relative to the sum of all, when that is `sum` times the highest's weight: a
+  // weight is off by two roundings of its exponent y, by 2^-22 for the exponential itself and as much for that of its section;
+  // ten additions and a product in its section.  The exponents' part is 2 * 2^-24 * ln 2 * |y|, and the weights' mean of ln 2 * |y| is their entropy less
+  // ln(sum), ln(vocab / sum) at most.
+  __device__ __forceinline__ double error(double sum) const
+  {
+    return (2.f * 0.6932f * fmaxf(0.f, log2f(float(vocab) / float(sum)) + 0.01f) + 20.f) * 0x1p-24;
+  }
+};
+
+__device__ __forceinline__ float warp_max(float x)
+{
+  float y;
+  asm volatile("redux.sync.max.f32 %0, %1, 0xFFFFFFFF;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ float warp_min(float x)
+{
+  float y;
+  asm volatile("redux.sync.min.f32 %0, %1, 0xFFFFFFFF;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <class N>
+__device__ __forceinline__ N warp_sum(N x)
+{
+#pragma unroll
+  for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, d);
+  return x;
+}
+template <class N>
+__device__ __forceinline__ N warp_upto(N x)  // the sum of the lanes up to the own one
+{
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const N l = __shfl_up_sync(0xFFFFFFFFu, x, d);
+    if (lane >= d) x += l;
+  }
+  return x;
+}
 
 struct Sum {
   double mass;
   int count;
 };
 
-// f(x, column) -> {weight, counted} over all columns, by all threads
-template <class T, class F>
-__device__ Sum sum_row(const T* x, int vocab, Scratch& S, F&& f)
+// The sums of weigh(x, column) by sections, to `section`, and their whole, by all threads; count(x, column) of the columns too.
+template <class T, class Weigh>
+__device__ __forceinline__ Sum sum_row(const Row<T>& row, double* section, Scratch& S, Weigh&& weigh)
 {
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int threads = blockDim.x, warps = threads >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   Sum s{0.0, 0};
-  for (int c = tid; c < vocab; c += kThreads) {
-    const Sum o = f(gtk::to_float(x[c]), c);
-    s.mass += o.mass, s.count += o.count;
-  }
-#pragma unroll
-  for (int d = 16; d; d >>= 1) {
-    s.mass += __shfl_xor_sync(0xFFFFFFFFu, s.mass, d);
-    s.count += __shfl_xor_sync(0xFFFFFFFFu, s.count, d);
-  }
   __syncthreads();
+  for (int i = warp; i < row.sections; i += warps) {
+    double sum = 0.0;
+#pragma unroll 1
+    for (int q = 0; q < Row<T>::kPacks; ++q) {
+      const int p     = (i * Row<T>::kPacks + q) * 32 + lane;
+      const uint4 raw = row.load(p);
+#pragma unroll
+      for (int j = 0; j < Row<T>::E; ++j) {
+        const Sum o = weigh(gtk::to_float(reinterpret_cast<const T*>(&raw)[j]), row.column(p) + j);
+        sum += o.mass, s.count += o.count;
+      }
+    }
+    sum = warp_sum(sum);
+    if (lane == 0 && GTK_IN(i, row.sections, 500)) section[i] = sum;
+    s.mass += sum;
+  }
+  s.count = warp_sum(s.count);
   if (lane == 0) S.mass[warp] = s.mass, S.count[warp] = s.count;
   __syncthreads();
   s = Sum{0.0, 0};
-  for (int w = 0; w < kWarps; ++w) s.mass += S.mass[w], s.count += S.count[w];
+  for (int w = 0; w < warps; ++w) s.mass += S.mass[w], s.count += S.count[w];
   return s;
 }
 
-// The first column at which the sum of f(x, column) exceeds the target, which is `share` of the whole where `of_whole`; the last column
-// with any weight where rounding leaves none, -1 where no column has any.  S.total is the whole.
-template <class T, class F>
-__device__ int locate(const T* x, int vocab, Scratch& S, bool of_whole, double share, F&& f)
+// A column, and the sums of the weights in front of it and with it.
+struct Place {
+  int column;
+  double before, upto;
+};
+
+// The first column at which the sum of weigh(x, column) exceeds the target, by one warp, whose sums by sections are there; the last one with
+// any weight where rounding leaves none, column -1 where none has any.
+template <class T, class Weigh>
+__device__ __forceinline__ Place locate(const Row<T>& row, const double* section, double target, Weigh&& weigh)
 {
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int sections = (vocab + kSection - 1) / kSection;
-  __syncthreads();
-  for (int s = warp; s < sections; s += kWarps) {
-    double sum = 0.0;
-    for (int c = s * kSection + lane; c < min(vocab, (s + 1) * kSection); c += 32) sum += f(gtk::to_float(x[c]), c);
-#pragma unroll
-    for (int d = 16; d; d >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, d);
-    if (lane == 0) S.section[s] = sum;
-  }
-  __syncthreads();
-  if (tid == 0) {
-    double total = 0.0;
-    for (int s = 0; s < sections; ++s) total += S.section[s];
-    const double target = of_whole ? share * total : share;
-    double front = 0.0;
-    int found = -1, last = -1;
-    double before_last = 0.0;
-    for (int s = 0; s < sections && found < 0; ++s) {
-      if (S.section[s] > 0.0) last = s, before_last = front;
-      if (front + S.section[s] > target) found = s;
-      else front += S.section[s];
+  const int lane = threadIdx.x & 31, each = (row.sections + 31) / 32;
+  constexpr uint32_t all = 0xFFFFFFFFu;
+  const int begin = min(lane * each, row.sections), end = min(begin + each, row.sections);
+  double mine = 0.0;
+  for (int i = begin; i < end; ++i) mine += section[i];
+  const double upto   = warp_upto(mine);
+  uint32_t over       = __ballot_sync(all, mine > 0.0 && upto > target);
+  const uint32_t some = __ballot_sync(all, mine > 0.0);
+  if (some == 0) return Place{-1, 0.0, 0.0};
+  int from = over ? __ffs(over) - 1 : 31 - __clz(some);
+  int s        = -1;
+  double front = upto - mine, next = front;
+  if (lane == from)
+    for (int i = begin; i < end; ++i) {
+      if (!(section[i] > 0.0)) continue;
+      s = i, front = next;
+      next += section[i];
+      if (next > target) break;
     }
-    if (found < 0) found = last, front = before_last;
-    S.column = found, S.at = front, S.total = total;
-  }
-  __syncthreads();
-  const int s = S.column;
-  const double target = of_whole ? share * S.total : share;
-  __syncthreads();
-  if (s >= 0 && warp == 0) {
-    double front = S.at;
-    int found = -1, last = -1;
-    for (int c0 = s * kSection; c0 < min(vocab, (s + 1) * kSection) && found < 0; c0 += 32) {
-      const int c    = c0 + lane;
-      const double w = c < vocab ? f(gtk::to_float(x[c]), c) : 0.0;
-      double upto    = w;
+  s     = __shfl_sync(all, s, from);
+  front = __shfl_sync(all, front, from);
+  // neighbouring packs to a lane
+  double w[Row<T>::kPacks];
+  mine = 0.0;
+  uint4 raw[Row<T>::kPacks];
 #pragma unroll
-      for (int d = 1; d < 32; d *= 2) {
-        const double l = __shfl_up_sync(0xFFFFFFFFu, upto, d);
-        if (lane >= d) upto += l;
+  for (int q = 0; q < Row<T>::kPacks; ++q) raw[q] = row.load((s * 32 + lane) * Row<T>::kPacks + q);
+#pragma unroll
+  for (int q = 0; q < Row<T>::kPacks; ++q) {
+    const int c = row.column((s * 32 + lane) * Row<T>::kPacks + q);
+    w[q]        = 0.0;
+#pragma unroll
+    for (int j = 0; j < Row<T>::E; ++j) w[q] += weigh(gtk::to_float(reinterpret_cast<const T*>(&raw[q])[j]), c + j);
+    mine += w[q];
+  }
+  const double upto_lane = front + warp_upto(mine);
+  over                   = __ballot_sync(all, mine > 0.0 && upto_lane > target);
+  const uint32_t some2   = __ballot_sync(all, mine > 0.0);
+  from                   = over ? __ffs(over) - 1 : some2 ? 31 - __clz(some2) : 0;
+  Place found{-1, 0.0, 0.0};
+  if (lane == from) {
+    double sum = upto_lane - mine;
+#pragma unroll
+    for (int q = 0; q < Row<T>::kPacks; ++q) {
+      const int c = row.column((s * 32 + lane) * Row<T>::kPacks + q);
+#pragma unroll
+      for (int j = 0; j < Row<T>::E; ++j) {
+        const double v = weigh(gtk::to_float(reinterpret_cast<const T*>(&raw[q])[j]), c + j);
+        if (v > 0.0 && !(found.column >= 0 && found.upto > target)) found = Place{c + j, sum, sum + v};
+        sum += v;
       }
-      const uint32_t over = __ballot_sync(0xFFFFFFFFu, w > 0.0 && front + upto > target), some = __ballot_sync(0xFFFFFFFFu, w > 0.0);
-      if (over) found = c0 + __ffs(over) - 1;
-      if (some) last = c0 + 31 - __clz(some);
-      front += __shfl_sync(0xFFFFFFFFu, upto, 31);
     }
-    if (lane == 0) S.column = found >= 0 ? found : last;
+  }
+  found.column = __shfl_sync(all, found.column, from);
+  found.before = __shfl_sync(all, found.before, from);
+  found.upto   = __shfl_sync(all, found.upto, from);
+  return found;
+}
+
+// Everything in 64 bits, by one CTA, in as many readings of the row as it takes: rows of which nothing else is known, or whose borders
+// the sums in 32 bits do not tell from each other.
+template <class T>
+struct Slowly {
+  const Row<T>& row;
+  const Limits& l;
+  double* section;
+  Scratch& S;
+  double m;
+  uint64_t floor = 1;  // what is left reaches it, see rank_key
+
+  __device__ double weight(float x) const { return x > -INFINITY ? exp((double(x) - m) * l.inverse) : 0.0; }
+  __device__ bool left(float x, int c) const { return rank_key(x, uint32_t(c)) >= floor; }
+
+  // the first column at which `weigh` exceeds the target, known to all threads
+  template <class Weigh>
+  __device__ Place find(double target, Weigh&& weigh)
+  {
+    __syncthreads();
+    if (threadIdx.x < 32) {
+      const Place found = locate(row, section, target, weigh);
+      if (threadIdx.x == 0) S.column = found.column, S.at = found.before, S.total = found.upto;
+    }
+    __syncthreads();
+    const Place found{S.column, S.at, S.total};
+    __syncthreads();
+    return found;
+  }
+
+  // Raises the floor to the highest value at which enough(sum over the columns that reach it) holds, and there to as many columns of that
+  // value as are wanted(sum over those above it).
+  template <class Enough, class Wanted>
+  __device__ void search(uint32_t most, Enough&& enough, Wanted&& wanted)
+  {
+    uint32_t lo = 1, hi = most;  // enough at lo
+    while (lo < hi) {
+      const uint32_t mid = lo + (hi - lo + 1) / 2;
+      const Sum s = sum_row(row, section, S, [&](float x, int c) { return value_key(x) >= mid && left(x, c) ? Sum{weight(x), 1} : Sum{0.0, 0}; });
+      if (enough(s)) lo = mid;
+      else hi = mid - 1;
+    }
+    const Sum above = sum_row(row, section, S, [&](float x, int c) { return value_key(x) > lo && left(x, c) ? Sum{weight(x), 1} : Sum{0.0, 0}; });
+    const float value  = key_value(uint64_t(lo) << 32);
+    auto equal         = [&](float x, int c) { return value_key(x) == lo && left(x, c) ? 1.0 : 0.0; };
+    sum_row(row, section, S, [&](float x, int c) { return Sum{equal(x, c), 0}; });
+    const int column = find(wanted(above, weight(value)) - 1.0, equal).column;
+    floor            = max(floor, rank_key(value, uint32_t(column)));
+  }
+
+  // the drawn column and its log probability; -1 for a row without one
+  __device__ int run(float& logprob)
+  {
+    const int threads = blockDim.x, warps = threads >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    bool broken   = false;
+    uint32_t most = 0;
+    const int some = sum_row(row, section, S, [&](float x, int c) {
+                       if (uint32_t(c) < uint32_t(row.vocab)) broken |= !(x < INFINITY), most = max(most, value_key(x));
+                       return Sum{0.0, x > -INFINITY ? 1 : 0};
+                     }).count;
+    logprob = __int_as_float(0x7FC00000);
+    if (__syncthreads_or(broken)) return -1;
+    most = __reduce_max_sync(0xFFFFFFFFu, most);
+    if (lane == 0) S.count[warp] = int(most);
+    __syncthreads();
+    for (int w = 0; w < warps; ++w) most = max(most, uint32_t(S.count[w]));
+    logprob = -INFINITY;
+    if (most == 0) return -1;
+    m = key_value(uint64_t(most) << 32);
+    if (l.k < some)
+      search(most, [&](const Sum& s) { return s.count >= l.k; }, [&](const Sum& s, double) { return double(l.k - s.count); });
+    if (l.cut_by_mass()) {
+      const double whole = sum_row(row, section, S, [&](float x, int c) { return left(x, c) ? Sum{weight(x), 1} : Sum{0.0, 0}; }).mass;
+      const double reach = fmax(0.0, double(l.p)) * whole;
+      search(most, [&](const Sum& s) { return s.mass >= reach; },
+             [&](const Sum& s, double w) {
+               double n = fmax(1.0, w > 0.0 ? ceil((reach - s.mass) / w) : 1.0);
+               if (n > 1.0 && s.mass + (n - 1.0) * w >= reach) n -= 1.0;
+               return n;
+             });
+    }
+    const double least_y = l.least > 0.f ? log(double(l.least)) : -INFINITY;
+    auto drawn           = [&](float x, int c) { return left(x, c) && (double(x) - m) * l.inverse >= least_y ? weight(x) : 0.0; };
+    const double total   = sum_row(row, section, S, [&](float x, int c) { return Sum{drawn(x, c), 0}; }).mass;
+    const int id         = find(l.u * total, drawn).column;
+    if (id < 0) return -1;
+    logprob = l.t == 0.f ? 0.f : float((double(row.value(id)) - m) * l.inverse - log(total));
+    return id;
+  }
+};
+
+template <class T>
+__device__ __noinline__ int draw_slowly(const Row<T>& row, const Limits& l, double* section, Scratch& S, float& logprob)
+{
+  Slowly<T> s{row, l, section, S, 0.0};
+  return s.run(logprob);
+}
+
+// The sum of all weights in 64 bits, by sections too.
+template <class T>
+__device__ __noinline__ double sum_exactly(const Row<T>& row, const Limits& l, double m, double* section, Scratch& S)
+{
+  return sum_row(row, section, S, [&](float x, int) { return Sum{x > -INFINITY ? exp((double(x) - m) * l.inverse) : 0.0, 0}; }).mass;
+}
+
+// Sorts n numbers, highest first, by all threads; there is room up to the next power of two.
+template <class N>
+__device__ void sort_down(N* a, int n)
+{
+  int size = 2;
+  while (size < n) size *= 2;
+  for (int i = n + int(threadIdx.x); i < size; i += blockDim.x) a[i] = 0;
+  __syncthreads();
+  for (int run = 2; run <= size; run *= 2)
+    for (int d = run / 2; d; d /= 2) {
+      for (int i = threadIdx.x; i < size / 2; i += blockDim.x) {
+        const int at = 2 * i - (i & (d - 1));
+        if (!GTK_IN(at + d, kMostKeys, 501)) continue;
+        const N lo = a[at], hi = a[at + d];
+        if ((lo < hi) == ((at & run) == 0)) a[at] = hi, a[at + d] = lo;
+      }
+      __syncthreads();
+    }
+}
+
+constexpr int kRanked = 192;  // up to so many keys are ranked by looking at each other
+
+// S.key[0 .. n), highest first.
+__device__ void sort_keys(Scratch& S, int n)
+{
+  if (n > kRanked) return sort_down(S.key, n);
+  constexpr int kEach = 2;
+  uint64_t key[kEach];
+  int place[kEach];
+#pragma unroll
+  for (int e = 0; e < kEach; ++e) {
+    const int i = e * blockDim.x + threadIdx.x;
+    key[e]      = i < n ? S.key[i] : 0;
+    place[e]    = 0;
+  }
+  for (int j = 0; j < n; ++j) {
+    const uint64_t other = S.key[j];
+#pragma unroll
+    for (int e = 0; e < kEach; ++e) place[e] += other > key[e];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int e = 0; e < kEach; ++e)
+    if (key[e] && GTK_IN(place[e], kMostKeys, 502)) S.key[place[e]] = key[e];
+  __syncthreads();
+}
+
+// The columns among S.key[0 .. n) that are left, their number and their weights' sum; `whole`: the sum that top-p is a part of, off
+// by `error` at most, < 0 where it is the sum of the keys.  By one warp, weights in place; false where the error leaves it open.
+__device__ bool cut_keys(const Limits& l, double m, Scratch& S, int n, double whole, double error, int& left, double& total)
+{
+  const int lane = threadIdx.x & 31;
+  n              = min(n, l.k);
+  const int each = (n + 31) / 32, begin = min(n, lane * each), end = min(n, begin + each);
+  double mine = 0.0;
+  for (int i = begin; i < end; ++i) mine += S.weight[i];
+  const double front = warp_upto(mine) - mine;
+  if (whole < 0.0) whole = __shfl_sync(0xFFFFFFFFu, front + mine, 31), error = 0.0;
+  const double reach   = fmax(0.0, double(l.p)) * whole;
+  const double least_y = l.least > 0.f ? log(double(l.least)) : -INFINITY;
+  int last     = INT_MAX;  // of those that top-p leaves
+  bool open    = false;
+  int allowed  = 0;
+  double upto  = front;
+  for (int i = begin; i < end; ++i) {
+    upto += S.weight[i];
+    if (l.cut_by_mass() && last == INT_MAX && upto >= reach - error) last = i, open = upto < reach + error;
+    allowed += (double(key_value(S.key[i])) - m) * l.inverse >= least_y;
+  }
+  const int first = __reduce_min_sync(0xFFFFFFFFu, last);
+  open            = __any_sync(0xFFFFFFFFu, open && last == first);
+  allowed         = __reduce_add_sync(0xFFFFFFFFu, allowed);
+  left            = max(1, min(min(n, allowed), first == INT_MAX ? n : first + 1));
+  if (open && left <= first) open = false;  // min-p cuts in front of it
+  upto = 0.0;
+  for (int i = begin; i < min(end, left); ++i) upto += S.weight[i];
+  total = warp_sum(upto);
+  return !open;
+}
+
+// The one of S.key[0 .. n) that is drawn, by all threads, by its place in the order of columns.
+__device__ int draw_key(Scratch& S, int n, double target)
+{
+  const int tid = threadIdx.x, lane = tid & 31;
+  if (tid == 0) S.column = INT_MAX, S.left = -1;
+  __syncthreads();
+  if (n <= kRanked) {
+    for (int i = tid; i < n; i += blockDim.x) {
+      const uint32_t c = key_column(S.key[i]);
+      double upto      = 0.0;
+      for (int j = 0; j < n; ++j)
+        if (key_column(S.key[j]) <= c) upto += S.weight[j];
+      if (S.weight[i] > 0.0) {
+        if (upto > target) atomicMin(&S.column, int(c));
+        atomicMax(&S.left, int(c));  // where rounding leaves none
+      }
+    }
+    __syncthreads();
+    return S.column == INT_MAX ? S.left : S.column;
+  }
+  // ranks by column, the lowest column first: 20 bits of column, 10 of rank
+  for (int i = tid; i < n; i += blockDim.x) S.order[i] = ~(key_column(S.key[i]) << 10 | uint32_t(i));
+  __syncthreads();
+  sort_down(S.order, n);
+  if (tid < 32) {
+    const int each = (n + 31) / 32, begin = min(n, lane * each), end = min(n, begin + each);
+    double mine = 0.0;
+    for (int i = begin; i < end; ++i) mine += S.weight[~S.order[i] & (kMostKeys - 1)];
+    double upto = warp_upto(mine) - mine;
+    int found = INT_MAX, last = -1;
+    for (int i = begin; i < end; ++i) {
+      const double w = S.weight[~S.order[i] & (kMostKeys - 1)];
+      upto += w;
+      if (w > 0.0) last = i;
+      if (w > 0.0 && upto > target && found == INT_MAX) found = i;
+    }
+    found = __reduce_min_sync(0xFFFFFFFFu, found);
+    last  = __reduce_max_sync(0xFFFFFFFFu, last);
+    if (lane == 0) S.column = int(~S.order[found == INT_MAX ? last : found] >> 10);
   }
   __syncthreads();
   return S.column;
 }
 
-template <class T>
-__global__ void __launch_bounds__(kThreads) k_sample(const T* __restrict__ logits, const SampleArgs a)
+template <class T, bool SPLIT>
+__global__ void __launch_bounds__(kThreads, 4) k_sample(const T* __restrict__ logits, const SampleArgs a, int n_parts)
 {
+  using P              = Pack16<T>;
+  constexpr int E      = P::kElems;
+  constexpr int kPacks = Row<T>::kPacks;
+  extern __shared__ double s_section[];  // a whole row's
   __shared__ Scratch S;
-  const int64_t r = blockIdx.x;
-  const T* x      = logits + r * a.stride;
-  const int tid = threadIdx.x, vocab = a.vocab;
-  const float nan = __int_as_float(0x7FC00000);
-  auto put        = [&](int id, float logprob) {
-    if (tid != 0) return;
+  const int parts = SPLIT ? n_parts : 1;
+  const int tid = threadIdx.x, threads = blockDim.x, warps = threads >> 5, warp = tid >> 5, lane = tid & 31;
+  const int64_t r = blockIdx.x / unsigned(parts);
+  const int part  = int(blockIdx.x % unsigned(parts));
+  const Row<T> row(logits + r * a.stride, a.vocab);
+  const Limits l(a, r);
+  auto put = [&](int id, float logprob) {
+    if (tid != 0 || part != 0) return;
     a.ids[r] = id;
     if (a.logprob) a.logprob[r] = logprob;
   };
-  const double u = a.uniform[r];
-  if (u < 0.0) return put(-1, 0.f);
-  const float t = a.temperature ? a.temperature[r] : 1.f, p = a.top_p ? a.top_p[r] : 1.f, least = a.min_p ? a.min_p[r] : 0.f;
-  const int k   = t == 0.f ? 1 : a.top_k ? a.top_k[r] : 0;
-  // the maximum; a row with a NaN or +inf is none
-  bool broken = !(t >= 0.f && t < INFINITY) || isnan(p) || isnan(least) || isnan(u);
-  uint32_t most = 0;
-  int some = 0;
-  for (int c = tid; c < vocab; c += kThreads) {
-    const float v = gtk::to_float(x[c]);
-    broken |= !(v < INFINITY);
-    most = max(most, value_key(v));
-    some += v > -INFINITY;
-  }
-  if (__syncthreads_or(broken)) return put(-1, nan);
+  if (l.u < 0.0) return put(-1, 0.f);
+  if (l.broken()) return put(-1, __int_as_float(0x7FC00000));
+  for (int i = tid; i < kBins; i += threads) S.hist[i] = 0;
+  if (tid == 0) S.keys = 0;
+
+  // ---- the row, once
+  const double k64  = 1.4426950408889634 * l.inverse;
+  const bool ranged = k64 > 0x1p-20 && k64 < 0x1p20;
+  const float k     = ranged ? float(k64) : 1.f;
+  const int share = (row.sections + parts - 1) / parts;
+  const int begin = min(row.sections, part * share), end = min(row.sections, begin + share);
+  float2* const piece = reinterpret_cast<float2*>(s_section);
+  typename P::Max best[kSets];
 #pragma unroll
-  for (int d = 16; d; d >>= 1) some += __shfl_xor_sync(0xFFFFFFFFu, some, d);
-  most = __reduce_max_sync(0xFFFFFFFFu, most);
-  if ((tid & 31) == 0) S.count[tid >> 5] = int(most), S.mass[tid >> 5] = some;
-  __syncthreads();
-  some = 0;
-  for (int w = 0; w < kWarps; ++w) most = max(most, uint32_t(S.count[w])), some += int(S.mass[w]);
-  if (some == 0) return put(-1, -INFINITY);
-  const double m = key_value(uint64_t(most) << 32), inverse = t == 0.f ? 1.0 : 1.0 / double(t);
-  auto weight    = [&](float v) { return v > -INFINITY ? exp((double(v) - m) * inverse) : 0.0; };
-  uint64_t floor = 0;  // what is left reaches it, see rank_key
-  auto left      = [&](float v, int c) { return rank_key(v, uint32_t(c)) >= max(floor, uint64_t(1)); };
-  // Lowers the floor from the highest: to the highest value at which enough(sum over the columns that reach it) holds, then to as many
-  // columns of that value as are wanted(sum over those above it).
-  auto search = [&](auto&& enough, auto&& wanted) {
-    uint32_t lo = 0, hi = most;  // enough at lo
-    while (lo < hi) {
-      const uint32_t mid = lo + (hi - lo + 1) / 2;
-      const Sum s = sum_row(x, vocab, S, [&](float v, int c) { return value_key(v) >= mid && left(v, c) ? Sum{weight(v), 1} : Sum{0.0, 0}; });
-      if (enough(s)) lo = mid;
-      else hi = mid - 1;
+  for (int q = 0; q < kSets; ++q) best[q] = P::lowest();
+  float top = -INFINITY, ref = kLow;
+  for (int s = begin + warp; s < end; s += warps) {
+    uint4 raw[kPacks];
+    const int p0 = s * 32 * kPacks + lane;
+    if (row.whole(s)) {
+#pragma unroll
+      for (int q = 0; q < kPacks; ++q) raw[q] = __ldg(row.base + p0 + q * 32);
+    } else {
+#pragma unroll
+      for (int q = 0; q < kPacks; ++q) raw[q] = row.load(p0 + q * 32);
     }
-    const Sum above = sum_row(x, vocab, S, [&](float v, int c) { return value_key(v) > lo && left(v, c) ? Sum{weight(v), 1} : Sum{0.0, 0}; });
-    const float value = key_value(uint64_t(lo) << 32);
-    const int column  = locate(x, vocab, S, false, wanted(above, weight(value)) - 1.0,
-                               [&](float v, int c) { return value_key(v) == lo && left(v, c) ? 1.0 : 0.0; });
-    floor             = max(floor, rank_key(value, uint32_t(column)));
-  };
-  if (k > 0 && k < some)
-    search([&](const Sum& s) { return s.count >= k; }, [&](const Sum& s, double) { return double(k - s.count); });
-  if (p < 1.f && t > 0.f) {
-    const double whole = sum_row(x, vocab, S, [&](float v, int c) { return left(v, c) ? Sum{weight(v), 1} : Sum{0.0, 0}; }).mass;
-    const double reach = max(0.0, double(p)) * whole;
-    search([&](const Sum& s) { return s.mass >= reach; },
-           [&](const Sum& s, double w) {
-             double n = max(1.0, w > 0.0 ? ceil((reach - s.mass) / w) : 1.0);
-             if (n > 1.0 && s.mass + (n - 1.0) * w >= reach) n -= 1.0;
-             return n;
-           });
+    typename P::Max most = P::highest(raw[0]);
+    best[0]              = P::higher(best[0], most);
+#pragma unroll
+    for (int q = 1; q < kPacks; ++q) {
+      const typename P::Max m = P::highest(raw[q]);
+      best[q % kSets]         = P::higher(best[q % kSets], m);
+      most                    = P::higher(most, m);
+    }
+    const float high = warp_max(P::kHalves == 2 ? fmaxf(P::of(most, 0), P::of(most, 1)) : P::of(most, 0));
+    top = fmaxf(top, high), ref = fmaxf(ref, high);
+    const float c = ref * k;
+    const Two k2(k, k), c2(-c, -c);
+    Two sum[kPacks];
+#pragma unroll
+    for (int q = 0; q < kPacks; ++q) {
+      Two x[E / 2];
+      P::pairs(raw[q], x);
+#pragma unroll
+      for (int j = 0; j < E / 2; ++j) {
+        float y0, y1;
+        gtk::fma2(x[j], k2, c2).get(y0, y1);
+        x[j] = Two(pow2(y0), pow2(y1));
+      }
+#pragma unroll
+      for (int d = 1; d < E / 2; d *= 2)
+#pragma unroll
+        for (int j = 0; j < E / 2; j += 2 * d) x[j] = x[j] + x[j + d];
+      sum[q] = x[0];
+    }
+#pragma unroll
+    for (int d = 1; d < kPacks; d *= 2)
+#pragma unroll
+      for (int q = 0; q < kPacks; q += 2 * d) sum[q] = sum[q] + sum[q + d];
+    float lo, hi;
+    sum[0].get(lo, hi);
+    lo = warp_sum(lo + hi);
+    if (lane == 0 && GTK_IN(s, row.sections, 503)) piece[s] = make_float2(c, lo);
   }
-  const double least_y = least > 0.f ? log(min(1.0, double(least))) : -INFINITY;
-  auto drawn           = [&](float v, int c) { return left(v, c) && (double(v) - m) * inverse >= least_y ? weight(v) : 0.0; };
-  const int id         = locate(x, vocab, S, true, min(u, 1.0), drawn);
-  put(id, t == 0.f ? 0.f : float((double(gtk::to_float(x[id])) - m) * inverse - log(S.total)));
+  float low = INFINITY;
+#pragma unroll
+  for (int q = 0; q < kSets; ++q) {
+    const float v = P::kHalves == 2 ? fmaxf(P::of(best[q], 0), P::of(best[q], 1)) : P::of(best[q], 0);
+    if (v > -INFINITY) low = fminf(low, v);
+  }
+  low = warp_min(low);
+  if (lane == 0) S.top[warp] = top, S.low[warp] = low;
+  __syncthreads();
+  for (int w = 0; w < warps; ++w) top = fmaxf(top, S.top[w]), low = fminf(low, S.low[w]);
+  if constexpr (SPLIT) {
+    cg::cluster_group cluster = cg::this_cluster();
+    if (tid == 0) S.part_top = top, S.part_low = low;
+    cluster.sync();
+    // lane c asks part c, here and below
+    if (lane < parts) {
+      const Scratch* other = cluster.map_shared_rank(&S, lane);
+      top = other->part_top, low = other->part_low;
+    }
+    top = warp_max(top), low = warp_min(low);
+  }
+
+  // ---- the sum of all weights relative to the highest's, and how the sets' highest are distributed
+  const float c_top = fmaxf(top, kLow) * k;
+  const float scale = fminf(float(kBins) / (top - low), 0x1p100f);
+  double sum = 0.0;
+  for (int s = begin + tid; s < end; s += threads) {
+    const float2 v   = piece[s];
+    const double w   = v.y * pow2(v.x - c_top);
+    s_section[s]     = w;
+    sum += w;
+  }
+  sum = warp_sum(sum);
+  if (lane == 0) S.mass[warp] = sum;
+  const bool all = l.all();
+  if (!all) {
+#pragma unroll
+    for (int q = 0; q < kSets; ++q) {
+      const float v = P::kHalves == 2 ? fmaxf(P::of(best[q], 0), P::of(best[q], 1)) : P::of(best[q], 0);
+      if (v > -INFINITY) {
+        const int at = int(fminf((top - v) * scale, float(kBins - 1)));
+        if (GTK_IN(at, kBins, 504)) atomicAdd(&S.hist[at], 1);
+      }
+    }
+  }
+  __syncthreads();
+  sum = 0.0;
+  for (int w = 0; w < warps; ++w) sum += S.mass[w];
+  const int* hist = S.hist;
+  if constexpr (SPLIT) {
+    cg::cluster_group cluster = cg::this_cluster();
+    if (tid == 0) S.part_sum = sum;
+    cluster.sync();
+    sum = warp_sum(lane < parts ? cluster.map_shared_rank(&S, lane)->part_sum : 0.0);
+    if (all) {
+      if (part == 0)  // the others' sections behind its own
+        for (int s = end + tid; s < row.sections; s += threads) s_section[s] = cluster.map_shared_rank(s_section, s / share)[s];
+    } else {
+      for (int i = tid; i < kBins; i += threads) {
+        int n = 0;
+        for (int c = 0; c < parts; ++c) n += cluster.map_shared_rank(&S, c)->hist[i];
+        S.bins[i] = n;
+      }
+      hist = S.bins;
+    }
+    __syncthreads();
+  }
+  // rows whose numbers 32 bits do not hold are looked at again, as are those without a distribution
+  bool fast          = ranged && fabsf(top) < 0x1p59f && fabsf(c_top) < 0x1p20f && sum > 0.0 && sum < 1e30;
+  const double m     = top;
+  const double shift = double(top) * double(k) - double(c_top);  // the highest's exponent
+  const double error = row.error(sum);
+
+  if (all || !fast) {
+    if constexpr (SPLIT) {
+      cg::this_cluster().sync();  // nobody leaves while its shared memory is read
+      if (part != 0) return;
+    }
+    if (fast) {
+      if (warp == 0) {
+        const double target = l.u * sum;
+        const Place at      = locate(row, s_section, target, [&](float x, int) { return double(pow2(fmaf(x, k, -c_top))); });
+        if (lane == 0) {
+          S.sure   = target - at.before >= error * sum && at.upto - target >= error * sum;
+          S.column = at.column;
+        }
+      }
+      __syncthreads();
+      if (S.sure) return put(S.column, float((double(row.value(S.column)) - m) * l.inverse + 0.6931471805599453 * shift - log(sum)));
+    }
+    float logprob;
+    const int id = draw_slowly(row, l, s_section, S, logprob);
+    return put(id, logprob);
+  }
+
+  // ---- a limit: how far down the columns have to be known
+  const bool by_mass = l.cut_by_mass();
+  sum *= exp2(-shift);
+  int reach = kBins;
+  {
+    constexpr int kEach = kBins / 32;
+    const float width   = 1.f / scale;
+    int counts[kEach], count = 0;
+    float masses[kEach], mass = 0.f;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      const int b = lane * kEach + i;
+      counts[i]   = hist[b];
+      masses[i]   = counts[i] ? float(counts[i]) * pow2(-float(b + 1) * width * k) * 0.999f : 0.f;  // no less than that
+      count += counts[i], mass += masses[i];
+    }
+    int count_upto  = warp_upto(count) - count;
+    float mass_upto = warp_upto(mass) - mass;
+    const float wanted = by_mass && l.k == INT_MAX ? fmaxf(l.p, 0.f) * float(sum) * 1.0001f : INFINITY;
+#pragma unroll
+    for (int i = 0; i < kEach; ++i) {
+      count_upto += counts[i], mass_upto += masses[i];
+      if (reach == kBins && counts[i] && (count_upto >= l.k || mass_upto >= wanted)) reach = lane * kEach + i;
+    }
+    reach = __reduce_min_sync(0xFFFFFFFFu, reach);
+    if (l.least > 0.f && (l.k == INT_MAX || !by_mass))
+      reach = min(reach, int(fminf(-logf(l.least) * l.t * scale * 1.0001f + 2.f, float(kBins))));
+  }
+  const bool everything = reach == kBins;
+  const float bound     = reach == kBins - 1 ? float(kBins + 1) : float(reach + 1);  // the last one holds the lowest too, however that is rounded
+  bool some             = !everything || row.vocab <= kMostKeys;
+  if (everything && !some) {  // where most columns are masked, what is left may be few
+    int n = 0;
+    for (int i = lane; i < kBins; i += 32) n += hist[i];
+    some = warp_sum(n) <= kMostKeys / 4;
+  }
+  if (some) {
+    auto reaches = [&](float x) { return everything || (top - x) * scale < bound; };
+    uint32_t* const set = S.order + warp * (kMostKeys / kWarps);
+    int sets            = 0;
+#pragma unroll
+    for (int q = 0; q < kSets; ++q) {
+      const float v       = P::kHalves == 2 ? fmaxf(P::of(best[q], 0), P::of(best[q], 1)) : P::of(best[q], 0);
+      const bool mine     = v > -INFINITY && reaches(v);
+      const uint32_t them = __ballot_sync(0xFFFFFFFFu, mine);
+      const int at        = sets + __popc(them & ((1u << lane) - 1u));
+      if (mine && GTK_IN(at, kMostKeys / kWarps, 505)) set[at] = q * 32 + lane;
+      sets += __popc(them);
+    }
+    __syncwarp();
+    const int sections = (end - begin - warp + warps - 1) / warps, packs = sets * max(0, sections) * (kPacks / kSets);
+    for (int i = lane; i < packs; i += 32) {
+      const int which = i % sets, rest = i / sets, s = begin + warp + rest / (kPacks / kSets) * warps;
+      const int p     = s * 32 * kPacks + int(set[which]) + rest % (kPacks / kSets) * 32 * kSets;
+      const uint4 raw = row.load(p);
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const float x = gtk::to_float(reinterpret_cast<const T*>(&raw)[j]);
+        if (x > -INFINITY && reaches(x)) {
+          const int at = atomicAdd(&S.keys, 1);
+          if (at < kMostKeys && GTK_IN(at, kMostKeys, 506)) S.key[at] = rank_key(x, uint32_t(row.column(p) + j));
+        }
+      }
+    }
+  }
+  __syncthreads();
+  int n = S.keys;
+  if constexpr (SPLIT) {
+    cg::cluster_group cluster = cg::this_cluster();
+    cluster.sync();
+    if (part == 0) {
+      const int keys = lane < parts ? cluster.map_shared_rank(&S, lane)->keys : 0;
+      const int upto = warp_upto(keys);
+      n              = __shfl_sync(0xFFFFFFFFu, upto, 31);
+      if (n <= kMostKeys)
+        for (int c = 1 + warp; c < parts; c += warps) {
+          const int count = __shfl_sync(0xFFFFFFFFu, keys, c), at = __shfl_sync(0xFFFFFFFFu, upto, c) - count;
+          for (int i = lane; i < count; i += 32)
+            if (GTK_IN(at + i, kMostKeys, 507)) S.key[at + i] = cluster.map_shared_rank(&S, c)->key[i];
+        }
+    }
+    cluster.sync();  // nobody leaves while its shared memory is read
+    if (part != 0) return;
+  }
+  if (!some || n > kMostKeys) {
+    float logprob;
+    const int id = draw_slowly(row, l, s_section, S, logprob);
+    return put(id, logprob);
+  }
+
+  // ---- the columns that are known, ranked
+  sort_keys(S, n);
+  for (int i = tid; i < n; i += threads) S.weight[i] = exp((double(key_value(S.key[i])) - m) * l.inverse);
+  __syncthreads();
+  double whole = everything || l.k != INT_MAX ? -1.0 : sum, off = error * sum;
+  for (int round = 0; round < 2; ++round) {
+    if (warp == 0) {
+      int left;
+      double total;
+      const bool sure = cut_keys(l, m, S, n, whole, off, left, total);
+      if (lane == 0) S.sure = sure, S.left = left, S.total = total;
+    }
+    __syncthreads();
+    if (S.sure) break;
+    whole = sum_exactly(row, l, m, s_section, S), off = 0.0;
+  }
+  const int left     = S.left;
+  const double total = S.total;
+  __syncthreads();
+  const int id = draw_key(S, left, l.u * total);
+  put(id, l.t == 0.f || id < 0 ? 0.f : float((double(row.value(id)) - m) * l.inverse - log(total)));
 }
 
-constexpr int64_t kMaxVocab = int64_t(kSection) * kMostSections, kMaxRows = (int64_t(1) << 31) - 1;
+struct Teams {
+  int parts, threads;
+};
+Teams teams_for(int64_t rows, int64_t bytes, int sm_count)
+{
+  Teams t{1, kThreads};
+  while (t.parts < kMaxParts && rows * t.parts * 2 <= sm_count && bytes / (t.parts * 2) >= (12 << 10)) t.parts *= 2;
+  return t;
+}
+
+template <class T>
+cudaError_t launch_sample(const gtk::HandleView& v, const void* logits, int64_t n_rows, const SampleArgs& a)
+{
+  const Teams t         = teams_for(n_rows, int64_t(a.vocab) * int64_t(sizeof(T)), v.sm_count);
+  const size_t sections = (size_t(a.vocab) + 16 / sizeof(T) + kSection - 1) / kSection;
+  return gtk::launch_clusters(t.parts > 1 ? k_sample<T, true> : k_sample<T, false>, dim3(unsigned(n_rows * t.parts)), dim3(unsigned(t.threads)),
+                              t.parts, sections * sizeof(double), v.stream, static_cast<const T*>(logits), a, t.parts);
+}
+
+constexpr int64_t kMaxRows = (int64_t(1) << 31) - 1;
 
 }  // namespace
 
@@ -208,7 +812,7 @@ extern "C" GTK_API int gtk_sample(gtk_tokenizer* h, const void* d_logits, int ty
   auto check = [&]() -> gtk::Refusal {
     if (!gtk::known_type(type)) return "unknown element type";
     if (n_rows < 0 || vocab <= 0 || stride < 0) return "n_rows and stride must be >= 0, vocab > 0";
-    if (n_rows > kMaxRows || vocab > kMaxVocab) return "n_rows of 2^31 and more, or vocab beyond 2^20";
+    if (n_rows > kMaxRows || vocab > GTK_MAX_SAMPLE_VOCAB) return "n_rows of 2^31 and more, or vocab beyond 2^20";
     if (n_rows == 0) return nullptr;
     if (!d_logits || !d_uniform || !d_ids) return "null device pointer";
     if (!gtk::aligned_to(d_logits, gtk::element_size(type)) || !gtk::aligned_to(d_uniform, 8)) return "a device pointer is not aligned to its elements";
@@ -220,10 +824,7 @@ extern "C" GTK_API int gtk_sample(gtk_tokenizer* h, const void* d_logits, int ty
   return gtk::run_operator(h, check, [&](const gtk::HandleView& v) -> cudaError_t {
     if (n_rows == 0) return cudaSuccess;
     const SampleArgs a{int(vocab), stride, d_uniform, d_temperature, d_top_p, d_min_p, d_top_k, d_ids, d_logprob};
-    return gtk::with_type(type, [&](auto x) {
-      using T = decltype(x);
-      return gtk::launch(k_sample<T>, dim3(unsigned(n_rows)), dim3(kThreads), 0, v.stream, static_cast<const T*>(d_logits), a);
-    });
+    return gtk::with_type(type, [&](auto x) { return launch_sample<decltype(x)>(v, d_logits, n_rows, a); });
   });
 }
 
