@@ -8,6 +8,7 @@
 // sum is held against a bound of its error (Row::error); where a border lies within the bound the row is summed again in 64 bits.
 #include <cooperative_groups.h>
 
+#include <cfloat>
 #include <climits>
 #include <cmath>
 
@@ -28,9 +29,10 @@ using gtk::value_key;
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMaxParts = 8;     // CTAs that share a row
 constexpr int kSection  = 1024;  // columns whose sum is kept, neighbours of each other, one warp's at a time
-constexpr int kSets     = 4;     // sets of its columns that a thread knows the highest of
 constexpr int kBins     = 256;
+constexpr int kFine     = 1024;  // bins of a wide row
 constexpr int kMostKeys = 1024;  // columns that are ranked at most
+constexpr int kSetsOfWarp = 256;  // of its columns that a warp knows the highest of, at most
 constexpr float kLow    = -0x1p60f;
 
 struct SampleArgs {
@@ -70,17 +72,23 @@ struct Limits {
 // What the threads of a CTA tell each other, and the columns that are ranked.
 struct Scratch {
   uint64_t key[kMostKeys];
-  double weight[kMostKeys];
-  uint32_t order[kMostKeys];  // before: sets, by warps
-  double mass[kWarps];
+  union {
+    double weight[kMostKeys];
+    struct {
+      uint32_t fine[kFine], fine_all[kFine];  // of this CTA, of all that share the row
+    };
+  };
+  uint32_t order[kWarps * kSetsOfWarp];  // sets, by warps; then places of keys
+  double power[64];           // 2^(i / 64)
+  double mass[kWarps], part_mass[2];
   int count[kWarps];
   float top[kWarps], low[kWarps];
   int hist[kBins], bins[kBins];  // of this CTA, of all that share the row
-  double at, total;
-  int column, keys, left;
+  double at, total, part_sum;
+  uint64_t floor;
+  int column, keys, left, part_count, solved;
   bool sure;
   float part_top, part_low;
-  double part_sum;
 };
 
 // A row as the packs of 16 bytes that it touches; what lies in them outside of it counts as -inf.
@@ -157,6 +165,37 @@ __device__ __forceinline__ N warp_upto(N x)  // the sum of the lanes up to the o
   return x;
 }
 
+// exp((x - m) / T) in 64 bits: with y = (x - m) log2(e) / T = n / 64 + f the product of 2^(n / 64), by a table of 64 entries, and
+// exp(f ln 2), |f ln 2| < 0.0055, whose series is cut behind the fifth power (3e-17).  About a quarter of the time of exp().
+struct Weight64 {
+  double m, k;  // k: log2(e) / T
+  const double* power;
+  __device__ __forceinline__ double operator()(float x) const
+  {
+    const double y = fmax((double(x) - m) * k, -2000.0);
+    const double a = fma(y, 64.0, 0x1.8p52);  // n in the low bits
+    const int n    = __double2loint(a);
+    const double z = fma(a - 0x1.8p52, -1.0 / 64, y) * 0.69314718055994531;
+    double s       = fma(z, 1.0 / 120, 1.0 / 24);
+    s              = fma(z, s, 1.0 / 6);
+    s              = fma(z, s, 0.5);
+    s              = fma(z, s, 1.0);
+    s              = fma(z, s, 1.0);
+    const double w = power[n & 63] * s;
+    const int e    = n >> 6;
+    if (e < -1000) return ldexp(w, e);
+    return w * __hiloint2double((e + 1023) << 20, 0);
+  }
+};
+
+// the table, by all threads
+__device__ __forceinline__ Weight64 weight64(const Limits& l, double m, Scratch& S)
+{
+  if (threadIdx.x < 64) S.power[threadIdx.x] = exp2(double(threadIdx.x) / 64);
+  __syncthreads();
+  return Weight64{m, 1.4426950408889634 * l.inverse, S.power};
+}
+
 struct Sum {
   double mass;
   int count;
@@ -168,17 +207,22 @@ __device__ __forceinline__ Sum sum_row(const Row<T>& row, double* section, Scrat
 {
   const int threads = blockDim.x, warps = threads >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   Sum s{0.0, 0};
+  constexpr int kAtOnce = 16 / Row<T>::E;  // packs
   __syncthreads();
   for (int i = warp; i < row.sections; i += warps) {
     double sum = 0.0;
 #pragma unroll 1
-    for (int q = 0; q < Row<T>::kPacks; ++q) {
-      const int p     = (i * Row<T>::kPacks + q) * 32 + lane;
-      const uint4 raw = row.load(p);
+    for (int q = 0; q < Row<T>::kPacks; q += kAtOnce) {
+      uint4 raw[kAtOnce];
 #pragma unroll
-      for (int j = 0; j < Row<T>::E; ++j) {
-        const Sum o = weigh(gtk::to_float(reinterpret_cast<const T*>(&raw)[j]), row.column(p) + j);
-        sum += o.mass, s.count += o.count;
+      for (int b = 0; b < kAtOnce; ++b) raw[b] = row.load((i * Row<T>::kPacks + q + b) * 32 + lane);
+#pragma unroll
+      for (int b = 0; b < kAtOnce; ++b) {
+#pragma unroll
+        for (int j = 0; j < Row<T>::E; ++j) {
+          const Sum o = weigh(gtk::to_float(reinterpret_cast<const T*>(&raw[b])[j]), row.column((i * Row<T>::kPacks + q + b) * 32 + lane) + j);
+          sum += o.mass, s.count += o.count;
+        }
       }
     }
     sum = warp_sum(sum);
@@ -272,9 +316,10 @@ struct Slowly {
   double* section;
   Scratch& S;
   double m;
-  uint64_t floor = 1;  // what is left reaches it, see rank_key
+  uint64_t floor;  // what is left reaches it, see rank_key
+  Weight64 power;
 
-  __device__ double weight(float x) const { return x > -INFINITY ? exp((double(x) - m) * l.inverse) : 0.0; }
+  __device__ double weight(float x) const { return x > -INFINITY ? power(x) : 0.0; }
   __device__ bool left(float x, int c) const { return rank_key(x, uint32_t(c)) >= floor; }
 
   // the first column at which `weigh` exceeds the target, known to all threads
@@ -330,7 +375,8 @@ struct Slowly {
     for (int w = 0; w < warps; ++w) most = max(most, uint32_t(S.count[w]));
     logprob = -INFINITY;
     if (most == 0) return -1;
-    m = key_value(uint64_t(most) << 32);
+    m     = key_value(uint64_t(most) << 32);
+    power = weight64(l, m, S);
     if (l.k < some)
       search(most, [&](const Sum& s) { return s.count >= l.k; }, [&](const Sum& s, double) { return double(l.k - s.count); });
     if (l.cut_by_mass()) {
@@ -356,7 +402,7 @@ struct Slowly {
 template <class T>
 __device__ __noinline__ int draw_slowly(const Row<T>& row, const Limits& l, double* section, Scratch& S, float& logprob)
 {
-  Slowly<T> s{row, l, section, S, 0.0};
+  Slowly<T> s{row, l, section, S, 0.0, 1, {}};
   return s.run(logprob);
 }
 
@@ -364,7 +410,23 @@ __device__ __noinline__ int draw_slowly(const Row<T>& row, const Limits& l, doub
 template <class T>
 __device__ __noinline__ double sum_exactly(const Row<T>& row, const Limits& l, double m, double* section, Scratch& S)
 {
-  return sum_row(row, section, S, [&](float x, int) { return Sum{x > -INFINITY ? exp((double(x) - m) * l.inverse) : 0.0, 0}; }).mass;
+  const Weight64 weight = weight64(l, m, S);
+  return sum_row(row, section, S, [&](float x, int) { return Sum{x > -INFINITY ? weight(x) : 0.0, 0}; }).mass;
+}
+
+// What is drawn of all columns, by sections whose sums are in 64 bits.
+template <class T>
+__device__ __noinline__ int draw_exactly(const Row<T>& row, const Limits& l, double m, double* section, Scratch& S, float& logprob)
+{
+  const double total    = sum_exactly(row, l, m, section, S);
+  const Weight64 weight = Weight64{m, 1.4426950408889634 * l.inverse, S.power};
+  if (threadIdx.x < 32) {
+    const Place found = locate(row, section, l.u * total, [&](float x, int) { return x > -INFINITY ? weight(x) : 0.0; });
+    if (threadIdx.x == 0) S.column = found.column;
+  }
+  __syncthreads();
+  logprob = float((double(row.value(S.column)) - m) * l.inverse - log(total));
+  return S.column;
 }
 
 // Sorts n numbers, highest first, by all threads; there is room up to the next power of two.
@@ -491,6 +553,327 @@ __device__ int draw_key(Scratch& S, int n, double target)
   return S.column;
 }
 
+// The CTAs that share a row, and this one's sections of it.
+template <bool SPLIT>
+struct Team {
+  int parts, part, share, begin, end;
+  __device__ __forceinline__ void sync() const
+  {
+    if constexpr (SPLIT) cg::this_cluster().sync();
+    else __syncthreads();
+  }
+  // an object of the c-th CTA that this one has at the same place
+  template <class N>
+  __device__ __forceinline__ N* of(N* mine, int c) const
+  {
+    if constexpr (SPLIT) return cg::this_cluster().map_shared_rank(mine, c);
+    else return mine;
+  }
+  // f(s, packs) for the warps' sections, packs as they lie
+  template <class T, class F>
+  __device__ __forceinline__ void each_section(const Row<T>& row, F&& f) const
+  {
+    constexpr int kPacks = Row<T>::kPacks;
+    const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    for (int s = begin + warp; s < end; s += warps) {
+      uint4 raw[kPacks];
+      const int p0 = s * 32 * kPacks + lane;
+      if (row.whole(s)) {
+#pragma unroll
+        for (int q = 0; q < kPacks; ++q) raw[q] = __ldg(row.base + p0 + q * 32);
+      } else {
+#pragma unroll
+        for (int q = 0; q < kPacks; ++q) raw[q] = row.load(p0 + q * 32);
+      }
+      f(s, raw);
+    }
+  }
+};
+
+// The keys of all CTAs behind those of the first: their number, known to all; they are there when it is kMostKeys at most.
+template <bool SPLIT>
+__device__ __forceinline__ int gather_keys(const Team<SPLIT>& team, Scratch& S)
+{
+  team.sync();
+  if constexpr (!SPLIT) {
+    return S.keys;
+  } else {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    // lane c asks part c
+    const int keys = lane < team.parts ? team.of(&S, lane)->keys : 0;
+    const int upto = warp_upto(keys), n = __shfl_sync(0xFFFFFFFFu, upto, 31);
+    if (team.part == 0 && n <= kMostKeys)
+      for (int c = 1 + warp; c < team.parts; c += warps) {
+        const int count = __shfl_sync(0xFFFFFFFFu, keys, c), at = __shfl_sync(0xFFFFFFFFu, upto, c) - count;
+        for (int i = lane; i < count; i += 32)
+          if (GTK_IN(at + i, kMostKeys, 507)) S.key[at + i] = team.of(&S, c)->key[i];
+      }
+    team.sync();
+    return n;
+  }
+}
+
+// The lowest of the numbers between those of the keys lo (for which holds() need not) and hi (for which it does) at which holds(); it does
+// for all above.
+template <class Holds>
+__device__ __forceinline__ uint32_t lowest_key(uint32_t lo, uint32_t hi, Holds&& holds)
+{
+  while (lo < hi) {
+    const uint32_t mid = lo + (hi - lo) / 2;
+    if (holds(key_value(uint64_t(mid) << 32))) hi = mid;
+    else lo = mid + 1;
+  }
+  return hi;
+}
+
+// Rows of which more columns are left than can be ranked.  For a limit by number or by mass the columns are counted by the interval of
+// logits that they lie in, kFine of them, with weights as whole numbers (so that their sum is one in whatever order), again in the one that the limit
+// falls in while that holds too many; then one pass in 64 bits sums what lies above it, by sections, and lists the columns within.
+// Which of these are left is known once they are ranked.
+// False where that finds nothing: more equal logits at a limit than can be ranked, or a limit beyond the intervals.  The answer is the
+// first CTA's.
+template <class T, bool SPLIT>
+__device__ __noinline__ bool draw_wide(const Row<T>& row, const Limits& l, const Team<SPLIT>& team, float top, float low, double* section, Scratch& S,
+                                       int& id, float& logprob)
+{
+  constexpr int E = Row<T>::E, kPacks = Row<T>::kPacks;
+  const int tid = threadIdx.x, threads = blockDim.x, warps = threads >> 5, warp = tid >> 5, lane = tid & 31;
+  const double m        = top;
+  const Weight64 weight = weight64(l, m, S);
+  const float k         = float(weight.k);
+  const uint32_t key_top = value_key(top);
+  // what min-p leaves
+  const uint32_t key_lowest = value_key(-FLT_MAX);
+  uint32_t key_least = key_lowest;
+  if (l.least > 0.f) {
+    const double least_y = log(double(l.least));
+    key_least            = lowest_key(key_lowest, key_top, [&](float x) { return (double(x) - m) * l.inverse >= least_y; });
+  }
+  uint64_t floor = 1;  // of the rank keys that are left
+  const bool by_number = l.k != INT_MAX, by_mass = l.cut_by_mass();
+  const int bits = min(15, 30 - (31 - __clz(row.vocab)));  // of the whole numbers, vocab of which 32 bits hold
+  for (int round = by_number ? 0 : 1; round < 2 || (round == 2 && !by_number && !by_mass); ++round) {
+    const bool mass = round == 1;
+    if (mass && !by_mass) {
+      if (by_number) break;
+      round = 2;  // min-p alone
+    }
+    // ---- between which logits the limit lies: from `above` on all columns are left, below `within` none
+    uint32_t above = key_least, within = key_least;
+    double whole_near = 0.0;
+    if (round < 2) {
+      // Columns of which vocab together weigh less than half of what is cut away are below the limit by mass.  By number it is among the
+      // sets' highest, or not far below.
+      float lo = mass ? top - (log2f(float(row.vocab) / (1.f - fmaxf(l.p, 0.f))) + 2.f) / k : low - 2.f * (top - low);
+      float hi = top;
+      uint32_t key_hi = key_top + 1;  // above it nothing is looked at
+      float front     = 0.f;          // what lies above it
+      for (int level = 0;; ++level) {
+        const float scale = float(kFine) / (hi - lo) * 0.9999f, step = k / scale;
+        if (!(scale > 0.f && scale < 0x1p100f) || level == 3) return false;
+        for (int i = tid; i < kFine; i += threads) S.fine[i] = 0;
+        __syncthreads();
+        const float beyond = key_hi > key_top ? INFINITY : key_value(uint64_t(key_hi) << 32);
+        double sum = 0.0;
+        team.each_section(row, [&](int s, const uint4 (&raw)[kPacks]) {
+          float part = 0.f;
+#pragma unroll
+          for (int q = 0; q < kPacks; ++q)
+#pragma unroll
+            for (int j = 0; j < E; ++j) {
+              const float x = gtk::to_float(reinterpret_cast<const T*>(&raw[q])[j]);
+              const int c   = row.column((s * kPacks + q) * 32 + lane) + j;
+              const bool left = floor == 1 || rank_key(x, uint32_t(c)) >= floor, in = left && x < beyond;
+              if (mass && left && (level == 0 || !in)) part += pow2((x - top) * k);
+              const float at = (hi - x) * scale;
+              if (in && at < float(kFine)) {
+                const int b       = int(at);
+                const float share = mass ? pow2(fmaf(float(b) - at, step, float(bits))) : 1.f;
+                if (GTK_IN(b, kFine, 508)) atomicAdd(&S.fine[b], uint32_t(__float2int_rn(share)));
+              }
+            }
+          sum += part;
+        });
+        sum = warp_sum(sum);
+        if (lane == 0) S.mass[warp] = sum;
+        __syncthreads();
+        sum = 0.0;
+        for (int w = 0; w < warps; ++w) sum += S.mass[w];
+        if (tid == 0) S.part_sum = sum;
+        const uint32_t* fine = S.fine;
+        if constexpr (SPLIT) {
+          team.sync();
+          sum = warp_sum(lane < team.parts ? team.of(&S, lane)->part_sum : 0.0);
+          for (int i = tid; i < kFine; i += threads) {
+            uint32_t n = 0;
+            for (int c = 0; c < team.parts; ++c) n += team.of(&S, c)->fine[i];
+            S.fine_all[i] = n;
+          }
+          fine = S.fine_all;
+          team.sync();  // the others' are cleared for the next level only when all have read them
+        }
+        if (mass && level == 0) whole_near = sum;
+        if (mass && level > 0) front = float(sum);
+        // the interval that the limit falls in, and those that rounding makes possible; by every warp
+        constexpr int kEach = kFine / 32;
+        const float slack  = mass ? ldexpf(1.f, -bits) : 0.f, base = front;
+        const float wanted = mass ? fmaxf(l.p, 0.f) * float(whole_near) : float(l.k);
+        const float unit   = mass ? ldexpf(1.f, -bits) : 1.f;
+        auto interval      = [&](int b) { return float(fine[b]) * unit * (mass ? pow2((hi - top) * k - float(b) * step) : 1.f); };
+        float mine = 0.f;
+        for (int i = 0; i < kEach; ++i) mine += interval(lane * kEach + i);
+        float upto = front + warp_upto(mine) - mine;
+        int first = kFine, last = kFine;
+        float before_first = 0.f;
+        for (int i = 0; i < kEach; ++i) {
+          const float now = interval(lane * kEach + i), next = upto + now;
+          const float off = mass ? slack * (next - base) + 1e-5f * wanted : 0.f;
+          if (first == kFine && next + off >= wanted) first = lane * kEach + i, before_first = upto;
+          if (last == kFine && next - off >= wanted) last = lane * kEach + i;
+          upto = next;
+        }
+        const int first_of_all = __reduce_min_sync(0xFFFFFFFFu, first);
+        if (first_of_all == kFine) return false;  // the limit is further down
+        front = __shfl_sync(0xFFFFFFFFu, before_first, first_of_all / kEach);
+        last  = min(__reduce_min_sync(0xFFFFFFFFu, last), kFine - 1);
+        first = first_of_all;
+        int n = 0;
+        for (int b = first + lane; b <= last; b += 32) n += int(float(fine[b]) * unit * 1.02f * (mass ? pow2(step * 0.5f) : 1.f)) + 1;
+        n = warp_sum(n);
+        // the intervals' ends as numbers
+        const uint32_t key_lo = value_key(fmaxf(lo - (hi - lo) * 1e-3f, -FLT_MAX));
+        above  = lowest_key(key_lo, key_top + 1, [&](float x) { return !(x <= hi) || (hi - x) * scale < float(first); });
+        within = lowest_key(key_lo, above, [&](float x) { return (hi - x) * scale < float(last + 1); });
+        above = min(above, key_hi);
+        if (n <= kMostKeys - 64) break;
+        if (above <= within) return false;
+        const float next_hi = key_value(uint64_t(above - 1) << 32), next_lo = key_value(uint64_t(within) << 32);
+        if (!(next_lo < next_hi)) return false;  // one number
+        hi = next_hi, lo = next_lo - (next_hi - next_lo) * 1e-3f, key_hi = above;
+        __syncthreads();
+      }
+    }
+    // ---- what lies above it, and the columns within
+    __syncthreads();
+    if (tid == 0) S.keys = 0;
+    __syncthreads();
+    const float x_above = above > key_top ? INFINITY : key_value(uint64_t(above) << 32), x_within = key_value(uint64_t(within) << 32),
+                x_least = key_value(uint64_t(key_least) << 32);
+    double sum_above = 0.0, sum_all = 0.0;
+    int count = 0;
+    team.each_section(row, [&](int s, const uint4 (&raw)[kPacks]) {
+      double part = 0.0;
+#pragma unroll 1
+      for (int q = 0; q < kPacks; ++q) {
+        uint4 one = raw[0];
+#pragma unroll
+        for (int i = 1; i < kPacks; ++i)
+          if (i == q) one = raw[i];
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          const float x = gtk::to_float(reinterpret_cast<const T*>(&one)[j]);
+          const int c   = row.column((s * kPacks + q) * 32 + lane) + j;
+          const uint64_t key = rank_key(x, uint32_t(c));
+          const bool in      = key >= floor;
+          const double w     = in ? weight(x) : 0.0;
+          sum_all += w;
+          if (in && x >= x_above) {
+            sum_above += w;
+            ++count;
+            if (x >= x_least) part += w;
+          } else if (in && x >= x_within) {
+            const int at = atomicAdd(&S.keys, 1);
+            if (at < kMostKeys && GTK_IN(at, kMostKeys, 509)) S.key[at] = key;
+          }
+        }
+      }
+      part = warp_sum(part);
+      if (lane == 0 && GTK_IN(s, row.sections, 510)) section[s] = part;
+    });
+    sum_above = warp_sum(sum_above), sum_all = warp_sum(sum_all), count = warp_sum(count);
+    if (lane == 0) S.mass[warp] = sum_above, S.count[warp] = count;
+    __syncthreads();
+    sum_above = 0.0, count = 0;
+    for (int w = 0; w < warps; ++w) sum_above += S.mass[w], count += S.count[w];
+    __syncthreads();
+    if (lane == 0) S.mass[warp] = sum_all;
+    __syncthreads();
+    sum_all = 0.0;
+    for (int w = 0; w < warps; ++w) sum_all += S.mass[w];
+    if (tid == 0) S.part_mass[0] = sum_above, S.part_mass[1] = sum_all, S.part_count = count;
+    const int n = gather_keys(team, S);
+    if (n > kMostKeys) return false;
+    if constexpr (SPLIT) {
+      if (team.part == 0) {
+        sum_above = warp_sum(lane < team.parts ? team.of(&S, lane)->part_mass[0] : 0.0);
+        sum_all   = warp_sum(lane < team.parts ? team.of(&S, lane)->part_mass[1] : 0.0);
+        count     = warp_sum(lane < team.parts ? team.of(&S, lane)->part_count : 0);
+        for (int s = team.end + tid; s < row.sections; s += threads) section[s] = team.of(section, s / team.share)[s];
+      }
+      team.sync();
+    }
+    // ---- which of these are left
+    if (team.part == 0) {
+      int left = 0;
+      if (n > 0) {
+        __syncthreads();
+        sort_keys(S, n);
+        for (int i = tid; i < n; i += threads) S.weight[i] = weight(key_value(S.key[i]));
+        __syncthreads();
+      }
+      bool solved = true;
+      if (round == 0) {
+        left   = l.k - count;
+        solved = left >= 0 && left <= n;
+      } else if (round == 1) {
+        const double reach = fmax(0.0, double(l.p)) * sum_all;
+        // the list's weights in front of every lane's share of it, by every warp
+        const int each = (n + 31) / 32, begin = min(n, lane * each), end = min(n, begin + each);
+        double mine = 0.0;
+        for (int i = begin; i < end; ++i) mine += S.weight[i];
+        double upto = sum_above + warp_upto(mine) - mine;
+        left        = INT_MAX;
+        for (int i = begin; i < end && left == INT_MAX; ++i)
+          if ((upto += S.weight[i]) >= reach) left = i + 1;
+        left   = __reduce_min_sync(0xFFFFFFFFu, left);
+        solved = sum_above < reach && left != INT_MAX;  // the limit is neither above nor below
+      }
+      if (solved && left > 0) floor = max(floor, S.key[left - 1]);
+      else floor = max(floor, uint64_t(above) << 32);
+      if (solved && !(round == 0 && by_mass)) {
+        floor = max(floor, uint64_t(key_least) << 32);
+        // the sections with what is left of the list, and the draw
+        for (int s = tid; s < row.sections; s += threads) {
+          double sum = section[s];
+          for (int i = 0; i < left; ++i)
+            if (S.key[i] >= floor && int(key_column(S.key[i]) + row.lead) / kSection == s) sum += S.weight[i];
+          section[s] = sum;
+        }
+        __syncthreads();
+        if (warp == 0) {
+          double total = 0.0;
+          for (int s = lane; s < row.sections; s += 32) total += section[s];
+          total            = warp_sum(total);
+          const Place found = locate(row, section, l.u * total, [&](float x, int c) { return rank_key(x, uint32_t(c)) >= floor ? weight(x) : 0.0; });
+          if (lane == 0) S.column = found.column, S.total = total;
+        }
+        __syncthreads();
+        id      = S.column;
+        logprob = id < 0 ? 0.f : float((double(row.value(id)) - m) * l.inverse - log(S.total));
+        solved  = id >= 0;
+      }
+      if (tid == 0) S.solved = solved, S.floor = floor;
+    }
+    team.sync();
+    const Scratch* first = team.of(&S, 0);
+    const bool solved    = first->solved;
+    floor                = first->floor;
+    team.sync();
+    if (!solved || !(round == 0 && by_mass)) return solved;
+  }
+  return false;
+}
+
 template <class T, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 4) k_sample(const T* __restrict__ logits, const SampleArgs a, int n_parts)
 {
@@ -521,27 +904,19 @@ __global__ void __launch_bounds__(kThreads, 4) k_sample(const T* __restrict__ lo
   const float k     = ranged ? float(k64) : 1.f;
   const int share = (row.sections + parts - 1) / parts;
   const int begin = min(row.sections, part * share), end = min(row.sections, begin + share);
+  const Team<SPLIT> team{parts, part, share, begin, end};
   float2* const piece = reinterpret_cast<float2*>(s_section);
-  typename P::Max best[kSets];
+  typename P::Max best[kPacks];
 #pragma unroll
-  for (int q = 0; q < kSets; ++q) best[q] = P::lowest();
+  for (int q = 0; q < kPacks; ++q) best[q] = P::lowest();
   float top = -INFINITY, ref = kLow;
-  for (int s = begin + warp; s < end; s += warps) {
-    uint4 raw[kPacks];
-    const int p0 = s * 32 * kPacks + lane;
-    if (row.whole(s)) {
-#pragma unroll
-      for (int q = 0; q < kPacks; ++q) raw[q] = __ldg(row.base + p0 + q * 32);
-    } else {
-#pragma unroll
-      for (int q = 0; q < kPacks; ++q) raw[q] = row.load(p0 + q * 32);
-    }
+  team.each_section(row, [&](int s, const uint4 (&raw)[kPacks]) {
     typename P::Max most = P::highest(raw[0]);
     best[0]              = P::higher(best[0], most);
 #pragma unroll
     for (int q = 1; q < kPacks; ++q) {
       const typename P::Max m = P::highest(raw[q]);
-      best[q % kSets]         = P::higher(best[q % kSets], m);
+      best[q] = P::higher(best[q], m);
       most                    = P::higher(most, m);
     }
     const float high = warp_max(P::kHalves == 2 ? fmaxf(P::of(most, 0), P::of(most, 1)) : P::of(most, 0));
@@ -573,10 +948,10 @@ __global__ void __launch_bounds__(kThreads, 4) k_sample(const T* __restrict__ lo
     sum[0].get(lo, hi);
     lo = warp_sum(lo + hi);
     if (lane == 0 && GTK_IN(s, row.sections, 503)) piece[s] = make_float2(c, lo);
-  }
+  });
   float low = INFINITY;
 #pragma unroll
-  for (int q = 0; q < kSets; ++q) {
+  for (int q = 0; q < kPacks; ++q) {
     const float v = P::kHalves == 2 ? fmaxf(P::of(best[q], 0), P::of(best[q], 1)) : P::of(best[q], 0);
     if (v > -INFINITY) low = fminf(low, v);
   }
@@ -611,7 +986,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_sample(const T* __restrict__ lo
   const bool all = l.all();
   if (!all) {
 #pragma unroll
-    for (int q = 0; q < kSets; ++q) {
+    for (int q = 0; q < kPacks; ++q) {
       const float v = P::kHalves == 2 ? fmaxf(P::of(best[q], 0), P::of(best[q], 1)) : P::of(best[q], 0);
       if (v > -INFINITY) {
         const int at = int(fminf((top - v) * scale, float(kBins - 1)));
@@ -665,7 +1040,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_sample(const T* __restrict__ lo
       if (S.sure) return put(S.column, float((double(row.value(S.column)) - m) * l.inverse + 0.6931471805599453 * shift - log(sum)));
     }
     float logprob;
-    const int id = draw_slowly(row, l, s_section, S, logprob);
+    const int id = fast ? draw_exactly(row, l, m, s_section, S, logprob) : draw_slowly(row, l, s_section, S, logprob);
     return put(id, logprob);
   }
 
@@ -707,22 +1082,22 @@ __global__ void __launch_bounds__(kThreads, 4) k_sample(const T* __restrict__ lo
   }
   if (some) {
     auto reaches = [&](float x) { return everything || (top - x) * scale < bound; };
-    uint32_t* const set = S.order + warp * (kMostKeys / kWarps);
+    uint32_t* const set = S.order + warp * kSetsOfWarp;
+    static_assert(kPacks * 32 <= kSetsOfWarp && kWarps * kSetsOfWarp >= kMostKeys, "");
     int sets            = 0;
 #pragma unroll
-    for (int q = 0; q < kSets; ++q) {
+    for (int q = 0; q < kPacks; ++q) {
       const float v       = P::kHalves == 2 ? fmaxf(P::of(best[q], 0), P::of(best[q], 1)) : P::of(best[q], 0);
       const bool mine     = v > -INFINITY && reaches(v);
       const uint32_t them = __ballot_sync(0xFFFFFFFFu, mine);
       const int at        = sets + __popc(them & ((1u << lane) - 1u));
-      if (mine && GTK_IN(at, kMostKeys / kWarps, 505)) set[at] = q * 32 + lane;
+      if (mine && GTK_IN(at, kSetsOfWarp, 505)) set[at] = q * 32 + lane;
       sets += __popc(them);
     }
     __syncwarp();
-    const int sections = (end - begin - warp + warps - 1) / warps, packs = sets * max(0, sections) * (kPacks / kSets);
+    const int sections = (end - begin - warp + warps - 1) / warps, packs = sets * max(0, sections);
     for (int i = lane; i < packs; i += 32) {
-      const int which = i % sets, rest = i / sets, s = begin + warp + rest / (kPacks / kSets) * warps;
-      const int p     = s * 32 * kPacks + int(set[which]) + rest % (kPacks / kSets) * 32 * kSets;
+      const int p     = (begin + warp + i / sets * warps) * 32 * kPacks + int(set[i % sets]);
       const uint4 raw = row.load(p);
 #pragma unroll
       for (int j = 0; j < E; ++j) {
@@ -734,30 +1109,17 @@ __global__ void __launch_bounds__(kThreads, 4) k_sample(const T* __restrict__ lo
       }
     }
   }
-  __syncthreads();
-  int n = S.keys;
-  if constexpr (SPLIT) {
-    cg::cluster_group cluster = cg::this_cluster();
-    cluster.sync();
-    if (part == 0) {
-      const int keys = lane < parts ? cluster.map_shared_rank(&S, lane)->keys : 0;
-      const int upto = warp_upto(keys);
-      n              = __shfl_sync(0xFFFFFFFFu, upto, 31);
-      if (n <= kMostKeys)
-        for (int c = 1 + warp; c < parts; c += warps) {
-          const int count = __shfl_sync(0xFFFFFFFFu, keys, c), at = __shfl_sync(0xFFFFFFFFu, upto, c) - count;
-          for (int i = lane; i < count; i += 32)
-            if (GTK_IN(at + i, kMostKeys, 507)) S.key[at + i] = cluster.map_shared_rank(&S, c)->key[i];
-        }
-    }
-    cluster.sync();  // nobody leaves while its shared memory is read
-    if (part != 0) return;
-  }
+  const int n = gather_keys(team, S);
   if (!some || n > kMostKeys) {
-    float logprob;
-    const int id = draw_slowly(row, l, s_section, S, logprob);
+    float logprob = 0.f;
+    int id        = -1;
+    const bool solved = draw_wide(row, l, team, top, low, s_section, S, id, logprob);
+    team.sync();  // nobody leaves while its shared memory is read
+    if (part != 0) return;
+    if (!solved) id = draw_slowly(row, l, s_section, S, logprob);
     return put(id, logprob);
   }
+  if (part != 0) return;
 
   // ---- the columns that are known, ranked
   sort_keys(S, n);
