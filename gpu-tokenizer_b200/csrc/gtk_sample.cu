@@ -28,11 +28,11 @@ using gtk::value_key;
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
 constexpr int kMaxParts = 8;     // CTAs that share a row
-constexpr int kSection  = 1024;  // columns whose sum is kept, neighbours of each other, one warp's at a time
+constexpr int kPacks    = 4;     // of 16 bytes that a thread has of a section: 32 * kPacks neighbouring packs, whose sum is kept
 constexpr int kBins     = 256;
 constexpr int kFine     = 1024;  // bins of a wide row
 constexpr int kMostKeys = 1024;  // columns that are ranked at most
-constexpr int kSetsOfWarp = 256;  // of its columns that a warp knows the highest of, at most
+constexpr int kSetsOfWarp = 32 * kPacks;  // of its columns that a warp knows the highest of, at most
 constexpr float kLow    = -0x1p60f;
 
 struct SampleArgs {
@@ -94,7 +94,7 @@ struct Scratch {
 // A row as the packs of 16 bytes that it touches; what lies in them outside of it counts as -inf.
 template <class T>
 struct Row {
-  static constexpr int E = Pack16<T>::kElems, kPacks = kSection / (32 * E);
+  static constexpr int E = Pack16<T>::kElems, kColumns = 32 * kPacks * E;  // of a section
   const uint4* base;
   int vocab, lead, packs, sections;
   __device__ Row(const T* x, int vocab_) : vocab(vocab_)
@@ -124,6 +124,17 @@ struct Row {
   }
   // The first and the last pack are in no such section.
   __device__ __forceinline__ bool whole(int s) const { return s > 0 && (s + 1) * 32 * kPacks < packs; }
+  __device__ __forceinline__ void load_section(int s, uint4 (&raw)[kPacks]) const
+  {
+    const int p0 = s * 32 * kPacks + int(threadIdx.x & 31);
+    if (whole(s)) {
+#pragma unroll
+      for (int q = 0; q < kPacks; ++q) raw[q] = __ldg(base + p0 + q * 32);
+    } else {
+#pragma unroll
+      for (int q = 0; q < kPacks; ++q) raw[q] = load(p0 + q * 32);
+    }
+  }
   // Of the sum of 32-bit weights, in any part of the row and relative to the sum of all, when that is `sum` times the highest's weight: a
   // weight is off by two roundings of its exponent y, by 2^-22 for the exponential itself and as much for that of its section;
   // ten additions and a product in its section.  The exponents' part is 2 * 2^-24 * ln 2 * |y|, and the weights' mean of ln 2 * |y| is their entropy less
@@ -208,19 +219,20 @@ __device__ __forceinline__ Sum sum_row(const Row<T>& row, double* section, Scrat
   const int threads = blockDim.x, warps = threads >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   Sum s{0.0, 0};
   constexpr int kAtOnce = 16 / Row<T>::E;  // packs
+  static_assert(kPacks % kAtOnce == 0, "");
   __syncthreads();
   for (int i = warp; i < row.sections; i += warps) {
     double sum = 0.0;
 #pragma unroll 1
-    for (int q = 0; q < Row<T>::kPacks; q += kAtOnce) {
+    for (int q = 0; q < kPacks; q += kAtOnce) {
       uint4 raw[kAtOnce];
 #pragma unroll
-      for (int b = 0; b < kAtOnce; ++b) raw[b] = row.load((i * Row<T>::kPacks + q + b) * 32 + lane);
+      for (int b = 0; b < kAtOnce; ++b) raw[b] = row.load((i * kPacks + q + b) * 32 + lane);
 #pragma unroll
       for (int b = 0; b < kAtOnce; ++b) {
 #pragma unroll
         for (int j = 0; j < Row<T>::E; ++j) {
-          const Sum o = weigh(gtk::to_float(reinterpret_cast<const T*>(&raw[b])[j]), row.column((i * Row<T>::kPacks + q + b) * 32 + lane) + j);
+          const Sum o = weigh(gtk::to_float(reinterpret_cast<const T*>(&raw[b])[j]), row.column((i * kPacks + q + b) * 32 + lane) + j);
           sum += o.mass, s.count += o.count;
         }
       }
@@ -270,14 +282,14 @@ __device__ __forceinline__ Place locate(const Row<T>& row, const double* section
   s     = __shfl_sync(all, s, from);
   front = __shfl_sync(all, front, from);
   // neighbouring packs to a lane
-  double w[Row<T>::kPacks];
+  double w[kPacks];
   mine = 0.0;
-  uint4 raw[Row<T>::kPacks];
+  uint4 raw[kPacks];
 #pragma unroll
-  for (int q = 0; q < Row<T>::kPacks; ++q) raw[q] = row.load((s * 32 + lane) * Row<T>::kPacks + q);
+  for (int q = 0; q < kPacks; ++q) raw[q] = row.load((s * 32 + lane) * kPacks + q);
 #pragma unroll
-  for (int q = 0; q < Row<T>::kPacks; ++q) {
-    const int c = row.column((s * 32 + lane) * Row<T>::kPacks + q);
+  for (int q = 0; q < kPacks; ++q) {
+    const int c = row.column((s * 32 + lane) * kPacks + q);
     w[q]        = 0.0;
 #pragma unroll
     for (int j = 0; j < Row<T>::E; ++j) w[q] += weigh(gtk::to_float(reinterpret_cast<const T*>(&raw[q])[j]), c + j);
@@ -291,8 +303,8 @@ __device__ __forceinline__ Place locate(const Row<T>& row, const double* section
   if (lane == from) {
     double sum = upto_lane - mine;
 #pragma unroll
-    for (int q = 0; q < Row<T>::kPacks; ++q) {
-      const int c = row.column((s * 32 + lane) * Row<T>::kPacks + q);
+    for (int q = 0; q < kPacks; ++q) {
+      const int c = row.column((s * 32 + lane) * kPacks + q);
 #pragma unroll
       for (int j = 0; j < Row<T>::E; ++j) {
         const double v = weigh(gtk::to_float(reinterpret_cast<const T*>(&raw[q])[j]), c + j);
@@ -573,18 +585,10 @@ struct Team {
   template <class T, class F>
   __device__ __forceinline__ void each_section(const Row<T>& row, F&& f) const
   {
-    constexpr int kPacks = Row<T>::kPacks;
-    const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    for (int s = begin + warp; s < end; s += warps) {
+    const int warps = blockDim.x >> 5;
+    for (int s = begin + (threadIdx.x >> 5); s < end; s += warps) {
       uint4 raw[kPacks];
-      const int p0 = s * 32 * kPacks + lane;
-      if (row.whole(s)) {
-#pragma unroll
-        for (int q = 0; q < kPacks; ++q) raw[q] = __ldg(row.base + p0 + q * 32);
-      } else {
-#pragma unroll
-        for (int q = 0; q < kPacks; ++q) raw[q] = row.load(p0 + q * 32);
-      }
+      row.load_section(s, raw);
       f(s, raw);
     }
   }
@@ -636,7 +640,7 @@ template <class T, bool SPLIT>
 __device__ __noinline__ bool draw_wide(const Row<T>& row, const Limits& l, const Team<SPLIT>& team, float top, float low, double* section, Scratch& S,
                                        int& id, float& logprob)
 {
-  constexpr int E = Row<T>::E, kPacks = Row<T>::kPacks;
+  constexpr int E = Row<T>::E;
   const int tid = threadIdx.x, threads = blockDim.x, warps = threads >> 5, warp = tid >> 5, lane = tid & 31;
   const double m        = top;
   const Weight64 weight = weight64(l, m, S);
@@ -846,7 +850,7 @@ __device__ __noinline__ bool draw_wide(const Row<T>& row, const Limits& l, const
         for (int s = tid; s < row.sections; s += threads) {
           double sum = section[s];
           for (int i = 0; i < left; ++i)
-            if (S.key[i] >= floor && int(key_column(S.key[i]) + row.lead) / kSection == s) sum += S.weight[i];
+            if (S.key[i] >= floor && int(key_column(S.key[i]) + row.lead) / Row<T>::kColumns == s) sum += S.weight[i];
           section[s] = sum;
         }
         __syncthreads();
@@ -879,7 +883,6 @@ __global__ void __launch_bounds__(kThreads, 4) k_sample(const T* __restrict__ lo
 {
   using P              = Pack16<T>;
   constexpr int E      = P::kElems;
-  constexpr int kPacks = Row<T>::kPacks;
   extern __shared__ double s_section[];  // a whole row's
   __shared__ Scratch S;
   const int parts = SPLIT ? n_parts : 1;
@@ -887,6 +890,11 @@ __global__ void __launch_bounds__(kThreads, 4) k_sample(const T* __restrict__ lo
   const int64_t r = blockIdx.x / unsigned(parts);
   const int part  = int(blockIdx.x % unsigned(parts));
   const Row<T> row(logits + r * a.stride, a.vocab);
+  const int share = (row.sections + parts - 1) / parts;
+  const int begin = min(row.sections, part * share), end = min(row.sections, begin + share);
+  const Team<SPLIT> team{parts, part, share, begin, end};
+  uint4 raw[kPacks];
+  if (begin + warp < end) row.load_section(begin + warp, raw);  // while the limits come in
   const Limits l(a, r);
   auto put = [&](int id, float logprob) {
     if (tid != 0 || part != 0) return;
@@ -902,15 +910,12 @@ __global__ void __launch_bounds__(kThreads, 4) k_sample(const T* __restrict__ lo
   const double k64  = 1.4426950408889634 * l.inverse;
   const bool ranged = k64 > 0x1p-20 && k64 < 0x1p20;
   const float k     = ranged ? float(k64) : 1.f;
-  const int share = (row.sections + parts - 1) / parts;
-  const int begin = min(row.sections, part * share), end = min(row.sections, begin + share);
-  const Team<SPLIT> team{parts, part, share, begin, end};
   float2* const piece = reinterpret_cast<float2*>(s_section);
   typename P::Max best[kPacks];
 #pragma unroll
   for (int q = 0; q < kPacks; ++q) best[q] = P::lowest();
   float top = -INFINITY, ref = kLow;
-  team.each_section(row, [&](int s, const uint4 (&raw)[kPacks]) {
+  auto take = [&](int s, const uint4 (&raw)[kPacks]) {
     typename P::Max most = P::highest(raw[0]);
     best[0]              = P::higher(best[0], most);
 #pragma unroll
@@ -948,7 +953,15 @@ __global__ void __launch_bounds__(kThreads, 4) k_sample(const T* __restrict__ lo
     sum[0].get(lo, hi);
     lo = warp_sum(lo + hi);
     if (lane == 0 && GTK_IN(s, row.sections, 503)) piece[s] = make_float2(c, lo);
-  });
+  };
+  for (int s = begin + warp; s < end; s += 2 * warps) {
+    uint4 next[kPacks];
+    if (s + warps < end) row.load_section(s + warps, next);
+    take(s, raw);
+    if (s + warps >= end) break;
+    if (s + 2 * warps < end) row.load_section(s + 2 * warps, raw);
+    take(s + warps, next);
+  }
   float low = INFINITY;
 #pragma unroll
   for (int q = 0; q < kPacks; ++q) {
@@ -1083,7 +1096,7 @@ __global__ void __launch_bounds__(kThreads, 4) k_sample(const T* __restrict__ lo
   if (some) {
     auto reaches = [&](float x) { return everything || (top - x) * scale < bound; };
     uint32_t* const set = S.order + warp * kSetsOfWarp;
-    static_assert(kPacks * 32 <= kSetsOfWarp && kWarps * kSetsOfWarp >= kMostKeys, "");
+    static_assert(kWarps * kSetsOfWarp >= kMostKeys, "");
     int sets            = 0;
 #pragma unroll
     for (int q = 0; q < kPacks; ++q) {
@@ -1144,6 +1157,8 @@ __global__ void __launch_bounds__(kThreads, 4) k_sample(const T* __restrict__ lo
   put(id, l.t == 0.f || id < 0 ? 0.f : float((double(row.value(id)) - m) * l.inverse - log(total)));
 }
 
+static_assert(sizeof(Scratch) + (GTK_MAX_SAMPLE_VOCAB / (32 * kPacks * 4) + 1) * sizeof(double) <= 48 << 10, "what a CTA has without asking");
+
 struct Teams {
   int parts, threads;
 };
@@ -1158,8 +1173,9 @@ template <class T>
 cudaError_t launch_sample(const gtk::HandleView& v, const void* logits, int64_t n_rows, const SampleArgs& a)
 {
   const Teams t         = teams_for(n_rows, int64_t(a.vocab) * int64_t(sizeof(T)), v.sm_count);
-  const size_t sections = (size_t(a.vocab) + 16 / sizeof(T) + kSection - 1) / kSection;
-  return gtk::launch_clusters(t.parts > 1 ? k_sample<T, true> : k_sample<T, false>, dim3(unsigned(n_rows * t.parts)), dim3(unsigned(t.threads)),
+  const size_t sections = (size_t(a.vocab) + Row<T>::E + Row<T>::kColumns - 1) / Row<T>::kColumns;
+  const auto kernel = t.parts > 1 ? k_sample<T, true> : k_sample<T, false>;
+  return gtk::launch_clusters(kernel, dim3(unsigned(n_rows * t.parts)), dim3(unsigned(t.threads)),
                               t.parts, sections * sizeof(double), v.stream, static_cast<const T*>(logits), a, t.parts);
 }
 
