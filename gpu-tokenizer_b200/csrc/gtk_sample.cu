@@ -88,7 +88,7 @@ struct Scratch {
   uint64_t floor;
   int column, keys, left, part_count, solved;
   bool sure;
-  float part_top, part_low;
+  float part_top;
 };
 
 // A row as the packs of 16 bytes that it touches; what lies in them outside of it counts as -inf.
@@ -135,13 +135,14 @@ struct Row {
       for (int q = 0; q < kPacks; ++q) raw[q] = load(p0 + q * 32);
     }
   }
-  // Of the sum of 32-bit weights, in any part of the row and relative to the sum of all, when that is `sum` times the highest's weight: a
-  // weight is off by two roundings of its exponent y, by 2^-22 for the exponential itself and as much for that of its section;
-  // ten additions and a product in its section.  The exponents' part is 2 * 2^-24 * ln 2 * |y|, and the weights' mean of ln 2 * |y| is their entropy less
-  // ln(sum), ln(vocab / sum) at most.
-  __device__ __forceinline__ double error(double sum) const
+  // Bounds of what 32 bits cost, in parts of 2^-24 of the sum of all weights, when that is at least `sum` times the highest's.  A weight 2^y, y =
+  // x k - c rounded once, with k rounded once: 2 ln 2 |y| such parts of itself, and 4 for the exponential (2^-22).  The weights' mean of
+  // ln 2 |y| is their entropy less ln(sum), ln(vocab / sum) at most, and c, a whole number, adds less than one to |y|.  The sum of a section:
+  // ten additions (four or five of a thread's, five of the warp's), and nothing more where sections are added, in 64 bits.
+  static constexpr float kWeightError = 4.f, kSumError = 10.f;
+  __device__ __forceinline__ float exponent_error(double sum) const
   {
-    return (2.f * 0.6932f * fmaxf(0.f, log2f(float(vocab) / float(sum)) + 0.01f) + 20.f) * 0x1p-24;
+    return 2.f * 0.6932f * (fmaxf(0.f, log2f(float(vocab) / float(sum))) + 1.1f);
   }
 };
 
@@ -249,74 +250,73 @@ __device__ __forceinline__ Sum sum_row(const Row<T>& row, double* section, Scrat
   return s;
 }
 
-// A column, and the sums of the weights in front of it and with it.
+// A column with its section and its logit, and the sums of the weights in front of it and with it.
 struct Place {
-  int column;
+  int column, section;
   double before, upto;
+  float x;
 };
 
-// The first column at which the sum of weigh(x, column) exceeds the target, by one warp, whose sums by sections are there; the last one with
-// any weight where rounding leaves none, column -1 where none has any.
-template <class T, class Weigh>
-__device__ __forceinline__ Place locate(const Row<T>& row, const double* section, double target, Weigh&& weigh)
+// The first column at which the sum of the weights exceeds the target, `share` of the sum of all, by one warp: section(s) is a section's sum, weigh(s)(x,
+// column) the weight of a column in it.  The last one with any weight where rounding leaves none, column -1 where none has any.
+template <class T, class Section, class Weigh>
+__device__ __forceinline__ Place locate(const Row<T>& row, double share, double& total, Section&& section, Weigh&& weigh)
 {
-  const int lane = threadIdx.x & 31, each = (row.sections + 31) / 32;
   constexpr uint32_t all = 0xFFFFFFFFu;
+  constexpr int kOwn     = kPacks * Row<T>::E;  // neighbouring columns of a lane
+  static_assert(kOwn <= 32, "");
+  const int lane = threadIdx.x & 31, each = (row.sections + 31) / 32;
+  // the lane in whose share the target lies, of those with any weight
+  auto lane_of = [&](double mine, double upto, double target) {
+    const uint32_t over = __ballot_sync(all, mine > 0.0 && upto > target), some = __ballot_sync(all, mine > 0.0);
+    return over ? __ffs(over) - 1 : some ? 31 - __clz(some) : -1;
+  };
   const int begin = min(lane * each, row.sections), end = min(begin + each, row.sections);
   double mine = 0.0;
-  for (int i = begin; i < end; ++i) mine += section[i];
-  const double upto   = warp_upto(mine);
-  uint32_t over       = __ballot_sync(all, mine > 0.0 && upto > target);
-  const uint32_t some = __ballot_sync(all, mine > 0.0);
-  if (some == 0) return Place{-1, 0.0, 0.0};
-  int from = over ? __ffs(over) - 1 : 31 - __clz(some);
+  for (int i = begin; i < end; ++i) mine += section(i);
+  double upto = warp_upto(mine);
+  total       = __shfl_sync(all, upto, 31);
+  const double target = share * total;
+  int from = lane_of(mine, upto, target);
+  if (from < 0) return Place{-1, -1, 0.0, 0.0, 0.f};
   int s        = -1;
   double front = upto - mine, next = front;
   if (lane == from)
     for (int i = begin; i < end; ++i) {
-      if (!(section[i] > 0.0)) continue;
+      const double w = section(i);
+      if (!(w > 0.0)) continue;
       s = i, front = next;
-      next += section[i];
+      next += w;
       if (next > target) break;
     }
   s     = __shfl_sync(all, s, from);
   front = __shfl_sync(all, front, from);
   // neighbouring packs to a lane
-  double w[kPacks];
-  mine = 0.0;
+  auto weight = weigh(s);
   uint4 raw[kPacks];
 #pragma unroll
   for (int q = 0; q < kPacks; ++q) raw[q] = row.load((s * 32 + lane) * kPacks + q);
+  double sums[kPacks];
 #pragma unroll
   for (int q = 0; q < kPacks; ++q) {
     const int c = row.column((s * 32 + lane) * kPacks + q);
-    w[q]        = 0.0;
+    sums[q]     = 0.0;
 #pragma unroll
-    for (int j = 0; j < Row<T>::E; ++j) w[q] += weigh(gtk::to_float(reinterpret_cast<const T*>(&raw[q])[j]), c + j);
-    mine += w[q];
+    for (int j = 0; j < Row<T>::E; ++j) sums[q] += weight(gtk::to_float(reinterpret_cast<const T*>(&raw[q])[j]), c + j);
   }
-  const double upto_lane = front + warp_upto(mine);
-  over                   = __ballot_sync(all, mine > 0.0 && upto_lane > target);
-  const uint32_t some2   = __ballot_sync(all, mine > 0.0);
-  from                   = over ? __ffs(over) - 1 : some2 ? 31 - __clz(some2) : 0;
-  Place found{-1, 0.0, 0.0};
-  if (lane == from) {
-    double sum = upto_lane - mine;
-#pragma unroll
-    for (int q = 0; q < kPacks; ++q) {
-      const int c = row.column((s * 32 + lane) * kPacks + q);
-#pragma unroll
-      for (int j = 0; j < Row<T>::E; ++j) {
-        const double v = weigh(gtk::to_float(reinterpret_cast<const T*>(&raw[q])[j]), c + j);
-        if (v > 0.0 && !(found.column >= 0 && found.upto > target)) found = Place{c + j, sum, sum + v};
-        sum += v;
-      }
-    }
-  }
-  found.column = __shfl_sync(all, found.column, from);
-  found.before = __shfl_sync(all, found.before, from);
-  found.upto   = __shfl_sync(all, found.upto, from);
-  return found;
+  mine = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+  static_assert(kPacks == 4, "");
+  upto = front + warp_upto(mine);
+  from = lane_of(mine, upto, target);
+  if (from < 0) return Place{-1, s, 0.0, 0.0, 0.f};
+  front = __shfl_sync(all, upto - mine, from);
+  // a column to a lane
+  const int c = row.column((s * 32 + from) * kPacks) + lane;
+  mine        = lane < kOwn && uint32_t(c) < uint32_t(row.vocab) ? weight(row.value(c), c) : 0.0;
+  upto        = front + warp_upto(mine);
+  from        = lane_of(mine, upto, target);
+  if (from < 0) return Place{-1, s, 0.0, 0.0, 0.f};
+  return Place{__shfl_sync(all, c, from), s, __shfl_sync(all, upto - mine, from), __shfl_sync(all, upto, from), __shfl_sync(all, row.value(min(max(c, 0), row.vocab - 1)), from)};
 }
 
 // Everything in 64 bits, by one CTA, in as many readings of the row as it takes: rows of which nothing else is known, or whose borders
@@ -330,23 +330,26 @@ struct Slowly {
   double m;
   uint64_t floor;  // what is left reaches it, see rank_key
   Weight64 power;
+  double total;  // of the last find
 
   __device__ double weight(float x) const { return x > -INFINITY ? power(x) : 0.0; }
   __device__ bool left(float x, int c) const { return rank_key(x, uint32_t(c)) >= floor; }
 
-  // the first column at which `weigh` exceeds the target, known to all threads
+  // the first column at which `weigh` exceeds a share of its sum, known to all threads
   template <class Weigh>
-  __device__ Place find(double target, Weigh&& weigh)
+  __device__ int find(double share, Weigh&& weigh)
   {
     __syncthreads();
     if (threadIdx.x < 32) {
-      const Place found = locate(row, section, target, weigh);
-      if (threadIdx.x == 0) S.column = found.column, S.at = found.before, S.total = found.upto;
+      double total;
+      const Place found = locate(row, share, total, [&](int s) { return section[s]; }, [&](int) { return weigh; });
+      if (threadIdx.x == 0) S.column = found.column, S.total = total;
     }
     __syncthreads();
-    const Place found{S.column, S.at, S.total};
+    const int column = S.column;
+    total            = S.total;
     __syncthreads();
-    return found;
+    return column;
   }
 
   // Raises the floor to the highest value at which enough(sum over the columns that reach it) holds, and there to as many columns of that
@@ -364,8 +367,8 @@ struct Slowly {
     const Sum above = sum_row(row, section, S, [&](float x, int c) { return value_key(x) > lo && left(x, c) ? Sum{weight(x), 1} : Sum{0.0, 0}; });
     const float value  = key_value(uint64_t(lo) << 32);
     auto equal         = [&](float x, int c) { return value_key(x) == lo && left(x, c) ? 1.0 : 0.0; };
-    sum_row(row, section, S, [&](float x, int c) { return Sum{equal(x, c), 0}; });
-    const int column = find(wanted(above, weight(value)) - 1.0, equal).column;
+    const double equals = sum_row(row, section, S, [&](float x, int c) { return Sum{equal(x, c), 0}; }).mass;
+    const int column    = find((wanted(above, weight(value)) - 0.5) / equals, equal);
     floor            = max(floor, rank_key(value, uint32_t(column)));
   }
 
@@ -403,8 +406,8 @@ struct Slowly {
     }
     const double least_y = l.least > 0.f ? log(double(l.least)) : -INFINITY;
     auto drawn           = [&](float x, int c) { return left(x, c) && (double(x) - m) * l.inverse >= least_y ? weight(x) : 0.0; };
-    const double total   = sum_row(row, section, S, [&](float x, int c) { return Sum{drawn(x, c), 0}; }).mass;
-    const int id         = find(l.u * total, drawn).column;
+    sum_row(row, section, S, [&](float x, int c) { return Sum{drawn(x, c), 0}; });
+    const int id = find(l.u, drawn);
     if (id < 0) return -1;
     logprob = l.t == 0.f ? 0.f : float((double(row.value(id)) - m) * l.inverse - log(total));
     return id;
@@ -414,7 +417,7 @@ struct Slowly {
 template <class T>
 __device__ __noinline__ int draw_slowly(const Row<T>& row, const Limits& l, double* section, Scratch& S, float& logprob)
 {
-  Slowly<T> s{row, l, section, S, 0.0, 1, {}};
+  Slowly<T> s{row, l, section, S, 0.0, 1, {}, 0.0};
   return s.run(logprob);
 }
 
@@ -426,19 +429,18 @@ __device__ __noinline__ double sum_exactly(const Row<T>& row, const Limits& l, d
   return sum_row(row, section, S, [&](float x, int) { return Sum{x > -INFINITY ? weight(x) : 0.0, 0}; }).mass;
 }
 
-// What is drawn of all columns, by sections whose sums are in 64 bits.
+// What is drawn of all columns, with everything in 64 bits.
 template <class T>
 __device__ __noinline__ int draw_exactly(const Row<T>& row, const Limits& l, double m, double* section, Scratch& S, float& logprob)
 {
-  const double total    = sum_exactly(row, l, m, section, S);
-  const Weight64 weight = Weight64{m, 1.4426950408889634 * l.inverse, S.power};
-  if (threadIdx.x < 32) {
-    const Place found = locate(row, section, l.u * total, [&](float x, int) { return x > -INFINITY ? weight(x) : 0.0; });
-    if (threadIdx.x == 0) S.column = found.column;
-  }
-  __syncthreads();
-  logprob = float((double(row.value(S.column)) - m) * l.inverse - log(total));
-  return S.column;
+  sum_exactly(row, l, m, section, S);
+  const Weight64 weight{m, 1.4426950408889634 * l.inverse, S.power};
+  if (threadIdx.x >= 32) return -1;
+  double total;
+  const Place found = locate(row, l.u, total, [&](int s) { return section[s]; },
+                             [&](int) { return [&](float x, int) { return x > -INFINITY ? weight(x) : 0.0; }; });
+  logprob           = float((double(found.x) - m) * l.inverse - log(total));
+  return found.column;
 }
 
 // Sorts n numbers, highest first, by all threads; there is room up to the next power of two.
@@ -855,10 +857,9 @@ __device__ __noinline__ bool draw_wide(const Row<T>& row, const Limits& l, const
         }
         __syncthreads();
         if (warp == 0) {
-          double total = 0.0;
-          for (int s = lane; s < row.sections; s += 32) total += section[s];
-          total            = warp_sum(total);
-          const Place found = locate(row, section, l.u * total, [&](float x, int c) { return rank_key(x, uint32_t(c)) >= floor ? weight(x) : 0.0; });
+          double total;
+          const Place found = locate(row, l.u, total, [&](int s) { return section[s]; },
+                                     [&](int) { return [&](float x, int c) { return rank_key(x, uint32_t(c)) >= floor ? weight(x) : 0.0; }; });
           if (lane == 0) S.column = found.column, S.total = total;
         }
         __syncthreads();
@@ -878,133 +879,130 @@ __device__ __noinline__ bool draw_wide(const Row<T>& row, const Limits& l, const
   return false;
 }
 
-template <class T, bool SPLIT>
-__global__ void __launch_bounds__(kThreads, 4) k_sample(const T* __restrict__ logits, const SampleArgs a, int n_parts)
-{
-  using P              = Pack16<T>;
-  constexpr int E      = P::kElems;
-  extern __shared__ double s_section[];  // a whole row's
-  __shared__ Scratch S;
-  const int parts = SPLIT ? n_parts : 1;
-  const int tid = threadIdx.x, threads = blockDim.x, warps = threads >> 5, warp = tid >> 5, lane = tid & 31;
-  const int64_t r = blockIdx.x / unsigned(parts);
-  const int part  = int(blockIdx.x % unsigned(parts));
-  const Row<T> row(logits + r * a.stride, a.vocab);
-  const int share = (row.sections + parts - 1) / parts;
-  const int begin = min(row.sections, part * share), end = min(row.sections, begin + share);
-  const Team<SPLIT> team{parts, part, share, begin, end};
-  uint4 raw[kPacks];
-  if (begin + warp < end) row.load_section(begin + warp, raw);  // while the limits come in
-  const Limits l(a, r);
-  auto put = [&](int id, float logprob) {
-    if (tid != 0 || part != 0) return;
-    a.ids[r] = id;
-    if (a.logprob) a.logprob[r] = logprob;
-  };
-  if (l.u < 0.0) return put(-1, 0.f);
-  if (l.broken()) return put(-1, __int_as_float(0x7FC00000));
-  for (int i = tid; i < kBins; i += threads) S.hist[i] = 0;
-  if (tid == 0) S.keys = 0;
-
-  // ---- the row, once
-  const double k64  = 1.4426950408889634 * l.inverse;
-  const bool ranged = k64 > 0x1p-20 && k64 < 0x1p20;
-  const float k     = ranged ? float(k64) : 1.f;
-  float2* const piece = reinterpret_cast<float2*>(s_section);
-  typename P::Max best[kPacks];
+// The highest of a thread's sets: the columns of the packs that are q-th in the sections that it has read.
+template <class T>
+struct Best {
+  using P = Pack16<T>;
+  typename P::Max of_set[kPacks];
+  __device__ __forceinline__ Best()
+  {
 #pragma unroll
-  for (int q = 0; q < kPacks; ++q) best[q] = P::lowest();
-  float top = -INFINITY, ref = kLow;
-  auto take = [&](int s, const uint4 (&raw)[kPacks]) {
-    typename P::Max most = P::highest(raw[0]);
-    best[0]              = P::higher(best[0], most);
-#pragma unroll
-    for (int q = 1; q < kPacks; ++q) {
-      const typename P::Max m = P::highest(raw[q]);
-      best[q] = P::higher(best[q], m);
-      most                    = P::higher(most, m);
-    }
-    const float high = warp_max(P::kHalves == 2 ? fmaxf(P::of(most, 0), P::of(most, 1)) : P::of(most, 0));
-    top = fmaxf(top, high), ref = fmaxf(ref, high);
-    const float c = ref * k;
-    const Two k2(k, k), c2(-c, -c);
-    Two sum[kPacks];
-#pragma unroll
-    for (int q = 0; q < kPacks; ++q) {
-      Two x[E / 2];
-      P::pairs(raw[q], x);
-#pragma unroll
-      for (int j = 0; j < E / 2; ++j) {
-        float y0, y1;
-        gtk::fma2(x[j], k2, c2).get(y0, y1);
-        x[j] = Two(pow2(y0), pow2(y1));
-      }
-#pragma unroll
-      for (int d = 1; d < E / 2; d *= 2)
-#pragma unroll
-        for (int j = 0; j < E / 2; j += 2 * d) x[j] = x[j] + x[j + d];
-      sum[q] = x[0];
-    }
-#pragma unroll
-    for (int d = 1; d < kPacks; d *= 2)
-#pragma unroll
-      for (int q = 0; q < kPacks; q += 2 * d) sum[q] = sum[q] + sum[q + d];
-    float lo, hi;
-    sum[0].get(lo, hi);
-    lo = warp_sum(lo + hi);
-    if (lane == 0 && GTK_IN(s, row.sections, 503)) piece[s] = make_float2(c, lo);
-  };
-  for (int s = begin + warp; s < end; s += 2 * warps) {
-    uint4 next[kPacks];
-    if (s + warps < end) row.load_section(s + warps, next);
-    take(s, raw);
-    if (s + warps >= end) break;
-    if (s + 2 * warps < end) row.load_section(s + 2 * warps, raw);
-    take(s + warps, next);
+    for (int q = 0; q < kPacks; ++q) of_set[q] = P::lowest();
   }
+  __device__ __forceinline__ float value(int q) const
+  {
+    return P::kHalves == 2 ? fmaxf(P::of(of_set[q], 0), P::of(of_set[q], 1)) : P::of(of_set[q], 0);
+  }
+};
+
+__device__ __forceinline__ double of_section(const float2& v, float c_top)  // its sum, relative to 2^c_top
+{
+  const int e = int(fmaxf(v.x - c_top, -1000.f));
+  return e > -1000 ? double(v.y) * __hiloint2double((e + 1023) << 20, 0) : 0.0;
+}
+
+// The row's highest logit, from the warps' own.
+template <bool SPLIT>
+__device__ __forceinline__ float highest(const Team<SPLIT>& team, Scratch& S, float top)
+{
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  if (lane == 0) S.top[warp] = top;
+  __syncthreads();
+  top = warp_max(lane < warps ? S.top[lane] : -INFINITY);
+  if constexpr (SPLIT) {
+    if (threadIdx.x == 0) S.part_top = top;
+    team.sync();
+    top = warp_max(lane < team.parts ? team.of(&S, lane)->part_top : -INFINITY);  // lane c asks part c, here and below
+  }
+  return top;
+}
+
+// Whether 32 bits hold a row's numbers and their sum, which is positive and finite then.
+__device__ __forceinline__ bool fits(bool ranged, float top, float c_top, double sum)
+{
+  return ranged && fabsf(top) < 0x1p59f && fabsf(c_top) < 0x1p20f && sum > 0.0 && sum < 1e30;
+}
+
+// A row without limits: the answer is its first warp's.
+template <class T, bool SPLIT>
+__device__ __noinline__ int draw_of_all(const Row<T>& row, const Limits& l, const Team<SPLIT>& team, float top, float k, bool ranged, double* section,
+                                        Scratch& S, float& logprob)
+{
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  top                = highest(team, S, top);
+  const float c_top  = ceilf(fmaxf(top, kLow) * k);
+  float2* const piece = reinterpret_cast<float2*>(section);
+  if constexpr (SPLIT) {
+    if (team.part == 0)  // the others' sections behind its own
+      for (int s = team.end + int(threadIdx.x); s < row.sections; s += blockDim.x) piece[s] = team.of(piece, s / team.share)[s];
+    team.sync();  // nobody leaves while its shared memory is read
+    if (team.part != 0) return -1;
+  }
+  int id = -1;
+  if (warp == 0) {
+    double total;
+    const Place at = locate(row, l.u, total, [&](int s) { return of_section(piece[s], c_top); },
+                            [&](int s) {
+                              const float c     = piece[s].x;
+                              const double unit = of_section(make_float2(c, 1.f), c_top);
+                              return [=](float x, int) { return double(pow2(fmaf(x, k, -c))) * unit; };
+                            });
+    bool sure = fits(ranged, top, c_top, total) && at.column >= 0;
+    if (sure) {
+      // u sum - (the weights in front): an error of a weight in front counts 1 - u times, of one behind u times, and those of the
+      // sections' sums likewise, but for the column's own section, whose weights in front are added one by one
+      const double u     = l.u, target = u * total, by_exponent = row.exponent_error(total) * fmax(u, 1.0 - u),
+                   by_sum = (Row<T>::kWeightError + Row<T>::kSumError) * 2.0 * u * (1.0 - u);
+      const double off = 0x1p-24 * (total * (by_exponent + by_sum + 0.1) + (Row<T>::kWeightError + Row<T>::kSumError) * of_section(piece[at.section], c_top));
+      sure             = target - at.before >= off && at.upto - target >= off;
+      const double shift = double(top) * double(k) - double(c_top);  // the highest's exponent
+      logprob            = float((double(at.x) - double(top)) * l.inverse + 0.6931471805599453 * shift - log(total));
+      id                 = at.column;
+    }
+    if (lane == 0) S.sure = sure, S.solved = fits(ranged, top, c_top, total);
+  }
+  __syncthreads();
+  if (S.sure) return id;
+  __syncthreads();
+  return S.solved ? draw_exactly(row, l, top, section, S, logprob) : draw_slowly(row, l, section, S, logprob);
+}
+
+// A row with limits: the answer is its first thread's.
+template <class T, bool SPLIT>
+__device__ __noinline__ int draw_limited(const Row<T>& row, const Limits& l, const Team<SPLIT>& team, const Best<T>& best, float top, float k,
+                                         bool ranged, double* section, Scratch& S, float& logprob)
+{
+  constexpr int E = Row<T>::E;
+  const int tid = threadIdx.x, threads = blockDim.x, warps = threads >> 5, warp = tid >> 5, lane = tid & 31;
   float low = INFINITY;
 #pragma unroll
-  for (int q = 0; q < kPacks; ++q) {
-    const float v = P::kHalves == 2 ? fmaxf(P::of(best[q], 0), P::of(best[q], 1)) : P::of(best[q], 0);
-    if (v > -INFINITY) low = fminf(low, v);
-  }
+  for (int q = 0; q < kPacks; ++q)
+    if (best.value(q) > -INFINITY) low = fminf(low, best.value(q));
   low = warp_min(low);
-  if (lane == 0) S.top[warp] = top, S.low[warp] = low;
-  __syncthreads();
-  for (int w = 0; w < warps; ++w) top = fmaxf(top, S.top[w]), low = fminf(low, S.low[w]);
+  if (lane == 0) S.low[warp] = low;
+  for (int i = tid; i < kBins; i += threads) S.hist[i] = 0;
+  if (tid == 0) S.keys = 0;
+  top = highest(team, S, top);
+  low = warp_min(lane < warps ? S.low[lane] : INFINITY);
   if constexpr (SPLIT) {
-    cg::cluster_group cluster = cg::this_cluster();
-    if (tid == 0) S.part_top = top, S.part_low = low;
-    cluster.sync();
-    // lane c asks part c, here and below
-    if (lane < parts) {
-      const Scratch* other = cluster.map_shared_rank(&S, lane);
-      top = other->part_top, low = other->part_low;
-    }
-    top = warp_max(top), low = warp_min(low);
+    // the parts' lowest, by way of all their warps
+    for (int c = 0; c < team.parts; ++c) low = fminf(low, warp_min(lane < warps ? team.of(&S, c)->low[lane] : INFINITY));
   }
 
   // ---- the sum of all weights relative to the highest's, and how the sets' highest are distributed
-  const float c_top = fmaxf(top, kLow) * k;
+  const float c_top = ceilf(fmaxf(top, kLow) * k);
   const float scale = fminf(float(kBins) / (top - low), 0x1p100f);
+  const float2* const piece = reinterpret_cast<const float2*>(section);
   double sum = 0.0;
-  for (int s = begin + tid; s < end; s += threads) {
-    const float2 v   = piece[s];
-    const double w   = v.y * pow2(v.x - c_top);
-    s_section[s]     = w;
-    sum += w;
-  }
+  for (int s = team.begin + tid; s < team.end; s += threads) sum += of_section(piece[s], c_top);
   sum = warp_sum(sum);
   if (lane == 0) S.mass[warp] = sum;
-  const bool all = l.all();
-  if (!all) {
 #pragma unroll
-    for (int q = 0; q < kPacks; ++q) {
-      const float v = P::kHalves == 2 ? fmaxf(P::of(best[q], 0), P::of(best[q], 1)) : P::of(best[q], 0);
-      if (v > -INFINITY) {
-        const int at = int(fminf((top - v) * scale, float(kBins - 1)));
-        if (GTK_IN(at, kBins, 504)) atomicAdd(&S.hist[at], 1);
-      }
+  for (int q = 0; q < kPacks; ++q) {
+    const float v = best.value(q);
+    if (v > -INFINITY) {
+      const int at = int(fminf((top - v) * scale, float(kBins - 1)));
+      if (GTK_IN(at, kBins, 504)) atomicAdd(&S.hist[at], 1);
     }
   }
   __syncthreads();
@@ -1012,52 +1010,27 @@ __global__ void __launch_bounds__(kThreads, 4) k_sample(const T* __restrict__ lo
   for (int w = 0; w < warps; ++w) sum += S.mass[w];
   const int* hist = S.hist;
   if constexpr (SPLIT) {
-    cg::cluster_group cluster = cg::this_cluster();
     if (tid == 0) S.part_sum = sum;
-    cluster.sync();
-    sum = warp_sum(lane < parts ? cluster.map_shared_rank(&S, lane)->part_sum : 0.0);
-    if (all) {
-      if (part == 0)  // the others' sections behind its own
-        for (int s = end + tid; s < row.sections; s += threads) s_section[s] = cluster.map_shared_rank(s_section, s / share)[s];
-    } else {
-      for (int i = tid; i < kBins; i += threads) {
-        int n = 0;
-        for (int c = 0; c < parts; ++c) n += cluster.map_shared_rank(&S, c)->hist[i];
-        S.bins[i] = n;
-      }
-      hist = S.bins;
+    team.sync();
+    sum = warp_sum(lane < team.parts ? team.of(&S, lane)->part_sum : 0.0);
+    for (int i = tid; i < kBins; i += threads) {
+      int n = 0;
+      for (int c = 0; c < team.parts; ++c) n += team.of(&S, c)->hist[i];
+      S.bins[i] = n;
     }
+    hist = S.bins;
     __syncthreads();
   }
   // rows whose numbers 32 bits do not hold are looked at again, as are those without a distribution
-  bool fast          = ranged && fabsf(top) < 0x1p59f && fabsf(c_top) < 0x1p20f && sum > 0.0 && sum < 1e30;
+  if (!fits(ranged, top, c_top, sum)) {
+    team.sync();  // nobody leaves while its shared memory is read
+    return team.part == 0 ? draw_slowly(row, l, section, S, logprob) : -1;
+  }
   const double m     = top;
   const double shift = double(top) * double(k) - double(c_top);  // the highest's exponent
-  const double error = row.error(sum);
+  const double error = 0x1p-24 * double(row.exponent_error(sum) + Row<T>::kWeightError + Row<T>::kSumError + 0.1f);
 
-  if (all || !fast) {
-    if constexpr (SPLIT) {
-      cg::this_cluster().sync();  // nobody leaves while its shared memory is read
-      if (part != 0) return;
-    }
-    if (fast) {
-      if (warp == 0) {
-        const double target = l.u * sum;
-        const Place at      = locate(row, s_section, target, [&](float x, int) { return double(pow2(fmaf(x, k, -c_top))); });
-        if (lane == 0) {
-          S.sure   = target - at.before >= error * sum && at.upto - target >= error * sum;
-          S.column = at.column;
-        }
-      }
-      __syncthreads();
-      if (S.sure) return put(S.column, float((double(row.value(S.column)) - m) * l.inverse + 0.6931471805599453 * shift - log(sum)));
-    }
-    float logprob;
-    const int id = fast ? draw_exactly(row, l, m, s_section, S, logprob) : draw_slowly(row, l, s_section, S, logprob);
-    return put(id, logprob);
-  }
-
-  // ---- a limit: how far down the columns have to be known
+  // ---- how far down the columns have to be known
   const bool by_mass = l.cut_by_mass();
   sum *= exp2(-shift);
   int reach = kBins;
@@ -1094,13 +1067,13 @@ __global__ void __launch_bounds__(kThreads, 4) k_sample(const T* __restrict__ lo
     some = warp_sum(n) <= kMostKeys / 4;
   }
   if (some) {
-    auto reaches = [&](float x) { return everything || (top - x) * scale < bound; };
+    auto reaches        = [&](float x) { return everything || (top - x) * scale < bound; };
     uint32_t* const set = S.order + warp * kSetsOfWarp;
     static_assert(kWarps * kSetsOfWarp >= kMostKeys, "");
-    int sets            = 0;
+    int sets = 0;
 #pragma unroll
     for (int q = 0; q < kPacks; ++q) {
-      const float v       = P::kHalves == 2 ? fmaxf(P::of(best[q], 0), P::of(best[q], 1)) : P::of(best[q], 0);
+      const float v       = best.value(q);
       const bool mine     = v > -INFINITY && reaches(v);
       const uint32_t them = __ballot_sync(0xFFFFFFFFu, mine);
       const int at        = sets + __popc(them & ((1u << lane) - 1u));
@@ -1108,9 +1081,9 @@ __global__ void __launch_bounds__(kThreads, 4) k_sample(const T* __restrict__ lo
       sets += __popc(them);
     }
     __syncwarp();
-    const int sections = (end - begin - warp + warps - 1) / warps, packs = sets * max(0, sections);
+    const int sections = (team.end - team.begin - warp + warps - 1) / warps, packs = sets * max(0, sections);
     for (int i = lane; i < packs; i += 32) {
-      const int p     = (begin + warp + i / sets * warps) * 32 * kPacks + int(set[i % sets]);
+      const int p     = (team.begin + warp + i / sets * warps) * 32 * kPacks + int(set[i % sets]);
       const uint4 raw = row.load(p);
 #pragma unroll
       for (int j = 0; j < E; ++j) {
@@ -1124,15 +1097,13 @@ __global__ void __launch_bounds__(kThreads, 4) k_sample(const T* __restrict__ lo
   }
   const int n = gather_keys(team, S);
   if (!some || n > kMostKeys) {
-    float logprob = 0.f;
-    int id        = -1;
-    const bool solved = draw_wide(row, l, team, top, low, s_section, S, id, logprob);
+    int id            = -1;
+    const bool solved = draw_wide(row, l, team, top, low, section, S, id, logprob);
     team.sync();  // nobody leaves while its shared memory is read
-    if (part != 0) return;
-    if (!solved) id = draw_slowly(row, l, s_section, S, logprob);
-    return put(id, logprob);
+    if (team.part != 0) return -1;
+    return solved ? id : draw_slowly(row, l, section, S, logprob);
   }
-  if (part != 0) return;
+  if (team.part != 0) return -1;
 
   // ---- the columns that are known, ranked
   sort_keys(S, n);
@@ -1148,13 +1119,99 @@ __global__ void __launch_bounds__(kThreads, 4) k_sample(const T* __restrict__ lo
     }
     __syncthreads();
     if (S.sure) break;
-    whole = sum_exactly(row, l, m, s_section, S), off = 0.0;
+    whole = sum_exactly(row, l, m, section, S), off = 0.0;
   }
   const int left     = S.left;
   const double total = S.total;
   __syncthreads();
   const int id = draw_key(S, left, l.u * total);
-  put(id, l.t == 0.f || id < 0 ? 0.f : float((double(row.value(id)) - m) * l.inverse - log(total)));
+  logprob      = l.t == 0.f || id < 0 ? 0.f : float((double(row.value(id)) - m) * l.inverse - log(total));
+  return id;
+}
+
+template <class T, bool SPLIT>
+__global__ void __launch_bounds__(kThreads, 4) k_sample(const T* __restrict__ logits, const SampleArgs a, int n_parts)
+{
+  using P         = Pack16<T>;
+  constexpr int E = P::kElems;
+  extern __shared__ double s_section[];  // a whole row's
+  __shared__ Scratch S;
+  const int parts = SPLIT ? n_parts : 1;
+  const int tid = threadIdx.x, warps = blockDim.x >> 5, warp = tid >> 5, lane = tid & 31;
+  const int64_t r = blockIdx.x / unsigned(parts);
+  const int part  = int(blockIdx.x % unsigned(parts));
+  const Row<T> row(logits + r * a.stride, a.vocab);
+  const int share = (row.sections + parts - 1) / parts;
+  const int begin = min(row.sections, part * share), end = min(row.sections, begin + share);
+  uint4 raw[kPacks];
+  if (begin + warp < end) row.load_section(begin + warp, raw);  // while the limits come in
+  const Limits l(a, r);
+  auto put = [&](int id, float logprob) {
+    if (tid != 0 || part != 0) return;
+    a.ids[r] = id;
+    if (a.logprob) a.logprob[r] = logprob;
+  };
+  if (l.u < 0.0) return put(-1, 0.f);
+  if (l.broken()) return put(-1, __int_as_float(0x7FC00000));
+
+  // ---- the row, once: a warp's section is summed relative to 2^c, c a whole number, no less than any exponent so far
+  const double k64  = 1.4426950408889634 * l.inverse;
+  const bool ranged = k64 > 0x1p-20 && k64 < 0x1p20;
+  const float k     = ranged ? float(k64) : 1.f;
+  float2* const piece = reinterpret_cast<float2*>(s_section);
+  Best<T> best;
+  float top = -INFINITY, ref = kLow;
+  auto take = [&](int s, const uint4 (&raw)[kPacks]) {
+    typename P::Max most = P::highest(raw[0]);
+    best.of_set[0]       = P::higher(best.of_set[0], most);
+#pragma unroll
+    for (int q = 1; q < kPacks; ++q) {
+      const typename P::Max m = P::highest(raw[q]);
+      best.of_set[q]          = P::higher(best.of_set[q], m);
+      most                    = P::higher(most, m);
+    }
+    top = fmaxf(top, warp_max(P::kHalves == 2 ? fmaxf(P::of(most, 0), P::of(most, 1)) : P::of(most, 0)));
+    const float c = ceilf(fmaxf(ref, top) * k);
+    const Two k2(k, k), c2(-c, -c);
+    Two sum[kPacks];
+#pragma unroll
+    for (int q = 0; q < kPacks; ++q) {
+      Two x[E / 2];
+      P::pairs(raw[q], x);
+#pragma unroll
+      for (int j = 0; j < E / 2; ++j) {
+        float y0, y1;
+        gtk::fma2(x[j], k2, c2).get(y0, y1);
+        x[j] = Two(pow2(y0), pow2(y1));
+      }
+#pragma unroll
+      for (int d = 1; d < E / 2; d *= 2)
+#pragma unroll
+        for (int j = 0; j < E / 2; j += 2 * d) x[j] = x[j] + x[j + d];
+      sum[q] = x[0];
+    }
+#pragma unroll
+    for (int d = 1; d < kPacks; d *= 2)
+#pragma unroll
+      for (int q = 0; q < kPacks; q += 2 * d) sum[q] = sum[q] + sum[q + d];
+    float lo, hi;
+    sum[0].get(lo, hi);
+    lo = warp_sum(lo + hi);
+    if (lane == 0 && GTK_IN(s, row.sections, 503)) piece[s] = make_float2(c, lo);
+  };
+  for (int s = begin + warp; s < end; s += 2 * warps) {
+    uint4 next[kPacks];
+    if (s + warps < end) row.load_section(s + warps, next);
+    take(s, raw);
+    if (s + warps >= end) break;
+    if (s + 2 * warps < end) row.load_section(s + 2 * warps, raw);
+    take(s + warps, next);
+  }
+  const Team<SPLIT> team{parts, part, share, begin, end};
+  float logprob = 0.f;
+  const int id  = l.all() ? draw_of_all(row, l, team, top, k, ranged, s_section, S, logprob)
+                          : draw_limited(row, l, team, best, top, k, ranged, s_section, S, logprob);
+  put(id, logprob);
 }
 
 static_assert(sizeof(Scratch) + (GTK_MAX_SAMPLE_VOCAB / (32 * kPacks * 4) + 1) * sizeof(double) <= 48 << 10, "what a CTA has without asking");
