@@ -70,8 +70,8 @@ struct Limits {
 };
 
 // What the threads of a CTA tell each other, and the columns that are ranked.
-struct Scratch {
-  uint64_t key[kMostKeys];
+struct alignas(16) Scratch {
+  uint64_t key[kMostKeys], ranked[kThreads];
   union {
     double weight[kMostKeys];
     struct {
@@ -138,8 +138,9 @@ struct Row {
   // Bounds of what 32 bits cost, in parts of 2^-24 of the sum of all weights, when that is at least `sum` times the highest's.  A weight 2^y, y =
   // x k - c rounded once, with k rounded once: 2 ln 2 |y| such parts of itself, and 4 for the exponential (2^-22).  The weights' mean of
   // ln 2 |y| is their entropy less ln(sum), ln(vocab / sum) at most, and c, a whole number, adds less than one to |y|.  The sum of a section:
-  // ten additions (four or five of a thread's, five of the warp's), and nothing more where sections are added, in 64 bits.
-  static constexpr float kWeightError = 4.f, kSumError = 10.f;
+  // ten additions (four or five of a thread's, five of the warp's), and nothing more where sections are added, in 64 bits.  The section that a
+  // column lies in: its sum's and its weights' errors, and 16 roundings more of what lies in front of the column (near_column).
+  static constexpr float kWeightError = 4.f, kSumError = 10.f, kOwnError = 28.f;
   __device__ __forceinline__ float exponent_error(double sum) const
   {
     return 2.f * 0.6932f * (fmaxf(0.f, log2f(float(vocab) / float(sum))) + 1.1f);
@@ -463,108 +464,64 @@ __device__ void sort_down(N* a, int n)
     }
 }
 
-constexpr int kRanked = 192;  // up to so many keys are ranked by looking at each other
-
-// S.key[0 .. n), highest first.
-__device__ void sort_keys(Scratch& S, int n)
-{
-  if (n > kRanked) return sort_down(S.key, n);
-  constexpr int kEach = 2;
-  uint64_t key[kEach];
-  int place[kEach];
-#pragma unroll
-  for (int e = 0; e < kEach; ++e) {
-    const int i = e * blockDim.x + threadIdx.x;
-    key[e]      = i < n ? S.key[i] : 0;
-    place[e]    = 0;
-  }
-  for (int j = 0; j < n; ++j) {
-    const uint64_t other = S.key[j];
-#pragma unroll
-    for (int e = 0; e < kEach; ++e) place[e] += other > key[e];
-  }
-  __syncthreads();
-#pragma unroll
-  for (int e = 0; e < kEach; ++e)
-    if (key[e] && GTK_IN(place[e], kMostKeys, 502)) S.key[place[e]] = key[e];
-  __syncthreads();
-}
-
-// The columns among S.key[0 .. n) that are left, their number and their weights' sum; `whole`: the sum that top-p is a part of, off
-// by `error` at most, < 0 where it is the sum of the keys.  By one warp, weights in place; false where the error leaves it open.
-__device__ bool cut_keys(const Limits& l, double m, Scratch& S, int n, double whole, double error, int& left, double& total)
+// The ones of n ranked keys that are left, their number and their weights' sum; `whole`: the sum that top-p is a part of, off by `error` at
+// most, < 0 where it is the sum of the keys.  By one warp; false where the error leaves it open.
+__device__ __forceinline__ bool cut_keys(const Limits& l, double m, const uint64_t* key, const double* weight, int n, double whole, double error,
+                                         int& left, double& total)
 {
   const int lane = threadIdx.x & 31;
   n              = min(n, l.k);
   const int each = (n + 31) / 32, begin = min(n, lane * each), end = min(n, begin + each);
   double mine = 0.0;
-  for (int i = begin; i < end; ++i) mine += S.weight[i];
-  const double front = warp_upto(mine) - mine;
-  if (whole < 0.0) whole = __shfl_sync(0xFFFFFFFFu, front + mine, 31), error = 0.0;
-  const double reach   = fmax(0.0, double(l.p)) * whole;
-  const double least_y = l.least > 0.f ? log(double(l.least)) : -INFINITY;
-  int last     = INT_MAX;  // of those that top-p leaves
-  bool open    = false;
-  int allowed  = 0;
-  double upto  = front;
-  for (int i = begin; i < end; ++i) {
-    upto += S.weight[i];
-    if (l.cut_by_mass() && last == INT_MAX && upto >= reach - error) last = i, open = upto < reach + error;
-    allowed += (double(key_value(S.key[i])) - m) * l.inverse >= least_y;
+  for (int i = begin; i < end; ++i) mine += weight[i];
+  const double upto = warp_upto(mine), front = upto - mine;
+  if (whole < 0.0) whole = __shfl_sync(0xFFFFFFFFu, upto, 31), error = 0.0;
+  left      = n;
+  bool open = false;
+  if (l.cut_by_mass()) {
+    const double reach = fmax(0.0, double(l.p)) * whole;
+    int last           = INT_MAX;
+    double so_far      = front;
+    for (int i = begin; i < end && last == INT_MAX; ++i)
+      if ((so_far += weight[i]) >= reach - error) last = i, open = so_far < reach + error;
+    const int first = __reduce_min_sync(0xFFFFFFFFu, last);
+    open            = __any_sync(0xFFFFFFFFu, open && last == first);
+    if (first != INT_MAX) left = first + 1;
   }
-  const int first = __reduce_min_sync(0xFFFFFFFFu, last);
-  open            = __any_sync(0xFFFFFFFFu, open && last == first);
-  allowed         = __reduce_add_sync(0xFFFFFFFFu, allowed);
-  left            = max(1, min(min(n, allowed), first == INT_MAX ? n : first + 1));
-  if (open && left <= first) open = false;  // min-p cuts in front of it
-  upto = 0.0;
-  for (int i = begin; i < min(end, left); ++i) upto += S.weight[i];
-  total = warp_sum(upto);
+  if (l.least > 0.f) {
+    const double least_y = log(double(l.least));
+    int allowed          = 0;
+    for (int i = begin; i < end; ++i) allowed += (double(key_value(key[i])) - m) * l.inverse >= least_y;
+    allowed = max(1, __reduce_add_sync(0xFFFFFFFFu, allowed));
+    if (allowed < left) left = allowed, open = false;  // whatever top-p leaves open
+  }
+  double so_far = front;
+  for (int i = begin; i < min(end, left); ++i) so_far += weight[i];
+  total = __shfl_sync(0xFFFFFFFFu, so_far, (left - 1) / each);
   return !open;
 }
 
-// The one of S.key[0 .. n) that is drawn, by all threads, by its place in the order of columns.
-__device__ int draw_key(Scratch& S, int n, double target)
+// The rank of the key that is drawn: of n ranks in the order of columns those below `left` count.  By one warp.
+__device__ __forceinline__ int draw_key(const uint32_t* order, const double* weight, int n, int left, double target)
 {
-  const int tid = threadIdx.x, lane = tid & 31;
-  if (tid == 0) S.column = INT_MAX, S.left = -1;
-  __syncthreads();
-  if (n <= kRanked) {
-    for (int i = tid; i < n; i += blockDim.x) {
-      const uint32_t c = key_column(S.key[i]);
-      double upto      = 0.0;
-      for (int j = 0; j < n; ++j)
-        if (key_column(S.key[j]) <= c) upto += S.weight[j];
-      if (S.weight[i] > 0.0) {
-        if (upto > target) atomicMin(&S.column, int(c));
-        atomicMax(&S.left, int(c));  // where rounding leaves none
-      }
-    }
-    __syncthreads();
-    return S.column == INT_MAX ? S.left : S.column;
-  }
-  // ranks by column, the lowest column first: 20 bits of column, 10 of rank
-  for (int i = tid; i < n; i += blockDim.x) S.order[i] = ~(key_column(S.key[i]) << 10 | uint32_t(i));
-  __syncthreads();
-  sort_down(S.order, n);
-  if (tid < 32) {
-    const int each = (n + 31) / 32, begin = min(n, lane * each), end = min(n, begin + each);
-    double mine = 0.0;
-    for (int i = begin; i < end; ++i) mine += S.weight[~S.order[i] & (kMostKeys - 1)];
-    double upto = warp_upto(mine) - mine;
-    int found = INT_MAX, last = -1;
+  const int lane = threadIdx.x & 31, each = (n + 31) / 32, begin = min(n, lane * each), end = min(n, begin + each);
+  auto weight_at = [&](int i) { return int(order[i]) < left ? weight[order[i]] : 0.0; };
+  double mine    = 0.0;
+  for (int i = begin; i < end; ++i) mine += weight_at(i);
+  const double upto   = warp_upto(mine);
+  const uint32_t over = __ballot_sync(0xFFFFFFFFu, mine > 0.0 && upto > target), some = __ballot_sync(0xFFFFFFFFu, mine > 0.0);
+  const int from      = over ? __ffs(over) - 1 : 31 - __clz(some);  // the last one with any weight where rounding leaves none
+  int at              = 0;
+  if (lane == from) {
+    double so_far = upto - mine;
     for (int i = begin; i < end; ++i) {
-      const double w = S.weight[~S.order[i] & (kMostKeys - 1)];
-      upto += w;
-      if (w > 0.0) last = i;
-      if (w > 0.0 && upto > target && found == INT_MAX) found = i;
+      const double w = weight_at(i);
+      if (!(w > 0.0)) continue;
+      at = int(order[i]);
+      if ((so_far += w) > target) break;
     }
-    found = __reduce_min_sync(0xFFFFFFFFu, found);
-    last  = __reduce_max_sync(0xFFFFFFFFu, last);
-    if (lane == 0) S.column = int(~S.order[found == INT_MAX ? last : found] >> 10);
   }
-  __syncthreads();
-  return S.column;
+  return __shfl_sync(0xFFFFFFFFu, at, from);
 }
 
 // The CTAs that share a row, and this one's sections of it.
@@ -823,7 +780,7 @@ __device__ __noinline__ bool draw_wide(const Row<T>& row, const Limits& l, const
       int left = 0;
       if (n > 0) {
         __syncthreads();
-        sort_keys(S, n);
+        sort_down(S.key, n);
         for (int i = tid; i < n; i += threads) S.weight[i] = weight(key_value(S.key[i]));
         __syncthreads();
       }
@@ -901,6 +858,82 @@ __device__ __forceinline__ double of_section(const float2& v, float c_top)  // i
   return e > -1000 ? double(v.y) * __hiloint2double((e + 1023) << 20, 0) : 0.0;
 }
 
+// locate() with the sums of the first reading, relative to 2^c_top: sections in 64 bits, within its section in 32.
+template <class T>
+__device__ __forceinline__ Place near_column(const Row<T>& row, const float2* piece, float c_top, float k, double share, double& total, Scratch& S)
+{
+  constexpr uint32_t all = 0xFFFFFFFFu;
+  constexpr int E = Row<T>::E, kOwn = kPacks * E;
+  static_assert(kOwn <= 32 && kPacks == 4, "");
+  const int lane = threadIdx.x & 31, each = (row.sections + 31) / 32;
+  const int begin = min(lane * each, row.sections), end = min(begin + each, row.sections);
+  double mine = 0.0;
+  for (int i = begin; i < end; ++i) mine += of_section(piece[i], c_top);
+  const double upto = warp_upto(mine);
+  total             = __shfl_sync(all, upto, 31);
+  const double target = share * total;
+  uint32_t over = __ballot_sync(all, mine > 0.0 && upto > target);
+  if (over == 0) return Place{-1, -1, 0.0, 0.0, 0.f};  // rounding has left none
+  int from     = __ffs(over) - 1, s = -1;
+  double front = upto - mine;
+  if (lane == from)
+    for (s = begin; s + 1 < end; ++s) {
+      const double w = of_section(piece[s], c_top);
+      if (w > 0.0 && front + w > target) break;
+      front += w;
+    }
+  s     = __shfl_sync(all, s, from);
+  front = __shfl_sync(all, front, from);
+  // neighbouring packs to a lane
+  uint4 raw[kPacks];
+#pragma unroll
+  for (int q = 0; q < kPacks; ++q) raw[q] = row.load((s * 32 + lane) * kPacks + q);
+  const float c   = piece[s].x;
+  const int shift = int(c_top - c);  // the section has weight, so that is below 1000
+  const float rest = float((target - front) * __hiloint2double((1023 + shift) << 20, 0));
+  const Two k2(k, k), c2(-c, -c);
+  Two sum[kPacks];
+#pragma unroll
+  for (int q = 0; q < kPacks; ++q) {
+    Two x[E / 2];
+    Pack16<T>::pairs(raw[q], x);
+#pragma unroll
+    for (int j = 0; j < E / 2; ++j) {
+      float y0, y1;
+      gtk::fma2(x[j], k2, c2).get(y0, y1);
+      x[j] = Two(pow2(y0), pow2(y1));
+    }
+#pragma unroll
+    for (int d = 1; d < E / 2; d *= 2)
+#pragma unroll
+      for (int j = 0; j < E / 2; j += 2 * d) x[j] = x[j] + x[j + d];
+    sum[q] = x[0];
+  }
+  float lo, hi;
+  ((sum[0] + sum[1]) + (sum[2] + sum[3])).get(lo, hi);
+  float own         = lo + hi;
+  const float so_far = warp_upto(own);
+  over              = __ballot_sync(all, own > 0.f && so_far > rest);
+  if (over == 0) return Place{-1, s, 0.0, 0.0, 0.f};
+  from = __ffs(over) - 1;
+  // a column to a lane
+  uint4* const shared = reinterpret_cast<uint4*>(S.order);
+  if (lane == from)
+#pragma unroll
+    for (int q = 0; q < kPacks; ++q) shared[q] = raw[q];
+  __syncwarp();
+  const float x = lane < kOwn ? gtk::to_float(reinterpret_cast<const T*>(shared)[lane]) : -INFINITY;
+  own           = pow2(fmaf(x, k, -c));
+  const float in_front = __shfl_sync(all, so_far, max(from - 1, 0));
+  const float now      = (from > 0 ? in_front : 0.f) + warp_upto(own);
+  over                 = __ballot_sync(all, own > 0.f && now > rest);
+  if (over == 0) return Place{-1, s, 0.0, 0.0, 0.f};
+  const int at      = __ffs(over) - 1;
+  const double unit = __hiloint2double((1023 - shift) << 20, 0);
+  const float here  = __shfl_sync(all, now, at), before = here - __shfl_sync(all, own, at);
+  return Place{row.column((s * 32 + from) * kPacks) + at, s, front + double(before) * unit, front + double(here) * unit, __shfl_sync(all, x, at)};
+}
+
 // The row's highest logit, from the warps' own.
 template <bool SPLIT>
 __device__ __forceinline__ float highest(const Team<SPLIT>& team, Scratch& S, float top)
@@ -941,19 +974,15 @@ __device__ __noinline__ int draw_of_all(const Row<T>& row, const Limits& l, cons
   int id = -1;
   if (warp == 0) {
     double total;
-    const Place at = locate(row, l.u, total, [&](int s) { return of_section(piece[s], c_top); },
-                            [&](int s) {
-                              const float c     = piece[s].x;
-                              const double unit = of_section(make_float2(c, 1.f), c_top);
-                              return [=](float x, int) { return double(pow2(fmaf(x, k, -c))) * unit; };
-                            });
+    const Place at = near_column(row, piece, c_top, k, l.u, total, S);
     bool sure = fits(ranged, top, c_top, total) && at.column >= 0;
     if (sure) {
       // u sum - (the weights in front): an error of a weight in front counts 1 - u times, of one behind u times, and those of the
-      // sections' sums likewise, but for the column's own section, whose weights in front are added one by one
-      const double u     = l.u, target = u * total, by_exponent = row.exponent_error(total) * fmax(u, 1.0 - u),
-                   by_sum = (Row<T>::kWeightError + Row<T>::kSumError) * 2.0 * u * (1.0 - u);
-      const double off = 0x1p-24 * (total * (by_exponent + by_sum + 0.1) + (Row<T>::kWeightError + Row<T>::kSumError) * of_section(piece[at.section], c_top));
+      // sections' sums likewise, but for the column's own section
+      const double u = l.u, target = u * total;
+      const float shares = fmaxf(float(u), 1.f - float(u)), both = 2.f * float(u) * (1.f - float(u));
+      const float of_all = row.exponent_error(total) * shares + (Row<T>::kWeightError + Row<T>::kSumError) * both + 0.1f;
+      const double off   = 0x1p-24 * (total * of_all + Row<T>::kOwnError * of_section(piece[at.section], c_top));
       sure             = target - at.before >= off && at.upto - target >= off;
       const double shift = double(top) * double(k) - double(c_top);  // the highest's exponent
       logprob            = float((double(at.x) - double(top)) * l.inverse + 0.6931471805599453 * shift - log(total));
@@ -972,7 +1001,7 @@ template <class T, bool SPLIT>
 __device__ __noinline__ int draw_limited(const Row<T>& row, const Limits& l, const Team<SPLIT>& team, const Best<T>& best, float top, float k,
                                          bool ranged, double* section, Scratch& S, float& logprob)
 {
-  constexpr int E = Row<T>::E;
+  constexpr int E = Row<T>::E, kAgain = 2;  // packs that a thread reads again at a time
   const int tid = threadIdx.x, threads = blockDim.x, warps = threads >> 5, warp = tid >> 5, lane = tid & 31;
   float low = INFINITY;
 #pragma unroll
@@ -1027,32 +1056,33 @@ __device__ __noinline__ int draw_limited(const Row<T>& row, const Limits& l, con
     return team.part == 0 ? draw_slowly(row, l, section, S, logprob) : -1;
   }
   const double m     = top;
-  const double shift = double(top) * double(k) - double(c_top);  // the highest's exponent
-  const double error = 0x1p-24 * double(row.exponent_error(sum) + Row<T>::kWeightError + Row<T>::kSumError + 0.1f);
-
   // ---- how far down the columns have to be known
-  const bool by_mass = l.cut_by_mass();
-  sum *= exp2(-shift);
+  const bool by_mass = l.cut_by_mass(), of_all = by_mass && l.k == INT_MAX;  // top-p of all columns
+  double error = 0.0;
+  if (of_all) {
+    error = 0x1p-24 * double(row.exponent_error(sum) + Row<T>::kWeightError + Row<T>::kSumError + 0.1f);
+    sum *= exp2(double(c_top) - double(top) * double(k));  // relative to the highest's
+  }
   int reach = kBins;
   {
     constexpr int kEach = kBins / 32;
-    const float width   = 1.f / scale;
     int counts[kEach], count = 0;
-    float masses[kEach], mass = 0.f;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      const int b = lane * kEach + i;
-      counts[i]   = hist[b];
-      masses[i]   = counts[i] ? float(counts[i]) * pow2(-float(b + 1) * width * k) * 0.999f : 0.f;  // no less than that
-      count += counts[i], mass += masses[i];
-    }
-    int count_upto  = warp_upto(count) - count;
-    float mass_upto = warp_upto(mass) - mass;
-    const float wanted = by_mass && l.k == INT_MAX ? fmaxf(l.p, 0.f) * float(sum) * 1.0001f : INFINITY;
+    for (int i = 0; i < kEach; ++i) count += counts[i] = hist[lane * kEach + i];
+    int count_upto = warp_upto(count) - count;
+    if (of_all) {
+      const float width = k / scale, wanted = fmaxf(l.p, 0.f) * float(sum) * 1.0001f;
+      float masses[kEach], mass = 0.f;
 #pragma unroll
-    for (int i = 0; i < kEach; ++i) {
-      count_upto += counts[i], mass_upto += masses[i];
-      if (reach == kBins && counts[i] && (count_upto >= l.k || mass_upto >= wanted)) reach = lane * kEach + i;
+      for (int i = 0; i < kEach; ++i) mass += masses[i] = counts[i] ? float(counts[i]) * pow2(-float(lane * kEach + i + 1) * width) * 0.999f : 0.f;
+      float mass_upto = warp_upto(mass) - mass;  // no less than that lies above
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        if ((mass_upto += masses[i]) >= wanted && reach == kBins && counts[i]) reach = lane * kEach + i;
+    } else {
+#pragma unroll
+      for (int i = 0; i < kEach; ++i)
+        if ((count_upto += counts[i]) >= l.k && reach == kBins && counts[i]) reach = lane * kEach + i;
     }
     reach = __reduce_min_sync(0xFFFFFFFFu, reach);
     if (l.least > 0.f && (l.k == INT_MAX || !by_mass))
@@ -1082,17 +1112,39 @@ __device__ __noinline__ int draw_limited(const Row<T>& row, const Limits& l, con
     }
     __syncwarp();
     const int sections = (team.end - team.begin - warp + warps - 1) / warps, packs = sets * max(0, sections);
-    for (int i = lane; i < packs; i += 32) {
-      const int p     = (team.begin + warp + i / sets * warps) * 32 * kPacks + int(set[i % sets]);
-      const uint4 raw = row.load(p);
+    const float per_set = 1.f / float(max(sets, 1));
+    for (int i0 = 0; i0 < packs; i0 += 32 * kAgain) {
+      uint4 raw[kAgain];
+      int column[kAgain];
+      uint32_t hits = 0;
 #pragma unroll
-      for (int j = 0; j < E; ++j) {
-        const float x = gtk::to_float(reinterpret_cast<const T*>(&raw)[j]);
-        if (x > -INFINITY && reaches(x)) {
-          const int at = atomicAdd(&S.keys, 1);
-          if (at < kMostKeys && GTK_IN(at, kMostKeys, 506)) S.key[at] = rank_key(x, uint32_t(row.column(p) + j));
-        }
+      for (int e = 0; e < kAgain; ++e) {
+        const int i = i0 + e * 32 + lane, s = int((float(i) + 0.5f) * per_set);  // i / sets
+        const int p = i < packs ? (team.begin + warp + s * warps) * 32 * kPacks + int(set[i - s * sets]) : row.packs;
+        column[e]   = row.column(p);
+        raw[e]      = row.load(p);
       }
+#pragma unroll
+      for (int e = 0; e < kAgain; ++e)
+#pragma unroll
+        for (int j = 0; j < E; ++j) {
+          const float x = gtk::to_float(reinterpret_cast<const T*>(&raw[e])[j]);
+          hits |= (x > -INFINITY && reaches(x) ? 1u : 0u) << (e * E + j);
+        }
+      const int mine = __popc(hits), upto = warp_upto(mine);
+      int at = 0;
+      if (lane == 31 && upto > 0) at = atomicAdd(&S.keys, upto);
+      at = __shfl_sync(0xFFFFFFFFu, at, 31) + upto - mine;
+      if (hits == 0) continue;
+#pragma unroll
+      for (int e = 0; e < kAgain; ++e)
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          if (hits >> (e * E + j) & 1u) {
+            if (at < kMostKeys && GTK_IN(at, kMostKeys, 506))
+              S.key[at] = rank_key(gtk::to_float(reinterpret_cast<const T*>(&raw[e])[j]), uint32_t(column[e] + j));
+            ++at;
+          }
     }
   }
   const int n = gather_keys(team, S);
@@ -1106,27 +1158,61 @@ __device__ __noinline__ int draw_limited(const Row<T>& row, const Limits& l, con
   if (team.part != 0) return -1;
 
   // ---- the columns that are known, ranked
-  sort_keys(S, n);
-  for (int i = tid; i < n; i += threads) S.weight[i] = exp((double(key_value(S.key[i])) - m) * l.inverse);
+  const bool few = n <= threads;
+  if (few) {
+    if (tid < n) {
+      const uint64_t key = S.key[tid];
+      const double w     = exp((double(key_value(key)) - m) * l.inverse);
+      int rank = 0, place = 0;
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) {
+        const uint64_t other = S.key[j];
+        rank += other > key;
+        place += uint32_t(other) > uint32_t(key);  // a lower column
+      }
+      if (GTK_IN(rank, kThreads, 511) && GTK_IN(place, kThreads, 512)) S.ranked[rank] = key, S.weight[rank] = w, S.order[place] = rank;
+    }
+  } else {
+    sort_down(S.key, n);
+    for (int i = tid; i < n; i += threads) S.weight[i] = exp((double(key_value(S.key[i])) - m) * l.inverse);
+  }
   __syncthreads();
-  double whole = everything || l.k != INT_MAX ? -1.0 : sum, off = error * sum;
+  const uint64_t* ranked = few ? S.ranked : S.key;
+  double whole = of_all && !everything ? sum : -1.0, off = error * sum;
   for (int round = 0; round < 2; ++round) {
     if (warp == 0) {
       int left;
       double total;
-      const bool sure = cut_keys(l, m, S, n, whole, off, left, total);
+      const bool sure = cut_keys(l, m, ranked, S.weight, n, whole, off, left, total);
       if (lane == 0) S.sure = sure, S.left = left, S.total = total;
+      if (few && sure) {
+        const int at = draw_key(S.order, S.weight, n, left, l.u * total);
+        if (lane == 0) S.column = at;
+      }
     }
     __syncthreads();
     if (S.sure) break;
+    __syncthreads();
     whole = sum_exactly(row, l, m, section, S), off = 0.0;
   }
-  const int left     = S.left;
-  const double total = S.total;
-  __syncthreads();
-  const int id = draw_key(S, left, l.u * total);
-  logprob      = l.t == 0.f || id < 0 ? 0.f : float((double(row.value(id)) - m) * l.inverse - log(total));
-  return id;
+  if (!few) {
+    // 20 bits of column, 10 of rank; the lowest column first
+    const int left = S.left;
+    for (int i = tid; i < left; i += threads) S.order[i] = ~(key_column(S.key[i]) << 10 | uint32_t(i));
+    __syncthreads();
+    sort_down(S.order, left);
+    for (int i = tid; i < left; i += threads) S.order[i] = ~S.order[i] & (kMostKeys - 1);
+    __syncthreads();
+    if (warp == 0) {
+      const int at = draw_key(S.order, S.weight, left, left, l.u * S.total);
+      if (lane == 0) S.column = at;
+    }
+    __syncthreads();
+  }
+  if (tid != 0) return -1;
+  const uint64_t drawn = ranked[S.column];
+  logprob              = l.t == 0.f ? 0.f : float((double(key_value(drawn)) - m) * l.inverse - log(S.total));
+  return int(key_column(drawn));
 }
 
 template <class T, bool SPLIT>
