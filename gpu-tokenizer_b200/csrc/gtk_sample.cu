@@ -31,7 +31,7 @@ constexpr int kMaxParts = 8;     // CTAs that share a row
 constexpr int kPacks    = 4;     // of 16 bytes that a thread has of a section: 32 * kPacks neighbouring packs, whose sum is kept
 constexpr int kBins     = 256;
 constexpr int kFine     = 1024;  // bins of a wide row
-constexpr int kMostKeys = 1024;  // columns that are ranked at most
+constexpr int kMostKeys = 512;   // columns that are ranked at most
 constexpr int kSetsOfWarp = 32 * kPacks;  // of its columns that a warp knows the highest of, at most
 constexpr float kLow    = -0x1p60f;
 
@@ -69,27 +69,45 @@ struct Limits {
   __device__ bool all() const { return k == INT_MAX && !cut_by_mass() && !(least > 0.f); }
 };
 
-// What the threads of a CTA tell each other, and the columns that are ranked.
+// What the threads of a CTA tell each other, and the columns that are ranked.  Small, for what shared memory takes the loads under way do
+// not have: 25 KiB a CTA cost 2048 rows of 50257 f32 a fifth.
 struct alignas(16) Scratch {
-  uint64_t key[kMostKeys], ranked[kThreads];
   union {
-    double weight[kMostKeys];
+    struct {
+      uint64_t key[kMostKeys];
+      double weight[kMostKeys];
+    };
     struct {
       uint32_t fine[kFine], fine_all[kFine];  // of this CTA, of all that share the row
     };
   };
-  uint32_t order[kWarps * kSetsOfWarp];  // sets, by warps; then places of keys
-  double power[64];           // 2^(i / 64)
+  union {
+    uint64_t ranked[kThreads];
+    uint32_t by_column[kMostKeys];
+  };
+  union {
+    uint8_t set[kWarps * kSetsOfWarp];
+    uint16_t order[kMostKeys];
+  };
+  double power[64];  // 2^(i / 64)
   double mass[kWarps], part_mass[2];
   int count[kWarps];
   float top[kWarps], low[kWarps];
   int hist[kBins], bins[kBins];  // of this CTA, of all that share the row
-  double at, total, part_sum;
+  double total, part_sum;
   uint64_t floor;
   int column, keys, left, part_count, solved;
   bool sure;
   float part_top;
 };
+
+// Past the first-level cache, in which the loads under way would otherwise take their places (2048 rows of 50257 f32 77 -> 68 us).
+__device__ __forceinline__ uint4 load_past(const uint4* p)
+{
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
 
 // A row as the packs of 16 bytes that it touches; what lies in them outside of it counts as -inf.
 template <class T>
@@ -129,7 +147,7 @@ struct Row {
     const int p0 = s * 32 * kPacks + int(threadIdx.x & 31);
     if (whole(s)) {
 #pragma unroll
-      for (int q = 0; q < kPacks; ++q) raw[q] = __ldg(base + p0 + q * 32);
+      for (int q = 0; q < kPacks; ++q) raw[q] = load_past(base + p0 + q * 32);
     } else {
 #pragma unroll
       for (int q = 0; q < kPacks; ++q) raw[q] = load(p0 + q * 32);
@@ -502,7 +520,7 @@ __device__ __forceinline__ bool cut_keys(const Limits& l, double m, const uint64
 }
 
 // The rank of the key that is drawn: of n ranks in the order of columns those below `left` count.  By one warp.
-__device__ __forceinline__ int draw_key(const uint32_t* order, const double* weight, int n, int left, double target)
+__device__ __forceinline__ int draw_key(const uint16_t* order, const double* weight, int n, int left, double target)
 {
   const int lane = threadIdx.x & 31, each = (n + 31) / 32, begin = min(n, lane * each), end = min(n, begin + each);
   auto weight_at = [&](int i) { return int(order[i]) < left ? weight[order[i]] : 0.0; };
@@ -917,7 +935,7 @@ __device__ __forceinline__ Place near_column(const Row<T>& row, const float2* pi
   if (over == 0) return Place{-1, s, 0.0, 0.0, 0.f};
   from = __ffs(over) - 1;
   // a column to a lane
-  uint4* const shared = reinterpret_cast<uint4*>(S.order);
+  uint4* const shared = reinterpret_cast<uint4*>(S.key);
   if (lane == from)
 #pragma unroll
     for (int q = 0; q < kPacks; ++q) shared[q] = raw[q];
@@ -1098,8 +1116,8 @@ __device__ __noinline__ int draw_limited(const Row<T>& row, const Limits& l, con
   }
   if (some) {
     auto reaches        = [&](float x) { return everything || (top - x) * scale < bound; };
-    uint32_t* const set = S.order + warp * kSetsOfWarp;
-    static_assert(kWarps * kSetsOfWarp >= kMostKeys, "");
+    uint8_t* const set  = S.set + warp * kSetsOfWarp;
+    static_assert(kSetsOfWarp <= 256, "");
     int sets = 0;
 #pragma unroll
     for (int q = 0; q < kPacks; ++q) {
@@ -1107,7 +1125,7 @@ __device__ __noinline__ int draw_limited(const Row<T>& row, const Limits& l, con
       const bool mine     = v > -INFINITY && reaches(v);
       const uint32_t them = __ballot_sync(0xFFFFFFFFu, mine);
       const int at        = sets + __popc(them & ((1u << lane) - 1u));
-      if (mine && GTK_IN(at, kSetsOfWarp, 505)) set[at] = q * 32 + lane;
+      if (mine && GTK_IN(at, kSetsOfWarp, 505)) set[at] = uint8_t(q * 32 + lane);
       sets += __popc(them);
     }
     __syncwarp();
@@ -1170,7 +1188,7 @@ __device__ __noinline__ int draw_limited(const Row<T>& row, const Limits& l, con
         rank += other > key;
         place += uint32_t(other) > uint32_t(key);  // a lower column
       }
-      if (GTK_IN(rank, kThreads, 511) && GTK_IN(place, kThreads, 512)) S.ranked[rank] = key, S.weight[rank] = w, S.order[place] = rank;
+      if (GTK_IN(rank, kThreads, 511) && GTK_IN(place, kThreads, 512)) S.ranked[rank] = key, S.weight[rank] = w, S.order[place] = uint16_t(rank);
     }
   } else {
     sort_down(S.key, n);
@@ -1196,12 +1214,13 @@ __device__ __noinline__ int draw_limited(const Row<T>& row, const Limits& l, con
     whole = sum_exactly(row, l, m, section, S), off = 0.0;
   }
   if (!few) {
-    // 20 bits of column, 10 of rank; the lowest column first
+    // 20 bits of column, 9 of rank; the lowest column first
     const int left = S.left;
-    for (int i = tid; i < left; i += threads) S.order[i] = ~(key_column(S.key[i]) << 10 | uint32_t(i));
+    for (int i = tid; i < left; i += threads) S.by_column[i] = ~(key_column(S.key[i]) << 9 | uint32_t(i));
     __syncthreads();
-    sort_down(S.order, left);
-    for (int i = tid; i < left; i += threads) S.order[i] = ~S.order[i] & (kMostKeys - 1);
+    static_assert(kMostKeys == 1 << 9 && GTK_MAX_SAMPLE_VOCAB == 1 << 20, "");
+    sort_down(S.by_column, left);
+    for (int i = tid; i < left; i += threads) S.order[i] = uint16_t(~S.by_column[i] & (kMostKeys - 1));
     __syncthreads();
     if (warp == 0) {
       const int at = draw_key(S.order, S.weight, left, left, l.u * S.total);
