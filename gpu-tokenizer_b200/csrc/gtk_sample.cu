@@ -90,13 +90,14 @@ struct alignas(16) Scratch {
     uint16_t order[kMostKeys];
   };
   double power[64];  // 2^(i / 64)
-  double mass[kWarps], part_mass[2];
+  double mass[kWarps];
   int count[kWarps];
   float top[kWarps], low[kWarps];
   int hist[kBins], bins[kBins];  // of this CTA, of all that share the row
   double total, part_sum;
   uint64_t floor;
-  int column, keys, left, part_count, solved;
+  int column, keys, left, part_count, solved, first, last;
+  float run[kFine / 128];
   bool sure;
   float part_top;
 };
@@ -197,25 +198,24 @@ __device__ __forceinline__ N warp_upto(N x)  // the sum of the lanes up to the o
 }
 
 // exp((x - m) / T) in 64 bits: with y = (x - m) log2(e) / T = n / 64 + f the product of 2^(n / 64), by a table of 64 entries, and
-// exp(f ln 2), |f ln 2| < 0.0055, whose series is cut behind the fifth power (3e-17).  About a quarter of the time of exp().
+// 2^f, |f| <= 1 / 128, whose series is cut behind the fifth power (3e-17).  No branch, so that several are under way at once; 2^e in two
+// factors, for the subnormal ones.
 struct Weight64 {
   double m, k;  // k: log2(e) / T
   const double* power;
   __device__ __forceinline__ double operator()(float x) const
   {
-    const double y = fmax((double(x) - m) * k, -2000.0);
+    constexpr double l2 = 0.69314718055994531;
+    const double y = fmax((double(x) - m) * k, -1990.0);
     const double a = fma(y, 64.0, 0x1.8p52);  // n in the low bits
-    const int n    = __double2loint(a);
-    const double z = fma(a - 0x1.8p52, -1.0 / 64, y) * 0.69314718055994531;
-    double s       = fma(z, 1.0 / 120, 1.0 / 24);
-    s              = fma(z, s, 1.0 / 6);
-    s              = fma(z, s, 0.5);
-    s              = fma(z, s, 1.0);
-    s              = fma(z, s, 1.0);
-    const double w = power[n & 63] * s;
-    const int e    = n >> 6;
-    if (e < -1000) return ldexp(w, e);
-    return w * __hiloint2double((e + 1023) << 20, 0);
+    const int n    = __double2loint(a), e = n >> 6, most = max(e, -1000);
+    const double f = fma(a - 0x1.8p52, -1.0 / 64, y);
+    double s       = fma(f, l2 * l2 * l2 * l2 * l2 / 120, l2 * l2 * l2 * l2 / 24);
+    s              = fma(f, s, l2 * l2 * l2 / 6);
+    s              = fma(f, s, l2 * l2 / 2);
+    s              = fma(f, s, l2);
+    s              = fma(f, s, 1.0);
+    return power[n & 63] * s * __hiloint2double((most + 1023) << 20, 0) * __hiloint2double((e - most + 1023) << 20, 0);
   }
 };
 
@@ -238,24 +238,21 @@ __device__ __forceinline__ Sum sum_row(const Row<T>& row, double* section, Scrat
 {
   const int threads = blockDim.x, warps = threads >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   Sum s{0.0, 0};
-  constexpr int kAtOnce = 16 / Row<T>::E;  // packs
-  static_assert(kPacks % kAtOnce == 0, "");
   __syncthreads();
   for (int i = warp; i < row.sections; i += warps) {
     double sum = 0.0;
 #pragma unroll 1
-    for (int q = 0; q < kPacks; q += kAtOnce) {
-      uint4 raw[kAtOnce];
+    for (int q = 0; q < kPacks; ++q) {
+      const int p     = (i * kPacks + q) * 32 + lane;
+      const uint4 raw = row.load(p);
+      Sum o[Row<T>::E];
 #pragma unroll
-      for (int b = 0; b < kAtOnce; ++b) raw[b] = row.load((i * kPacks + q + b) * 32 + lane);
+      for (int j = 0; j < Row<T>::E; ++j) o[j] = weigh(gtk::to_float(reinterpret_cast<const T*>(&raw)[j]), row.column(p) + j);
 #pragma unroll
-      for (int b = 0; b < kAtOnce; ++b) {
+      for (int d = 1; d < Row<T>::E; d *= 2)
 #pragma unroll
-        for (int j = 0; j < Row<T>::E; ++j) {
-          const Sum o = weigh(gtk::to_float(reinterpret_cast<const T*>(&raw[b])[j]), row.column((i * kPacks + q + b) * 32 + lane) + j);
-          sum += o.mass, s.count += o.count;
-        }
-      }
+        for (int j = 0; j < Row<T>::E; j += 2 * d) o[j].mass += o[j + d].mass, o[j].count += o[j + d].count;
+      sum += o[0].mass, s.count += o[0].count;
     }
     sum = warp_sum(sum);
     if (lane == 0 && GTK_IN(i, row.sections, 500)) section[i] = sum;
@@ -312,19 +309,20 @@ __device__ __forceinline__ Place locate(const Row<T>& row, double share, double&
   front = __shfl_sync(all, front, from);
   // neighbouring packs to a lane
   auto weight = weigh(s);
-  uint4 raw[kPacks];
-#pragma unroll
-  for (int q = 0; q < kPacks; ++q) raw[q] = row.load((s * 32 + lane) * kPacks + q);
-  double sums[kPacks];
-#pragma unroll
+  mine        = 0.0;
+#pragma unroll 1
   for (int q = 0; q < kPacks; ++q) {
-    const int c = row.column((s * 32 + lane) * kPacks + q);
-    sums[q]     = 0.0;
+    const int p     = (s * 32 + lane) * kPacks + q, c = row.column(p);
+    const uint4 raw = row.load(p);
+    double w[Row<T>::E];
 #pragma unroll
-    for (int j = 0; j < Row<T>::E; ++j) sums[q] += weight(gtk::to_float(reinterpret_cast<const T*>(&raw[q])[j]), c + j);
+    for (int j = 0; j < Row<T>::E; ++j) w[j] = weight(gtk::to_float(reinterpret_cast<const T*>(&raw)[j]), c + j);
+#pragma unroll
+    for (int d = 1; d < Row<T>::E; d *= 2)
+#pragma unroll
+      for (int j = 0; j < Row<T>::E; j += 2 * d) w[j] += w[j + d];
+    mine += w[0];
   }
-  mine = (sums[0] + sums[1]) + (sums[2] + sums[3]);
-  static_assert(kPacks == 4, "");
   upto = front + warp_upto(mine);
   from = lane_of(mine, upto, target);
   if (from < 0) return Place{-1, s, 0.0, 0.0, 0.f};
@@ -351,7 +349,7 @@ struct Slowly {
   Weight64 power;
   double total;  // of the last find
 
-  __device__ double weight(float x) const { return x > -INFINITY ? power(x) : 0.0; }
+  __device__ double weight(float x) const { return power(x); }
   __device__ bool left(float x, int c) const { return rank_key(x, uint32_t(c)) >= floor; }
 
   // the first column at which `weigh` exceeds a share of its sum, known to all threads
@@ -445,7 +443,7 @@ template <class T>
 __device__ __noinline__ double sum_exactly(const Row<T>& row, const Limits& l, double m, double* section, Scratch& S)
 {
   const Weight64 weight = weight64(l, m, S);
-  return sum_row(row, section, S, [&](float x, int) { return Sum{x > -INFINITY ? weight(x) : 0.0, 0}; }).mass;
+  return sum_row(row, section, S, [&](float x, int) { return Sum{weight(x), 0}; }).mass;
 }
 
 // What is drawn of all columns, with everything in 64 bits.
@@ -457,7 +455,7 @@ __device__ __noinline__ int draw_exactly(const Row<T>& row, const Limits& l, dou
   if (threadIdx.x >= 32) return -1;
   double total;
   const Place found = locate(row, l.u, total, [&](int s) { return section[s]; },
-                             [&](int) { return [&](float x, int) { return x > -INFINITY ? weight(x) : 0.0; }; });
+                             [&](int) { return [&](float x, int) { return weight(x); }; });
   logprob           = float((double(found.x) - m) * l.inverse - log(total));
   return found.column;
 }
@@ -558,16 +556,33 @@ struct Team {
     if constexpr (SPLIT) return cg::this_cluster().map_shared_rank(mine, c);
     else return mine;
   }
-  // f(s, packs) for the warps' sections, packs as they lie
+  // f(s, each_pack) for the warps' sections, where each_pack(g) calls g(p, pack) for the thread's packs of it
   template <class T, class F>
-  __device__ __forceinline__ void each_section(const Row<T>& row, F&& f) const
+  __device__ __forceinline__ void each_section_packs(const Row<T>& row, F&& f) const
   {
     const int warps = blockDim.x >> 5;
-    for (int s = begin + (threadIdx.x >> 5); s < end; s += warps) {
+    uint4 next[kPacks];
+    int s = begin + int(threadIdx.x >> 5);
+    if (s < end) row.load_section(s, next);
+    for (; s < end; s += warps) {
       uint4 raw[kPacks];
-      row.load_section(s, raw);
-      f(s, raw);
+#pragma unroll
+      for (int q = 0; q < kPacks; ++q) raw[q] = next[q];
+      if (s + warps < end) row.load_section(s + warps, next);
+      f(s, [&](auto&& g) {
+#pragma unroll 1
+        for (int q = 0; q < kPacks; ++q) {  // one after the other: the code is run few times, and has to come in first
+          g((s * kPacks + q) * 32 + int(threadIdx.x & 31), raw[0]);
+#pragma unroll
+          for (int i = 1; i < kPacks; ++i) raw[i - 1] = raw[i];
+        }
+      });
     }
+  }
+  template <class T, class F>
+  __device__ __forceinline__ void each_pack(const Row<T>& row, F&& f) const
+  {
+    each_section_packs(row, [&](int, auto&& each) { each(f); });
   }
 };
 
@@ -639,40 +654,34 @@ __device__ __noinline__ bool draw_wide(const Row<T>& row, const Limits& l, const
       if (by_number) break;
       round = 2;  // min-p alone
     }
-    // ---- between which logits the limit lies: from `above` on all columns are left, below `within` none
-    uint32_t above = key_least, within = key_least;
-    double whole_near = 0.0;
+    // ---- between which logits the limit lies: those from `beyond` on, and those in intervals in front of the first-th, are left; those
+    // behind the last-th are not
+    float lo = 0.f, hi = top, scale = 0.f, beyond = INFINITY;
+    int first = 0, last = -1;
     if (round < 2) {
       // Columns of which vocab together weigh less than half of what is cut away are below the limit by mass.  By number it is among the
       // sets' highest, or not far below.
-      float lo = mass ? top - (log2f(float(row.vocab) / (1.f - fmaxf(l.p, 0.f))) + 2.f) / k : low - 2.f * (top - low);
-      float hi = top;
-      uint32_t key_hi = key_top + 1;  // above it nothing is looked at
-      float front     = 0.f;          // what lies above it
+      lo = mass ? top - (log2f(float(row.vocab) / (1.f - fmaxf(l.p, 0.f))) + 2.f) / k : low - 2.f * (top - low);
+      float front = 0.f, whole = 0.f;  // the sums of what lies from `beyond` on, of all that is left of rounds before
       for (int level = 0;; ++level) {
-        const float scale = float(kFine) / (hi - lo) * 0.9999f, step = k / scale;
+        scale            = float(kFine) / (hi - lo) * 0.9999f;
+        const float step = k / scale;
         if (!(scale > 0.f && scale < 0x1p100f) || level == 3) return false;
         for (int i = tid; i < kFine; i += threads) S.fine[i] = 0;
         __syncthreads();
-        const float beyond = key_hi > key_top ? INFINITY : key_value(uint64_t(key_hi) << 32);
         double sum = 0.0;
-        team.each_section(row, [&](int s, const uint4 (&raw)[kPacks]) {
+        team.each_pack(row, [&](int p, const uint4& raw) {
           float part = 0.f;
 #pragma unroll
-          for (int q = 0; q < kPacks; ++q)
-#pragma unroll
-            for (int j = 0; j < E; ++j) {
-              const float x = gtk::to_float(reinterpret_cast<const T*>(&raw[q])[j]);
-              const int c   = row.column((s * kPacks + q) * 32 + lane) + j;
-              const bool left = floor == 1 || rank_key(x, uint32_t(c)) >= floor, in = left && x < beyond;
-              if (mass && left && (level == 0 || !in)) part += pow2((x - top) * k);
-              const float at = (hi - x) * scale;
-              if (in && at < float(kFine)) {
-                const int b       = int(at);
-                const float share = mass ? pow2(fmaf(float(b) - at, step, float(bits))) : 1.f;
-                if (GTK_IN(b, kFine, 508)) atomicAdd(&S.fine[b], uint32_t(__float2int_rn(share)));
-              }
-            }
+          for (int j = 0; j < E; ++j) {
+            const float x   = gtk::to_float(reinterpret_cast<const T*>(&raw)[j]);
+            const bool left = floor == 1 || rank_key(x, uint32_t(row.column(p) + j)) >= floor, in = left && x < beyond;
+            if (mass) part += left && (level == 0 || !in) ? pow2((x - top) * k) : 0.f;
+            const float at = (hi - x) * scale;
+            const int b    = int(fminf(at, float(kFine)));
+            const float as = mass ? pow2(fmaf(float(b) - at, step, float(bits))) : 1.f;
+            if (in && b < kFine && GTK_IN(b, kFine, 508)) atomicAdd(&S.fine[b], uint32_t(__float2int_rn(as)));
+          }
           sum += part;
         });
         sum = warp_sum(sum);
@@ -681,56 +690,75 @@ __device__ __noinline__ bool draw_wide(const Row<T>& row, const Limits& l, const
         sum = 0.0;
         for (int w = 0; w < warps; ++w) sum += S.mass[w];
         if (tid == 0) S.part_sum = sum;
-        const uint32_t* fine = S.fine;
+        const uint4* fine = reinterpret_cast<const uint4*>(S.fine);
         if constexpr (SPLIT) {
           team.sync();
           sum = warp_sum(lane < team.parts ? team.of(&S, lane)->part_sum : 0.0);
-          for (int i = tid; i < kFine; i += threads) {
-            uint32_t n = 0;
-            for (int c = 0; c < team.parts; ++c) n += team.of(&S, c)->fine[i];
-            S.fine_all[i] = n;
+          for (int i = tid; i < kFine / 4; i += threads) {
+            uint4 n = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+            for (int c = 0; c < kMaxParts; ++c)
+              if (c < team.parts) {
+                const uint4 o = reinterpret_cast<const uint4*>(team.of(&S, c)->fine)[i];
+                n = make_uint4(n.x + o.x, n.y + o.y, n.z + o.z, n.w + o.w);
+              }
+            reinterpret_cast<uint4*>(S.fine_all)[i] = n;
           }
-          fine = S.fine_all;
+          fine = reinterpret_cast<const uint4*>(S.fine_all);
           team.sync();  // the others' are cleared for the next level only when all have read them
         }
-        if (mass && level == 0) whole_near = sum;
+        if (mass && level == 0) whole = float(sum);
         if (mass && level > 0) front = float(sum);
-        // the interval that the limit falls in, and those that rounding makes possible; by every warp
-        constexpr int kEach = kFine / 32;
-        const float slack  = mass ? ldexpf(1.f, -bits) : 0.f, base = front;
-        const float wanted = mass ? fmaxf(l.p, 0.f) * float(whole_near) : float(l.k);
-        const float unit   = mass ? ldexpf(1.f, -bits) : 1.f;
-        auto interval      = [&](int b) { return float(fine[b]) * unit * (mass ? pow2((hi - top) * k - float(b) * step) : 1.f); };
-        float mine = 0.f;
-        for (int i = 0; i < kEach; ++i) mine += interval(lane * kEach + i);
-        float upto = front + warp_upto(mine) - mine;
-        int first = kFine, last = kFine;
-        float before_first = 0.f;
-        for (int i = 0; i < kEach; ++i) {
-          const float now = interval(lane * kEach + i), next = upto + now;
-          const float off = mass ? slack * (next - base) + 1e-5f * wanted : 0.f;
-          if (first == kFine && next + off >= wanted) first = lane * kEach + i, before_first = upto;
-          if (last == kFine && next - off >= wanted) last = lane * kEach + i;
-          upto = next;
+        // the interval that the limit falls in, and those that rounding makes possible: four to a lane, by warps
+        const float unit = mass ? ldexpf(1.f, -bits) : 1.f, wanted = mass ? fmaxf(l.p, 0.f) * whole : float(l.k);
+        const float lead = (hi - top) * k;
+        auto weigh       = [&](uint32_t n, int b) { return float(n) * unit * (mass ? pow2(lead - float(b) * step) : 1.f); };
+        for (int i = warp; i < kFine / 128; i += warps) {
+          const uint4 n = fine[i * 32 + lane];
+          const int b   = (i * 32 + lane) * 4;
+          const float w = warp_sum((weigh(n.x, b) + weigh(n.y, b + 1)) + (weigh(n.z, b + 2) + weigh(n.w, b + 3)));
+          if (lane == 0) S.run[i] = w;
         }
-        const int first_of_all = __reduce_min_sync(0xFFFFFFFFu, first);
-        if (first_of_all == kFine) return false;  // the limit is further down
-        front = __shfl_sync(0xFFFFFFFFu, before_first, first_of_all / kEach);
-        last  = min(__reduce_min_sync(0xFFFFFFFFu, last), kFine - 1);
-        first = first_of_all;
+        if (tid == 0) S.first = kFine, S.last = kFine - 1;
+        __syncthreads();
+        for (int i = warp; i < kFine / 128; i += warps) {
+          const uint4 n = fine[i * 32 + lane];
+          const int b   = (i * 32 + lane) * 4;
+          float w[4]    = {weigh(n.x, b), weigh(n.y, b + 1), weigh(n.z, b + 2), weigh(n.w, b + 3)};
+          float upto    = 0.f;
+          for (int j = 0; j < i; ++j) upto += S.run[j];
+          upto += warp_upto((w[0] + w[1]) + (w[2] + w[3])) - ((w[0] + w[1]) + (w[2] + w[3]));
+          int from = kFine, to = kFine - 1;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            upto += w[j];
+            const float off = mass ? upto * unit + 1e-5f * wanted : 0.f;
+            if (from == kFine && front + upto + off >= wanted) from = b + j;
+            if (to == kFine - 1 && front + upto - off >= wanted) to = b + j;
+          }
+          from = __reduce_min_sync(0xFFFFFFFFu, from), to = __reduce_min_sync(0xFFFFFFFFu, to);
+          if (lane == 0) atomicMin(&S.first, from), atomicMin(&S.last, to);
+        }
+        __syncthreads();
+        first = S.first, last = S.last;
+        if (first == kFine) return false;  // the limit is further down
+        // how many columns that may be
         int n = 0;
-        for (int b = first + lane; b <= last; b += 32) n += int(float(fine[b]) * unit * 1.02f * (mass ? pow2(step * 0.5f) : 1.f)) + 1;
+        for (int b = first + lane; b <= last; b += 32) n += int(float(reinterpret_cast<const uint32_t*>(fine)[b]) * unit * 1.02f * (mass ? pow2(step * 0.5f) : 1.f)) + 1;
         n = warp_sum(n);
-        // the intervals' ends as numbers
-        const uint32_t key_lo = value_key(fmaxf(lo - (hi - lo) * 1e-3f, -FLT_MAX));
-        above  = lowest_key(key_lo, key_top + 1, [&](float x) { return !(x <= hi) || (hi - x) * scale < float(first); });
-        within = lowest_key(key_lo, above, [&](float x) { return (hi - x) * scale < float(last + 1); });
-        above = min(above, key_hi);
+        float so_far = 0.f;  // by number, which front and these are exactly
+        if (!mass)
+          for (int b = lane; b < first; b += 32) so_far += float(reinterpret_cast<const uint32_t*>(fine)[b]);
         if (n <= kMostKeys - 64) break;
-        if (above <= within) return false;
-        const float next_hi = key_value(uint64_t(above - 1) << 32), next_lo = key_value(uint64_t(within) << 32);
-        if (!(next_lo < next_hi)) return false;  // one number
-        hi = next_hi, lo = next_lo - (next_hi - next_lo) * 1e-3f, key_hi = above;
+        front += warp_sum(so_far);
+        // those intervals alone, from one number to another
+        const uint32_t key_lo = value_key(fmaxf(lo - (hi - lo) * 1e-3f, -FLT_MAX)), key_hi = value_key(hi) + 1;
+        const uint32_t above  = lowest_key(key_lo, key_hi, [&](float x) { return (hi - x) * scale < float(first); });
+        const uint32_t within = lowest_key(key_lo, above, [&](float x) { return (hi - x) * scale < float(last + 1); });
+        if (above <= within + 1) return false;  // one number
+        if (above < key_hi || beyond == INFINITY) beyond = above <= key_top ? key_value(uint64_t(above) << 32) : INFINITY;
+        const float next_lo = key_value(uint64_t(within) << 32);
+        hi = key_value(uint64_t(above - 1) << 32), lo = next_lo - (hi - next_lo) * 1e-3f;
         __syncthreads();
       }
     }
@@ -738,103 +766,121 @@ __device__ __noinline__ bool draw_wide(const Row<T>& row, const Limits& l, const
     __syncthreads();
     if (tid == 0) S.keys = 0;
     __syncthreads();
-    const float x_above = above > key_top ? INFINITY : key_value(uint64_t(above) << 32), x_within = key_value(uint64_t(within) << 32),
-                x_least = key_value(uint64_t(key_least) << 32);
-    double sum_above = 0.0, sum_all = 0.0;
-    int count = 0;
-    team.each_section(row, [&](int s, const uint4 (&raw)[kPacks]) {
+    const float x_least = key_value(uint64_t(key_least) << 32), from_first = float(first), upto_last = float(last + 1);
+    double sum_all = 0.0;
+    int count      = 0;
+    bool cut_short = false;  // min-p cuts above the limit
+    team.each_section_packs(row, [&](int s, auto&& each_pack) {
       double part = 0.0;
-#pragma unroll 1
-      for (int q = 0; q < kPacks; ++q) {
-        uint4 one = raw[0];
-#pragma unroll
-        for (int i = 1; i < kPacks; ++i)
-          if (i == q) one = raw[i];
+      each_pack([&](int p, const uint4& raw) {
+        double w[E];
+        uint32_t hits = 0;
 #pragma unroll
         for (int j = 0; j < E; ++j) {
-          const float x = gtk::to_float(reinterpret_cast<const T*>(&one)[j]);
-          const int c   = row.column((s * kPacks + q) * 32 + lane) + j;
-          const uint64_t key = rank_key(x, uint32_t(c));
-          const bool in      = key >= floor;
-          const double w     = in ? weight(x) : 0.0;
-          sum_all += w;
-          if (in && x >= x_above) {
-            sum_above += w;
-            ++count;
-            if (x >= x_least) part += w;
-          } else if (in && x >= x_within) {
-            const int at = atomicAdd(&S.keys, 1);
-            if (at < kMostKeys && GTK_IN(at, kMostKeys, 509)) S.key[at] = key;
-          }
+          const float x   = gtk::to_float(reinterpret_cast<const T*>(&raw)[j]);
+          const bool in   = rank_key(x, uint32_t(row.column(p) + j)) >= floor;
+          const float at  = (hi - x) * scale;
+          const bool above = in && (round == 2 || x >= beyond || at < from_first);
+          hits |= (in && !above && at < upto_last ? 1u : 0u) << j;
+          w[j] = weight(x);
+          w[j] = in ? w[j] : 0.0;
+          count += above;
+          cut_short |= above && x < x_least;
+          part += above && x >= x_least ? w[j] : 0.0;
         }
-      }
+#pragma unroll
+        for (int d = 1; d < E; d *= 2)
+#pragma unroll
+          for (int j = 0; j < E; j += 2 * d) w[j] += w[j + d];
+        sum_all += w[0];
+        if (hits) {
+          int i = atomicAdd(&S.keys, __popc(hits));
+#pragma unroll
+          for (int j = 0; j < E; ++j)
+            if (hits >> j & 1u) {
+              if (i < kMostKeys && GTK_IN(i, kMostKeys, 509)) S.key[i] = rank_key(gtk::to_float(reinterpret_cast<const T*>(&raw)[j]), uint32_t(row.column(p) + j));
+              ++i;
+            }
+        }
+      });
       part = warp_sum(part);
       if (lane == 0 && GTK_IN(s, row.sections, 510)) section[s] = part;
     });
-    sum_above = warp_sum(sum_above), sum_all = warp_sum(sum_all), count = warp_sum(count);
-    if (lane == 0) S.mass[warp] = sum_above, S.count[warp] = count;
+    sum_all = warp_sum(sum_all), count = warp_sum(count);
+    cut_short = __any_sync(0xFFFFFFFFu, cut_short);
+    if (lane == 0) S.mass[warp] = sum_all, S.count[warp] = count << 1 | int(cut_short);
     __syncthreads();
-    sum_above = 0.0, count = 0;
-    for (int w = 0; w < warps; ++w) sum_above += S.mass[w], count += S.count[w];
-    __syncthreads();
-    if (lane == 0) S.mass[warp] = sum_all;
-    __syncthreads();
-    sum_all = 0.0;
-    for (int w = 0; w < warps; ++w) sum_all += S.mass[w];
-    if (tid == 0) S.part_mass[0] = sum_above, S.part_mass[1] = sum_all, S.part_count = count;
+    sum_all = 0.0, count = 0;
+    for (int w = 0; w < warps; ++w) sum_all += S.mass[w], count += S.count[w] >> 1, cut_short |= S.count[w] & 1;
+    if (tid == 0) S.part_sum = sum_all, S.part_count = count << 1 | int(cut_short);
     const int n = gather_keys(team, S);
     if (n > kMostKeys) return false;
     if constexpr (SPLIT) {
       if (team.part == 0) {
-        sum_above = warp_sum(lane < team.parts ? team.of(&S, lane)->part_mass[0] : 0.0);
-        sum_all   = warp_sum(lane < team.parts ? team.of(&S, lane)->part_mass[1] : 0.0);
-        count     = warp_sum(lane < team.parts ? team.of(&S, lane)->part_count : 0);
+        sum_all         = warp_sum(lane < team.parts ? team.of(&S, lane)->part_sum : 0.0);
+        const int other = lane < team.parts ? team.of(&S, lane)->part_count : 0;
+        count           = warp_sum(other >> 1);
+        cut_short       = __any_sync(0xFFFFFFFFu, other & 1);
         for (int s = team.end + tid; s < row.sections; s += threads) section[s] = team.of(section, s / team.share)[s];
       }
       team.sync();
     }
     // ---- which of these are left
     if (team.part == 0) {
-      int left = 0;
+      int left    = 0;
+      bool solved = true;
       if (n > 0) {
         __syncthreads();
         sort_down(S.key, n);
         for (int i = tid; i < n; i += threads) S.weight[i] = weight(key_value(S.key[i]));
-        __syncthreads();
       }
-      bool solved = true;
+      __syncthreads();
       if (round == 0) {
         left   = l.k - count;
         solved = left >= 0 && left <= n;
-      } else if (round == 1) {
+      } else if (round == 1 && !cut_short) {
         const double reach = fmax(0.0, double(l.p)) * sum_all;
+        double above       = 0.0;
+        for (int s = lane; s < row.sections; s += 32) above += section[s];
+        above = warp_sum(above);
         // the list's weights in front of every lane's share of it, by every warp
         const int each = (n + 31) / 32, begin = min(n, lane * each), end = min(n, begin + each);
         double mine = 0.0;
         for (int i = begin; i < end; ++i) mine += S.weight[i];
-        double upto = sum_above + warp_upto(mine) - mine;
+        double upto = above + warp_upto(mine) - mine;
         left        = INT_MAX;
         for (int i = begin; i < end && left == INT_MAX; ++i)
           if ((upto += S.weight[i]) >= reach) left = i + 1;
         left   = __reduce_min_sync(0xFFFFFFFFu, left);
-        solved = sum_above < reach && left != INT_MAX;  // the limit is neither above nor below
+        solved = above < reach && left != INT_MAX;  // the limit is neither above nor below
       }
-      if (solved && left > 0) floor = max(floor, S.key[left - 1]);
-      else floor = max(floor, uint64_t(above) << 32);
+      if (solved && left > 0) {
+        floor = max(floor, S.key[left - 1]);
+      } else if (solved && (round == 0 || (round == 1 && !cut_short))) {  // as many as lie above it
+        const uint32_t above = lowest_key(key_lowest, key_top, [&](float x) { return x >= beyond || (hi - x) * scale < from_first; });
+        floor                = max(floor, uint64_t(above) << 32);
+      }
       if (solved && !(round == 0 && by_mass)) {
         floor = max(floor, uint64_t(key_least) << 32);
         // the sections with what is left of the list, and the draw
+        for (int i = tid; i < left; i += threads) S.order[i] = uint16_t(S.key[i] >= floor ? int(key_column(S.key[i]) + row.lead) / Row<T>::kColumns : 0xFFFF);
+        __syncthreads();
         for (int s = tid; s < row.sections; s += threads) {
-          double sum = section[s];
+          double sum = 0.0;
+#pragma unroll 4
           for (int i = 0; i < left; ++i)
-            if (S.key[i] >= floor && int(key_column(S.key[i]) + row.lead) / Row<T>::kColumns == s) sum += S.weight[i];
-          section[s] = sum;
+            if (S.order[i] == s) sum += S.weight[i];
+          section[s] += sum;
         }
         __syncthreads();
         if (warp == 0) {
           double total;
-          const Place found = locate(row, l.u, total, [&](int s) { return section[s]; },
-                                     [&](int) { return [&](float x, int c) { return rank_key(x, uint32_t(c)) >= floor ? weight(x) : 0.0; }; });
+          const Place found = locate(row, l.u, total, [&](int s) { return section[s]; }, [&](int) {
+            return [&](float x, int c) {
+              const double w = weight(x);
+              return rank_key(x, uint32_t(c)) >= floor ? w : 0.0;
+            };
+          });
           if (lane == 0) S.column = found.column, S.total = total;
         }
         __syncthreads();
@@ -845,9 +891,9 @@ __device__ __noinline__ bool draw_wide(const Row<T>& row, const Limits& l, const
       if (tid == 0) S.solved = solved, S.floor = floor;
     }
     team.sync();
-    const Scratch* first = team.of(&S, 0);
-    const bool solved    = first->solved;
-    floor                = first->floor;
+    const Scratch* leader = team.of(&S, 0);
+    const bool solved     = leader->solved;
+    floor                 = leader->floor;
     team.sync();
     if (!solved || !(round == 0 && by_mass)) return solved;
   }
