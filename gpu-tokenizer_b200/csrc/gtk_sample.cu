@@ -102,6 +102,34 @@ struct alignas(16) Scratch {
   float part_top;
 };
 
+template <class T>
+__device__ __forceinline__ void unpack(const uint4& raw, float (&x)[Pack16<T>::kElems])
+{
+  Two pairs[Pack16<T>::kElems / 2];
+  Pack16<T>::pairs(raw, pairs);
+#pragma unroll
+  for (int j = 0; j < Pack16<T>::kElems / 2; ++j) pairs[j].get(x[2 * j], x[2 * j + 1]);
+}
+
+// their sum, by halves
+template <class N, int E>
+__device__ __forceinline__ N sum_of(N (&x)[E])
+{
+#pragma unroll
+  for (int d = 1; d < E; d *= 2)
+#pragma unroll
+    for (int j = 0; j < E; j += 2 * d) x[j] += x[j + d];
+  return x[0];
+}
+
+// adds to a word of shared memory where `yes`, without a branch
+__device__ __forceinline__ void add_shared(uint32_t* p, uint32_t n, bool yes)
+{
+  asm volatile("{\n .reg .pred p;\n setp.ne.u32 p, %2, 0;\n @p red.shared.add.u32 [%0], %1;\n}" ::"r"(uint32_t(__cvta_generic_to_shared(p))), "r"(n),
+               "r"(uint32_t(yes))
+               : "memory");
+}
+
 // Past the first-level cache, in which the loads under way would otherwise take their places (2048 rows of 50257 f32 77 -> 68 us).
 __device__ __forceinline__ uint4 load_past(const uint4* p)
 {
@@ -205,17 +233,46 @@ struct Weight64 {
   const double* power;
   __device__ __forceinline__ double operator()(float x) const
   {
+    const float one[1] = {x};
+    double w[1];
+    of(one, w);
+    return w[0];
+  }
+  // of N numbers, step by step for all of them: a step waits for the one before it some 30 clocks
+  template <int N>
+  __device__ __forceinline__ void of(const float (&x)[N], double (&w)[N]) const
+  {
     constexpr double l2 = 0.69314718055994531;
-    const double y = fmax((double(x) - m) * k, -1990.0);
-    const double a = fma(y, 64.0, 0x1.8p52);  // n in the low bits
-    const int n    = __double2loint(a), e = n >> 6, most = max(e, -1000);
-    const double f = fma(a - 0x1.8p52, -1.0 / 64, y);
-    double s       = fma(f, l2 * l2 * l2 * l2 * l2 / 120, l2 * l2 * l2 * l2 / 24);
-    s              = fma(f, s, l2 * l2 * l2 / 6);
-    s              = fma(f, s, l2 * l2 / 2);
-    s              = fma(f, s, l2);
-    s              = fma(f, s, 1.0);
-    return power[n & 63] * s * __hiloint2double((most + 1023) << 20, 0) * __hiloint2double((e - most + 1023) << 20, 0);
+    double y[N], a[N];
+    int n[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) y[i] = double(x[i]) - m;
+#pragma unroll
+    for (int i = 0; i < N; ++i) y[i] = fmax(y[i] * k, -1990.0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) a[i] = fma(y[i], 64.0, 0x1.8p52);  // n in the low bits
+#pragma unroll
+    for (int i = 0; i < N; ++i) n[i] = __double2loint(a[i]), a[i] -= 0x1.8p52;
+#pragma unroll
+    for (int i = 0; i < N; ++i) y[i] = fma(a[i], -1.0 / 64, y[i]);
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = fma(y[i], l2 * l2 * l2 * l2 * l2 / 120, l2 * l2 * l2 * l2 / 24);
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = fma(y[i], w[i], l2 * l2 * l2 / 6);
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = fma(y[i], w[i], l2 * l2 / 2);
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = fma(y[i], w[i], l2);
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] = fma(y[i], w[i], 1.0);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = n[i] >> 6, most = max(e, -1000);
+      w[i] *= power[n[i] & 63] * __hiloint2double((most + 1023) << 20, 0);
+      n[i] = e - most;
+    }
+#pragma unroll
+    for (int i = 0; i < N; ++i) w[i] *= __hiloint2double((n[i] + 1023) << 20, 0);
   }
 };
 
@@ -232,7 +289,8 @@ struct Sum {
   int count;
 };
 
-// The sums of weigh(x, column) by sections, to `section`, and their whole, by all threads; count(x, column) of the columns too.
+// The sums of weights by sections, to `section`, and their whole, by all threads.  weigh(x, column, w, count): the weights of some neighbouring
+// columns, and how many of them count.
 template <class T, class Weigh>
 __device__ __forceinline__ Sum sum_row(const Row<T>& row, double* section, Scratch& S, Weigh&& weigh)
 {
@@ -245,14 +303,15 @@ __device__ __forceinline__ Sum sum_row(const Row<T>& row, double* section, Scrat
     for (int q = 0; q < kPacks; ++q) {
       const int p     = (i * kPacks + q) * 32 + lane;
       const uint4 raw = row.load(p);
-      Sum o[Row<T>::E];
+      float all[Row<T>::E];
+      unpack<T>(raw, all);
 #pragma unroll
-      for (int j = 0; j < Row<T>::E; ++j) o[j] = weigh(gtk::to_float(reinterpret_cast<const T*>(&raw)[j]), row.column(p) + j);
-#pragma unroll
-      for (int d = 1; d < Row<T>::E; d *= 2)
-#pragma unroll
-        for (int j = 0; j < Row<T>::E; j += 2 * d) o[j].mass += o[j + d].mass, o[j].count += o[j + d].count;
-      sum += o[0].mass, s.count += o[0].count;
+      for (int j = 0; j < Row<T>::E; j += 4) {
+        const float x[4] = {all[j], all[j + 1], all[j + 2], all[j + 3]};
+        double w[4];
+        weigh(x, row.column(p) + j, w, s.count);
+        sum += sum_of(w);
+      }
     }
     sum = warp_sum(sum);
     if (lane == 0 && GTK_IN(i, row.sections, 500)) section[i] = sum;
@@ -266,6 +325,18 @@ __device__ __forceinline__ Sum sum_row(const Row<T>& row, double* section, Scrat
   return s;
 }
 
+// the same from f(x, column) -> {weight, whether it counts}
+template <class T, class F>
+__device__ __forceinline__ Sum sum_columns(const Row<T>& row, double* section, Scratch& S, F&& f)
+{
+  return sum_row(row, section, S, [&](const auto& x, int c, auto& w, int& count) {
+    for (int j = 0; j < int(sizeof(x) / sizeof(x[0])); ++j) {
+      const Sum o = f(x[j], c + j);
+      w[j] = o.mass, count += o.count;
+    }
+  });
+}
+
 // A column with its section and its logit, and the sums of the weights in front of it and with it.
 struct Place {
   int column, section;
@@ -274,7 +345,7 @@ struct Place {
 };
 
 // The first column at which the sum of the weights exceeds the target, `share` of the sum of all, by one warp: section(s) is a section's sum, weigh(s)(x,
-// column) the weight of a column in it.  The last one with any weight where rounding leaves none, column -1 where none has any.
+// column, w) the weights of columns in it.  The last one with any weight where rounding leaves none, column -1 where none has any.
 template <class T, class Section, class Weigh>
 __device__ __forceinline__ Place locate(const Row<T>& row, double share, double& total, Section&& section, Weigh&& weigh)
 {
@@ -314,14 +385,15 @@ __device__ __forceinline__ Place locate(const Row<T>& row, double share, double&
   for (int q = 0; q < kPacks; ++q) {
     const int p     = (s * 32 + lane) * kPacks + q, c = row.column(p);
     const uint4 raw = row.load(p);
-    double w[Row<T>::E];
+    float all_of[Row<T>::E];
+    unpack<T>(raw, all_of);
 #pragma unroll
-    for (int j = 0; j < Row<T>::E; ++j) w[j] = weight(gtk::to_float(reinterpret_cast<const T*>(&raw)[j]), c + j);
-#pragma unroll
-    for (int d = 1; d < Row<T>::E; d *= 2)
-#pragma unroll
-      for (int j = 0; j < Row<T>::E; j += 2 * d) w[j] += w[j + d];
-    mine += w[0];
+    for (int j = 0; j < Row<T>::E; j += 4) {
+      const float x[4] = {all_of[j], all_of[j + 1], all_of[j + 2], all_of[j + 3]};
+      double w[4];
+      weight(x, c + j, w);
+      mine += sum_of(w);
+    }
   }
   upto = front + warp_upto(mine);
   from = lane_of(mine, upto, target);
@@ -329,11 +401,14 @@ __device__ __forceinline__ Place locate(const Row<T>& row, double share, double&
   front = __shfl_sync(all, upto - mine, from);
   // a column to a lane
   const int c = row.column((s * 32 + from) * kPacks) + lane;
-  mine        = lane < kOwn && uint32_t(c) < uint32_t(row.vocab) ? weight(row.value(c), c) : 0.0;
+  const float own[1] = {lane < kOwn && uint32_t(c) < uint32_t(row.vocab) ? row.value(c) : -INFINITY};
+  double w[1];
+  weight(own, c, w);
+  mine        = own[0] > -INFINITY ? w[0] : 0.0;
   upto        = front + warp_upto(mine);
   from        = lane_of(mine, upto, target);
   if (from < 0) return Place{-1, s, 0.0, 0.0, 0.f};
-  return Place{__shfl_sync(all, c, from), s, __shfl_sync(all, upto - mine, from), __shfl_sync(all, upto, from), __shfl_sync(all, row.value(min(max(c, 0), row.vocab - 1)), from)};
+  return Place{__shfl_sync(all, c, from), s, __shfl_sync(all, upto - mine, from), __shfl_sync(all, upto, from), __shfl_sync(all, own[0], from)};
 }
 
 // Everything in 64 bits, by one CTA, in as many readings of the row as it takes: rows of which nothing else is known, or whose borders
@@ -359,7 +434,11 @@ struct Slowly {
     __syncthreads();
     if (threadIdx.x < 32) {
       double total;
-      const Place found = locate(row, share, total, [&](int s) { return section[s]; }, [&](int) { return weigh; });
+      const Place found = locate(row, share, total, [&](int s) { return section[s]; }, [&](int) {
+        return [&](const auto& x, int c, auto& w) {
+          for (int j = 0; j < int(sizeof(x) / sizeof(x[0])); ++j) w[j] = weigh(x[j], c + j);
+        };
+      });
       if (threadIdx.x == 0) S.column = found.column, S.total = total;
     }
     __syncthreads();
@@ -377,14 +456,14 @@ struct Slowly {
     uint32_t lo = 1, hi = most;  // enough at lo
     while (lo < hi) {
       const uint32_t mid = lo + (hi - lo + 1) / 2;
-      const Sum s = sum_row(row, section, S, [&](float x, int c) { return value_key(x) >= mid && left(x, c) ? Sum{weight(x), 1} : Sum{0.0, 0}; });
+      const Sum s = sum_columns(row, section, S, [&](float x, int c) { return value_key(x) >= mid && left(x, c) ? Sum{weight(x), 1} : Sum{0.0, 0}; });
       if (enough(s)) lo = mid;
       else hi = mid - 1;
     }
-    const Sum above = sum_row(row, section, S, [&](float x, int c) { return value_key(x) > lo && left(x, c) ? Sum{weight(x), 1} : Sum{0.0, 0}; });
+    const Sum above = sum_columns(row, section, S, [&](float x, int c) { return value_key(x) > lo && left(x, c) ? Sum{weight(x), 1} : Sum{0.0, 0}; });
     const float value  = key_value(uint64_t(lo) << 32);
     auto equal         = [&](float x, int c) { return value_key(x) == lo && left(x, c) ? 1.0 : 0.0; };
-    const double equals = sum_row(row, section, S, [&](float x, int c) { return Sum{equal(x, c), 0}; }).mass;
+    const double equals = sum_columns(row, section, S, [&](float x, int c) { return Sum{equal(x, c), 0}; }).mass;
     const int column    = find((wanted(above, weight(value)) - 0.5) / equals, equal);
     floor            = max(floor, rank_key(value, uint32_t(column)));
   }
@@ -395,7 +474,7 @@ struct Slowly {
     const int threads = blockDim.x, warps = threads >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     bool broken   = false;
     uint32_t most = 0;
-    const int some = sum_row(row, section, S, [&](float x, int c) {
+    const int some = sum_columns(row, section, S, [&](float x, int c) {
                        if (uint32_t(c) < uint32_t(row.vocab)) broken |= !(x < INFINITY), most = max(most, value_key(x));
                        return Sum{0.0, x > -INFINITY ? 1 : 0};
                      }).count;
@@ -412,7 +491,7 @@ struct Slowly {
     if (l.k < some)
       search(most, [&](const Sum& s) { return s.count >= l.k; }, [&](const Sum& s, double) { return double(l.k - s.count); });
     if (l.cut_by_mass()) {
-      const double whole = sum_row(row, section, S, [&](float x, int c) { return left(x, c) ? Sum{weight(x), 1} : Sum{0.0, 0}; }).mass;
+      const double whole = sum_columns(row, section, S, [&](float x, int c) { return left(x, c) ? Sum{weight(x), 1} : Sum{0.0, 0}; }).mass;
       const double reach = fmax(0.0, double(l.p)) * whole;
       search(most, [&](const Sum& s) { return s.mass >= reach; },
              [&](const Sum& s, double w) {
@@ -423,7 +502,7 @@ struct Slowly {
     }
     const double least_y = l.least > 0.f ? log(double(l.least)) : -INFINITY;
     auto drawn           = [&](float x, int c) { return left(x, c) && (double(x) - m) * l.inverse >= least_y ? weight(x) : 0.0; };
-    sum_row(row, section, S, [&](float x, int c) { return Sum{drawn(x, c), 0}; });
+    sum_columns(row, section, S, [&](float x, int c) { return Sum{drawn(x, c), 0}; });
     const int id = find(l.u, drawn);
     if (id < 0) return -1;
     logprob = l.t == 0.f ? 0.f : float((double(row.value(id)) - m) * l.inverse - log(total));
@@ -443,7 +522,7 @@ template <class T>
 __device__ __noinline__ double sum_exactly(const Row<T>& row, const Limits& l, double m, double* section, Scratch& S)
 {
   const Weight64 weight = weight64(l, m, S);
-  return sum_row(row, section, S, [&](float x, int) { return Sum{weight(x), 0}; }).mass;
+  return sum_row(row, section, S, [&](const auto& x, int, auto& w, int&) { weight.of(x, w); }).mass;
 }
 
 // What is drawn of all columns, with everything in 64 bits.
@@ -455,7 +534,7 @@ __device__ __noinline__ int draw_exactly(const Row<T>& row, const Limits& l, dou
   if (threadIdx.x >= 32) return -1;
   double total;
   const Place found = locate(row, l.u, total, [&](int s) { return section[s]; },
-                             [&](int) { return [&](float x, int) { return weight(x); }; });
+                             [&](int) { return [&](const auto& x, int, auto& w) { weight.of(x, w); }; });
   logprob           = float((double(found.x) - m) * l.inverse - log(total));
   return found.column;
 }
@@ -561,14 +640,9 @@ struct Team {
   __device__ __forceinline__ void each_section_packs(const Row<T>& row, F&& f) const
   {
     const int warps = blockDim.x >> 5;
-    uint4 next[kPacks];
-    int s = begin + int(threadIdx.x >> 5);
-    if (s < end) row.load_section(s, next);
-    for (; s < end; s += warps) {
+    for (int s = begin + int(threadIdx.x >> 5); s < end; s += warps) {
       uint4 raw[kPacks];
-#pragma unroll
-      for (int q = 0; q < kPacks; ++q) raw[q] = next[q];
-      if (s + warps < end) row.load_section(s + warps, next);
+      row.load_section(s, raw);
       f(s, [&](auto&& g) {
 #pragma unroll 1
         for (int q = 0; q < kPacks; ++q) {  // one after the other: the code is run few times, and has to come in first
@@ -578,11 +652,6 @@ struct Team {
         }
       });
     }
-  }
-  template <class T, class F>
-  __device__ __forceinline__ void each_pack(const Row<T>& row, F&& f) const
-  {
-    each_section_packs(row, [&](int, auto&& each) { each(f); });
   }
 };
 
@@ -620,6 +689,120 @@ __device__ __forceinline__ uint32_t lowest_key(uint32_t lo, uint32_t hi, Holds&&
     else lo = mid + 1;
   }
   return hi;
+}
+
+// What a pass over a wide row goes by: x is in interval int((hi - x) * scale), or above all of them from `beyond` on.
+struct Interval {
+  uint64_t floor;
+  float hi, scale, beyond;
+  float a, b, c, d;
+  bool yes, all;
+};
+
+// Counts the columns in S.fine, or with v.yes adds their weights, as whole numbers relative to the interval's upper end: v.a the highest
+// logit, v.b an exponent's part of a logit, v.c of an interval, v.d the bits of a one.  The sum of the weights from `beyond` on, or of v.all.
+template <class T, bool SPLIT>
+__device__ __noinline__ double count_columns(const Row<T>& row, const Team<SPLIT>& team, const Interval v, Scratch& S)
+{
+  constexpr int E = Row<T>::E;
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  double sum = 0.0;
+  team.each_section_packs(row, [&](int, auto&& each) {
+    float of_section = 0.f;
+    each([&](int p, const uint4& raw) {
+      float x[E], at[E], part[E];
+      unpack<T>(raw, x);
+      int b[E];
+      bool in[E];
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const bool left = v.floor == 1 || rank_key(x[j], uint32_t(row.column(p) + j)) >= v.floor;
+        at[j]   = (v.hi - x[j]) * v.scale;
+        in[j]   = left && x[j] < v.beyond;
+        b[j]    = int(fminf(at[j], float(kFine)));
+        part[j] = v.yes && left && (v.all || !in[j]) ? pow2((x[j] - v.a) * v.b) : 0.f;
+      }
+#pragma unroll
+      for (int j = 0; j < E; ++j) at[j] = v.yes ? pow2(fmaf(float(b[j]) - at[j], v.c, v.d)) : 1.f;
+#pragma unroll
+      for (int j = 0; j < E; ++j) {
+        const bool counts = in[j] && b[j] < kFine && GTK_IN(b[j], kFine, 508);
+        add_shared(S.fine + (counts ? b[j] : 0), uint32_t(__float2int_rn(at[j])), counts);
+      }
+      of_section += sum_of(part);
+    });
+    sum += of_section;
+  });
+  sum = warp_sum(sum);
+  if (lane == 0) S.mass[warp] = sum;
+  __syncthreads();
+  sum = 0.0;
+  for (int w = 0; w < warps; ++w) sum += S.mass[w];
+  if (threadIdx.x == 0) S.part_sum = sum;
+  return sum;
+}
+
+// Sums in 64 bits, of columns that reach v.floor: those above interval v.b (v.yes: all) and at least v.a by sections, all of them together; lists those in
+// front of interval v.c, and tells how many are above and whether some of these are below v.a.
+struct Above {
+  double all;
+  int count;
+  bool cut_short;
+};
+template <class T, bool SPLIT>
+__device__ __noinline__ Above sum_above(const Row<T>& row, const Team<SPLIT>& team, const Weight64 weight, const Interval v, double* section, Scratch& S)
+{
+  constexpr int E = Row<T>::E, kOnce = 4;  // columns at a time
+  const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  Above found{0.0, 0, false};
+  team.each_section_packs(row, [&](int s, auto&& each_pack) {
+    double part = 0.0;
+    each_pack([&](int p, const uint4& raw) {
+      float all[E];
+      unpack<T>(raw, all);
+      uint32_t hits = 0;
+#pragma unroll
+      for (int i = 0; i < E; i += kOnce) {
+        float x[kOnce];
+        double w[kOnce], kept[kOnce];
+#pragma unroll
+        for (int j = 0; j < kOnce; ++j) x[j] = all[i + j];
+        weight.of(x, w);
+#pragma unroll
+        for (int j = 0; j < kOnce; ++j) {
+          const bool in    = rank_key(x[j], uint32_t(row.column(p) + i + j)) >= v.floor;
+          const float at   = (v.hi - x[j]) * v.scale;
+          const bool above = in && (v.yes || x[j] >= v.beyond || at < v.b), high = x[j] >= v.a;
+          hits |= (in && !above && at < v.c ? 1u : 0u) << (i + j);
+          w[j]    = in ? w[j] : 0.0;
+          kept[j] = above && high ? w[j] : 0.0;
+          found.count += above;
+          found.cut_short |= above && !high;
+        }
+        part += sum_of(kept);
+        found.all += sum_of(w);
+      }
+      if (hits) {
+        int i = atomicAdd(&S.keys, __popc(hits));
+#pragma unroll
+        for (int j = 0; j < E; ++j)
+          if (hits >> j & 1u) {
+            if (i < kMostKeys && GTK_IN(i, kMostKeys, 509)) S.key[i] = rank_key(all[j], uint32_t(row.column(p) + j));
+            ++i;
+          }
+      }
+    });
+    part = warp_sum(part);
+    if (lane == 0 && GTK_IN(s, row.sections, 510)) section[s] = part;
+  });
+  found.all = warp_sum(found.all), found.count = warp_sum(found.count);
+  found.cut_short = __any_sync(0xFFFFFFFFu, found.cut_short);
+  if (lane == 0) S.mass[warp] = found.all, S.count[warp] = found.count << 1 | int(found.cut_short);
+  __syncthreads();
+  found.all = 0.0, found.count = 0;
+  for (int w = 0; w < warps; ++w) found.all += S.mass[w], found.count += S.count[w] >> 1, found.cut_short |= S.count[w] & 1;
+  if (threadIdx.x == 0) S.part_sum = found.all, S.part_count = found.count << 1 | int(found.cut_short);
+  return found;
 }
 
 // Rows of which more columns are left than can be ranked.  For a limit by number or by mass the columns are counted by the interval of
@@ -669,27 +852,7 @@ __device__ __noinline__ bool draw_wide(const Row<T>& row, const Limits& l, const
         if (!(scale > 0.f && scale < 0x1p100f) || level == 3) return false;
         for (int i = tid; i < kFine; i += threads) S.fine[i] = 0;
         __syncthreads();
-        double sum = 0.0;
-        team.each_pack(row, [&](int p, const uint4& raw) {
-          float part = 0.f;
-#pragma unroll
-          for (int j = 0; j < E; ++j) {
-            const float x   = gtk::to_float(reinterpret_cast<const T*>(&raw)[j]);
-            const bool left = floor == 1 || rank_key(x, uint32_t(row.column(p) + j)) >= floor, in = left && x < beyond;
-            if (mass) part += left && (level == 0 || !in) ? pow2((x - top) * k) : 0.f;
-            const float at = (hi - x) * scale;
-            const int b    = int(fminf(at, float(kFine)));
-            const float as = mass ? pow2(fmaf(float(b) - at, step, float(bits))) : 1.f;
-            if (in && b < kFine && GTK_IN(b, kFine, 508)) atomicAdd(&S.fine[b], uint32_t(__float2int_rn(as)));
-          }
-          sum += part;
-        });
-        sum = warp_sum(sum);
-        if (lane == 0) S.mass[warp] = sum;
-        __syncthreads();
-        sum = 0.0;
-        for (int w = 0; w < warps; ++w) sum += S.mass[w];
-        if (tid == 0) S.part_sum = sum;
+        double sum = count_columns(row, team, Interval{floor, hi, scale, beyond, top, k, step, float(bits), mass, level == 0}, S);
         const uint4* fine = reinterpret_cast<const uint4*>(S.fine);
         if constexpr (SPLIT) {
           team.sync();
@@ -767,52 +930,10 @@ __device__ __noinline__ bool draw_wide(const Row<T>& row, const Limits& l, const
     if (tid == 0) S.keys = 0;
     __syncthreads();
     const float x_least = key_value(uint64_t(key_least) << 32), from_first = float(first), upto_last = float(last + 1);
-    double sum_all = 0.0;
-    int count      = 0;
-    bool cut_short = false;  // min-p cuts above the limit
-    team.each_section_packs(row, [&](int s, auto&& each_pack) {
-      double part = 0.0;
-      each_pack([&](int p, const uint4& raw) {
-        double w[E];
-        uint32_t hits = 0;
-#pragma unroll
-        for (int j = 0; j < E; ++j) {
-          const float x   = gtk::to_float(reinterpret_cast<const T*>(&raw)[j]);
-          const bool in   = rank_key(x, uint32_t(row.column(p) + j)) >= floor;
-          const float at  = (hi - x) * scale;
-          const bool above = in && (round == 2 || x >= beyond || at < from_first);
-          hits |= (in && !above && at < upto_last ? 1u : 0u) << j;
-          w[j] = weight(x);
-          w[j] = in ? w[j] : 0.0;
-          count += above;
-          cut_short |= above && x < x_least;
-          part += above && x >= x_least ? w[j] : 0.0;
-        }
-#pragma unroll
-        for (int d = 1; d < E; d *= 2)
-#pragma unroll
-          for (int j = 0; j < E; j += 2 * d) w[j] += w[j + d];
-        sum_all += w[0];
-        if (hits) {
-          int i = atomicAdd(&S.keys, __popc(hits));
-#pragma unroll
-          for (int j = 0; j < E; ++j)
-            if (hits >> j & 1u) {
-              if (i < kMostKeys && GTK_IN(i, kMostKeys, 509)) S.key[i] = rank_key(gtk::to_float(reinterpret_cast<const T*>(&raw)[j]), uint32_t(row.column(p) + j));
-              ++i;
-            }
-        }
-      });
-      part = warp_sum(part);
-      if (lane == 0 && GTK_IN(s, row.sections, 510)) section[s] = part;
-    });
-    sum_all = warp_sum(sum_all), count = warp_sum(count);
-    cut_short = __any_sync(0xFFFFFFFFu, cut_short);
-    if (lane == 0) S.mass[warp] = sum_all, S.count[warp] = count << 1 | int(cut_short);
-    __syncthreads();
-    sum_all = 0.0, count = 0;
-    for (int w = 0; w < warps; ++w) sum_all += S.mass[w], count += S.count[w] >> 1, cut_short |= S.count[w] & 1;
-    if (tid == 0) S.part_sum = sum_all, S.part_count = count << 1 | int(cut_short);
+    const Above found = sum_above(row, team, weight, Interval{floor, hi, scale, beyond, x_least, from_first, upto_last, 0.f, round == 2, false}, section, S);
+    double sum_all    = found.all;
+    int count         = found.count;
+    bool cut_short    = found.cut_short;
     const int n = gather_keys(team, S);
     if (n > kMostKeys) return false;
     if constexpr (SPLIT) {
@@ -876,9 +997,10 @@ __device__ __noinline__ bool draw_wide(const Row<T>& row, const Limits& l, const
         if (warp == 0) {
           double total;
           const Place found = locate(row, l.u, total, [&](int s) { return section[s]; }, [&](int) {
-            return [&](float x, int c) {
-              const double w = weight(x);
-              return rank_key(x, uint32_t(c)) >= floor ? w : 0.0;
+            return [&](const auto& x, int c, auto& w) {
+              weight.of(x, w);
+#pragma unroll
+              for (int j = 0; j < int(sizeof(x) / sizeof(x[0])); ++j) w[j] = rank_key(x[j], uint32_t(c + j)) >= floor ? w[j] : 0.0;
             };
           });
           if (lane == 0) S.column = found.column, S.total = total;
