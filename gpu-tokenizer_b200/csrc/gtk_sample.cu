@@ -701,7 +701,8 @@ struct Interval {
 
 // Counts the columns in S.fine, or with v.yes adds their weights, as whole numbers relative to the interval's upper end: v.a the highest
 // logit, v.b an exponent's part of a logit, v.c of an interval, v.d the bits of a one.  The sum of the weights from `beyond` on, or of v.all.
-template <class T, bool SPLIT>
+// PLAIN: by weight, and no round has been before.
+template <bool PLAIN, class T, bool SPLIT>
 __device__ __noinline__ double count_columns(const Row<T>& row, const Team<SPLIT>& team, const Interval v, Scratch& S)
 {
   constexpr int E = Row<T>::E;
@@ -716,14 +717,14 @@ __device__ __noinline__ double count_columns(const Row<T>& row, const Team<SPLIT
       bool in[E];
 #pragma unroll
       for (int j = 0; j < E; ++j) {
-        const bool left = v.floor == 1 || rank_key(x[j], uint32_t(row.column(p) + j)) >= v.floor;
+        const bool left = PLAIN || v.floor == 1 || rank_key(x[j], uint32_t(row.column(p) + j)) >= v.floor;
         at[j]   = (v.hi - x[j]) * v.scale;
         in[j]   = left && x[j] < v.beyond;
         b[j]    = int(fminf(at[j], float(kFine)));
-        part[j] = v.yes && left && (v.all || !in[j]) ? pow2((x[j] - v.a) * v.b) : 0.f;
+        part[j] = (PLAIN || v.yes) && left && (v.all || !in[j]) ? pow2((x[j] - v.a) * v.b) : 0.f;
       }
 #pragma unroll
-      for (int j = 0; j < E; ++j) at[j] = v.yes ? pow2(fmaf(float(b[j]) - at[j], v.c, v.d)) : 1.f;
+      for (int j = 0; j < E; ++j) at[j] = PLAIN || v.yes ? pow2(fmaf(float(b[j]) - at[j], v.c, v.d)) : 1.f;
 #pragma unroll
       for (int j = 0; j < E; ++j) {
         const bool counts = in[j] && b[j] < kFine && GTK_IN(b[j], kFine, 508);
@@ -749,7 +750,8 @@ struct Above {
   int count;
   bool cut_short;
 };
-template <class T, bool SPLIT>
+// PLAIN: by weight, no round before, no min-p.
+template <bool PLAIN, class T, bool SPLIT>
 __device__ __noinline__ Above sum_above(const Row<T>& row, const Team<SPLIT>& team, const Weight64 weight, const Interval v, double* section, Scratch& S)
 {
   constexpr int E = Row<T>::E, kOnce = 4;  // columns at a time
@@ -770,14 +772,20 @@ __device__ __noinline__ Above sum_above(const Row<T>& row, const Team<SPLIT>& te
         weight.of(x, w);
 #pragma unroll
         for (int j = 0; j < kOnce; ++j) {
-          const bool in    = rank_key(x[j], uint32_t(row.column(p) + i + j)) >= v.floor;
-          const float at   = (v.hi - x[j]) * v.scale;
-          const bool above = in && (v.yes || x[j] >= v.beyond || at < v.b), high = x[j] >= v.a;
-          hits |= (in && !above && at < v.c ? 1u : 0u) << (i + j);
-          w[j]    = in ? w[j] : 0.0;
-          kept[j] = above && high ? w[j] : 0.0;
-          found.count += above;
-          found.cut_short |= above && !high;
+          const float at = (v.hi - x[j]) * v.scale;
+          if constexpr (PLAIN) {  // -inf weighs nothing and lies in no interval
+            const bool above = x[j] >= v.beyond || at < v.b;
+            hits |= (!above && at < v.c ? 1u : 0u) << (i + j);
+            kept[j] = above ? w[j] : 0.0;
+          } else {
+            const bool in    = rank_key(x[j], uint32_t(row.column(p) + i + j)) >= v.floor;
+            const bool above = in && (v.yes || x[j] >= v.beyond || at < v.b), high = x[j] >= v.a;
+            hits |= (in && !above && at < v.c ? 1u : 0u) << (i + j);
+            w[j]    = in ? w[j] : 0.0;
+            kept[j] = above && high ? w[j] : 0.0;
+            found.count += above;
+            found.cut_short |= above && !high;
+          }
         }
         part += sum_of(kept);
         found.all += sum_of(w);
@@ -815,7 +823,6 @@ template <class T, bool SPLIT>
 __device__ __noinline__ bool draw_wide(const Row<T>& row, const Limits& l, const Team<SPLIT>& team, float top, float low, double* section, Scratch& S,
                                        int& id, float& logprob)
 {
-  constexpr int E = Row<T>::E;
   const int tid = threadIdx.x, threads = blockDim.x, warps = threads >> 5, warp = tid >> 5, lane = tid & 31;
   const double m        = top;
   const Weight64 weight = weight64(l, m, S);
@@ -852,7 +859,8 @@ __device__ __noinline__ bool draw_wide(const Row<T>& row, const Limits& l, const
         if (!(scale > 0.f && scale < 0x1p100f) || level == 3) return false;
         for (int i = tid; i < kFine; i += threads) S.fine[i] = 0;
         __syncthreads();
-        double sum = count_columns(row, team, Interval{floor, hi, scale, beyond, top, k, step, float(bits), mass, level == 0}, S);
+        const Interval v{floor, hi, scale, beyond, top, k, step, float(bits), mass, level == 0};
+        double sum = mass && floor == 1 ? count_columns<true>(row, team, v, S) : count_columns<false>(row, team, v, S);
         const uint4* fine = reinterpret_cast<const uint4*>(S.fine);
         if constexpr (SPLIT) {
           team.sync();
@@ -930,7 +938,8 @@ __device__ __noinline__ bool draw_wide(const Row<T>& row, const Limits& l, const
     if (tid == 0) S.keys = 0;
     __syncthreads();
     const float x_least = key_value(uint64_t(key_least) << 32), from_first = float(first), upto_last = float(last + 1);
-    const Above found = sum_above(row, team, weight, Interval{floor, hi, scale, beyond, x_least, from_first, upto_last, 0.f, round == 2, false}, section, S);
+    const Interval v{floor, hi, scale, beyond, x_least, from_first, upto_last, 0.f, round == 2, false};
+    const Above found = round == 1 && floor == 1 && !(l.least > 0.f) ? sum_above<true>(row, team, weight, v, section, S) : sum_above<false>(row, team, weight, v, section, S);
     double sum_all    = found.all;
     int count         = found.count;
     bool cut_short    = found.cut_short;
@@ -1489,13 +1498,20 @@ __global__ void __launch_bounds__(kThreads, 4) k_sample(const T* __restrict__ lo
 
 static_assert(sizeof(Scratch) + (GTK_MAX_SAMPLE_VOCAB / (32 * kPacks * 4) + 1) * sizeof(double) <= 48 << 10, "what a CTA has without asking");
 
+// How many CTAs share a row, and how many threads they have.
+// In 1 / 2 / 4 / 8 parts of 256 threads, us: one row of 50257 bf16 without limits - / 9.8 / 8.9 / 8.4, 64 of 131072 f32 23.7 / 15.9 / 12.7 / 14, with
+// the 50 highest 42 / 25 / 19 / 22; 148 of 50257 bf16 9.8 / 9.8 / 13.1, with limits 16.7 / 16.9 / 27; 256 of f32 21.6 / 23.2 / 28.
+// Rows in numbers take 128 threads, so that more of them are under way while others are at their ends: of 256 / 128, 2048 rows of 50257 f32 80 / 73,
+// bf16 50 / 45, with min-p 73 / 63; 512 of bf16 24 / 28.
 struct Teams {
   int parts, threads;
 };
 Teams teams_for(int64_t rows, int64_t bytes, int sm_count)
 {
   Teams t{1, kThreads};
-  while (t.parts < kMaxParts && rows * t.parts * 2 <= sm_count && bytes / (t.parts * 2) >= (12 << 10)) t.parts *= 2;
+  const int64_t room = int64_t(sm_count) * (bytes >= (160 << 10) ? 2 : 1);
+  while (t.parts < kMaxParts && rows * t.parts * 2 <= room && bytes / (t.parts * 2) >= (12 << 10)) t.parts *= 2;
+  if (rows > int64_t(sm_count) * 8 && bytes <= (256 << 10)) t.threads = 128;
   return t;
 }
 
