@@ -11,10 +11,27 @@ namespace {
 
 constexpr int kThreads = 1024, kWarps = kThreads / 32;
 
-struct StepArgs {
+// Division by a number that stays the same, of numbers below 2^31: a multiplication by ceil(2^(31 + s) / d), s = ceil(log2 d), is off by less
+// than one part in 2^31 of the quotient's last place (Granlund and Montgomery 1994).
+struct Divisor {
+  uint32_t d, m;
+  int s;
+  __host__ explicit Divisor(int by) : d(uint32_t(by)), s(0)
+  {
+    while ((uint64_t(1) << s) < d) ++s;
+    m = uint32_t(((uint64_t(1) << (31 + s)) + d - 1) / d);
+  }
+  __device__ __forceinline__ uint32_t of(uint32_t x) const { return uint32_t((uint64_t(x) * m) >> (31 + s)); }
+};
+
+struct Requests {
   const int32_t *old_lengths, *new_lengths;
   int64_t n;
-  int block;
+  Divisor block;
+};
+
+struct StepArgs {
+  Requests q;
   int32_t* tables;
   int64_t columns, stride;
   int32_t* queue;
@@ -26,16 +43,16 @@ struct StepArgs {
 // Blocks that a request holds before the step and after it; none of either where it is no request.
 struct Blocks {
   uint32_t have = 0, need = 0;
-  __device__ Blocks(const StepArgs& a, int64_t r)
+  __device__ __forceinline__ Blocks(const Requests& q, int64_t r)
   {
-    if (r >= a.n) return;
-    const int32_t before = __ldg(a.old_lengths + r), after = __ldg(a.new_lengths + r);
+    if (r >= q.n) return;
+    const int32_t before = __ldg(q.old_lengths + r), after = __ldg(q.new_lengths + r);
     if (before < 0 || after < 0) return;
-    have = (uint32_t(before) + uint32_t(a.block) - 1u) / uint32_t(a.block);
-    need = (uint32_t(after) + uint32_t(a.block) - 1u) / uint32_t(a.block);
+    have = before ? q.block.of(uint32_t(before) - 1u) + 1u : 0u;
+    need = after ? q.block.of(uint32_t(after) - 1u) + 1u : 0u;
   }
-  __device__ uint32_t taken() const { return need > have ? need - have : 0u; }
-  __device__ uint32_t given() const { return have > need ? have - need : 0u; }
+  __device__ __forceinline__ uint32_t taken() const { return need > have ? need - have : 0u; }
+  __device__ __forceinline__ uint32_t given() const { return have > need ? have - need : 0u; }
 };
 
 __device__ __forceinline__ int64_t warp_sum(int64_t x)
@@ -44,70 +61,142 @@ __device__ __forceinline__ int64_t warp_sum(int64_t x)
   for (int d = 16; d; d >>= 1) x += __shfl_xor_sync(0xFFFFFFFFu, x, d);
   return x;
 }
-
-__global__ void __launch_bounds__(kThreads) k_block_tables(const StepArgs a)
+__device__ __forceinline__ int64_t warp_upto(int64_t x)
 {
-  __shared__ int64_t s_taken[kWarps], s_given[kWarps];
-  __shared__ uint32_t s_have[kThreads], s_need[kThreads];
-  __shared__ int64_t s_from[kThreads];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int64_t head = a.state[0], tail = a.state[1];
-  int64_t taken = 0, given = 0;
-  bool beyond   = false;
-  for (int64_t r = tid; r < a.n; r += kThreads) {
-    const Blocks b(a, r);
-    taken += b.taken(), given += b.given();
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int d = 1; d < 32; d *= 2) {
+    const int64_t l = __shfl_up_sync(0xFFFFFFFFu, x, d);
+    if (lane >= d) x += l;
+  }
+  return x;
+}
+
+struct Pair {
+  int64_t a, b;
+};
+
+// Of two numbers per thread the sums up to the own ones, and of all; every thread of the CTA.
+__device__ __forceinline__ Pair block_upto(Pair x, Pair& all, Pair (&s_sum)[kWarps])
+{
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  x.a = warp_upto(x.a), x.b = warp_upto(x.b);
+  __syncthreads();
+  if (lane == 31) s_sum[warp] = x;
+  __syncthreads();
+  const Pair w = s_sum[lane];  // as many warps as lanes
+  all          = Pair{warp_sum(w.a), warp_sum(w.b)};
+  x.a += warp_sum(lane < warp ? w.a : 0), x.b += warp_sum(lane < warp ? w.b : 0);
+  return x;
+}
+static_assert(kWarps == 32, "");
+
+// Each CTA has the sums over all requests formed by itself (they are read from L2: 64 KiB for 8192 of them), and then moves the blocks of a share of
+// the requests, in tiles of a thread each; a warp moves those of one request after the other.  The state is written by the kernel behind this one, when all
+// have read it.
+struct StepStatus {
+  int64_t taken, given, status;
+};
+__device__ __forceinline__ StepStatus look_at_step(const StepArgs& a, int64_t begin, Pair& before, Pair (&s_sum)[kWarps])
+{
+  const int tid = threadIdx.x;
+  Pair front{0, 0}, rest{0, 0};  // of the requests in front of `begin`, and from there on
+  bool beyond = false;
+#pragma unroll 4
+  for (int64_t r = tid; r < a.q.n; r += kThreads) {
+    const Blocks b(a.q, r);
+    Pair& to = r < begin ? front : rest;
+    to.a += b.taken(), to.b += b.given();
     beyond |= int64_t(max(b.have, b.need)) > a.columns;
   }
-  taken = warp_sum(taken), given = warp_sum(given);
-  if (lane == 0) s_taken[warp] = taken, s_given[warp] = given;
   beyond = __syncthreads_or(beyond);
-  taken  = warp_sum(s_taken[lane]);
-  given  = warp_sum(s_given[lane]);
-  __syncthreads();
-  const int64_t waiting = tail - head;
-  int64_t status        = 0;
-  if (beyond) status = -1;
-  else if (head < 0 || waiting < 0 || waiting + given > a.capacity) status = -2;
-  else if (taken > waiting) status = taken - waiting;
-  if (tid == 0) {
-    a.state_out[0] = status ? head : head + taken;
-    a.state_out[1] = status ? tail : tail + given;
-    a.state_out[2] = status;
+  Pair all;
+  block_upto(front, before, s_sum);
+  block_upto(rest, all, s_sum);
+  StepStatus s{before.a + all.a, before.b + all.b, 0};
+  const int64_t head = a.state[0], tail = a.state[1], waiting = tail - head;
+  if (beyond) s.status = -1;
+  else if (head < 0 || waiting < 0 || waiting + s.given > a.capacity) s.status = -2;
+  else if (s.taken > waiting) s.status = s.taken - waiting;
+  return s;
+}
+
+__device__ __forceinline__ void put_state(const StepArgs& a, const StepStatus& s)
+{
+  const int64_t head = a.state[0], tail = a.state[1];
+  a.state_out[0] = s.status ? head : head + s.taken;
+  a.state_out[1] = s.status ? tail : tail + s.given;
+  a.state_out[2] = s.status;
+}
+
+template <bool ALONE>
+__global__ void __launch_bounds__(kThreads) k_block_tables(const StepArgs a, int64_t share)
+{
+  __shared__ Pair s_sum[kWarps];
+  __shared__ uint32_t s_have[kThreads], s_need[kThreads], s_from[kThreads];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int64_t begin = min(a.q.n, blockIdx.x * share), end = min(a.q.n, begin + share);
+  Pair before;
+  const StepStatus s = look_at_step(a, begin, before, s_sum);
+  const int64_t head = a.state[0], tail = a.state[1];
+  if constexpr (ALONE) {
+    __syncthreads();  // all have read the state
+    if (tid == 0) put_state(a, s);
   }
-  if (status) return;
-  int64_t took = 0, gave = 0;  // by the requests in front of the tile
-  for (int64_t first = 0; first < a.n; first += kThreads) {
-    const Blocks b(a, first + tid);
-    int64_t t = b.taken(), g = b.given();
-#pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-      const int64_t tl = __shfl_up_sync(0xFFFFFFFFu, t, d), gl = __shfl_up_sync(0xFFFFFFFFu, g, d);
-      if (lane >= d) t += tl, g += gl;
-    }
-    if (lane == 31) s_taken[warp] = t, s_given[warp] = g;
+  if (s.status) return;
+  const uint32_t capacity = uint32_t(a.capacity), at_head = uint32_t(head % a.capacity), at_tail = uint32_t(tail % a.capacity);
+  // places in the ring; a step moves no more blocks than it has
+  auto place = [&](uint32_t from, uint32_t i) {
+    const uint32_t p = from + i;  // both below 2^31
+    return p >= capacity ? p - capacity : p;
+  };
+  for (int64_t first = begin; first < end; first += kThreads) {
+    Blocks b(a.q, first + tid);
+    if (first + tid >= end) b.have = b.need = 0;
+    Pair all;
+    const Pair upto = block_upto(Pair{int64_t(b.taken()), int64_t(b.given())}, all, s_sum);
     s_have[tid] = b.have, s_need[tid] = b.need;
+    s_from[tid] = b.need > b.have ? place(at_head, uint32_t(before.a + upto.a - b.taken())) : place(at_tail, uint32_t(before.b + upto.b - b.given()));
+    before.a += all.a, before.b += all.b;
     __syncthreads();
-    const int64_t taken_before = warp_sum(lane < warp ? s_taken[lane] : 0), given_before = warp_sum(lane < warp ? s_given[lane] : 0);
-    s_from[tid] = b.need > b.have ? head + took + taken_before + t - b.taken() : tail + gave + given_before + g - b.given();
-    took += warp_sum(s_taken[lane]), gave += warp_sum(s_given[lane]);
-    __syncthreads();
-    const int rows = int(min(int64_t(kThreads), a.n - first));
-    for (int r = warp; r < rows; r += kWarps) {
-      const uint32_t have = s_have[r], need = s_need[r];
-      const int64_t at = s_from[r];
-      int32_t* row     = a.tables + (first + r) * a.stride;
-      for (uint32_t i = have + lane; i < need; i += 32) row[i] = a.queue[(at + (i - have)) % a.capacity];
-      for (uint32_t i = need + lane; i < have; i += 32) a.queue[(at + (i - need)) % a.capacity] = row[i];
+    const int rows = int(min(int64_t(kThreads), end - first));
+    // a warp's requests lie kWarps apart: lane l knows of the l-th of them
+    const int own     = warp + lane * kWarps;
+    uint32_t some     = __ballot_sync(0xFFFFFFFFu, own < rows && s_have[own] != s_need[own]);
+    static_assert(kThreads == 32 * kWarps, "");
+    while (some) {
+      const int r = warp + (__ffs(some) - 1) * kWarps;
+      some &= some - 1;
+      const uint32_t have = s_have[r], need = s_need[r], from = s_from[r];
+      int32_t* row = a.tables + (first + r) * a.stride;
+#pragma unroll 4
+      for (uint32_t i = have + lane; i < need; i += 32) {
+        const uint32_t p = place(from, i - have);
+        if (GTK_IN(p, capacity, 400) && GTK_IN(i, a.columns, 401)) row[i] = __ldcg(a.queue + p);
+      }
+#pragma unroll 4
+      for (uint32_t i = need + lane; i < have; i += 32) {
+        const uint32_t p = place(from, i - need);
+        if (GTK_IN(p, capacity, 402) && GTK_IN(i, a.columns, 403)) a.queue[p] = row[i];
+      }
     }
     __syncthreads();
   }
 }
 
+// What k_block_tables<false> has found, again, when all of its CTAs are through.
+__global__ void __launch_bounds__(kThreads) k_block_state(const StepArgs a)
+{
+  __shared__ Pair s_sum[kWarps];
+  Pair before;
+  const StepStatus s = look_at_step(a, 0, before, s_sum);
+  gtk::await_kernel();
+  __syncthreads();
+  if (threadIdx.x == 0) put_state(a, s);
+}
+
 struct SlotArgs {
-  const int32_t *old_lengths, *new_lengths;
-  int64_t n;
-  int block;
+  Requests q;
   const int32_t* tables;
   int64_t columns, stride;
   const int64_t* state;
@@ -119,58 +208,120 @@ struct SlotArgs {
 
 __device__ __forceinline__ int64_t new_tokens(const SlotArgs& a, int64_t r)
 {
-  if (r >= a.n) return 0;
-  const int32_t before = __ldg(a.old_lengths + r), after = __ldg(a.new_lengths + r);
+  const int32_t before = __ldg(a.q.old_lengths + r), after = __ldg(a.q.new_lengths + r);
   return before >= 0 && after > before ? int64_t(after) - before : 0;
 }
 
+// The tokens [begin, end) of the step, which offset_at(request) tells the owners of, by all threads; a warp takes neighbouring ones, and looks for a request
+// among all only where it is not the one of the token 32 places before.
+template <class OffsetAt>
+__device__ __forceinline__ void put_slots(const SlotArgs& a, int64_t begin, int64_t end, int64_t n, OffsetAt&& offset_at)
+{
+  constexpr int kOnce = 4;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int64_t total = offset_at(n), each = ((end - begin + kWarps - 1) / kWarps + 31) / 32 * 32;
+  // the last request from lo on that begins at i or before, for i < total
+  auto owner = [&](int64_t lo, int64_t i) {
+    int64_t hi = n;
+    while (hi - lo > 1) {
+      const int64_t mid = (lo + hi) / 2;
+      if (offset_at(mid) <= i) lo = mid;
+      else hi = mid;
+    }
+    return lo;
+  };
+  const int64_t from = begin + warp * each, to = min(end, from + each);
+  int64_t lo = from < to && from < total ? owner(0, from) : 0, next = n > 0 ? offset_at(lo + 1) : 0;
+  for (int64_t i0 = from; i0 < to; i0 += 32 * kOnce) {
+    int32_t position[kOnce], request[kOnce], entry[kOnce];
+#pragma unroll
+    for (int e = 0; e < kOnce; ++e) {
+      const int64_t i = i0 + e * 32 + lane;
+      position[e] = request[e] = entry[e] = -1;
+      if (i < to && i < total) {
+        if (i >= next) lo = owner(lo, i), next = offset_at(lo + 1);
+        request[e]  = int32_t(lo);
+        position[e] = __ldg(a.q.old_lengths + lo) + int32_t(i - offset_at(lo));
+        const uint32_t column = a.q.block.of(uint32_t(position[e]));
+        if (int64_t(column) < a.columns) entry[e] = __ldg(a.tables + lo * a.stride + column);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < kOnce; ++e) {
+      const int64_t i = i0 + e * 32 + lane;
+      if (i >= to) break;
+      const uint32_t in_block = uint32_t(position[e]) - a.q.block.of(uint32_t(position[e])) * a.q.block.d;
+      a.slots[i] = entry[e] >= 0 ? int64_t(entry[e]) * a.q.block.d + in_block : -1;
+      if (a.positions) a.positions[i] = position[e];
+      if (a.requests) a.requests[i] = request[e];
+    }
+  }
+}
+
+// Few requests: each CTA adds up all of them, in shared memory, and puts a share of the tokens; the first one puts the offsets too.
+constexpr int kFewRequests = 4096, kEachRequest = kFewRequests / kThreads;
+__global__ void __launch_bounds__(kThreads) k_slots_of_few(const SlotArgs a, int64_t share)
+{
+  __shared__ int64_t s_offset[kFewRequests + 1];
+  __shared__ Pair s_sum[kWarps];
+  const int tid = threadIdx.x;
+  const bool not_done = a.state && __ldg(a.state + 2) != 0;
+  // neighbouring requests to a thread
+  const int each = int((a.q.n + kThreads - 1) / kThreads), first = tid * each;
+  int64_t more[kEachRequest], mine = 0;
+#pragma unroll
+  for (int e = 0; e < kEachRequest; ++e) {
+    more[e] = e < each && first + e < a.q.n && !not_done ? new_tokens(a, first + e) : 0;
+    mine += more[e];
+  }
+  Pair all;
+  int64_t upto = block_upto(Pair{mine, 0}, all, s_sum).a - mine;
+  if (tid == 0) s_offset[0] = 0;
+#pragma unroll
+  for (int e = 0; e < kEachRequest; ++e) {
+    upto += more[e];
+    if (e < each && first + e < a.q.n && GTK_IN(first + e + 1, kFewRequests + 1, 404)) s_offset[first + e + 1] = upto;
+  }
+  __syncthreads();
+  if (blockIdx.x == 0)
+    for (int r = tid; r <= a.q.n; r += kThreads) a.offsets[r] = s_offset[r];
+  const int64_t begin = blockIdx.x * share;
+  put_slots(a, begin, min(a.capacity, begin + share), a.q.n, [&](int64_t r) { return s_offset[r]; });
+}
+
+// Many requests: offsets first, then the tokens.
 __global__ void __launch_bounds__(kThreads) k_slot_offsets(const SlotArgs a)
 {
-  __shared__ int64_t s_sum[kWarps];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const bool done = a.state && a.state[2] != 0;
-  int64_t before  = 0;
+  __shared__ Pair s_sum[kWarps];
+  constexpr int kEach = 8;
+  const int tid  = threadIdx.x;
+  const bool not_done = a.state && __ldg(a.state + 2) != 0;
+  int64_t before = 0;
   if (tid == 0) a.offsets[0] = 0;
-  for (int64_t first = 0; first < a.n; first += kThreads) {
-    int64_t t = done ? 0 : new_tokens(a, first + tid);
+  for (int64_t tile = 0; tile < a.q.n; tile += kThreads * kEach) {
+    const int64_t first = tile + tid * kEach;
+    int64_t more[kEach], mine = 0;
 #pragma unroll
-    for (int d = 1; d < 32; d *= 2) {
-      const int64_t l = __shfl_up_sync(0xFFFFFFFFu, t, d);
-      if (lane >= d) t += l;
+    for (int e = 0; e < kEach; ++e) {
+      more[e] = first + e < a.q.n && !not_done ? new_tokens(a, first + e) : 0;
+      mine += more[e];
     }
-    if (lane == 31) s_sum[warp] = t;
-    __syncthreads();
-    const int64_t front = warp_sum(lane < warp ? s_sum[lane] : 0);
-    if (first + tid < a.n) a.offsets[first + tid + 1] = before + front + t;
-    before += warp_sum(s_sum[lane]);
-    __syncthreads();
+    Pair all;
+    int64_t upto = before + block_upto(Pair{mine, 0}, all, s_sum).a - mine;
+#pragma unroll
+    for (int e = 0; e < kEach; ++e)
+      if (first + e < a.q.n) a.offsets[first + e + 1] = upto += more[e];
+    before += all.a;
   }
 }
-
-__global__ void __launch_bounds__(256) k_slots(const SlotArgs a)
+__global__ void __launch_bounds__(kThreads) k_slots_of_many(const SlotArgs a, int64_t share)
 {
-  for (int64_t i = blockIdx.x * int64_t(blockDim.x) + threadIdx.x; i < a.capacity; i += int64_t(gridDim.x) * blockDim.x) {
-    int64_t slot = -1;
-    int32_t position = -1, request = -1;
-    if (i < a.offsets[a.n]) {
-      int64_t lo = 0, hi = a.n;  // offsets[lo] <= i < offsets[hi]
-      while (hi - lo > 1) {
-        const int64_t mid = (lo + hi) / 2;
-        if (a.offsets[mid] <= i) lo = mid;
-        else hi = mid;
-      }
-      request  = int32_t(lo);
-      position = __ldg(a.old_lengths + lo) + int32_t(i - a.offsets[lo]);
-      const int column = position / a.block;
-      const int32_t b  = column < a.columns ? a.tables[lo * a.stride + column] : -1;
-      if (b >= 0) slot = int64_t(b) * a.block + position % a.block;
-    }
-    a.slots[i] = slot;
-    if (a.positions) a.positions[i] = position;
-    if (a.requests) a.requests[i] = request;
-  }
+  gtk::await_kernel();
+  const int64_t begin = blockIdx.x * share;
+  put_slots(a, begin, min(a.capacity, begin + share), a.q.n, [&](int64_t r) { return __ldcg(a.offsets + r); });
 }
 
+constexpr int64_t kAlone = 1024, kShare = 32;  // requests of a CTA that is the only one, at most, and of one of several, at least
 constexpr int64_t kMost = (int64_t(1) << 31) - 1;
 
 gtk::Refusal refuse_step(const void* before, const void* after, int64_t n, int block, const void* tables, int64_t columns, int64_t stride)
@@ -199,8 +350,12 @@ extern "C" GTK_API int gtk_block_tables(gtk_tokenizer* h, const int32_t* d_old_l
     return nullptr;
   };
   return gtk::run_operator(h, check, [&](const gtk::HandleView& v) -> cudaError_t {
-    const StepArgs a{d_old_lengths, d_new_lengths, n_requests, block_tokens, d_tables, columns, table_stride, d_queue, queue_capacity, d_state, d_state_out};
-    return gtk::launch(k_block_tables, dim3(1), dim3(kThreads), 0, v.stream, a);
+    const StepArgs a{{d_old_lengths, d_new_lengths, n_requests, Divisor(block_tokens)}, d_tables, columns, table_stride, d_queue, queue_capacity, d_state, d_state_out};
+    const int64_t ctas = n_requests > kAlone ? std::min<int64_t>((n_requests + kShare - 1) / kShare, v.sm_count) : 1;
+    if (ctas == 1) return gtk::launch(k_block_tables<true>, dim3(1), dim3(kThreads), 0, v.stream, a, n_requests);
+    const int64_t share = (n_requests + ctas - 1) / ctas;
+    const cudaError_t e = gtk::launch(k_block_tables<false>, dim3(unsigned(ctas)), dim3(kThreads), 0, v.stream, a, share);
+    return e != cudaSuccess ? e : gtk::launch_behind(k_block_state, dim3(1), dim3(kThreads), 0, v.stream, a);
   });
 }
 
@@ -218,11 +373,15 @@ extern "C" GTK_API int gtk_slot_map(gtk_tokenizer* h, const int32_t* d_old_lengt
     return nullptr;
   };
   return gtk::run_operator(h, check, [&](const gtk::HandleView& v) -> cudaError_t {
-    const SlotArgs a{d_old_lengths, d_new_lengths, n_requests, block_tokens, d_tables, columns, table_stride, d_state, capacity,
+    const SlotArgs a{{d_old_lengths, d_new_lengths, n_requests, Divisor(block_tokens)}, d_tables, columns, table_stride, d_state, capacity,
                      d_slots, d_positions, d_requests, d_offsets};
-    cudaError_t e = gtk::launch(k_slot_offsets, dim3(1), dim3(kThreads), 0, v.stream, a);
-    if (e != cudaSuccess || capacity == 0) return e;
-    return gtk::launch(k_slots, dim3(unsigned(std::min<int64_t>((capacity + 255) / 256, int64_t(v.sm_count) * 8))), dim3(256), 0, v.stream, a);
+    const bool few = n_requests <= kFewRequests;
+    if (!few)
+      if (const cudaError_t e = gtk::launch(k_slot_offsets, dim3(1), dim3(kThreads), 0, v.stream, a); e != cudaSuccess) return e;
+    const int64_t ctas  = std::max<int64_t>(1, std::min<int64_t>((capacity + kThreads - 1) / kThreads, int64_t(v.sm_count)));
+    const int64_t share = (capacity + ctas - 1) / ctas;
+    return few ? gtk::launch(k_slots_of_few, dim3(unsigned(ctas)), dim3(kThreads), 0, v.stream, a, share)
+               : gtk::launch_behind(k_slots_of_many, dim3(unsigned(ctas)), dim3(kThreads), 0, v.stream, a, share);
   });
 }
 

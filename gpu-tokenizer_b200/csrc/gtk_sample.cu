@@ -297,14 +297,17 @@ __device__ __forceinline__ Sum sum_row(const Row<T>& row, double* section, Scrat
   const int threads = blockDim.x, warps = threads >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   Sum s{0.0, 0};
   __syncthreads();
+  uint4 raw[kPacks];
+  if (warp < row.sections) row.load_section(warp, raw);
   for (int i = warp; i < row.sections; i += warps) {
+    uint4 next[kPacks];
+    if (i + warps < row.sections) row.load_section(i + warps, next);
     double sum = 0.0;
 #pragma unroll 1
-    for (int q = 0; q < kPacks; ++q) {
-      const int p     = (i * kPacks + q) * 32 + lane;
-      const uint4 raw = row.load(p);
+    for (int q = 0; q < kPacks; ++q) {  // one after the other: the code is run few times, and has to come in first
+      const int p = (i * kPacks + q) * 32 + lane;
       float all[Row<T>::E];
-      unpack<T>(raw, all);
+      unpack<T>(raw[0], all);
 #pragma unroll
       for (int j = 0; j < Row<T>::E; j += 4) {
         const float x[4] = {all[j], all[j + 1], all[j + 2], all[j + 3]};
@@ -312,7 +315,11 @@ __device__ __forceinline__ Sum sum_row(const Row<T>& row, double* section, Scrat
         weigh(x, row.column(p) + j, w, s.count);
         sum += sum_of(w);
       }
+#pragma unroll
+      for (int e = 1; e < kPacks; ++e) raw[e - 1] = raw[e];
     }
+#pragma unroll
+    for (int e = 0; e < kPacks; ++e) raw[e] = next[e];
     sum = warp_sum(sum);
     if (lane == 0 && GTK_IN(i, row.sections, 500)) section[i] = sum;
     s.mass += sum;
@@ -641,7 +648,7 @@ struct Team {
   {
     const int warps = blockDim.x >> 5;
     for (int s = begin + int(threadIdx.x >> 5); s < end; s += warps) {
-      uint4 raw[kPacks];
+      uint4 raw[kPacks];  // the next section's too do not fit into the registers (64 rows of 131072 f32: 116 us, as it is 75)
       row.load_section(s, raw);
       f(s, [&](auto&& g) {
 #pragma unroll 1
