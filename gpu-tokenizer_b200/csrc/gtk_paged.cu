@@ -212,14 +212,14 @@ __device__ __forceinline__ int64_t new_tokens(const SlotArgs& a, int64_t r)
   return before >= 0 && after > before ? int64_t(after) - before : 0;
 }
 
-// The tokens [begin, end) of the step, which offset_at(request) tells the owners of, by all threads; a warp takes neighbouring ones, and looks for a request
+// The tokens [begin, end) of the step, those below `total` of requests [first, n), which offset_at(request) tells the owners of, by all threads; a warp takes neighbouring ones, and looks for a request
 // among all only where it is not the one of the token 32 places before.
 template <class OffsetAt>
-__device__ __forceinline__ void put_slots(const SlotArgs& a, int64_t begin, int64_t end, int64_t n, OffsetAt&& offset_at)
+__device__ __forceinline__ void put_slots(const SlotArgs& a, int64_t begin, int64_t end, int64_t first, int64_t n, int64_t total, OffsetAt&& offset_at)
 {
   constexpr int kOnce = 4;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int64_t total = offset_at(n), each = ((end - begin + kWarps - 1) / kWarps + 31) / 32 * 32;
+  const int64_t each = ((end - begin + kWarps - 1) / kWarps + 31) / 32 * 32;
   // the last request from lo on that begins at i or before, for i < total
   auto owner = [&](int64_t lo, int64_t i) {
     int64_t hi = n;
@@ -231,7 +231,7 @@ __device__ __forceinline__ void put_slots(const SlotArgs& a, int64_t begin, int6
     return lo;
   };
   const int64_t from = begin + warp * each, to = min(end, from + each);
-  int64_t lo = from < to && from < total ? owner(0, from) : 0, next = n > 0 ? offset_at(lo + 1) : 0;
+  int64_t lo = from < to && from < total ? owner(first, from) : first, next = from < to && from < total ? offset_at(lo + 1) : 0;
   for (int64_t i0 = from; i0 < to; i0 += 32 * kOnce) {
     int32_t position[kOnce], request[kOnce], entry[kOnce];
 #pragma unroll
@@ -258,35 +258,41 @@ __device__ __forceinline__ void put_slots(const SlotArgs& a, int64_t begin, int6
   }
 }
 
-// Few requests: each CTA adds up all of them, in shared memory, and puts a share of the tokens; the first one puts the offsets too.
-constexpr int kFewRequests = 4096, kEachRequest = kFewRequests / kThreads;
+// Up to kFewRequests: each CTA adds up all of them, in shared memory, and puts a share of the tokens; the first one puts the offsets too.  What
+// begins at 2^31 or later is behind every token that has a place.
+constexpr int kFewRequests = 8192;
+template <int EACH>  // neighbouring requests to a thread
 __global__ void __launch_bounds__(kThreads) k_slots_of_few(const SlotArgs a, int64_t share)
 {
-  __shared__ int64_t s_offset[kFewRequests + 1];
+  constexpr int kMine = EACH * kThreads;  // requests at most
+  __shared__ uint32_t s_offset[kMine + 1];
   __shared__ Pair s_sum[kWarps];
   const int tid = threadIdx.x;
   const bool not_done = a.state && __ldg(a.state + 2) != 0;
-  // neighbouring requests to a thread
-  const int each = int((a.q.n + kThreads - 1) / kThreads), first = tid * each;
-  int64_t more[kEachRequest], mine = 0;
+  const int first     = tid * EACH;
+  int64_t more[EACH], mine = 0;
 #pragma unroll
-  for (int e = 0; e < kEachRequest; ++e) {
-    more[e] = e < each && first + e < a.q.n && !not_done ? new_tokens(a, first + e) : 0;
+  for (int e = 0; e < EACH; ++e) {
+    more[e] = first + e < a.q.n && !not_done ? new_tokens(a, first + e) : 0;
     mine += more[e];
   }
   Pair all;
   int64_t upto = block_upto(Pair{mine, 0}, all, s_sum).a - mine;
-  if (tid == 0) s_offset[0] = 0;
+  if (tid == 0) {
+    s_offset[0] = 0;
+    if (blockIdx.x == 0) a.offsets[0] = 0;
+  }
 #pragma unroll
-  for (int e = 0; e < kEachRequest; ++e) {
+  for (int e = 0; e < EACH; ++e) {
     upto += more[e];
-    if (e < each && first + e < a.q.n && GTK_IN(first + e + 1, kFewRequests + 1, 404)) s_offset[first + e + 1] = upto;
+    if (first + e < a.q.n && GTK_IN(first + e + 1, kMine + 1, 404)) {
+      s_offset[first + e + 1] = uint32_t(min(upto, int64_t(1) << 31));
+      if (blockIdx.x == 0) a.offsets[first + e + 1] = upto;
+    }
   }
   __syncthreads();
-  if (blockIdx.x == 0)
-    for (int r = tid; r <= a.q.n; r += kThreads) a.offsets[r] = s_offset[r];
   const int64_t begin = blockIdx.x * share;
-  put_slots(a, begin, min(a.capacity, begin + share), a.q.n, [&](int64_t r) { return s_offset[r]; });
+  put_slots(a, begin, min(a.capacity, begin + share), 0, a.q.n, all.a, [&](int64_t r) { return int64_t(s_offset[r]); });
 }
 
 // Many requests: offsets first, then the tokens.
@@ -316,12 +322,30 @@ __global__ void __launch_bounds__(kThreads) k_slot_offsets(const SlotArgs a)
 }
 __global__ void __launch_bounds__(kThreads) k_slots_of_many(const SlotArgs a, int64_t share)
 {
+  __shared__ int64_t s_offset[kFewRequests / 2 + 1];
   gtk::await_kernel();
-  const int64_t begin = blockIdx.x * share;
-  put_slots(a, begin, min(a.capacity, begin + share), a.q.n, [&](int64_t r) { return __ldcg(a.offsets + r); });
+  const int64_t begin = blockIdx.x * share, end = min(a.capacity, begin + share), total = __ldcg(a.offsets + a.q.n);
+  auto owner = [&](int64_t i) {
+    int64_t lo = 0, hi = a.q.n;
+    while (hi - lo > 1) {
+      const int64_t mid = (lo + hi) / 2;
+      if (__ldcg(a.offsets + mid) <= i) lo = mid;
+      else hi = mid;
+    }
+    return lo;
+  };
+  // the requests of these tokens, in shared memory where they are few enough
+  const int64_t first = begin < total ? owner(begin) : 0, last = begin < total ? owner(min(end, total) - 1) : 0;
+  if (last - first + 1 <= kFewRequests / 2) {
+    for (int64_t r = first + threadIdx.x; r <= last + 1; r += kThreads) s_offset[r - first] = __ldcg(a.offsets + r);
+    __syncthreads();
+    put_slots(a, begin, end, first, last + 1, total, [&](int64_t r) { return s_offset[r - first]; });
+  } else {
+    put_slots(a, begin, end, first, last + 1, total, [&](int64_t r) { return __ldcg(a.offsets + r); });
+  }
 }
 
-constexpr int64_t kAlone = 1024, kShare = 32;  // requests of a CTA that is the only one, at most, and of one of several, at least
+constexpr int64_t kAlone = 512, kShare = 32;  // requests of a CTA that is the only one, at most, and of one of several, at least
 constexpr int64_t kMost = (int64_t(1) << 31) - 1;
 
 gtk::Refusal refuse_step(const void* before, const void* after, int64_t n, int block, const void* tables, int64_t columns, int64_t stride)
@@ -380,7 +404,8 @@ extern "C" GTK_API int gtk_slot_map(gtk_tokenizer* h, const int32_t* d_old_lengt
       if (const cudaError_t e = gtk::launch(k_slot_offsets, dim3(1), dim3(kThreads), 0, v.stream, a); e != cudaSuccess) return e;
     const int64_t ctas  = std::max<int64_t>(1, std::min<int64_t>((capacity + kThreads - 1) / kThreads, int64_t(v.sm_count)));
     const int64_t share = (capacity + ctas - 1) / ctas;
-    return few ? gtk::launch(k_slots_of_few, dim3(unsigned(ctas)), dim3(kThreads), 0, v.stream, a, share)
+    const auto of_few = n_requests <= kThreads ? k_slots_of_few<1> : n_requests <= 4 * kThreads ? k_slots_of_few<4> : k_slots_of_few<kFewRequests / kThreads>;
+    return few ? gtk::launch(of_few, dim3(unsigned(ctas)), dim3(kThreads), 0, v.stream, a, share)
                : gtk::launch_behind(k_slots_of_many, dim3(unsigned(ctas)), dim3(kThreads), 0, v.stream, a, share);
   });
 }
