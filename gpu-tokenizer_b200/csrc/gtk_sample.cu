@@ -461,8 +461,8 @@ struct Slowly {
   __device__ void search(uint32_t most, Enough&& enough, Wanted&& wanted)
   {
     uint32_t lo = 1, hi = most;  // enough at lo
-    while (lo < hi) {
-      const uint32_t mid = lo + (hi - lo + 1) / 2;
+    for (bool first = true; lo < hi; first = false) {
+      const uint32_t mid = first ? most : lo + (hi - lo + 1) / 2;  // rows of equal logits end with the first
       const Sum s = sum_columns(row, section, S, [&](float x, int c) { return value_key(x) >= mid && left(x, c) ? Sum{weight(x), 1} : Sum{0.0, 0}; });
       if (enough(s)) lo = mid;
       else hi = mid - 1;
@@ -1228,10 +1228,11 @@ __device__ __noinline__ int draw_limited(const Row<T>& row, const Limits& l, con
   for (int s = team.begin + tid; s < team.end; s += threads) sum += of_section(piece[s], c_top);
   sum = warp_sum(sum);
   if (lane == 0) S.mass[warp] = sum;
+  const bool only = l.k == 1;  // the highest alone
 #pragma unroll
   for (int q = 0; q < kPacks; ++q) {
     const float v = best.value(q);
-    if (v > -INFINITY) {
+    if (v > -INFINITY && !only) {
       const int at = int(fminf((top - v) * scale, float(kBins - 1)));
       if (GTK_IN(at, kBins, 504)) atomicAdd(&S.hist[at], 1);
     }
@@ -1265,8 +1266,8 @@ __device__ __noinline__ int draw_limited(const Row<T>& row, const Limits& l, con
     error = 0x1p-24 * double(row.exponent_error(sum) + Row<T>::kWeightError + Row<T>::kSumError + 0.1f);
     sum *= exp2(double(c_top) - double(top) * double(k));  // relative to the highest's
   }
-  int reach = kBins;
-  {
+  int reach = only ? 0 : kBins;
+  if (!only) {
     constexpr int kEach = kBins / 32;
     int counts[kEach], count = 0;
 #pragma unroll
@@ -1299,7 +1300,7 @@ __device__ __noinline__ int draw_limited(const Row<T>& row, const Limits& l, con
     some = warp_sum(n) <= kMostKeys / 4;
   }
   if (some) {
-    auto reaches        = [&](float x) { return everything || (top - x) * scale < bound; };
+    auto reaches        = [&](float x) { return only ? x == top : everything || (top - x) * scale < bound; };
     uint8_t* const set  = S.set + warp * kSetsOfWarp;
     static_assert(kSetsOfWarp <= 256, "");
     int sets = 0;

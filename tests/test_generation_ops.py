@@ -341,6 +341,22 @@ def test_equal_logits_are_drawn_in_even_parts(tok, name, vocab):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("name", TYPES)
+def test_more_equal_logits_than_can_be_ranked(tok, name):
+    """Limits that fall among a thousand and more equal logits: at the top, and below others."""
+    import torch
+
+    x = some_logits(4, 4, 9001, "plain").clamp_(max=0.0).to(dtype(name))   # half of them are zero
+    x[1, 77] = x[1, 5000] = 3.0
+    x[2] = -7.0
+    x[2, ::2] = -math.inf
+    x[3, 4000:] = 1.0
+    for t, k, p, m in ((1.0, 0, 0.0, 0.0), (1.0, 0, 0.3, 0.0), (1.0, 2000, 1.0, 0.0), (0.7, 2000, 0.4, 0.0), (0.9, 0, 0.99, 0.3), (1.0, 1, 1.0, 0.0)):
+        limits = Limits(3, 4, temperature=t, top_k=k, top_p=p, min_p=m)
+        check_draws(x, limits, *draw(tok, x, name, limits))
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("which", ["none", "k and p", "p", "nearly all", "min", "many k"])
 @pytest.mark.parametrize("name", TYPES)
 def test_every_column_is_drawn_as_often_as_it_should_be(tok, name, which):
