@@ -1198,6 +1198,47 @@ __device__ __noinline__ int draw_of_all(const Row<T>& row, const Limits& l, cons
   return S.solved ? draw_exactly(row, l, top, section, S, logprob) : draw_slowly(row, l, section, S, logprob);
 }
 
+// A row of which the highest alone is left, of equal ones the lowest column: the answer is its first thread's.
+template <class T, bool SPLIT>
+__device__ __noinline__ int draw_highest(const Row<T>& row, const Limits& l, const Team<SPLIT>& team, const Best<T>& best, float top, double* section,
+                                         Scratch& S, float& logprob)
+{
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+  if (threadIdx.x == 0) S.column = INT_MAX;
+  top = highest(team, S, top);
+  const float2* const piece = reinterpret_cast<const float2*>(section);
+  bool broken = !(fabsf(top) < 0x1p59f);
+  for (int s = team.begin + int(threadIdx.x); s < team.end; s += blockDim.x) broken |= !(piece[s].y < 1e30f);  // a NaN, or +inf
+  uint32_t column = INT_MAX;
+#pragma unroll
+  for (int q = 0; q < kPacks; ++q)
+    if (best.value(q) == top) {
+#pragma unroll 4
+      for (int s = team.begin + warp; s < team.end; s += warps) {
+        const int p     = (s * kPacks + q) * 32 + lane;
+        const uint4 raw = row.load(p);
+#pragma unroll
+        for (int j = Row<T>::E - 1; j >= 0; --j)
+          if (gtk::to_float(reinterpret_cast<const T*>(&raw)[j]) == top) column = min(column, uint32_t(row.column(p) + j));
+      }
+    }
+  column = __reduce_min_sync(0xFFFFFFFFu, column);
+  if (lane == 0 && column != INT_MAX) atomicMin(&S.column, int(column));
+  broken = __syncthreads_or(broken);
+  column = uint32_t(S.column);
+  if constexpr (SPLIT) {
+    if (threadIdx.x == 0) S.solved = broken;
+    team.sync();
+    column = __reduce_min_sync(0xFFFFFFFFu, lane < team.parts ? uint32_t(team.of(&S, lane)->column) : INT_MAX);
+    broken = __any_sync(0xFFFFFFFFu, lane < team.parts && team.of(&S, lane)->solved);
+    team.sync();  // nobody leaves while its shared memory is read
+    if (team.part != 0) return -1;
+  }
+  if (broken) return draw_slowly(row, l, section, S, logprob);
+  logprob = 0.f;
+  return int(column);
+}
+
 // A row with limits: the answer is its first thread's.
 template <class T, bool SPLIT>
 __device__ __noinline__ int draw_limited(const Row<T>& row, const Limits& l, const Team<SPLIT>& team, const Best<T>& best, float top, float k,
@@ -1228,11 +1269,10 @@ __device__ __noinline__ int draw_limited(const Row<T>& row, const Limits& l, con
   for (int s = team.begin + tid; s < team.end; s += threads) sum += of_section(piece[s], c_top);
   sum = warp_sum(sum);
   if (lane == 0) S.mass[warp] = sum;
-  const bool only = l.k == 1;  // the highest alone
 #pragma unroll
   for (int q = 0; q < kPacks; ++q) {
     const float v = best.value(q);
-    if (v > -INFINITY && !only) {
+    if (v > -INFINITY) {
       const int at = int(fminf((top - v) * scale, float(kBins - 1)));
       if (GTK_IN(at, kBins, 504)) atomicAdd(&S.hist[at], 1);
     }
@@ -1266,8 +1306,8 @@ __device__ __noinline__ int draw_limited(const Row<T>& row, const Limits& l, con
     error = 0x1p-24 * double(row.exponent_error(sum) + Row<T>::kWeightError + Row<T>::kSumError + 0.1f);
     sum *= exp2(double(c_top) - double(top) * double(k));  // relative to the highest's
   }
-  int reach = only ? 0 : kBins;
-  if (!only) {
+  int reach = kBins;
+  {
     constexpr int kEach = kBins / 32;
     int counts[kEach], count = 0;
 #pragma unroll
@@ -1300,7 +1340,7 @@ __device__ __noinline__ int draw_limited(const Row<T>& row, const Limits& l, con
     some = warp_sum(n) <= kMostKeys / 4;
   }
   if (some) {
-    auto reaches        = [&](float x) { return only ? x == top : everything || (top - x) * scale < bound; };
+    auto reaches        = [&](float x) { return everything || (top - x) * scale < bound; };
     uint8_t* const set  = S.set + warp * kSetsOfWarp;
     static_assert(kSetsOfWarp <= 256, "");
     int sets = 0;
@@ -1499,8 +1539,9 @@ __global__ void __launch_bounds__(kThreads, 4) k_sample(const T* __restrict__ lo
   }
   const Team<SPLIT> team{parts, part, share, begin, end};
   float logprob = 0.f;
-  const int id  = l.all() ? draw_of_all(row, l, team, top, k, ranged, s_section, S, logprob)
-                          : draw_limited(row, l, team, best, top, k, ranged, s_section, S, logprob);
+  const int id  = l.all()    ? draw_of_all(row, l, team, top, k, ranged, s_section, S, logprob)
+                  : l.k == 1 ? draw_highest(row, l, team, best, top, s_section, S, logprob)
+                             : draw_limited(row, l, team, best, top, k, ranged, s_section, S, logprob);
   put(id, logprob);
 }
 
