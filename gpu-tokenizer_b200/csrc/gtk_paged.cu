@@ -2,6 +2,10 @@
 //
 // With B tokens per block, a request of L tokens holds ceil(L / B) blocks, and its token j lies in slot
 // table[j / B] * B + j % B.  Blocks that nobody holds wait in a ring: taken at its head, given back at its tail.
+//
+// A step moves little: what it takes is launches, sums over all requests, and loads that wait for each other.  Measured: blocks of 256 requests 7 us,
+// of 8192 of which half are replaced 17 (205 by one CTA that moves all of them); slots of 256 tokens 3.9, of a million of 512 requests 10 (floor 2.6; 18
+// with a search for each token), of 8192 requests 17.
 #include <climits>
 
 #include "gtk_checked.cuh"
@@ -91,7 +95,7 @@ __device__ __forceinline__ Pair block_upto(Pair x, Pair& all, Pair (&s_sum)[kWar
 }
 static_assert(kWarps == 32, "");
 
-// Each CTA has the sums over all requests formed by itself (they are read from L2: 64 KiB for 8192 of them), and then moves the blocks of a share of
+// Each CTA forms the sums over all requests by itself (they are read from L2: 64 KiB for 8192 of them), and then moves the blocks of a share of
 // the requests, in tiles of a thread each; a warp moves those of one request after the other.  The state is written by the kernel behind this one, when all
 // have read it.
 struct StepStatus {
@@ -345,7 +349,9 @@ __global__ void __launch_bounds__(kThreads) k_slots_of_many(const SlotArgs a, in
   }
 }
 
-constexpr int64_t kAlone = 512, kShare = 32;  // requests of a CTA that is the only one, at most, and of one of several, at least
+// Requests of a CTA that is the only one, at most, and of one of several, at least.  Alone and with others, us: 512 requests that are replaced 13.0 and 11.4,
+// in a decoding step 8.4 and 10; 1024 of them 19.0 and 10.7, 12.5 and 10.5.
+constexpr int64_t kAlone = 512, kShare = 32;
 constexpr int64_t kMost = (int64_t(1) << 31) - 1;
 
 gtk::Refusal refuse_step(const void* before, const void* after, int64_t n, int block, const void* tables, int64_t columns, int64_t stride)

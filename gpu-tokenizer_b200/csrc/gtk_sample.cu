@@ -5,7 +5,15 @@
 // column, in the order of columns, at which the sum of the weights that are left exceeds u times the whole of it.
 //
 // A row is read once.  Its weights are summed in 32 bits, by sections of neighbouring columns, and every decision that hangs on such a
-// sum is held against a bound of its error (Row::error); where a border lies within the bound the row is summed again in 64 bits.
+// sum is held against a bound of its error (Row::exponent_error); where a border lies within the bound the row is summed again in 64 bits.
+//
+// The reading is bound by memory, what follows it by phases that wait for each other.  Measured against a copy (6.57 TB/s):
+//   1024 rows of 131072 bf16, no limits   52 us, 78 %, the reading alone 47; where a model is unsure of thousands of ids, some ten of them are looked
+//                                         at again, which takes one CTA 80 us each: 129
+//   2048 rows of 50257 f32                73 us, 86 %, with min-p 80, with the 50 highest 123
+//   512 rows of 50257 bf16, the highest   17 us
+//   one row of 50257 bf16                 5.9 us without limits, 14 with top-k and top-p
+//   64 rows of 131072 f32, wide nuclei    76 us: three readings, 120 instructions an element, 17 of them in 64 bits
 #include <cooperative_groups.h>
 
 #include <cfloat>
@@ -1550,16 +1558,19 @@ static_assert(sizeof(Scratch) + (GTK_MAX_SAMPLE_VOCAB / (32 * kPacks * 4) + 1) *
 // How many CTAs share a row, and how many threads they have.
 // In 1 / 2 / 4 / 8 parts of 256 threads, us: one row of 50257 bf16 without limits - / 9.8 / 8.9 / 8.4, 64 of 131072 f32 23.7 / 15.9 / 12.7 / 14, with
 // the 50 highest 42 / 25 / 19 / 22; 148 of 50257 bf16 9.8 / 9.8 / 13.1, with limits 16.7 / 16.9 / 27; 256 of f32 21.6 / 23.2 / 28.
+// A nucleus may be wide, and a wide row is bound by instructions: 256 rows of 50304 f32, a few of them wide, take 102 / 74 / 66, with none 27 / 25 / 36; 333
+// of 32003 fp16, all of them wide, 84 / 119 / 162.
 // Rows in numbers take 128 threads, so that more of them are under way while others are at their ends: of 256 / 128, 2048 rows of 50257 f32 80 / 73,
 // bf16 50 / 45, with min-p 73 / 63; 512 of bf16 24 / 28.
 struct Teams {
   int parts, threads;
 };
-Teams teams_for(int64_t rows, int64_t bytes, int sm_count)
+Teams teams_for(int64_t rows, int64_t bytes, bool nuclei, int sm_count)
 {
   Teams t{1, kThreads};
   const int64_t room = int64_t(sm_count) * (bytes >= (160 << 10) ? 2 : 1);
   while (t.parts < kMaxParts && rows * t.parts * 2 <= room && bytes / (t.parts * 2) >= (12 << 10)) t.parts *= 2;
+  if (nuclei && t.parts == 1 && bytes >= (160 << 10) && rows * 2 <= int64_t(sm_count) * 4) t.parts = 2;
   if (rows > int64_t(sm_count) * 8 && bytes <= (256 << 10)) t.threads = 128;
   return t;
 }
@@ -1567,7 +1578,7 @@ Teams teams_for(int64_t rows, int64_t bytes, int sm_count)
 template <class T>
 cudaError_t launch_sample(const gtk::HandleView& v, const void* logits, int64_t n_rows, const SampleArgs& a)
 {
-  const Teams t         = teams_for(n_rows, int64_t(a.vocab) * int64_t(sizeof(T)), v.sm_count);
+  const Teams t         = teams_for(n_rows, int64_t(a.vocab) * int64_t(sizeof(T)), a.top_p != nullptr, v.sm_count);
   const size_t sections = (size_t(a.vocab) + Row<T>::E + Row<T>::kColumns - 1) / Row<T>::kColumns;
   const auto kernel = t.parts > 1 ? k_sample<T, true> : k_sample<T, false>;
   return gtk::launch_clusters(kernel, dim3(unsigned(n_rows * t.parts)), dim3(unsigned(t.threads)),
