@@ -1062,10 +1062,12 @@ struct Best {
   }
 };
 
-__device__ __forceinline__ double of_section(const float2& v, float c_top)  // its sum, relative to 2^c_top
+// A section's sum, relative to 2^c_top.  A NaN stays one however far below the section's reference lies (a section that is masked but for it, or one that
+// a cold temperature leaves nothing of): a sum is NaN where, and only where, its section has a NaN or +inf, and rows are told broken by it.
+__device__ __forceinline__ double of_section(const float2& v, float c_top)
 {
   const int e = int(fmaxf(v.x - c_top, -1000.f));
-  return e > -1000 ? double(v.y) * __hiloint2double((e + 1023) << 20, 0) : 0.0;
+  return e > -1000 || isnan(v.y) ? double(v.y) * __hiloint2double((e + 1023) << 20, 0) : 0.0;
 }
 
 // locate() with the sums of the first reading, relative to 2^c_top: sections in 64 bits, within its section in 32.

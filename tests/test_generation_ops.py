@@ -415,6 +415,46 @@ def test_sample_at_the_ends(tok, name, vocab):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("t", [1.0, 0.02, 0.01])
+@pytest.mark.parametrize("n", [1, 9, 320, 1250])  # eight CTAs to a row or four, one of 256 threads, one of 128
+def test_sample_finds_a_nan_wherever_it_lies(tok, name, t, n):
+    """A NaN among columns that weigh nothing beside the rest: in sections that are masked otherwise, in front, within and at the end; in
+    sections of nothing but NaN; and among logits so far below the highest that a cold temperature leaves nothing of them.  Rows with the
+    same masks and no NaN are drawn from."""
+    import torch
+
+    vocab = 50257 if n < 100 else 20011
+    kinds = 9
+    for turn in range(kinds if n < kinds else 1):
+        x = some_logits(n + turn, n, vocab, "plain").clamp_(-6.0, 6.0)
+        kind = (torch.arange(n, device="cuda") + turn) % kinds
+        x[kind == 0, :1024] = -math.inf           # 1024 columns are two sections in 32 bits, one in 16
+        x[kind == 0, 700] = math.nan
+        x[kind == 1, :1024] = math.nan
+        x[kind == 2, :8192] = -math.inf           # the first section of every warp
+        x[kind == 2, 8191] = math.nan
+        x[kind == 3, vocab - 3000:] = -math.inf
+        x[kind == 3, vocab - 1] = math.nan
+        x[kind == 4, 0] = math.nan
+        x[kind == 4, vocab // 2] = 26.0           # 20 above all others
+        x[kind == 5, vocab - 1500] = math.nan
+        x[kind == 5, 3] = 26.0
+        x[kind == 6, :vocab // 2 + 1] = -math.inf
+        x[kind == 6, 5000] = math.nan
+        x[kind == 7, :8192] = -math.inf           # no NaN, here and in the last kind
+        x[kind == 8, 3] = 26.0
+        x = rows(x.to(dtype(name)), name, vocab + 3, 1)
+        broken = (kind < 7).cpu().numpy()
+        whole = np.flatnonzero(~broken)[:: max(1, n // 40)]
+        for which in ("none", "greedy", "k", "many k", "p", "nearly all", "min", "k and p", "all"):
+            limits = Limits(n, n, **{**LIMITS[which], **({} if which == "greedy" else {"temperature": t})})
+            ids, lp = draw(tok, x, name, limits)
+            assert (ids[broken] == -1).all() and np.isnan(lp[broken]).all(), (which, kind[torch.from_numpy(broken).cuda()][:9], ids[broken][:9])
+            check_draws(x, limits, ids, lp, only=whole)
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("name", ["f32", "bf16"])
 def test_logits_that_32_bits_hardly_hold(tok, name):
     """Logits up to the largest numbers: differences that no 32-bit float holds, and rows of the type's lowest number alone."""
