@@ -118,9 +118,12 @@ __device__ __forceinline__ StepStatus look_at_step(const StepArgs& a, int64_t be
   block_upto(front, before, s_sum);
   block_upto(rest, all, s_sum);
   StepStatus s{before.a + all.a, before.b + all.b, 0};
-  const int64_t head = a.state[0], tail = a.state[1], waiting = tail - head;
+  // whatever the counts are, nothing here passes 64 bits
+  const int64_t head = a.state[0], tail = a.state[1];
+  const bool counts  = head >= 0 && tail >= head && s.given <= LLONG_MAX - tail;
+  const int64_t waiting = counts ? tail - head : 0;
   if (beyond) s.status = -1;
-  else if (head < 0 || waiting < 0 || waiting + s.given > a.capacity) s.status = -2;
+  else if (!counts || waiting > a.capacity || s.given > a.capacity - waiting) s.status = -2;
   else if (s.taken > waiting) s.status = s.taken - waiting;
   return s;
 }

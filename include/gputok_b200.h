@@ -404,7 +404,8 @@ GTK_API int gtk_sample(gtk_tokenizer* h, const void* d_logits, int type, int64_t
  *   0     done
  *   > 0   so many blocks are missing
  *   -1    a request has, or would have, more blocks than `columns`
- *   -2    the queue cannot be: a negative count, more blocks in it, or more after the step, than it has places
+ *   -2    the queue cannot be: a negative count, or one that passes 64 bits, more blocks taken than given, or more in it, with
+ *         those that this step gives back and without what it takes, than it has places
  * Unless it is 0 nothing is taken, given or written, but for the counts as they were.  n_requests, columns and queue_capacity
  * < 2^31, block_tokens <= 2^20. */
 GTK_API int gtk_block_tables(gtk_tokenizer* h, const int32_t* d_old_lengths, const int32_t* d_new_lengths, int64_t n_requests,

@@ -703,6 +703,34 @@ def test_steps_that_are_not_done(tok, n):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("n", [1, 50, 512, 3000])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_steps_with_queues_that_cannot_be(tok, n, in_place):
+    """Counts at the ends of 64 bits, whose differences and sums pass them; a full queue that gets blocks back though as many are taken."""
+    most, least, block, columns = (1 << 63) - 1, -(1 << 63), 16, 4
+    pool = Pool(n, n, block, columns, columns, n * columns, old=np.full(n, 33))  # three blocks each
+    size = len(pool.queue)
+    back = np.full(n, 33)
+    back[n // 2] = 0
+    both = back.copy()
+    both[-1] = 64 if n > 1 else 0
+    for head, tail in ((0, most), (1, least), (0, least), (least, most), (least, least), (-1, 5), (-5, -1), (most, 0), (most, least), (5, 4),
+                       (most - 1, most), (most, most), (most - 2, most - 2), (0, size + 1), (most - size - 1, most), (7, 7 + size)):
+        pool.head, pool.tail = head, tail
+        for new in (back, both):
+            table, queue, state = run_tables(tok, pool, new, in_place)
+            assert state == [head, tail, -2], (head, tail)
+            assert np.array_equal(table, pool.table) and np.array_equal(queue, pool.queue)
+    # the last counts that there are
+    pool.head, pool.tail = most - 4, most - 3
+    assert check_step(tok, pool, back, in_place) == 0 and (pool.head, pool.tail) == (most - 4, most)
+    grown = pool.old.copy()
+    grown[0] += 16
+    if n > 1:
+        assert check_step(tok, pool, grown, in_place) == 0 and pool.head == most - 3
+
+
+@pytest.mark.gpu
 def test_steps_of_no_requests(tok):
     import torch
 
