@@ -477,6 +477,41 @@ def test_logits_that_32_bits_hardly_hold(tok, name):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("mask", [-1e9, -1e10, -math.inf])
+def test_sample_with_whole_ranges_masked(tok, name, mask):
+    """Stretches of columns at a number that no other column comes near (-inf here: the type's lowest), at the beginning, within and at the
+    end, so that sections and sets of nothing else are looked at."""
+    import torch
+
+    low = float(torch.finfo(dtype(name)).min)
+    n, vocab = 6, 50257
+    x = some_logits(8, n, vocab, "text")
+    x[0, 9000:30000] = x[1, :9000] = x[2, 2000:] = x[3, 40000:] = max(mask, low)
+    x[4, :16384] = x[4, 16500:] = max(mask, low)
+    x[5] = max(mask, low)
+    x = rows(x.to(dtype(name)), name, 50304, 1)
+    for which in ("none", "greedy", "k", "many k", "many k and p", "p", "nearly all", "little min", "all"):
+        limits = Limits(n, n, **LIMITS[which])
+        check_draws(x, limits, *draw(tok, x, name, limits))
+    limits = Limits(n, n, top_k=45000)       # masked columns are among the first where too few others are there
+    check_draws(x, limits, *draw(tok, x, name, limits))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", TYPES)
+@pytest.mark.parametrize("mean,deviation", [(10.0, 2.0), (-6.0, 2.0), (18.0, 3.0), (300.0, 2.0)])
+def test_sample_of_logits_off_zero(tok, name, mean, deviation):
+    """16-bit logits are coarse away from zero: hundreds and thousands of columns are equal at the border of a wide limit."""
+    import torch
+
+    x = (torch.randn(3, 131072, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda") * deviation + mean).to(dtype(name))
+    for limits in (Limits(1, 3, top_p=0.95), Limits(2, 3, top_k=2000), Limits(3, 3, temperature=0.8, top_k=5000, top_p=0.9), Limits(4, 3),
+                   Limits(5, 3, temperature=0.9, top_p=0.9, min_p=1e-3)):
+        check_draws(x, limits, *draw(tok, x, name, limits))
+
+
+@pytest.mark.gpu
 def test_sample_without_logprob_and_of_nothing(tok):
     import torch
 
@@ -666,6 +701,36 @@ def test_block_tables_and_slots(tok, n, block, columns, stride, kind):
     for capacity in {min(total, 1 << 20), min(total, 1 << 20) + 37, max(0, min(total, 1 << 20) - 5), 0}:
         check_slots(tok, pool, old, new, capacity)
     assert check_step(tok, pool, next_lengths(n + 1, np.maximum(pool.old, 0), columns * block, "replace"), in_place=True) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [152000, 200001])
+def test_more_requests_than_ctas_have_threads(tok, n):
+    """More than 1024 requests to each CTA of any GPU's: tiles behind the first go on where it has ended."""
+    pool = Pool(n, n, 16, 2, 2, 2 * n + 5, head=77)
+    for i, kind in enumerate(("replace", "full", "step", "gone")):
+        old = pool.old.copy()
+        new = next_lengths(i, old, 32, kind)
+        assert check_step(tok, pool, new, in_place=i % 2 == 1) == 0
+        total = int(np.where(new > old, new - old, 0).sum())
+        check_slots(tok, pool, old, new, min(total, 1 << 20) + 5)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n,every", [(20000, 10), (20000, 9999), (100000, 100), (8193, 8193)])
+def test_slots_of_few_among_many_requests(tok, n, every):
+    """Few of many requests have new tokens: those of a CTA lie among more requests than its shared memory has room for."""
+    pool = Pool(n, n, 16, 3, 3, 3 * n)
+    new = pool.old.copy()
+    new[every // 2::every] = np.minimum(new[every // 2::every] + 1, 48)
+    new[every // 3::every] = np.maximum(new[every // 3::every] - 1, 0)
+    total = int(np.where(new > pool.old, new - pool.old, 0).sum())
+    far = pool.old.copy()
+    far[[0, n - 1]] += 700
+    assert check_step(tok, Pool(n, n, 16, 3, 3, 3 * n, old=pool.old), new) == 0
+    for capacity in (total, total + 3000, max(1, total // 2)):
+        check_slots(tok, pool, pool.old, new, capacity)
+    check_slots(tok, pool, pool.old, far, 1500)
 
 
 @pytest.mark.gpu
@@ -897,6 +962,52 @@ def test_a_step_captured_and_replayed(native_built, merges_path):
         assert np.array_equal(table.cpu().numpy(), pool.table) and np.array_equal(queue.cpu().numpy(), pool.queue)
         assert np.array_equal(slots.cpu().numpy(), want_slots(pool, now, now + 1, n)[0])
         check_draws(x, limits, ids.cpu().numpy(), lp.cpu().numpy(), only=range(step % 7, n, 7))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("n", [600, 9000])
+def test_steps_of_many_requests_captured_and_replayed(native_built, merges_path, n):
+    """Calls of two kernels each, in one graph behind each other and behind what moves their lengths on."""
+    import torch
+
+    t = Tokenizer(merges_path, 2048, 50, device=0)
+    block, columns, vocab = 4, 6, 300
+    pool = Pool(5, n, block, columns, columns, n * columns, old=np.arange(n) % 3)
+    old, new = (torch.from_numpy(a.astype(np.int32)).cuda() for a in (pool.old, pool.old + 1))
+    table, queue = torch.from_numpy(pool.table.copy()).cuda(), torch.from_numpy(pool.queue.copy()).cuda()
+    state = torch.tensor([pool.head, pool.tail, 0], dtype=torch.int64, device="cuda")
+    capacity = 5 * n
+    slots, offsets = (torch.empty(k, dtype=torch.int64, device="cuda") for k in (capacity, n + 1))
+    positions, requests = (torch.empty(capacity, dtype=torch.int32, device="cuda") for _ in range(2))
+    x = typed_logits(1, n, vocab, "text", "bf16")
+    limits = Limits(1, n, **LIMITS["mixed"])
+    u, temp, k, p, m = limits.device()
+    ids, lp = torch.empty(n, dtype=torch.int32, device="cuda"), torch.empty(n, device="cuda")
+    s = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    t.set_stream(s.cuda_stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=s):
+        t.block_tables(old.data_ptr(), new.data_ptr(), n, block, table.data_ptr(), columns, queue.data_ptr(), len(pool.queue),
+                       state.data_ptr(), state.data_ptr())
+        t.slot_map(old.data_ptr(), new.data_ptr(), n, block, table.data_ptr(), columns, capacity, slots.data_ptr(), offsets.data_ptr(),
+                   positions.data_ptr(), requests.data_ptr(), state.data_ptr())
+        t.sample(x.data_ptr(), "bf16", n, vocab, u.data_ptr(), ids.data_ptr(), lp.data_ptr(), temp.data_ptr(), k.data_ptr(), p.data_ptr(),
+                 m.data_ptr())
+        old.copy_(new)
+        new.add_(torch.where(new % 7 == 3, 5, 1)).remainder_(columns * block)  # some bring several, some end
+    for step in range(12):
+        x.copy_(some_logits(step + 5, n, vocab, "text"))
+        now, then = pool.old.copy(), new.cpu().numpy().astype(np.int64)
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert pool.step(then) == 0
+        assert state.tolist() == [pool.head, pool.tail, 0]
+        assert np.array_equal(table.cpu().numpy(), pool.table) and np.array_equal(queue.cpu().numpy(), pool.queue)
+        for got, want in zip((slots, positions, requests, offsets), want_slots(pool, now, then, capacity)):
+            assert np.array_equal(got.cpu().numpy(), want)
+        check_draws(x, limits, ids.cpu().numpy(), lp.cpu().numpy(), only=range(step, n, 61))
 
 
 @pytest.mark.gpu
