@@ -1062,12 +1062,12 @@ struct Best {
   }
 };
 
-// A section's sum, relative to 2^c_top.  A NaN stays one however far below the section's reference lies (a section that is masked but for it, or one that
-// a cold temperature leaves nothing of): a sum is NaN where, and only where, its section has a NaN or +inf, and rows are told broken by it.
+// A section's sum, relative to 2^c_top.  A broken section's reference is NaN, so that its sum is one too however far below the highest its numbers
+// lie (all masked but one, or nothing left of them by a cold temperature).
 __device__ __forceinline__ double of_section(const float2& v, float c_top)
 {
-  const int e = int(fmaxf(v.x - c_top, -1000.f));
-  return e > -1000 || isnan(v.y) ? double(v.y) * __hiloint2double((e + 1023) << 20, 0) : 0.0;
+  const float d = v.x - c_top;
+  return d <= -1000.f ? 0.0 : double(v.y) * __hiloint2double((int(d) + 1023) << 20, 0);
 }
 
 // locate() with the sums of the first reading, relative to 2^c_top: sections in 64 bits, within its section in 32.
@@ -1537,7 +1537,8 @@ __global__ void __launch_bounds__(kThreads, 4) k_sample(const T* __restrict__ lo
     float lo, hi;
     sum[0].get(lo, hi);
     lo = warp_sum(lo + hi);
-    if (lane == 0 && GTK_IN(s, row.sections, 503)) piece[s] = make_float2(c, lo);
+    // NaN where, and only where, the section has a NaN or +inf: rows are told broken by it
+    if (lane == 0 && GTK_IN(s, row.sections, 503)) piece[s] = make_float2(isnan(lo) ? lo : c, lo);
   };
   for (int s = begin + warp; s < end; s += 2 * warps) {
     uint4 next[kPacks];
