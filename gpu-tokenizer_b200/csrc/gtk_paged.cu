@@ -118,13 +118,13 @@ __device__ __forceinline__ StepStatus look_at_step(const StepArgs& a, int64_t be
   block_upto(front, before, s_sum);
   block_upto(rest, all, s_sum);
   StepStatus s{before.a + all.a, before.b + all.b, 0};
-  // whatever the counts are, nothing here passes 64 bits
-  const int64_t head = a.state[0], tail = a.state[1];
-  const bool counts  = head >= 0 && tail >= head && s.given <= LLONG_MAX - tail;
-  const int64_t waiting = counts ? tail - head : 0;
+  // The counts may be anything.  Their difference and sum wrap: with a head and a new tail that are not negative and a difference that is
+  // no more than the places for what comes back, neither has.
+  const uint64_t head = uint64_t(a.state[0]), tail = uint64_t(a.state[1]), waiting = tail - head;
+  const int64_t room = a.capacity - s.given;
   if (beyond) s.status = -1;
-  else if (!counts || waiting > a.capacity || s.given > a.capacity - waiting) s.status = -2;
-  else if (s.taken > waiting) s.status = s.taken - waiting;
+  else if ((int64_t(head) | int64_t(tail + uint64_t(s.given)) | room) < 0 || waiting > uint64_t(room)) s.status = -2;
+  else if (s.taken > int64_t(waiting)) s.status = s.taken - int64_t(waiting);
   return s;
 }
 
