@@ -3,9 +3,10 @@
 // With B tokens per block, a request of L tokens holds ceil(L / B) blocks, and its token j lies in slot
 // table[j / B] * B + j % B.  Blocks that nobody holds wait in a ring: taken at its head, given back at its tail.
 //
-// A step moves little: what it takes is launches, sums over all requests, and loads that wait for each other.  Measured: blocks of 256 requests 7 us,
-// of 8192 of which half are replaced 17 (205 by one CTA that moves all of them); slots of 256 tokens 3.9, of a million of 512 requests 10 (floor 2.6; 18
-// with a search for each token), of 8192 requests 17.
+// A step moves little: what it takes is launches, sums over all requests, and loads that wait for each other.  Measured in a graph of calls behind
+// each other: blocks of 256 requests 7.9 us, of 8192 of which half are replaced 17 (205 by one CTA that moves all of them); slots of 256
+// tokens 4.2, of a million of 512 requests 9.6 (floor 2.6; 18 with a search for each token), of 8192 requests 19.6, of one token each 12.7,
+// and of 8193, offsets first, 23.7.
 #include <climits>
 
 #include "gtk_checked.cuh"
@@ -96,8 +97,8 @@ __device__ __forceinline__ Pair block_upto(Pair x, Pair& all, Pair (&s_sum)[kWar
 static_assert(kWarps == 32, "");
 
 // Each CTA forms the sums over all requests by itself (they are read from L2: 64 KiB for 8192 of them), and then moves the blocks of a share of
-// the requests, in tiles of a thread each; a warp moves those of one request after the other.  The state is written by the kernel behind this one, when all
-// have read it.
+// the requests, in tiles of a thread each; a warp moves those of one request after the other.  The state is written by the kernel behind this
+// one, when all have read it.
 struct StepStatus {
   int64_t taken, given, status;
 };
@@ -219,10 +220,11 @@ __device__ __forceinline__ int64_t new_tokens(const SlotArgs& a, int64_t r)
   return before >= 0 && after > before ? int64_t(after) - before : 0;
 }
 
-// The tokens [begin, end) of the step, those below `total` of requests [first, n), which offset_at(request) tells the owners of, by all threads; a warp takes neighbouring ones, and looks for a request
-// among all only where it is not the one of the token 32 places before.
+// The tokens [begin, end) of the step, those below `total` of requests [first, n), which offset_at(request) tells the owners of, by all threads; a
+// warp takes neighbouring ones, and looks for a request among all only where it is not the one of the token 32 places before.
 template <class OffsetAt>
-__device__ __forceinline__ void put_slots(const SlotArgs& a, int64_t begin, int64_t end, int64_t first, int64_t n, int64_t total, OffsetAt&& offset_at)
+__device__ __forceinline__ void put_slots(const SlotArgs& a, int64_t begin, int64_t end, int64_t first, int64_t n, int64_t total,
+                                          OffsetAt&& offset_at)
 {
   constexpr int kOnce = 4;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -352,8 +354,10 @@ __global__ void __launch_bounds__(kThreads) k_slots_of_many(const SlotArgs a, in
   }
 }
 
-// Requests of a CTA that is the only one, at most, and of one of several, at least.  Alone and with others, us: 512 requests that are replaced 13.0 and 11.4,
-// in a decoding step 8.4 and 10; 1024 of them 19.0 and 10.7, 12.5 and 10.5.
+// Requests of a CTA that is the only one, at most, and of one of several, at least.  Alone and with others, us (512 and 513 requests, in a graph): in
+// a decoding step 9.3 and 10.5; half of them replaced by others of up to 8192 tokens 17.5 and 10.5.  The rule knows of requests and not of
+// their blocks, whose number is in device memory: 512 new ones of 131072 tokens each in blocks of 16, four million blocks, take one CTA 1630,
+// 513 take all CTAs 123.
 constexpr int64_t kAlone = 512, kShare = 32;
 constexpr int64_t kMost = (int64_t(1) << 31) - 1;
 
@@ -364,7 +368,8 @@ gtk::Refusal refuse_step(const void* before, const void* after, int64_t n, int b
   if (columns <= 0 || columns > kMost) return "columns must be 1 .. 2^31 - 1";
   if (stride < columns) return "table_stride must be >= columns";
   if (n > 0 && (!before || !after || !tables)) return "null device pointer";
-  if (!gtk::aligned_to(before, 4) || !gtk::aligned_to(after, 4) || !gtk::aligned_to(tables, 4)) return "a device pointer is not aligned to its elements";
+  if (!gtk::aligned_to(before, 4) || !gtk::aligned_to(after, 4) || !gtk::aligned_to(tables, 4))
+    return "a device pointer is not aligned to its elements";
   return nullptr;
 }
 
@@ -383,7 +388,8 @@ extern "C" GTK_API int gtk_block_tables(gtk_tokenizer* h, const int32_t* d_old_l
     return nullptr;
   };
   return gtk::run_operator(h, check, [&](const gtk::HandleView& v) -> cudaError_t {
-    const StepArgs a{{d_old_lengths, d_new_lengths, n_requests, Divisor(block_tokens)}, d_tables, columns, table_stride, d_queue, queue_capacity, d_state, d_state_out};
+    const StepArgs a{{d_old_lengths, d_new_lengths, n_requests, Divisor(block_tokens)},
+                     d_tables, columns, table_stride, d_queue, queue_capacity, d_state, d_state_out};
     const int64_t ctas = n_requests > kAlone ? std::min<int64_t>((n_requests + kShare - 1) / kShare, v.sm_count) : 1;
     if (ctas == 1) return gtk::launch(k_block_tables<true>, dim3(1), dim3(kThreads), 0, v.stream, a, n_requests);
     const int64_t share = (n_requests + ctas - 1) / ctas;
@@ -413,7 +419,9 @@ extern "C" GTK_API int gtk_slot_map(gtk_tokenizer* h, const int32_t* d_old_lengt
       if (const cudaError_t e = gtk::launch(k_slot_offsets, dim3(1), dim3(kThreads), 0, v.stream, a); e != cudaSuccess) return e;
     const int64_t ctas  = std::max<int64_t>(1, std::min<int64_t>((capacity + kThreads - 1) / kThreads, int64_t(v.sm_count)));
     const int64_t share = (capacity + ctas - 1) / ctas;
-    const auto of_few = n_requests <= kThreads ? k_slots_of_few<1> : n_requests <= 4 * kThreads ? k_slots_of_few<4> : k_slots_of_few<kFewRequests / kThreads>;
+    const auto of_few = n_requests <= kThreads       ? k_slots_of_few<1>
+                        : n_requests <= 4 * kThreads ? k_slots_of_few<4>
+                                                     : k_slots_of_few<kFewRequests / kThreads>;
     return few ? gtk::launch(of_few, dim3(unsigned(ctas)), dim3(kThreads), 0, v.stream, a, share)
                : gtk::launch_behind(k_slots_of_many, dim3(unsigned(ctas)), dim3(kThreads), 0, v.stream, a, share);
   });

@@ -7,13 +7,16 @@
 // A row is read once.  Its weights are summed in 32 bits, by sections of neighbouring columns, and every decision that hangs on such a
 // sum is held against a bound of its error (Row::exponent_error); where a border lies within the bound the row is summed again in 64 bits.
 //
-// The reading is bound by memory, what follows it by phases that wait for each other.  Measured against a copy (6.57 TB/s):
-//   1024 rows of 131072 bf16, no limits   52 us, 78 %, the reading alone 47; where a model is unsure of thousands of ids, some ten of them are looked
-//                                         at again, which takes one CTA 80 us each: 129
-//   2048 rows of 50257 f32                73 us, 86 %, with min-p 80, with the 50 highest 123
-//   512 rows of 50257 bf16, the highest   17 us
-//   one row of 50257 bf16                 5.9 us without limits, 14 with top-k and top-p
-//   64 rows of 131072 f32, wide nuclei    76 us: three readings, 120 instructions an element, 17 of them in 64 bits
+// The reading is bound by memory, what follows it by phases that wait for each other.  Measured against a copy (6.57 TB/s), in a graph of calls
+// whose inputs together pass L2; logits normal with a head of 64 likely ids, whose lead differs from row to row, "sure" with one far above all:
+//   1024 rows of 131072 bf16, no limits   sure 53.7 us, 76 %; where a model is unsure of thousands of ids, some ten of them are looked
+//                                         at again, which takes one CTA 80 us each: 137
+//   2048 rows of 50257, no limits, sure   f32 71.8 us, 87 %, bf16 47.5, fp16 46.7; unsure 111, 91, 88
+//   the same, unsure, with the 50 highest f32 136 us, bf16 90, fp16 87; with min-p 0.05 instead 153, 106, 103
+//   512 rows of 50257, the highest        f32 23.4 us, bf16 17.5, fp16 17.2; weights are summed in these too, for the NaN that they tell of
+//   one row of 50257 bf16                 6.1 us without limits, 14.7 with top-k and top-p
+//   64 rows of 131072 f32, wide nuclei    77 us: three readings, 120 instructions an element, 17 of them in 64 bits
+//   64 rows of 131072 bf16, top-p 0.95, normal with deviation 2, T = 1: mean 0 1255 us, mean 10 5370; see Slowly::search
 #include <cooperative_groups.h>
 
 #include <cfloat>
@@ -359,8 +362,8 @@ struct Place {
   float x;
 };
 
-// The first column at which the sum of the weights exceeds the target, `share` of the sum of all, by one warp: section(s) is a section's sum, weigh(s)(x,
-// column, w) the weights of columns in it.  The last one with any weight where rounding leaves none, column -1 where none has any.
+// The first column at which the sum of the weights exceeds the target, `share` of the sum of all, by one warp: section(s) is a section's sum,
+// weigh(s)(x, column, w) the weights of columns in it.  The last one with any weight where rounding leaves none, column -1 where none has any.
 template <class T, class Section, class Weigh>
 __device__ __forceinline__ Place locate(const Row<T>& row, double share, double& total, Section&& section, Weigh&& weigh)
 {
@@ -464,7 +467,10 @@ struct Slowly {
   }
 
   // Raises the floor to the highest value at which enough(sum over the columns that reach it) holds, and there to as many columns of that
-  // value as are wanted(sum over those above it).
+  // value as are wanted(sum over those above it).  A reading in 64 bits for each halving, up to 32 of them, and four more: 80 us each for 131072
+  // columns.  Rows come here with some hundreds of equal logits at the border of a wide limit, which 16-bit logits away from 0 have (bf16 of
+  // mean 10 and deviation 2, 131072 of them, top-p 0.95: 1596), and by a top-k with more than 512 candidates where sets of columns are masked
+  // by a finite number far below (64 rows of 50257 f32, top-k 700, 21000 columns at -1e9: 1238 us, at -inf 65).
   template <class Enough, class Wanted>
   __device__ void search(uint32_t most, Enough&& enough, Wanted&& wanted)
   {
@@ -758,8 +764,8 @@ __device__ __noinline__ double count_columns(const Row<T>& row, const Team<SPLIT
   return sum;
 }
 
-// Sums in 64 bits, of columns that reach v.floor: those above interval v.b (v.yes: all) and at least v.a by sections, all of them together; lists those in
-// front of interval v.c, and tells how many are above and whether some of these are below v.a.
+// Sums in 64 bits, of columns that reach v.floor: those above interval v.b (v.yes: all) and at least v.a by sections, all of them together; lists
+// those in front of interval v.c, and tells how many are above and whether some of these are below v.a.
 struct Above {
   double all;
   int count;
@@ -767,7 +773,8 @@ struct Above {
 };
 // PLAIN: by weight, no round before, no min-p.
 template <bool PLAIN, class T, bool SPLIT>
-__device__ __noinline__ Above sum_above(const Row<T>& row, const Team<SPLIT>& team, const Weight64 weight, const Interval v, double* section, Scratch& S)
+__device__ __noinline__ Above sum_above(const Row<T>& row, const Team<SPLIT>& team, const Weight64 weight, const Interval v, double* section,
+                                        Scratch& S)
 {
   constexpr int E = Row<T>::E, kOnce = 4;  // columns at a time
   const int warps = blockDim.x >> 5, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -930,7 +937,8 @@ __device__ __noinline__ bool draw_wide(const Row<T>& row, const Limits& l, const
         if (first == kFine) return false;  // the limit is further down
         // how many columns that may be
         int n = 0;
-        for (int b = first + lane; b <= last; b += 32) n += int(float(reinterpret_cast<const uint32_t*>(fine)[b]) * unit * 1.02f * (mass ? pow2(step * 0.5f) : 1.f)) + 1;
+        for (int b = first + lane; b <= last; b += 32)
+          n += int(float(reinterpret_cast<const uint32_t*>(fine)[b]) * unit * 1.02f * (mass ? pow2(step * 0.5f) : 1.f)) + 1;
         n = warp_sum(n);
         float so_far = 0.f;  // by number, which front and these are exactly
         if (!mass)
@@ -954,7 +962,8 @@ __device__ __noinline__ bool draw_wide(const Row<T>& row, const Limits& l, const
     __syncthreads();
     const float x_least = key_value(uint64_t(key_least) << 32), from_first = float(first), upto_last = float(last + 1);
     const Interval v{floor, hi, scale, beyond, x_least, from_first, upto_last, 0.f, round == 2, false};
-    const Above found = round == 1 && floor == 1 && !(l.least > 0.f) ? sum_above<true>(row, team, weight, v, section, S) : sum_above<false>(row, team, weight, v, section, S);
+    const Above found = round == 1 && floor == 1 && !(l.least > 0.f) ? sum_above<true>(row, team, weight, v, section, S)
+                                                                     : sum_above<false>(row, team, weight, v, section, S);
     double sum_all    = found.all;
     int count         = found.count;
     bool cut_short    = found.cut_short;
@@ -1008,7 +1017,8 @@ __device__ __noinline__ bool draw_wide(const Row<T>& row, const Limits& l, const
       if (solved && !(round == 0 && by_mass)) {
         floor = max(floor, uint64_t(key_least) << 32);
         // the sections with what is left of the list, and the draw
-        for (int i = tid; i < left; i += threads) S.order[i] = uint16_t(S.key[i] >= floor ? int(key_column(S.key[i]) + row.lead) / Row<T>::kColumns : 0xFFFF);
+        for (int i = tid; i < left; i += threads)
+          S.order[i] = uint16_t(S.key[i] >= floor ? int(key_column(S.key[i]) + row.lead) / Row<T>::kColumns : 0xFFFF);
         __syncthreads();
         for (int s = tid; s < row.sections; s += threads) {
           double sum = 0.0;
@@ -1559,12 +1569,14 @@ __global__ void __launch_bounds__(kThreads, 4) k_sample(const T* __restrict__ lo
 static_assert(sizeof(Scratch) + (GTK_MAX_SAMPLE_VOCAB / (32 * kPacks * 4) + 1) * sizeof(double) <= 48 << 10, "what a CTA has without asking");
 
 // How many CTAs share a row, and how many threads they have.
-// In 1 / 2 / 4 / 8 parts of 256 threads, us: one row of 50257 bf16 without limits - / 9.8 / 8.9 / 8.4, 64 of 131072 f32 23.7 / 15.9 / 12.7 / 14, with
-// the 50 highest 42 / 25 / 19 / 22; 148 of 50257 bf16 9.8 / 9.8 / 13.1, with limits 16.7 / 16.9 / 27; 256 of f32 21.6 / 23.2 / 28.
-// A nucleus may be wide, and a wide row is bound by instructions: 256 rows of 50304 f32, a few of them wide, take 102 / 74 / 66, with none 27 / 25 / 36; 333
-// of 32003 fp16, all of them wide, 84 / 119 / 162.
-// Rows in numbers take 128 threads, so that more of them are under way while others are at their ends: of 256 / 128, 2048 rows of 50257 f32 80 / 73,
-// bf16 50 / 45, with min-p 73 / 63; 512 of bf16 24 / 28.
+// When the rule was chosen, in 1 / 2 / 4 / 8 parts of 256 threads, us: one row of 50257 bf16 without limits - / 9.8 / 8.9 / 8.4, 64 of 131072 f32
+// 23.7 / 15.9 / 12.7 / 14, with the 50 highest 42 / 25 / 19 / 22; 148 of 50257 bf16 9.8 / 9.8 / 13.1, with limits 16.7 / 16.9 / 27; 256 of f32
+// 21.6 / 23.2 / 28.  A nucleus may be wide, and a wide row is bound by instructions: 256 rows of 50304 f32, a few of them wide, took 102 / 74 / 66,
+// with none 27 / 25 / 36; 333 of 32003 fp16, all of them wide, 84 / 119 / 162.
+// At its borders now, a row less in two parts and a row more in one: 74 and 75 nuclei of 50257 bf16 (0.95 at T = 0.8) 60 and 72, 0.99 at 1.3
+// 67 and 80; 296 and 297 of f32 102 and 112, 112 and 119.  Nuclei of rows between were not measured in both ways.
+// Rows in numbers take 128 threads, so that more of them are under way while others are at their ends: of 256 / 128, 2048 rows of 50257 f32
+// 80 / 73, bf16 50 / 45, with min-p 73 / 63; 512 of bf16 24 / 28.
 struct Teams {
   int parts, threads;
 };
@@ -1602,7 +1614,8 @@ extern "C" GTK_API int gtk_sample(gtk_tokenizer* h, const void* d_logits, int ty
     if (n_rows > kMaxRows || vocab > GTK_MAX_SAMPLE_VOCAB) return "n_rows of 2^31 and more, or vocab beyond 2^20";
     if (n_rows == 0) return nullptr;
     if (!d_logits || !d_uniform || !d_ids) return "null device pointer";
-    if (!gtk::aligned_to(d_logits, gtk::element_size(type)) || !gtk::aligned_to(d_uniform, 8)) return "a device pointer is not aligned to its elements";
+    if (!gtk::aligned_to(d_logits, gtk::element_size(type)) || !gtk::aligned_to(d_uniform, 8))
+      return "a device pointer is not aligned to its elements";
     for (const void* q : {static_cast<const void*>(d_temperature), static_cast<const void*>(d_top_k), static_cast<const void*>(d_top_p),
                           static_cast<const void*>(d_min_p), static_cast<const void*>(d_ids), static_cast<const void*>(d_logprob)})
       if (!gtk::aligned_to(q, 4)) return "a device pointer is not aligned to its elements";

@@ -383,8 +383,8 @@ GTK_API int gtk_token_logprobs_grad(gtk_tokenizer* h, const void* d_logits, int 
  * d_temperature (then 1), d_top_k, d_top_p, d_min_p (then all) and d_logprob may be NULL.  Which columns stay and which one is
  * drawn is decided as in 64-bit arithmetic, and does not depend on the run.
  *   T == 0              the highest logit, of equal ones the lowest column, with log probability 0
- *   d_uniform[r] < 0    no request: id -1, log probability 0, the row is not looked at
- *   d_uniform[r] >= 1   the last column that is left
+ *   d_uniform[r] < 0    no request: id -1, log probability 0, whatever the row holds (its memory may be read)
+ *   d_uniform[r] >= 1   the last column that is left with a weight above 0 in 64 bits
  *   a row of -inf       id -1, log probability -inf
  *   a row with a NaN or +inf, a NaN limit or random number, a negative, infinite or NaN temperature: id -1, log probability NaN
  * n_rows < 2^31, vocab <= GTK_MAX_SAMPLE_VOCAB. */
